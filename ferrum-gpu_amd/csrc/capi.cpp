@@ -21,6 +21,7 @@
 #include "hip_backend.hpp"
 #include "host_stage.hpp"
 #include "scratch.hpp"
+#include "ssm_ops.hpp"
 
 using fg::Buffer;
 using fg::Cf32;
@@ -47,6 +48,7 @@ struct fg_device {
     Buffer<Cf32, HipBackend> staging;
     Buffer<Cf32, HipBackend> staging_out;  // out-of-place outputs (plans whose in-place form differs)
     fg::Pointwise pointwise;  // elementwise kernels of fft_module
+    fg::SsmKernels ssm;       // the sequence filters' code objects
     std::atomic<int> dependents{0};  // live plans and captured graphs made on this device
     std::unique_ptr<fg::HostStager> stager;  // pinned pieces of the host path (first large call)
     // fg_fft_exec_split_noalloc: calls on this device take turns at the
@@ -86,6 +88,16 @@ struct fg_fft_plan {
     std::unique_ptr<FftPlan> plan;
     fg_device* dev = nullptr;
     std::atomic<int> graphs{0};  // live fg_graph objects that replay this plan
+};
+
+struct fg_conv_plan {
+    std::unique_ptr<fg::ConvPlan> plan;
+    fg_device* dev = nullptr;
+};
+
+struct fg_scan_plan {
+    std::unique_ptr<fg::ScanPlan> plan;
+    fg_device* dev = nullptr;
 };
 
 struct fg_graph {
@@ -129,6 +141,7 @@ fg_device* open_device(int ordinal) {
     d->dev.reset(new HipDevice(h));
     d->fft_module = d->dev->load_or_cache(fg::fft_code_object());
     d->pointwise = fg::Pointwise(d->fft_module);
+    d->ssm = fg::SsmKernels(*d->dev);
     // The allocation-free entry point's scratch area: its address on this
     // device, resolved once with the device current (scratch.hip).
     HipBackend::bind(h);
@@ -865,6 +878,106 @@ int fg_stream_copy(fg_device_t dev, const void* d_in, void* d_out, size_t bytes,
         need(d_in, "d_in");
         need(d_out, "d_out");
         dev->pointwise.stream_copy(dev->dev->handle(), d_in, d_out, bytes, (hipStream_t)stream);
+    });
+}
+
+int fg_conv_plan_create(fg_device_t dev, const fg_conv_shape* shape, fg_conv_plan_t* out) {
+    return guarded([&] {
+        need(out, "out");
+        *out = nullptr;
+        need(dev, "device");
+        need(shape, "shape");
+        std::unique_ptr<fg_conv_plan> p(new fg_conv_plan);
+        p->dev = dev;
+        p->plan.reset(new fg::ConvPlan(dev->dev->handle(), dev->ssm, *shape));
+        dev->dependents.fetch_add(1);
+        *out = p.release();
+    });
+}
+
+int fg_conv_plan_destroy(fg_conv_plan_t plan) {
+    return guarded([&] {
+        if (!plan) return;
+        plan->dev->dependents.fetch_sub(1);
+        delete plan;
+    });
+}
+
+int fg_conv_forward(fg_conv_plan_t plan, const fg_conv_forward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->forward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_conv_backward(fg_conv_plan_t plan, const fg_conv_backward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->backward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_conv_step(fg_device_t dev, const fg_conv_step_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(dev, "device");
+        need(args, "args");
+        dev->ssm.conv_step(dev->dev->handle(), *args, (hipStream_t)stream);
+    });
+}
+
+int fg_scan_plan_create(fg_device_t dev, const fg_scan_shape* shape, fg_scan_plan_t* out) {
+    return guarded([&] {
+        need(out, "out");
+        *out = nullptr;
+        need(dev, "device");
+        need(shape, "shape");
+        std::unique_ptr<fg_scan_plan> p(new fg_scan_plan);
+        p->dev = dev;
+        p->plan.reset(new fg::ScanPlan(dev->dev->handle(), dev->ssm, *shape));
+        dev->dependents.fetch_add(1);
+        *out = p.release();
+    });
+}
+
+int fg_scan_plan_destroy(fg_scan_plan_t plan) {
+    return guarded([&] {
+        if (!plan) return;
+        plan->dev->dependents.fetch_sub(1);
+        delete plan;
+    });
+}
+
+int fg_scan_checkpoint_bytes(fg_scan_plan_t plan, size_t* bytes) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(bytes, "bytes");
+        *bytes = plan->plan->checkpoint_bytes();
+    });
+}
+
+int fg_scan_forward(fg_scan_plan_t plan, const fg_scan_forward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->forward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_scan_backward(fg_scan_plan_t plan, const fg_scan_backward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->backward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_scan_step(fg_device_t dev, const fg_scan_step_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(dev, "device");
+        need(args, "args");
+        dev->ssm.scan_step(dev->dev->handle(), *args, (hipStream_t)stream);
     });
 }
 

@@ -1,0 +1,91 @@
+/* ssm_args.h -- kernel arguments and tile sizes of the sequence filters
+ * (ssm_conv.hpp, ssm_scan.hpp), shared by the kernels and their host
+ * launchers (ssm_ops.cpp). */
+#ifndef FG_SSM_ARGS_H
+#define FG_SSM_ARGS_H
+
+#include <stdint.h>
+
+#define FG_SSM_WAVES 4            /* waves of a workgroup of the scan */
+#define FG_SSM_WAVE_CHANNELS 16   /* channels of a wave */
+#define FG_SSM_GROUP_CHANNELS (FG_SSM_WAVES * FG_SSM_WAVE_CHANNELS)
+#define FG_SSM_MAX_STATES 64
+#define FG_CONV_MAX_WIDTH 8
+
+/* States of a channel that one lane holds: the channel's states are spread
+ * over four lanes.  1, 2, 4, 8 or 16. */
+static inline uint32_t fg_ssm_lane_states(uint32_t states) {
+    uint32_t s = 1;
+    while (4 * s < states) s *= 2;
+    return s;
+}
+/* Tokens of a segment, the unit that the scan works through; the states at
+ * the start of each are what a forward pass leaves for its backward pass. */
+#define FG_SSM_SEGMENT(lane_states) ((lane_states) <= 4 ? 16 : 64 / (lane_states))
+
+/* Rows of a [sequences, tokens, n] array, strides in elements. */
+typedef struct {
+    void* p;
+    int64_t seq, row;
+} fg_ssm_view;
+
+typedef struct {
+    fg_ssm_view u, delta, b, c, z, out;      /* z.p null: no gate */
+    fg_ssm_view gu, gdelta, gb, gc, gz, gout; /* gradients; out.p and those may be null */
+    const float *a, *skip, *bias, *initial;
+    float* final;
+    const float* gfinal;
+    float *ga, *gskip, *gbias, *ginitial;
+    const int32_t* offsets; /* packed: sequences + 1 of them; null: dense */
+    float* check;           /* states at segment starts */
+    float* carry;           /* [sequences][chunks + 1][wave blocks][64 * lane states]: what a chunk adds;
+                               the last place: the initial states */
+    float* carry_dt;        /* [sequences][chunks + 1][wave blocks][16]: its summed time steps */
+    float* part_bc;         /* [channel blocks of a group][tokens][groups][2][states] */
+    float* part_p;          /* [sequences * chunks][channels * (states + 2)] */
+    uint64_t tokens;        /* packed: of all sequences */
+    uint32_t seqs, length, channels, states, groups;
+    uint32_t group_channels, group_blocks; /* channels of a group, workgroups over them */
+    uint32_t chunks, chunk_len;            /* chunk_len: a multiple of the segment */
+    uint32_t check_segs;                   /* dense: segments of a sequence */
+    uint32_t softplus;
+} fg_scan_kargs;
+
+typedef struct {
+    fg_ssm_view u, delta, b, c, z, out; /* .seq: of rows; .row unused */
+    const float *a, *skip, *bias, *state;
+    float* state_out;
+    const int32_t* slots;
+    uint64_t state_rows;
+    uint32_t rows, channels, states, groups, group_channels;
+    uint32_t lanes; /* lanes of a channel */
+    uint32_t softplus;
+} fg_scan_step_kargs;
+
+typedef struct {
+    fg_ssm_view x, out;       /* backward: x and the output's gradient */
+    fg_ssm_view gx;
+    const float *weight, *bias;
+    const void* initial;      /* [sequences][width - 1][channels] */
+    void* final;
+    const void* gfinal;
+    void* ginitial;
+    float* part;              /* [parts][channels * (width + 1)] */
+    const int32_t* offsets;
+    uint64_t tokens;
+    uint32_t seqs, length, channels, run; /* run: tokens of a thread */
+    uint32_t runs;                        /* runs of the longest sequence */
+    uint32_t silu;
+} fg_conv_kargs;
+
+typedef struct {
+    fg_ssm_view x, out;
+    const float *weight, *bias;
+    const void* state;
+    void* state_out;
+    const int32_t* slots;
+    uint64_t state_rows;
+    uint32_t rows, channels, silu;
+} fg_conv_step_kargs;
+
+#endif

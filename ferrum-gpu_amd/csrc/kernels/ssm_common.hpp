@@ -1,0 +1,94 @@
+// ssm_common.hpp -- element types, activations and lane exchanges of the
+// sequence filters' kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "ssm_args.h"
+
+namespace fg {
+namespace ssm {
+
+struct F32 {
+    using raw = float;
+    static __device__ __forceinline__ float up(raw x) { return x; }
+    static __device__ __forceinline__ raw down(float x) { return x; }
+};
+struct BF16 {
+    using raw = unsigned short;
+    static __device__ __forceinline__ float up(raw x) { return __uint_as_float((uint32_t)x << 16); }
+    static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
+};
+struct F16 {
+    using raw = unsigned short;
+    static __device__ __forceinline__ float up(raw x) { return (float)__builtin_bit_cast(_Float16, x); }
+    static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
+};
+
+template <int I>
+struct Int {
+    static constexpr int value = I;
+    constexpr operator int() const { return I; }
+};
+// f(Int<0>), f(Int<1>), ... f(Int<N - 1>): a loop whose index is a constant.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F&& f) {
+    if constexpr (I < N) {
+        f(Int<I>{});
+        each<N, I + 1>(f);
+    }
+}
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 1 / (1 + exp(-x)).
+__device__ __forceinline__ float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + exp2_(-kLog2e * x));
+}
+
+// log(1 + exp(x)) and its derivative 1 / (1 + exp(-x)), both from
+// e = exp(-|x|): max(x, 0) + log1p(e), and (x >= 0 ? 1 : e) / (1 + e).
+// log1p(e) = log(w) + (e - (w - 1)) / w for the rounded w = 1 + e: the second
+// term is what the rounding took away, so time steps far below 1 keep their
+// relative accuracy.
+struct Softplus {
+    float value, slope;
+};
+__device__ __forceinline__ Softplus softplus(float x) {
+    const float e = exp2_(-kLog2e * fabsf(x));
+    const float w = 1.0f + e, r = __builtin_amdgcn_rcpf(w);
+    const float l = fmaf(e - (w - 1.0f), r, kLn2 * __builtin_amdgcn_logf(w));
+    return {fmaxf(x, 0.0f) + l, x >= 0.0f ? r : e * r};
+}
+
+// Lane I of each row of 16 lanes to the whole row.  The compiler folds the
+// move into a product that takes it.
+template <int I>
+__device__ __forceinline__ float row_bcast(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kXor1 = 0xb1, kXor2 = 0x4e;
+
+__device__ __forceinline__ float swap32_add(float a, float b) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(a), __float_as_int(b), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+__device__ __forceinline__ float swap16_add(float a, float b) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(a), __float_as_int(b), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+// Sums over the four rows of a wave (lanes l, l + 16, l + 32, l + 48): row i
+// gets the sum of v[i].  Swapping the upper half of one register with the
+// lower half of another and adding the two sums both at once.
+__device__ __forceinline__ float rows_sum(const float (&v)[4]) {
+    return swap16_add(swap32_add(v[0], v[2]), swap32_add(v[1], v[3]));
+}
+
+}  // namespace ssm
+}  // namespace fg

@@ -1,0 +1,79 @@
+// ssm_kernels.hip -- the gfx950 code object of the sequence filters: the short
+// causal convolution (ssm_conv.hpp) and the selective scan (ssm_scan.hpp).
+//
+// Names: fg_<operator>_<element type>[_...]; the host composes them
+// (ssm_ops.cpp).  Built like the FFT code object, by ferrum-gpu_amd/csrc/Makefile.
+#include "ssm_conv.hpp"
+#include "ssm_scan.hpp"
+
+using namespace fg::ssm;
+
+// S: states of a lane; _pad: the channel has fewer than 4 S states.
+#define FG_SCAN(NAME, T, S, SUFFIX, PAD)                                                                       \
+    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_local_##NAME##_s##S##SUFFIX(       \
+        fg_scan_kargs g) {                                                                                      \
+        Scan<T, S, PAD>::forward<true>(g);                                                                     \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_##NAME##_s##S##SUFFIX(             \
+        fg_scan_kargs g) {                                                                                      \
+        Scan<T, S, PAD>::forward<false>(g);                                                                    \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_back_local_##NAME##_s##S##SUFFIX(  \
+        fg_scan_kargs g) {                                                                                      \
+        Scan<T, S, PAD>::backward<true>(g);                                                                    \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_back_##NAME##_s##S##SUFFIX(        \
+        fg_scan_kargs g) {                                                                                      \
+        Scan<T, S, PAD>::backward<false>(g);                                                                   \
+    }
+#define FG_SCAN_BOTH(NAME, T, S) FG_SCAN(NAME, T, S, , false) FG_SCAN(NAME, T, S, _pad, true)
+
+// W taps, V channels of a thread: 16 bytes of a row forward, at most four
+// channels backward; V = 1 for any stride and alignment.
+#define FG_CONV(NAME, T, W, V, B)                                                                               \
+    extern "C" __global__ __launch_bounds__(256) void fg_conv_##NAME##_w##W##_v##V(fg_conv_kargs g) {            \
+        Conv<T, V, W>::forward(g);                                                                             \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void fg_conv_back_##NAME##_w##W##_v##B(fg_conv_kargs g) {       \
+        Conv<T, B, W>::backward(g);                                                                            \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void fg_conv_step_##NAME##_w##W##_v##V(fg_conv_step_kargs g) {  \
+        Conv<T, V, W>::step(g);                                                                                \
+    }
+#define FG_CONV_BOTH(NAME, T, W, V) FG_CONV(NAME, T, W, V, 4) FG_CONV(NAME, T, W, 1, 1)
+
+#define FG_SSM_TYPE(NAME, T, V)                                                                                 \
+    FG_SCAN_BOTH(NAME, T, 1)                                                                                    \
+    FG_SCAN_BOTH(NAME, T, 2)                                                                                    \
+    FG_SCAN_BOTH(NAME, T, 4)                                                                                    \
+    FG_SCAN_BOTH(NAME, T, 8)                                                                                    \
+    FG_SCAN_BOTH(NAME, T, 16)                                                                                   \
+    FG_CONV_BOTH(NAME, T, 2, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 3, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 4, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 5, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 6, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 7, V)                                                                                 \
+    FG_CONV_BOTH(NAME, T, 8, V)                                                                                 \
+    extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_bc_##NAME(fg_scan_kargs g) {                \
+        scan_reduce_bc<T>(g);                                                                                  \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void fg_scan_step_##NAME(fg_scan_step_kargs g) {                \
+        scan_step_body<T>(g);                                                                                  \
+    }
+
+// One code object, three builds of this file in parallel: FG_SSM_F32, _BF16, _F16.
+#if defined(FG_SSM_F32)
+FG_SSM_TYPE(f32, F32, 4)
+extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_p(fg_scan_kargs g) { scan_reduce_p(g); }
+extern "C" __global__ __launch_bounds__(256) void fg_conv_reduce(fg_conv_kargs g, uint32_t width, float* gweight,
+                                                                float* gbias) {
+    conv_reduce(g, width, gweight, gbias);
+}
+#elif defined(FG_SSM_BF16)
+FG_SSM_TYPE(bf16, BF16, 8)
+#elif defined(FG_SSM_F16)
+FG_SSM_TYPE(f16, F16, 8)
+#else
+#error "build with FG_SSM_F32, FG_SSM_BF16 or FG_SSM_F16"
+#endif

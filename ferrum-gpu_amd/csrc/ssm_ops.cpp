@@ -1,0 +1,533 @@
+// ssm_ops.cpp -- see ssm_ops.hpp.
+#include "ssm_ops.hpp"
+
+#include <algorithm>
+#include <initializer_list>
+#include <string>
+#include <vector>
+
+extern "C" {
+extern const unsigned char fg_ssm_f32_code_object_start[], fg_ssm_f32_code_object_end[];
+extern const unsigned char fg_ssm_bf16_code_object_start[], fg_ssm_bf16_code_object_end[];
+extern const unsigned char fg_ssm_f16_code_object_start[], fg_ssm_f16_code_object_end[];
+}
+
+namespace fg {
+
+namespace {
+
+const char* const kTypes[3] = {"f32", "bf16", "f16"};
+const uint32_t kBytes[3] = {4, 2, 2};
+constexpr int64_t kMaxRowStride = 1 << 25;   // 32-bit offsets within a segment's rows
+constexpr int64_t kMaxCount = 0x7fffffff;
+
+KernelArtifact ssm_code_object(int dtype) {
+    static const unsigned char* const start[3] = {fg_ssm_f32_code_object_start, fg_ssm_bf16_code_object_start,
+                                                  fg_ssm_f16_code_object_start};
+    static const unsigned char* const end[3] = {fg_ssm_f32_code_object_end, fg_ssm_bf16_code_object_end,
+                                                fg_ssm_f16_code_object_end};
+    KernelArtifact a;
+    a.backend = BackendId::Hip;
+    a.name = std::string("ferrum-gpu-ssm-kernels-") + kTypes[dtype];
+    a.target = "gfx950";
+    a.image = start[dtype];
+    a.size = (size_t)(end[dtype] - start[dtype]);
+    return a;
+}
+
+void check_dtype(const char* op, int64_t dtype) {
+    if (dtype < 0 || dtype > 2)
+        invalid(std::string(op) + ": dtype must be FG_DTYPE_F32, FG_DTYPE_BF16 or FG_DTYPE_F16, got " +
+                std::to_string(dtype));
+}
+
+void check_range(const char* op, const char* what, int64_t v, int64_t lo, int64_t hi) {
+    if (v < lo || v > hi)
+        invalid(std::string(op) + ": " + what + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) +
+                "], got " + std::to_string(v));
+}
+
+// The extent of an array of rows, in bytes from its first element.
+struct Extent {
+    std::string name;
+    const char* p = nullptr;
+    int64_t bytes = 0;              // up to its last element
+    int64_t seq = 0, row = 0;       // bytes
+    int64_t width = 0;              // bytes of a row
+    bool out = false;
+};
+
+// A call's arrays: each is checked when it is added, outputs also against
+// everything that was added before and after.
+class Arrays {
+public:
+    Arrays(const char* op, int64_t seqs, int64_t rows, uint32_t es) : op_(op), seqs_(seqs), rows_(rows), es_(es) {}
+
+    fg_ssm_view rows(const char* name, const fg_rows& r, int64_t width, bool out, bool optional = false) {
+        fg_ssm_view v{nullptr, 0, 0};
+        if (!r.ptr) {
+            if (!optional && seqs_ > 0 && rows_ > 0) invalid(std::string(op_) + ": " + name + ": null buffer");
+            return v;
+        }
+        v.p = r.ptr;
+        v.seq = seqs_ > 1 ? r.seq_stride : 0;
+        v.row = rows_ > 1 ? r.row_stride : 0;
+        if (reinterpret_cast<uintptr_t>(r.ptr) % es_)
+            invalid(std::string(op_) + ": " + name + ": not aligned to its elements");
+        if (v.seq < 0 || v.row < 0) invalid(std::string(op_) + ": " + name + ": negative stride");
+        if (v.row > kMaxRowStride)
+            invalid(std::string(op_) + ": " + name + ": row stride " + std::to_string(v.row) + " exceeds " +
+                    std::to_string(kMaxRowStride));
+        if (seqs_ == 0 || rows_ == 0) return v;
+        if (out) {
+            // rows of all sequences apart: the larger stride steps over all that the smaller one covers
+            int64_t small = v.row, small_n = rows_, large = v.seq, large_n = seqs_;
+            if (small_n == 1 || (large_n > 1 && large < small)) std::swap(small, large), std::swap(small_n, large_n);
+            if ((small_n > 1 && small < width) || (large_n > 1 && large < (small_n - 1) * small + width))
+                invalid(std::string(op_) + ": " + name + ": rows of an output overlap");
+        }
+        Extent e;
+        e.name = name;
+        e.p = (const char*)r.ptr;
+        e.seq = v.seq * es_;
+        e.row = v.row * es_;
+        e.width = width * es_;
+        e.bytes = (seqs_ - 1) * e.seq + (rows_ - 1) * e.row + e.width;
+        e.out = out;
+        add(e);
+        return v;
+    }
+    void flat(const char* name, const void* p, int64_t bytes, bool out, bool optional, uint32_t align = 4) {
+        if (!p) {
+            if (!optional && bytes > 0) invalid(std::string(op_) + ": " + name + ": null buffer");
+            return;
+        }
+        if (reinterpret_cast<uintptr_t>(p) % align)
+            invalid(std::string(op_) + ": " + name + ": not aligned to its elements");
+        if (bytes <= 0) return;
+        Extent e;
+        e.name = name;
+        e.p = (const char*)p;
+        e.bytes = e.width = bytes;
+        e.out = out;
+        add(e);
+    }
+
+private:
+    static bool apart(const Extent& a, const Extent& b) {
+        if (a.p + a.bytes <= b.p || b.p + b.bytes <= a.p) return true;
+        // column windows of one array: the same strides, and the windows apart within a row
+        if (a.row <= 0 || a.row != b.row || a.seq != b.seq || a.seq % a.row) return false;
+        int64_t off = (b.p - a.p) % a.row;
+        if (off < 0) off += a.row;
+        return off >= a.width && off + b.width <= a.row;
+    }
+    void add(const Extent& e) {
+        for (const Extent& x : all_)
+            if ((e.out || x.out) && !apart(e, x)) invalid(std::string(op_) + ": " + x.name + " and " + e.name + " overlap");
+        all_.push_back(e);
+    }
+    const char* op_;
+    int64_t seqs_, rows_;
+    uint32_t es_;
+    std::vector<Extent> all_;
+};
+
+void refuse_capture(const char* op, const HipBackend::DeviceHandle& dev, hipStream_t stream) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HipBackend::bind(dev);
+    hip_check(hipStreamIsCapturing(stream ? stream : dev->stream, &cap), "hipStreamIsCapturing");
+    if (cap != hipStreamCaptureStatusNone)
+        invalid(std::string(op) + ": a plan's first backward call allocates its workspace and cannot be captured");
+}
+
+// Device pointers and strides of `v` multiples of a vector of n elements.
+bool vector_rows(const fg_ssm_view& v, uint32_t n, uint32_t es) {
+    return reinterpret_cast<uintptr_t>(v.p) % (n * es) == 0 && v.seq % n == 0 && v.row % n == 0;
+}
+bool vector_ptr(const void* p, uint32_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+void launch(const HipBackend::DeviceHandle& dev, hipStream_t stream, HipBackend::KernelHandle k, uint64_t blocks,
+            uint32_t threads, void** args, const char* op) {
+    if (blocks == 0) return;
+    if (blocks > 0xffffffffull / threads) invalid(std::string(op) + ": too large for one launch");
+    HipBackend::launch(dev, stream, k, Dim3((uint32_t)blocks), Dim3(threads), 0, args);
+}
+
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+}  // namespace
+
+SsmKernels::SsmKernels(Device<HipBackend>& dev) {
+    for (int t = 0; t < 3; ++t) {
+        mod_[t] = dev.load_or_cache(ssm_code_object(t));
+        for (int w = 2; w <= FG_CONV_MAX_WIDTH; ++w)
+            for (int v = 0; v < 2; ++v)
+                conv_step_[t][w][v] = get(t, std::string("fg_conv_step_") + kTypes[t] + "_w" + std::to_string(w) +
+                                                 "_v" + std::to_string(v ? 16 / kBytes[t] : 1));
+        scan_step_[t] = get(t, std::string("fg_scan_step_") + kTypes[t]);
+    }
+}
+
+HipBackend::KernelHandle SsmKernels::get(int dtype, const std::string& name) const {
+    return HipBackend::get_kernel(mod_[dtype], name.c_str());
+}
+
+void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_step_args& a,
+                           hipStream_t stream) const {
+    const char* op = "conv_step";
+    check_dtype(op, a.dtype);
+    check_range(op, "rows", a.rows, 0, kMaxCount);
+    check_range(op, "channels", a.channels, 1, kMaxCount);
+    check_range(op, "width", a.width, 2, FG_CONV_MAX_WIDTH);
+    check_range(op, "state_rows", a.state_rows, a.slots ? 0 : a.rows, kMaxCount);
+    const uint32_t es = kBytes[a.dtype], n = 16 / es;
+    Arrays all(op, a.rows, 1, es);
+    fg_conv_step_kargs g{};
+    g.x = all.rows("x", a.x, a.channels, false);
+    g.out = all.rows("out", a.out, a.channels, true);
+    all.flat("weight", a.weight, 4 * a.channels * a.width, false, false);
+    all.flat("bias", a.bias, 4 * a.channels, false, true);
+    const int64_t state = a.state_rows * (a.width - 1) * a.channels * es;
+    all.flat("state", a.state, state, a.state_out == a.state, false, es);
+    if (a.state_out != a.state || !a.state_out) all.flat("state_out", a.state_out, state, true, false, es);
+    all.flat("slots", a.slots, 4 * a.rows, false, true);
+    if (a.rows == 0) return;
+    g.weight = a.weight;
+    g.bias = a.bias;
+    g.state = a.state;
+    g.state_out = a.state_out;
+    g.slots = a.slots;
+    g.state_rows = (uint64_t)a.state_rows;
+    g.rows = (uint32_t)a.rows;
+    g.channels = (uint32_t)a.channels;
+    g.silu = a.silu != 0;
+    const bool vec = a.channels % n == 0 && vector_rows(g.x, n, es) && vector_rows(g.out, n, es) &&
+                     vector_ptr(a.state, 16) && vector_ptr(a.state_out, 16);
+    const uint64_t waves = ceil_div(g.channels / (vec ? n : 1), 64) * g.rows;
+    void* args[] = {&g};
+    launch(dev, stream, conv_step_[a.dtype][a.width][vec], ceil_div(waves, 4), 256, args, op);
+}
+
+void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_step_args& a,
+                           hipStream_t stream) const {
+    const char* op = "scan_step";
+    check_dtype(op, a.dtype);
+    check_range(op, "rows", a.rows, 0, kMaxCount);
+    check_range(op, "channels", a.channels, 1, kMaxCount);
+    check_range(op, "states", a.states, 1, FG_SSM_MAX_STATES);
+    check_range(op, "groups", a.groups, 1, a.channels);
+    if (a.channels % a.groups) invalid("scan_step: groups must divide channels");
+    check_range(op, "state_rows", a.state_rows, a.slots ? 0 : a.rows, kMaxCount);
+    Arrays all(op, a.rows, 1, kBytes[a.dtype]);
+    fg_scan_step_kargs g{};
+    g.u = all.rows("u", a.u, a.channels, false);
+    g.delta = all.rows("delta", a.delta, a.channels, false);
+    g.b = all.rows("B", a.b, a.groups * a.states, false);
+    g.c = all.rows("C", a.c, a.groups * a.states, false);
+    g.z = all.rows("z", a.z, a.channels, false, true);
+    g.out = all.rows("out", a.out, a.channels, true);
+    all.flat("A", a.a, 4 * a.channels * a.states, false, false);
+    all.flat("D", a.d, 4 * a.channels, false, true);
+    all.flat("delta_bias", a.delta_bias, 4 * a.channels, false, true);
+    const int64_t state = 4 * a.state_rows * a.channels * a.states;
+    all.flat("state", a.state, state, a.state_out == a.state, false);
+    if (a.state_out != a.state || !a.state_out) all.flat("state_out", a.state_out, state, true, false);
+    all.flat("slots", a.slots, 4 * a.rows, false, true);
+    if (a.rows == 0) return;
+    g.a = a.a;
+    g.skip = a.d;
+    g.bias = a.delta_bias;
+    g.state = a.state;
+    g.state_out = a.state_out;
+    g.slots = a.slots;
+    g.state_rows = (uint64_t)a.state_rows;
+    g.rows = (uint32_t)a.rows;
+    g.channels = (uint32_t)a.channels;
+    g.states = (uint32_t)a.states;
+    g.groups = (uint32_t)a.groups;
+    g.group_channels = g.channels / g.groups;
+    g.lanes = 1;
+    while (4 * g.lanes < g.states) g.lanes *= 2;
+    g.softplus = a.softplus != 0;
+    const uint64_t threads = (uint64_t)g.rows * g.channels * g.lanes;
+    void* args[] = {&g};
+    launch(dev, stream, scan_step_[a.dtype], ceil_div(threads, 256), 256, args, op);
+}
+
+// ------------------------------------------------------------- convolution
+
+namespace {
+
+// Shared by both plans' constructors: sequences, length, tokens.
+void check_sequences(const char* op, int64_t sequences, int64_t length, int64_t tokens, int64_t packed) {
+    check_range(op, "sequences", sequences, 0, kMaxCount);
+    check_range(op, "length", length, 0, kMaxCount);
+    if (packed) check_range(op, "tokens", tokens, 0, int64_t(1) << 40);
+}
+
+}  // namespace
+
+ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_conv_shape& s)
+    : dev_(dev), s_(s) {
+    const char* op = "conv plan";
+    check_dtype(op, s.dtype);
+    check_sequences(op, s.sequences, s.length, s.tokens, s.packed);
+    check_range(op, "channels", s.channels, 1, kMaxCount);
+    check_range(op, "width", s.width, 2, FG_CONV_MAX_WIDTH);
+    if (!s_.packed) s_.tokens = s_.sequences * s_.length;
+    run_forward_ = 16;
+    run_backward_ = 32;
+    const std::string type = kTypes[s.dtype], w = "_w" + std::to_string(s.width);
+    for (int v = 0; v < 2; ++v) {
+        forward_[v] = k.get((int)s.dtype, "fg_conv_" + type + w + "_v" + std::to_string(v ? 16 / kBytes[s.dtype] : 1));
+        backward_[v] = k.get((int)s.dtype, "fg_conv_back_" + type + w + "_v" + std::to_string(v ? 4 : 1));
+    }
+    reduce_ = k.get(FG_DTYPE_F32, "fg_conv_reduce");
+}
+
+fg_conv_kargs ConvPlan::base(const int32_t* offsets) const {
+    if (s_.packed && !offsets) invalid("conv: packed sequences need offsets");
+    if (!s_.packed && offsets) invalid("conv: offsets are for packed sequences");
+    fg_conv_kargs g{};
+    g.offsets = offsets;
+    g.tokens = (uint64_t)s_.tokens;
+    g.seqs = (uint32_t)s_.sequences;
+    g.length = (uint32_t)s_.length;
+    g.channels = (uint32_t)s_.channels;
+    g.silu = s_.silu != 0;
+    return g;
+}
+
+void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const {
+    const char* op = "conv forward";
+    const uint32_t es = kBytes[s_.dtype], n = 16 / es;
+    fg_conv_kargs g = base(a.offsets);
+    Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, es);
+    g.x = all.rows("x", a.x, s_.channels, false);
+    g.out = all.rows("out", a.out, s_.channels, true);
+    all.flat("weight", a.weight, 4 * s_.channels * s_.width, false, false);
+    all.flat("bias", a.bias, 4 * s_.channels, false, true);
+    const int64_t state = s_.sequences * (s_.width - 1) * s_.channels * es;
+    all.flat("initial", a.initial, state, a.initial == a.final, true, es);
+    if (a.final != a.initial) all.flat("final", a.final, state, true, true, es);
+    all.flat("offsets", a.offsets, 4 * (s_.sequences + 1), false, true);
+    if (s_.sequences == 0) return;
+    g.weight = a.weight;
+    g.bias = a.bias;
+    g.initial = a.initial;
+    g.final = a.final;
+    g.run = run_forward_;
+    g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
+    const bool vec = s_.channels % n == 0 && vector_rows(g.x, n, es) && vector_rows(g.out, n, es) &&
+                     vector_ptr(a.initial, 16) && vector_ptr(a.final, 16);
+    const uint64_t waves = ceil_div(g.channels / (vec ? n : 1), 64) * g.runs * g.seqs;
+    void* args[] = {&g};
+    launch(dev_, stream, forward_[vec], ceil_div(waves, 4), 256, args, op);
+}
+
+void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
+    const char* op = "conv backward";
+    const uint32_t es = kBytes[s_.dtype];
+    fg_conv_kargs g = base(a.offsets);
+    Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, es);
+    g.x = all.rows("x", a.x, s_.channels, false);
+    g.out = all.rows("grad_out", a.grad_out, s_.channels, false);
+    g.gx = all.rows("grad_x", a.grad_x, s_.channels, true, true);
+    all.flat("weight", a.weight, 4 * s_.channels * s_.width, false, false);
+    all.flat("bias", a.bias, 4 * s_.channels, false, true);
+    const int64_t state = s_.sequences * (s_.width - 1) * s_.channels * es;
+    all.flat("initial", a.initial, state, false, true, es);
+    all.flat("grad_final", a.grad_final, state, false, true, es);
+    all.flat("grad_initial", a.grad_initial, state, true, true, es);
+    all.flat("grad_weight", a.grad_weight, 4 * s_.channels * s_.width, true, true);
+    all.flat("grad_bias", a.grad_bias, 4 * s_.channels, true, true);
+    all.flat("offsets", a.offsets, 4 * (s_.sequences + 1), false, true);
+    g.weight = a.weight;
+    g.bias = a.bias;
+    g.initial = a.initial;
+    g.gfinal = a.grad_final;
+    g.ginitial = a.grad_initial;
+    g.run = run_backward_;
+    g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
+    const uint64_t n = (uint64_t)s_.channels * (s_.width + 1);
+    {
+        std::lock_guard<std::mutex> lock(mu_);
+        if (!part_.data() && g.seqs) {
+            refuse_capture(op, dev_, stream);
+            part_ = Buffer<float, HipBackend>(dev_, n * g.runs * g.seqs);
+        }
+    }
+    g.part = part_.data();
+    const bool vec = s_.channels % 4 == 0 && vector_rows(g.x, 4, es) && vector_rows(g.out, 4, es) &&
+                     vector_rows(g.gx, 4, es) && vector_ptr(a.initial, 4 * es) && vector_ptr(a.grad_final, 4 * es) &&
+                     vector_ptr(a.grad_initial, 4 * es);
+    const uint64_t waves = ceil_div(g.channels / (vec ? 4 : 1), 64) * g.runs * g.seqs;
+    void* args[] = {&g};
+    launch(dev_, stream, backward_[vec], ceil_div(waves, 4), 256, args, op);
+    uint32_t width = (uint32_t)s_.width;
+    float *gw = a.grad_weight, *gb = a.grad_bias;
+    void* rargs[] = {&g, &width, &gw, &gb};
+    if (gw || gb) launch(dev_, stream, reduce_, ceil_div(n, 256), 256, rargs, op);
+}
+
+// -------------------------------------------------------------------- scan
+
+ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_scan_shape& s)
+    : dev_(dev), s_(s) {
+    const char* op = "scan plan";
+    check_dtype(op, s.dtype);
+    check_sequences(op, s.sequences, s.length, s.tokens, s.packed);
+    check_range(op, "channels", s.channels, 1, kMaxCount);
+    check_range(op, "states", s.states, 1, FG_SSM_MAX_STATES);
+    check_range(op, "groups", s.groups, 1, s.channels);
+    if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
+    if (!s_.packed) s_.tokens = s_.sequences * s_.length;
+    lane_states_ = fg_ssm_lane_states((uint32_t)s.states);
+    segment_ = FG_SSM_SEGMENT(lane_states_);
+    group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, FG_SSM_GROUP_CHANNELS);
+    blocks_ = group_blocks_ * (uint32_t)s.groups;
+    chunks_forward_ = chunks_for(1024);
+    chunks_backward_ = chunks_for(1024);
+    const uint64_t waves =
+        (uint64_t)s.sequences * (std::max(chunks_forward_, chunks_backward_) + 1) * blocks_ * FG_SSM_WAVES;
+    if (chunks_forward_ > 1 || chunks_backward_ > 1) {
+        carry_ = Buffer<float, HipBackend>(dev, waves * 64 * lane_states_);
+        carry_dt_ = Buffer<float, HipBackend>(dev, waves * FG_SSM_WAVE_CHANNELS);
+    }
+    const std::string type = kTypes[s.dtype], tail = type + "_s" + std::to_string(lane_states_) +
+                                                     (4 * lane_states_ > (uint32_t)s.states ? "_pad" : "");
+    local_ = k.get((int)s.dtype, "fg_scan_local_" + tail);
+    forward_ = k.get((int)s.dtype, "fg_scan_" + tail);
+    back_local_ = k.get((int)s.dtype, "fg_scan_back_local_" + tail);
+    backward_ = k.get((int)s.dtype, "fg_scan_back_" + tail);
+    reduce_bc_ = k.get((int)s.dtype, "fg_scan_reduce_bc_" + type);
+    reduce_p_ = k.get(FG_DTYPE_F32, "fg_scan_reduce_p");
+}
+
+// Parts of the token axis that work at the same time, so that `target` waves do.
+uint32_t ScanPlan::chunks_for(uint32_t target) const {
+    const uint64_t waves = std::max<uint64_t>(1, (uint64_t)s_.sequences * blocks_ * FG_SSM_WAVES);
+    const uint64_t most = std::max<uint64_t>(1, ceil_div(s_.length, 4 * segment_));
+    return (uint32_t)std::min<uint64_t>({ceil_div(target, waves), most, 64});
+}
+
+size_t ScanPlan::checkpoint_bytes() const {
+    const uint64_t segs = s_.packed ? (uint64_t)s_.tokens / segment_ + s_.sequences
+                                    : s_.sequences * ceil_div(s_.length, segment_);
+    return segs * blocks_ * FG_SSM_WAVES * 64 * lane_states_ * sizeof(float);
+}
+
+fg_scan_kargs ScanPlan::base(const fg_scan_inputs& in, uint32_t chunks) const {
+    fg_scan_kargs g{};
+    g.a = in.a;
+    g.skip = in.d;
+    g.bias = in.delta_bias;
+    g.initial = in.initial;
+    g.offsets = in.offsets;
+    g.carry = carry_.data();
+    g.carry_dt = carry_dt_.data();
+    g.tokens = (uint64_t)s_.tokens;
+    g.seqs = (uint32_t)s_.sequences;
+    g.length = (uint32_t)s_.length;
+    g.channels = (uint32_t)s_.channels;
+    g.states = (uint32_t)s_.states;
+    g.groups = (uint32_t)s_.groups;
+    g.group_channels = g.channels / g.groups;
+    g.group_blocks = group_blocks_;
+    g.chunk_len = (uint32_t)ceil_div(ceil_div(s_.length, chunks), segment_) * segment_;
+    if (g.chunk_len == 0) g.chunk_len = segment_;
+    g.chunks = (uint32_t)std::max<uint64_t>(1, ceil_div(s_.length, g.chunk_len));
+    g.check_segs = (uint32_t)ceil_div(s_.length, segment_);
+    g.softplus = s_.softplus != 0;
+    return g;
+}
+
+void ScanPlan::check_inputs(const char* op, const fg_scan_inputs& in) const {
+    if (s_.packed && !in.offsets) invalid(std::string(op) + ": packed sequences need offsets");
+    if (!s_.packed && in.offsets) invalid(std::string(op) + ": offsets are for packed sequences");
+}
+
+void ScanPlan::forward(const fg_scan_forward_args& a, hipStream_t stream) const {
+    const char* op = "scan forward";
+    const fg_scan_inputs& in = a.in;
+    check_inputs(op, in);
+    fg_scan_kargs g = base(in, chunks_forward_);
+    Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, kBytes[s_.dtype]);
+    const int64_t state = 4 * s_.sequences * s_.channels * s_.states;
+    g.u = all.rows("u", in.u, s_.channels, false);
+    g.delta = all.rows("delta", in.delta, s_.channels, false);
+    g.b = all.rows("B", in.b, s_.groups * s_.states, false);
+    g.c = all.rows("C", in.c, s_.groups * s_.states, false);
+    g.z = all.rows("z", in.z, s_.channels, false, true);
+    g.out = all.rows("out", a.out, s_.channels, true);
+    all.flat("A", in.a, 4 * s_.channels * s_.states, false, false);
+    all.flat("D", in.d, 4 * s_.channels, false, true);
+    all.flat("delta_bias", in.delta_bias, 4 * s_.channels, false, true);
+    all.flat("initial", in.initial, state, in.initial == a.final, true);
+    if (a.final != in.initial) all.flat("final", a.final, state, true, true);
+    all.flat("offsets", in.offsets, 4 * (s_.sequences + 1), false, true);
+    all.flat("checkpoints", a.checkpoints, (int64_t)checkpoint_bytes(), true, true);
+    g.final = a.final;
+    g.check = (float*)a.checkpoints;
+    void* args[] = {&g};
+    const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
+    if (g.chunks > 1) launch(dev_, stream, local_, blocks, 64 * FG_SSM_WAVES, args, op);
+    launch(dev_, stream, forward_, blocks, 64 * FG_SSM_WAVES, args, op);
+}
+
+void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
+    const char* op = "scan backward";
+    const fg_scan_inputs& in = a.in;
+    check_inputs(op, in);
+    if (a.grad_z.ptr && !in.z.ptr) invalid("scan backward: grad_z without z");
+    fg_scan_kargs g = base(in, chunks_backward_);
+    Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, kBytes[s_.dtype]);
+    const int64_t state = 4 * s_.sequences * s_.channels * s_.states;
+    g.u = all.rows("u", in.u, s_.channels, false);
+    g.delta = all.rows("delta", in.delta, s_.channels, false);
+    g.b = all.rows("B", in.b, s_.groups * s_.states, false);
+    g.c = all.rows("C", in.c, s_.groups * s_.states, false);
+    g.z = all.rows("z", in.z, s_.channels, false, true);
+    g.gout = all.rows("grad_out", a.grad_out, s_.channels, false);
+    g.gu = all.rows("grad_u", a.grad_u, s_.channels, true, true);
+    g.gdelta = all.rows("grad_delta", a.grad_delta, s_.channels, true, true);
+    g.gb = all.rows("grad_B", a.grad_b, s_.groups * s_.states, true, true);
+    g.gc = all.rows("grad_C", a.grad_c, s_.groups * s_.states, true, true);
+    g.gz = all.rows("grad_z", a.grad_z, s_.channels, true, true);
+    all.flat("A", in.a, 4 * s_.channels * s_.states, false, false);
+    all.flat("D", in.d, 4 * s_.channels, false, true);
+    all.flat("delta_bias", in.delta_bias, 4 * s_.channels, false, true);
+    all.flat("offsets", in.offsets, 4 * (s_.sequences + 1), false, true);
+    all.flat("checkpoints", a.checkpoints, (int64_t)checkpoint_bytes(), false, false);
+    all.flat("grad_final", a.grad_final, state, false, true);
+    all.flat("grad_initial", a.grad_initial, state, true, true);
+    all.flat("grad_A", a.grad_a, 4 * s_.channels * s_.states, true, true);
+    all.flat("grad_D", a.grad_d, 4 * s_.channels, true, true);
+    all.flat("grad_delta_bias", a.grad_delta_bias, 4 * s_.channels, true, true);
+    g.check = (float*)a.checkpoints;
+    g.gfinal = a.grad_final;
+    g.ginitial = a.grad_initial;
+    g.ga = a.grad_a;
+    g.gskip = a.grad_d;
+    g.gbias = a.grad_delta_bias;
+    const uint64_t row = 2ull * s_.groups * s_.states, params = (uint64_t)s_.channels * (s_.states + 2);
+    {
+        std::lock_guard<std::mutex> lock(mu_);
+        if (!part_p_.data() && g.seqs) {
+            refuse_capture(op, dev_, stream);
+            part_bc_ = Buffer<float, HipBackend>(dev_, group_blocks_ * (uint64_t)s_.tokens * row);
+            part_p_ = Buffer<float, HipBackend>(dev_, params * g.seqs * g.chunks);
+        }
+    }
+    g.part_bc = part_bc_.data();
+    g.part_p = part_p_.data();
+    void* args[] = {&g};
+    const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
+    if (g.chunks > 1) launch(dev_, stream, back_local_, blocks, 64 * FG_SSM_WAVES, args, op);
+    launch(dev_, stream, backward_, blocks, 64 * FG_SSM_WAVES, args, op);
+    if (g.gb.p || g.gc.p) launch(dev_, stream, reduce_bc_, ceil_div(g.tokens * row, 256), 256, args, op);
+    if (g.ga || g.gskip || g.gbias) launch(dev_, stream, reduce_p_, ceil_div(params, 256), 256, args, op);
+}
+
+}  // namespace fg

@@ -1,0 +1,73 @@
+// ssm_ops.hpp -- host side of the sequence filters (kernels/ssm_conv.hpp,
+// kernels/ssm_scan.hpp): argument checks, launch geometry and workspaces of
+// the short causal convolution and the selective scan.
+//
+// The kernels are a code object for each element type, loaded with the device,
+// so that no call loads anything (a call may be captured into a graph).
+#pragma once
+
+#include <cstdint>
+#include <mutex>
+
+#include "device.hpp"
+#include "hip_backend.hpp"
+#include "kernels/ssm_args.h"
+
+namespace fg {
+
+// The code objects of the three element types and the handles of the kernels
+// that need no plan.
+class SsmKernels {
+public:
+    SsmKernels() = default;
+    explicit SsmKernels(Device<HipBackend>& dev);
+
+    HipBackend::KernelHandle get(int dtype, const std::string& name) const;
+
+    void conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_step_args& a, hipStream_t stream) const;
+    void scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_step_args& a, hipStream_t stream) const;
+
+private:
+    HipBackend::Module mod_[3];
+    HipBackend::KernelHandle conv_step_[3][FG_CONV_MAX_WIDTH + 1][2] = {};  // [dtype][width][any alignment, 16 bytes]
+    HipBackend::KernelHandle scan_step_[3] = {};
+};
+
+class ConvPlan {
+public:
+    ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_conv_shape& s);
+    void forward(const fg_conv_forward_args& a, hipStream_t stream) const;
+    void backward(const fg_conv_backward_args& a, hipStream_t stream);
+
+private:
+    fg_conv_kargs base(const int32_t* offsets) const;
+    HipBackend::DeviceHandle dev_;
+    fg_conv_shape s_;
+    uint32_t run_forward_, run_backward_;
+    HipBackend::KernelHandle forward_[2], backward_[2], reduce_;  // [any alignment, vectors]
+    std::mutex mu_;
+    Buffer<float, HipBackend> part_;
+};
+
+class ScanPlan {
+public:
+    ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_scan_shape& s);
+    size_t checkpoint_bytes() const;
+    void forward(const fg_scan_forward_args& a, hipStream_t stream) const;
+    void backward(const fg_scan_backward_args& a, hipStream_t stream);
+
+private:
+    fg_scan_kargs base(const fg_scan_inputs& in, uint32_t chunks) const;
+    void check_inputs(const char* op, const fg_scan_inputs& in) const;
+    uint32_t chunks_for(uint32_t target_waves) const;
+    HipBackend::DeviceHandle dev_;
+    fg_scan_shape s_;
+    uint32_t lane_states_, segment_, group_blocks_, blocks_;  // blocks_: workgroups over all channels
+    uint32_t chunks_forward_, chunks_backward_;
+    HipBackend::KernelHandle local_, forward_, back_local_, backward_, reduce_bc_, reduce_p_;
+    Buffer<float, HipBackend> carry_, carry_dt_;
+    std::mutex mu_;
+    Buffer<float, HipBackend> part_bc_, part_p_;
+};
+
+}  // namespace fg

@@ -132,6 +132,14 @@ _sig("fg_graph_capture_begin", _vp, _P(_vp))
 _sig("fg_graph_capture_end", _vp, _vp, _P(_vp))
 _sig("fg_graph_node_count", _vp, _P(_sz))
 _sig("fg_graph_destroy", _vp)
+for _name in ("fg_conv_plan_create", "fg_scan_plan_create"):
+    _sig(_name, _vp, ctypes.c_char_p, _P(_vp))
+for _name in ("fg_conv_forward", "fg_conv_backward", "fg_conv_step", "fg_scan_forward", "fg_scan_backward",
+              "fg_scan_step"):
+    _sig(_name, _vp, ctypes.c_char_p, _vp)  # the argument struct, packed
+_sig("fg_conv_plan_destroy", _vp)
+_sig("fg_scan_plan_destroy", _vp)
+_sig("fg_scan_checkpoint_bytes", _vp, _P(_sz))
 
 
 def last_error() -> str:

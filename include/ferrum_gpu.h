@@ -374,6 +374,155 @@ FG_API int fg_fill_normal_c64(fg_device_t dev, void *d_out, size_t n, uint64_t s
 FG_API int fg_stream_copy(fg_device_t dev, const void *d_in, void *d_out, size_t bytes,
                    fg_stream_t stream);
 
+/* ------------------------------------------------------ sequence filters */
+
+/* The short causal convolution and the selective state space scan over
+ * sequences of tokens (prompts, training), and for single tokens against a
+ * cache of states (generation).  No counterpart in the reference: they stand
+ * beside the FFT's filters (transform, product, inverse) for filters of a few
+ * taps and for filters whose coefficients change from token to token.
+ *
+ * Arrays of rows, one row of `channels` (b, c: groups * states) elements a
+ * token, are given as fg_rows: row t of sequence s starts seq_stride * s +
+ * row_stride * t elements from ptr, its elements are adjacent.  Rows of inputs
+ * may overlap or repeat (stride 0); rows of outputs may not, and outputs may
+ * not overlap inputs unless stated, though both may be column windows of one
+ * array.  Row strides are at most 2^25 elements.  Everything else is
+ * contiguous.  `dtype` is the type of the rows (and of the convolution's
+ * states); parameters, their gradients and the scan's states are float32, and
+ * so is all arithmetic.
+ *
+ * Dense calls (packed = 0) have `sequences` sequences of `length` tokens.
+ * Packed ones have the rows of all sequences one after another, `tokens` rows
+ * in all; seq_stride is not used.  offsets[s] <= row < offsets[s + 1] are
+ * sequence s's, at most `length` of them; `offsets` is on the device, and its
+ * values are taken as the nearest valid ones (no row outside `tokens` is
+ * touched whatever they are).  Rows outside every sequence are not written.
+ *
+ * All calls are stream-ordered and asynchronous (stream NULL: the device's
+ * default stream).  A plan's workspaces serve one call at a time.  The structs
+ * hold 8-byte members only. */
+#define FG_DTYPE_F32 0
+#define FG_DTYPE_BF16 1
+#define FG_DTYPE_F16 2
+
+typedef struct fg_rows {
+    void *ptr;
+    int64_t seq_stride, row_stride; /* elements */
+} fg_rows;
+
+typedef struct fg_conv_plan *fg_conv_plan_t;
+typedef struct fg_scan_plan *fg_scan_plan_t;
+
+typedef struct fg_conv_shape {
+    int64_t sequences, length, tokens; /* tokens: packed only */
+    int64_t channels, width;           /* width: 2 .. 8 taps */
+    int64_t dtype, packed, silu;       /* silu: out = p sigmoid(p), else p */
+} fg_conv_shape;
+
+/* out[t,d] = act(bias[d] + sum_k weight[d,k] x[t - (width - 1) + k, d]).
+ * Optional (NULL): bias; initial, the [sequences][width - 1][channels] rows
+ * before each sequence (NULL: zeros); final, the last width - 1 rows of
+ * (initial, x), may be initial; offsets unless packed. */
+typedef struct fg_conv_forward_args {
+    fg_rows x, out;
+    const float *weight, *bias; /* [channels][width], [channels] */
+    const void *initial;
+    void *final;
+    const int32_t *offsets;
+} fg_conv_forward_args;
+
+/* Gradients from grad_out, that of out, and grad_final (NULL: zeros), that of
+ * final.  Each output may be NULL. */
+typedef struct fg_conv_backward_args {
+    fg_rows x, grad_out, grad_x;
+    const float *weight, *bias;
+    const void *initial, *grad_final;
+    float *grad_weight, *grad_bias;
+    void *grad_initial;
+    const int32_t *offsets;
+} fg_conv_backward_args;
+
+FG_API int fg_conv_plan_create(fg_device_t dev, const fg_conv_shape *shape, fg_conv_plan_t *out);
+FG_API int fg_conv_plan_destroy(fg_conv_plan_t plan);
+FG_API int fg_conv_forward(fg_conv_plan_t plan, const fg_conv_forward_args *args, fg_stream_t stream);
+/* The first call allocates the plan's workspace for the parameters' gradients,
+ * so it cannot be captured into a graph; later ones can. */
+FG_API int fg_conv_backward(fg_conv_plan_t plan, const fg_conv_backward_args *args, fg_stream_t stream);
+
+/* One token of each row.  slots[i] is row i's place among the state_rows
+ * [width - 1][channels] windows of `state` (NULL: i itself); a row whose slot
+ * is negative or beyond them gets zeros and leaves the states alone.  Two rows
+ * of one call must not share a slot.  state_out may be state. */
+typedef struct fg_conv_step_args {
+    int64_t rows, channels, width, dtype, silu, state_rows;
+    fg_rows x, out; /* row i: seq_stride * i; row_stride is not used */
+    const float *weight, *bias;
+    const void *state;
+    void *state_out;
+    const int32_t *slots;
+} fg_conv_step_args;
+FG_API int fg_conv_step(fg_device_t dev, const fg_conv_step_args *args, fg_stream_t stream);
+
+typedef struct fg_scan_shape {
+    int64_t sequences, length, tokens; /* tokens: packed only */
+    int64_t channels, states, groups;  /* states: 1 .. 64; groups divides channels */
+    int64_t dtype, packed, softplus;
+} fg_scan_shape;
+
+/* dt = softplus(delta + delta_bias) (softplus = 0: without it);
+ * h_t[d,n] = exp(dt a[d,n]) h_{t-1}[d,n] + dt u b_t[g,n];
+ * out = (sum_n c_t[g,n] h_t[d,n] + d[d] u) * (z sigmoid(z)), where channel d
+ * belongs to group g = d / (channels / groups).  Optional (NULL): d, delta_bias
+ * (zeros), z.ptr (no gate), initial (zeros), offsets unless packed. */
+typedef struct fg_scan_inputs {
+    fg_rows u, delta, b, c, z;
+    const float *a, *d, *delta_bias; /* [channels][states], [channels], [channels] */
+    const float *initial;            /* [sequences][channels][states] */
+    const int32_t *offsets;
+} fg_scan_inputs;
+
+/* final (NULL: not wanted): the states after the last token, may be initial.
+ * checkpoints (NULL: no backward pass follows): fg_scan_checkpoint_bytes()
+ * that the backward pass of the same inputs takes. */
+typedef struct fg_scan_forward_args {
+    fg_scan_inputs in;
+    fg_rows out;
+    float *final;
+    void *checkpoints;
+} fg_scan_forward_args;
+
+/* Gradients from grad_out, that of out, and grad_final (NULL: zeros), that of
+ * final.  Each output may be NULL. */
+typedef struct fg_scan_backward_args {
+    fg_scan_inputs in;
+    fg_rows grad_out;
+    const void *checkpoints;
+    const float *grad_final;
+    fg_rows grad_u, grad_delta, grad_b, grad_c, grad_z;
+    float *grad_a, *grad_d, *grad_delta_bias, *grad_initial;
+} fg_scan_backward_args;
+
+FG_API int fg_scan_plan_create(fg_device_t dev, const fg_scan_shape *shape, fg_scan_plan_t *out);
+FG_API int fg_scan_plan_destroy(fg_scan_plan_t plan);
+FG_API int fg_scan_checkpoint_bytes(fg_scan_plan_t plan, size_t *bytes);
+FG_API int fg_scan_forward(fg_scan_plan_t plan, const fg_scan_forward_args *args, fg_stream_t stream);
+/* The first call allocates the plan's workspace for the gradients' sums, so it
+ * cannot be captured into a graph; later ones can. */
+FG_API int fg_scan_backward(fg_scan_plan_t plan, const fg_scan_backward_args *args, fg_stream_t stream);
+
+/* One token of each row; slots as for fg_conv_step, over the state_rows
+ * [channels][states] states.  state_out may be state. */
+typedef struct fg_scan_step_args {
+    int64_t rows, channels, states, groups, dtype, softplus, state_rows;
+    fg_rows u, delta, b, c, z, out; /* row i: seq_stride * i; row_stride is not used */
+    const float *a, *d, *delta_bias;
+    const float *state;
+    float *state_out;
+    const int32_t *slots;
+} fg_scan_step_args;
+FG_API int fg_scan_step(fg_device_t dev, const fg_scan_step_args *args, fg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
