@@ -63,6 +63,13 @@ __device__ __forceinline__ Softplus softplus(float x) {
     return {fmaxf(x, 0.0f) + l, x >= 0.0f ? r : e * r};
 }
 
+// A value that is the same in every lane, as a scalar: what is worked out from
+// it (addresses, loop bounds) stays out of the vector registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)(((uint64_t)uniform((uint32_t)((uint64_t)x >> 32)) << 32) | uniform((uint32_t)x));
+}
+
 // Lane I of each row of 16 lanes to the whole row.  The compiler folds the
 // move into a product that takes it.
 template <int I>

@@ -125,7 +125,7 @@ struct Place {
 __device__ __forceinline__ Place place(const fg_scan_kargs& g) {
     Place p;
     const uint32_t lane = threadIdx.x & 63;
-    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    p.wave = uniform(threadIdx.x >> 6);
     p.q = lane >> 4;
     p.c = lane & 15;
     const uint32_t blocks = g.groups * g.group_blocks;
@@ -142,8 +142,8 @@ __device__ __forceinline__ Place place(const fg_scan_kargs& g) {
         const int64_t all = (int64_t)g.tokens;
         a = a < 0 ? 0 : a > all ? all : a;
         b = b < a ? a : b > all ? all : b;
-        p.start = a;
-        p.len = (uint32_t)(b - a < (int64_t)g.length ? b - a : (int64_t)g.length);
+        p.start = uniform(a);
+        p.len = uniform((uint32_t)(b - a < (int64_t)g.length ? b - a : (int64_t)g.length));
     }
     const uint64_t first = (uint64_t)p.chunk * g.chunk_len;
     p.t0 = first < p.len ? (uint32_t)first : p.len;
@@ -196,38 +196,58 @@ struct Scan {
         return l;
     }
 
-    // Row 4 i + q of n rows of a channel array (row 0 at base): beyond the
-    // last, the last one.
-    static __device__ __forceinline__ uint32_t row_of(const Place& p, int i, uint32_t n) {
-        const uint32_t r = 4 * i + p.q;
-        return r < n ? r : n - 1;
-    }
-    static __device__ __forceinline__ void load_channels(float (&v)[NG], const fg_ssm_view& w, const Place& p,
-                                                         uint32_t t, uint32_t n) {
-        const char* base = rows(w, p, t);
+    // A view's rows of a segment: the uniform address of its first row, moved
+    // on from segment to segment, and the lane's offsets from it.
+    struct Cursor {
+        const char* at;
+        uint32_t row;  // bytes
+        __device__ __forceinline__ void set(const fg_ssm_view& v, const Place& p, uint32_t t, uint32_t column = 0) {
+            at = rows(v, p, t) + (uint64_t)column * ES;
+            row = (uint32_t)v.row * ES;
+        }
+        __device__ __forceinline__ const char* group(int i) const { return at + (uint64_t)(4 * i) * row; }
+        __device__ __forceinline__ void forth() { at += (uint64_t)SEG * row; }
+        __device__ __forceinline__ void back() { at -= (uint64_t)SEG * row; }
+    };
+
+    // A segment's rows as they lie in memory.  TAIL: n < SEG of them; beyond
+    // the last, the last.
+    template <bool TAIL>
+    static __device__ __forceinline__ void load_channels(raw (&v)[NG], const Cursor& w, const Place& p, uint32_t n) {
         each<NG>([&](auto i) {
-            v[i] = at(base, (row_of(p, i, n) * (uint32_t)w.row + p.ch) * ES);
+            if constexpr (TAIL) {
+                const uint32_t r = 4 * i + p.q;
+                v[i] = *(const raw*)(w.at + ((r < n ? r : n - 1) * w.row + p.ch * ES));
+            } else {
+                v[i] = *(const raw*)(w.group(i) + (p.q * w.row + p.ch * ES));
+            }
         });
     }
-    static __device__ __forceinline__ void load_states(float (&v)[NG][NB], const fg_ssm_view& w, const fg_scan_kargs& g,
-                                                       const Place& p, const Lane& l, uint32_t t, uint32_t n) {
-        const char* base = rows(w, p, t) + (uint64_t)p.group * g.states * ES;
+    template <bool TAIL>
+    static __device__ __forceinline__ void load_states(raw (&v)[NG][NB], const Cursor& w, const Lane& l, uint32_t n) {
         each<NG>([&](auto i) {
             each<NB>([&](auto k) {
-                uint32_t r = 4 * i + l.tok[k];
-                r = r < n ? r : n - 1;
-                const float x = at(base, (r * (uint32_t)w.row + l.st[k]) * ES);
-                v[i][k] = !PAD || l.has[k] ? x : 0.0f;
+                if constexpr (TAIL) {
+                    const uint32_t r = 4 * i + l.tok[k];
+                    v[i][k] = *(const raw*)(w.at + ((r < n ? r : n - 1) * w.row + l.st[k] * ES));
+                } else {
+                    v[i][k] = *(const raw*)(w.group(i) + (l.tok[k] * w.row + l.st[k] * ES));
+                }
             });
         });
     }
-    static __device__ __forceinline__ void store_channels(const fg_ssm_view& w, const Place& p, uint32_t t, int i,
-                                                          uint32_t n, float v) {
-        const uint32_t r = 4 * i + p.q;
-        if (p.valid && r < n) {
-            char* base = (char*)rows(w, p, t);
-            *(raw*)(base + (r * (uint32_t)w.row + p.ch) * ES) = T::down(v);
-        }
+    static __device__ __forceinline__ void up_channels(float (&x)[NG], const raw (&v)[NG]) {
+        each<NG>([&](auto i) { x[i] = T::up(v[i]); });
+    }
+    static __device__ __forceinline__ void up_states(float (&x)[NG][NB], const raw (&v)[NG][NB], const Lane& l) {
+        each<NG>([&](auto i) {
+            each<NB>([&](auto k) { x[i][k] = !PAD || l.has[k] ? T::up(v[i][k]) : 0.0f; });
+        });
+    }
+    template <bool TAIL>
+    static __device__ __forceinline__ void store_channels(const Cursor& w, const Place& p, int i, uint32_t n, float v) {
+        if (p.valid && (!TAIL || 4 * i + p.q < n))
+            *(raw*)(const_cast<char*>(w.group(i)) + (p.q * w.row + p.ch * ES)) = T::down(v);
     }
     static __device__ __forceinline__ uint64_t check_at(const fg_scan_kargs& g, const Place& p, uint32_t t) {
         const uint64_t seg = g.offsets ? (uint64_t)p.start / SEG + p.seq : (uint64_t)p.seq * g.check_segs;
@@ -262,20 +282,113 @@ struct Scan {
     // Time steps of the segment's rows: dt and its slope.
     static __device__ __forceinline__ void steps(const fg_scan_kargs& g, const Lane& l, const float (&d)[NG],
                                                  float (&dt)[NG], float (&slope)[NG]) {
-        each<NG>([&](auto i) {
-            const float x = d[i] + l.bias;
-            if (g.softplus) {
-                const Softplus s = softplus(x);
+        each<NG>([&](auto i) { dt[i] = d[i] + l.bias, slope[i] = 1.0f; });
+        if (g.softplus) {
+            each<NG>([&](auto i) {
+                const Softplus s = softplus(dt[i]);
                 dt[i] = s.value;
                 slope[i] = s.slope;
-            } else {
-                dt[i] = x;
-                slope[i] = 1.0f;
-            }
-        });
+            });
+        }
     }
 
     // ------------------------------------------------------------ forward
+
+    template <bool LOCAL>
+    struct Segment {
+        raw u[NG], d[NG], z[NG], b[NG][NB], c[NG][NB];
+    };
+    // The forward pass's views, at the segment that is loaded next; `out` at
+    // the one that is stored next.
+    template <bool LOCAL>
+    struct Cursors {
+        Cursor u, d, z, b, c, out;
+        bool gate;
+        __device__ __forceinline__ void set(const fg_scan_kargs& g, const Place& p) {
+            u.set(g.u, p, p.t0);
+            d.set(g.delta, p, p.t0);
+            b.set(g.b, p, p.t0, p.group * g.states);
+            gate = false;
+            if constexpr (!LOCAL) {
+                c.set(g.c, p, p.t0, p.group * g.states);
+                gate = g.z.p != nullptr;
+                z.set(g.z, p, p.t0);
+                out.set(g.out, p, p.t0);
+            }
+        }
+        template <bool TAIL>
+        __device__ __forceinline__ void load(Segment<LOCAL>& s, const Place& p, const Lane& l, uint32_t n) {
+            load_channels<TAIL>(s.d, d, p, n);
+            load_channels<TAIL>(s.u, u, p, n);
+            load_states<TAIL>(s.b, b, l, n);
+            if constexpr (!LOCAL) {
+                load_states<TAIL>(s.c, c, l, n);
+                if (gate) load_channels<TAIL>(s.z, z, p, n);
+                c.forth();
+                z.forth();
+            }
+            d.forth();
+            u.forth();
+            b.forth();
+        }
+    };
+    template <bool LOCAL>
+    struct Values {
+        float u[NG], d[NG], z[NG], b[NG][NB], c[NG][NB];
+        __device__ __forceinline__ void take(const Segment<LOCAL>& s, const Lane& l) {
+            up_channels(d, s.d);
+            up_channels(u, s.u);
+            up_states(b, s.b, l);
+            if constexpr (!LOCAL) {
+                up_states(c, s.c, l);
+                up_channels(z, s.z);
+            }
+        }
+    };
+
+    template <bool LOCAL, bool TAIL>
+    static __device__ __forceinline__ void forward_segment(const fg_scan_kargs& g, const Place& p, const Lane& l,
+                                                           float* x, float (&h)[S], float& sum_dt,
+                                                           const Values<LOCAL>& v, Cursors<LOCAL>& at, uint32_t t,
+                                                           uint32_t n) {
+        float dt[NG], slope[NG], out[NG];
+        if constexpr (!LOCAL) {
+            if (g.check) {  // lanes without a channel too: the backward pass reads them
+                float* to = g.check + check_at(g, p, t);
+                each<S>([&](auto s) { to[s] = h[s]; });
+            }
+        }
+        steps(g, l, v.d, dt, slope);
+        wave_sync();
+        each<NG>([&](auto i) {
+            const float2 e = {dt[i], dt[i] * v.u[i]};
+            *(float2*)(x + (4 * i + p.q) * 2) = e;
+            if constexpr (LOCAL) sum_dt += !TAIL || 4 * i + p.q < n ? dt[i] : 0.0f;
+        });
+        wave_sync();
+        each<NG>([&](auto i) {
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float e[8];
+            *(float4*)e = *(const float4*)(x + 8 * i);
+            *(float4*)(e + 4) = *(const float4*)(x + 8 * i + 4);
+            each<4>([&](auto j) {
+                if (!TAIL || 4 * i + j < n) {
+                    each<S>([&](auto s) {
+                        constexpr int I = j * S + s;
+                        h[s] = fmaf(exp2_(e[2 * j] * l.a2[s]), h[s], row_bcast<I % 16>(v.b[i][I / 16]) * e[2 * j + 1]);
+                        if (PAD && l.pad[s]) h[s] = 0.0f;
+                    });
+                    if constexpr (!LOCAL) bcast_dot<S, j>(y[j], v.c[i], h);
+                }
+            });
+            if constexpr (!LOCAL) out[i] = fmaf(l.skip, v.u[i], rows_sum(y));
+        });
+        if constexpr (!LOCAL) {
+            if (at.gate) each<NG>([&](auto i) { out[i] *= v.z[i] * sigmoid(v.z[i]); });
+            each<NG>([&](auto i) { store_channels<TAIL>(at.out, p, i, n, out[i]); });
+            at.out.forth();
+        }
+    }
 
     // LOCAL: the states that the chunk's own tokens leave, from none, and the
     // sum of its time steps; else outputs, from the states before the chunk.
@@ -311,47 +424,23 @@ struct Scan {
             }
         }
         float sum_dt = 0.0f;
-        for (uint32_t t = p.t0; t < p.t1; t += SEG) {
-            const uint32_t n = p.t1 - t < SEG ? p.t1 - t : SEG;
-            float u[NG], d[NG], dt[NG], slope[NG], z[NG], b[NG][NB], cc[NG][NB];
-            load_channels(u, g.u, p, t, n);
-            load_channels(d, g.delta, p, t, n);
-            load_states(b, g.b, g, p, l, t, n);
-            if constexpr (!LOCAL) {
-                load_states(cc, g.c, g, p, l, t, n);
-                if (g.z.p) load_channels(z, g.z, p, t, n);
-                if (g.check) {  // lanes without a channel too: the backward pass reads them
-                    float* to = g.check + check_at(g, p, t);
-                    each<S>([&](auto s) { to[s] = h[s]; });
-                }
-            }
-            steps(g, l, d, dt, slope);
-            wave_sync();
-            each<NG>([&](auto i) {
-                x[(4 * i + p.q) * 2] = dt[i];
-                x[(4 * i + p.q) * 2 + 1] = dt[i] * u[i];
-                if constexpr (LOCAL) sum_dt += 4 * i + p.q < n ? dt[i] : 0.0f;
-            });
-            wave_sync();
-            each<NG>([&](auto i) {
-                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                each<4>([&](auto j) {
-                    if (4 * i + j < n) {
-                        const float dtj = x[(4 * i + j) * 2], dtu = x[(4 * i + j) * 2 + 1];
-                        each<S>([&](auto s) {
-                            constexpr int I = j * S + s;
-                            h[s] = fmaf(exp2_(dtj * l.a2[s]), h[s], row_bcast<I % 16>(b[i][I / 16]) * dtu);
-                            if (PAD && l.pad[s]) h[s] = 0.0f;
-                        });
-                        if constexpr (!LOCAL) bcast_dot<S, j>(y[j], cc[i], h);
-                    }
-                });
-                if constexpr (!LOCAL) {
-                    float o = fmaf(l.skip, u[i], rows_sum(y));
-                    if (g.z.p) o *= z[i] * sigmoid(z[i]);
-                    store_channels(g.out, p, t, i, n, o);
-                }
-            });
+        Cursors<LOCAL> at;
+        at.set(g, p);
+        Segment<LOCAL> next;
+        Values<LOCAL> now;
+        uint32_t t = p.t0;
+        if (t + SEG <= p.t1) at.template load<false>(next, p, l, SEG);
+        while (t + SEG <= p.t1) {
+            now.take(next, l);
+            // the next segment's rows, while this one is worked through
+            if (t + 2 * SEG <= p.t1) at.template load<false>(next, p, l, SEG);
+            forward_segment<LOCAL, false>(g, p, l, x, h, sum_dt, now, at, t, SEG);
+            t += SEG;
+        }
+        if (t < p.t1) {
+            at.template load<true>(next, p, l, p.t1 - t);
+            now.take(next, l);
+            forward_segment<LOCAL, true>(g, p, l, x, h, sum_dt, now, at, t, p.t1 - t);
         }
         if constexpr (LOCAL) {
             const float v[4] = {sum_dt, sum_dt, sum_dt, sum_dt};
@@ -401,17 +490,31 @@ struct Scan {
             const uint32_t t = p.t0 + k * SEG;
             const uint32_t n = p.t1 - t < SEG ? p.t1 - t : SEG;
             float u[NG], d[NG], dt[NG], slope[NG], dy[NG], b[NG][NB], cc[NG][NB], ds[NG], zs[NG];
-            load_channels(d, g.delta, p, t, n);
-            load_channels(dy, g.gout, p, t, n);
-            load_states(cc, g.c, g, p, l, t, n);
+            raw rv[NG], rs[NG][NB];
+            Cursor cur;
+            cur.set(g.delta, p, t);
+            load_channels<true>(rv, cur, p, n);
+            up_channels(d, rv);
+            cur.set(g.gout, p, t);
+            load_channels<true>(rv, cur, p, n);
+            up_channels(dy, rv);
+            cur.set(g.c, p, t, p.group * g.states);
+            load_states<true>(rs, cur, l, n);
+            up_states(cc, rs, l);
             if constexpr (!LOCAL) {
-                load_channels(u, g.u, p, t, n);
-                load_states(b, g.b, g, p, l, t, n);
+                cur.set(g.u, p, t);
+            load_channels<true>(rv, cur, p, n);
+                up_channels(u, rv);
+                cur.set(g.b, p, t, p.group * g.states);
+                load_states<true>(rs, cur, l, n);
+                up_states(b, rs, l);
             }
             each<NG>([&](auto i) { ds[i] = dy[i], zs[i] = 0.0f; });
             if (g.z.p) {
                 float z[NG];
-                load_channels(z, g.z, p, t, n);
+                cur.set(g.z, p, t);
+            load_channels<true>(rv, cur, p, n);
+                up_channels(z, rv);
                 each<NG>([&](auto i) {
                     const float sg = sigmoid(z[i]);
                     ds[i] = dy[i] * z[i] * sg;
@@ -468,7 +571,7 @@ struct Scan {
                     });
                     if (g.gz.p) {
                         const float o = fmaf(l.skip, u[i], rows_sum(y));
-                        store_channels(g.gz, p, t, i, n, zs[i] * o);
+                        { cur.set(g.gz, p, t); store_channels<true>(cur, p, i, n, zs[i] * o); }
                     }
                 });
                 // and back
@@ -500,8 +603,8 @@ struct Scan {
                         gbias += gdelta;
                         gskip = fmaf(ds[i], u[i], gskip);
                     }
-                    if (g.gdelta.p) store_channels(g.gdelta, p, t, i, n, gdelta);
-                    if (g.gu.p) store_channels(g.gu, p, t, i, n, fmaf(dt[i], gbu, l.skip * ds[i]));
+                    if (g.gdelta.p) { cur.set(g.gdelta, p, t); store_channels<true>(cur, p, i, n, gdelta); }
+                    if (g.gu.p) { cur.set(g.gu, p, t); store_channels<true>(cur, p, i, n, fmaf(dt[i], gbu, l.skip * ds[i])); }
                     channels_sum(gb, p.c);
                     channels_sum(gc, p.c);
                     constexpr int R = S >= 4 ? S / 4 : 1;
