@@ -21,7 +21,7 @@ static inline uint32_t fg_ssm_lane_states(uint32_t states) {
 }
 /* Tokens of a segment, the unit that the scan works through; the states at
  * the start of each are what a forward pass leaves for its backward pass. */
-#define FG_SSM_SEGMENT(lane_states) ((lane_states) <= 4 ? 16 : 64 / (lane_states))
+#define FG_SSM_SEGMENT 16
 
 /* Rows of a [sequences, tokens, n] array, strides in elements. */
 typedef struct {
@@ -49,6 +49,7 @@ typedef struct {
     uint32_t chunks, chunk_len;            /* chunk_len: a multiple of the segment */
     uint32_t check_segs;                   /* dense: segments of a sequence */
     uint32_t softplus;
+    uint32_t wide; /* all rows take vector loads and stores */
 } fg_scan_kargs;
 
 typedef struct {

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "ssm_args.h"
 
 namespace fg {
@@ -68,6 +70,14 @@ __device__ __forceinline__ Softplus softplus(float x) {
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) {
     return (int64_t)(((uint64_t)uniform((uint32_t)((uint64_t)x >> 32)) << 32) | uniform((uint32_t)x));
+}
+
+// A 32-bit offset that the compiler takes as new here: it then adds it to a
+// uniform address within the load or store, where an offset extended to 64
+// bits far above costs a vector addition for each of them.
+__device__ __forceinline__ uint32_t fresh(uint32_t off) {
+    asm volatile("" : "+v"(off));
+    return off;
 }
 
 // Lane I of each row of 16 lanes to the whole row.  The compiler folds the

@@ -22,8 +22,8 @@ using namespace fg::ssm;
         fg_scan_kargs g) {                                                                                      \
         Scan<T, S, PAD>::backward<true>(g);                                                                    \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_back_##NAME##_s##S##SUFFIX(        \
-        fg_scan_kargs g) {                                                                                      \
+    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES)                  \
+    __attribute__((amdgpu_waves_per_eu(S <= 4 ? 2 : 1))) void fg_scan_back_##NAME##_s##S##SUFFIX(fg_scan_kargs g) {                                                                                      \
         Scan<T, S, PAD>::backward<false>(g);                                                                   \
     }
 #define FG_SCAN_BOTH(NAME, T, S) FG_SCAN(NAME, T, S, , false) FG_SCAN(NAME, T, S, _pad, true)

@@ -384,7 +384,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     lane_states_ = fg_ssm_lane_states((uint32_t)s.states);
-    segment_ = FG_SSM_SEGMENT(lane_states_);
+    segment_ = FG_SSM_SEGMENT;
     group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, FG_SSM_GROUP_CHANNELS);
     blocks_ = group_blocks_ * (uint32_t)s.groups;
     chunks_forward_ = chunks_for(1024);
@@ -448,6 +448,17 @@ void ScanPlan::check_inputs(const char* op, const fg_scan_inputs& in) const {
     if (!s_.packed && in.offsets) invalid(std::string(op) + ": offsets are for packed sequences");
 }
 
+// Vector accesses where every row and every lane's part of it allow them: four
+// channels, and the lane's states of a channel that has all of them.
+bool ScanPlan::wide(const fg_scan_kargs& g, std::initializer_list<const fg_ssm_view*> channels,
+                    std::initializer_list<const fg_ssm_view*> states) const {
+    const uint32_t es = kBytes[s_.dtype];
+    bool yes = g.group_channels % 4 == 0 && g.states == 4 * lane_states_;
+    for (const fg_ssm_view* v : channels) yes = yes && vector_rows(*v, 4, es);
+    for (const fg_ssm_view* v : states) yes = yes && vector_rows(*v, std::min(lane_states_, 16 / es), es);
+    return yes;
+}
+
 void ScanPlan::forward(const fg_scan_forward_args& a, hipStream_t stream) const {
     const char* op = "scan forward";
     const fg_scan_inputs& in = a.in;
@@ -470,6 +481,7 @@ void ScanPlan::forward(const fg_scan_forward_args& a, hipStream_t stream) const 
     all.flat("checkpoints", a.checkpoints, (int64_t)checkpoint_bytes(), true, true);
     g.final = a.final;
     g.check = (float*)a.checkpoints;
+    g.wide = wide(g, {&g.u, &g.delta, &g.z, &g.out}, {&g.b, &g.c});
     void* args[] = {&g};
     const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
     if (g.chunks > 1) launch(dev_, stream, local_, blocks, 64 * FG_SSM_WAVES, args, op);
@@ -522,6 +534,7 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
     }
     g.part_bc = part_bc_.data();
     g.part_p = part_p_.data();
+    g.wide = wide(g, {&g.u, &g.delta, &g.z, &g.gout, &g.gu, &g.gdelta, &g.gz}, {&g.b, &g.c});
     void* args[] = {&g};
     const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
     if (g.chunks > 1) launch(dev_, stream, back_local_, blocks, 64 * FG_SSM_WAVES, args, op);

@@ -7,6 +7,7 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 
 #include "device.hpp"
@@ -59,6 +60,8 @@ public:
 private:
     fg_scan_kargs base(const fg_scan_inputs& in, uint32_t chunks) const;
     void check_inputs(const char* op, const fg_scan_inputs& in) const;
+    bool wide(const fg_scan_kargs& g, std::initializer_list<const fg_ssm_view*> channels,
+              std::initializer_list<const fg_ssm_view*> states) const;
     uint32_t chunks_for(uint32_t target_waves) const;
     HipBackend::DeviceHandle dev_;
     fg_scan_shape s_;
