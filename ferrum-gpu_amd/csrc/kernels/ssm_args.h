@@ -6,22 +6,15 @@
 
 #include <stdint.h>
 
-#define FG_SSM_WAVES 4            /* waves of a workgroup of the scan */
-#define FG_SSM_WAVE_CHANNELS 16   /* channels of a wave */
-#define FG_SSM_GROUP_CHANNELS (FG_SSM_WAVES * FG_SSM_WAVE_CHANNELS)
+#define FG_SSM_SEGMENT 16         /* tokens that the scan works through at a time; the
+                                    states before each segment are what a forward
+                                    pass leaves for its backward pass */
 #define FG_SSM_MAX_STATES 64
 #define FG_CONV_MAX_WIDTH 8
 
-/* States of a channel that one lane holds: the channel's states are spread
- * over four lanes.  1, 2, 4, 8 or 16. */
-static inline uint32_t fg_ssm_lane_states(uint32_t states) {
-    uint32_t s = 1;
-    while (4 * s < states) s *= 2;
-    return s;
-}
-/* Tokens of a segment, the unit that the scan works through; the states at
- * the start of each are what a forward pass leaves for its backward pass. */
-#define FG_SSM_SEGMENT 16
+/* A scan's workgroup has FG_SSM_BLOCKS(W) blocks of 16 channels with W waves
+ * each; 4 W rows of 16 lanes share a channel's states. */
+#define FG_SSM_BLOCKS(w) ((w) == 1 ? 4 : 2)
 
 /* Rows of a [sequences, tokens, n] array, strides in elements. */
 typedef struct {
@@ -38,9 +31,9 @@ typedef struct {
     float *ga, *gskip, *gbias, *ginitial;
     const int32_t* offsets; /* packed: sequences + 1 of them; null: dense */
     float* check;           /* states at segment starts */
-    float* carry;           /* [sequences][chunks + 1][wave blocks][64 * lane states]: what a chunk adds;
+    float* carry;           /* [sequences][chunks + 1][blocks of 16 channels][16 * 4 W S]: what a chunk adds;
                                the last place: the initial states */
-    float* carry_dt;        /* [sequences][chunks + 1][wave blocks][16]: its summed time steps */
+    float* carry_dt;        /* [sequences][chunks + 1][blocks of 16 channels][16]: its summed time steps */
     float* part_bc;         /* [channel blocks of a group][tokens][groups][2][states] */
     float* part_p;          /* [sequences * chunks][channels * (states + 2)] */
     uint64_t tokens;        /* packed: of all sequences */
@@ -49,7 +42,6 @@ typedef struct {
     uint32_t chunks, chunk_len;            /* chunk_len: a multiple of the segment */
     uint32_t check_segs;                   /* dense: segments of a sequence */
     uint32_t softplus;
-    uint32_t wide; /* all rows take vector loads and stores */
 } fg_scan_kargs;
 
 typedef struct {

@@ -8,25 +8,23 @@
 
 using namespace fg::ssm;
 
-// S: states of a lane; _pad: the channel has fewer than 4 S states.
-#define FG_SCAN(NAME, T, S, SUFFIX, PAD)                                                                       \
-    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_local_##NAME##_s##S##SUFFIX(       \
-        fg_scan_kargs g) {                                                                                      \
-        Scan<T, S, PAD>::forward<true>(g);                                                                     \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_##NAME##_s##S##SUFFIX(             \
-        fg_scan_kargs g) {                                                                                      \
-        Scan<T, S, PAD>::forward<false>(g);                                                                    \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES) void fg_scan_back_local_##NAME##_s##S##SUFFIX(  \
-        fg_scan_kargs g) {                                                                                      \
-        Scan<T, S, PAD>::backward<true>(g);                                                                    \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64 * FG_SSM_WAVES)                  \
-    __attribute__((amdgpu_waves_per_eu(S <= 4 ? 2 : 1))) void fg_scan_back_##NAME##_s##S##SUFFIX(fg_scan_kargs g) {                                                                                      \
-        Scan<T, S, PAD>::backward<false>(g);                                                                   \
+// S: states of a lane, W: waves that share a channel's states; _any: for any
+// alignment, and channels with fewer than 4 S W states.  The backward kernel holds two states
+// and decays for each of its 16 S, so S = 4 is held to two waves per SIMD.
+#define FG_SCAN_KERNEL(NAME, T, S, W, WIDE, CALL)                                                               \
+    extern "C" __global__ __launch_bounds__((Scan<T, S, W, WIDE>::THREADS))                                     \
+    __attribute__((amdgpu_waves_per_eu(2, 3))) void NAME(fg_scan_kargs g) {                                    \
+        Scan<T, S, W, WIDE>::CALL(g);                                                                           \
     }
-#define FG_SCAN_BOTH(NAME, T, S) FG_SCAN(NAME, T, S, , false) FG_SCAN(NAME, T, S, _pad, true)
+#define FG_SCAN_ONE(NAME, T, S, W, SUFFIX, WIDE)                                                                \
+    FG_SCAN_KERNEL(fg_scan_local_##NAME##_s##S##w##W##SUFFIX, T, S, W, WIDE, template forward<true>)            \
+    FG_SCAN_KERNEL(fg_scan_##NAME##_s##S##w##W##SUFFIX, T, S, W, WIDE, template forward<false>)                 \
+    FG_SCAN_KERNEL(fg_scan_back_local_##NAME##_s##S##w##W##SUFFIX, T, S, W, WIDE, template backward<true>)      \
+    extern "C" __global__ __launch_bounds__((Scan<T, S, W, WIDE>::THREADS))                                     \
+    __attribute__((amdgpu_waves_per_eu(2))) void fg_scan_back_##NAME##_s##S##w##W##SUFFIX(fg_scan_kargs g) {   \
+        Scan<T, S, W, WIDE>::template backward<false>(g);                                                       \
+    }
+#define FG_SCAN(NAME, T, S, W) FG_SCAN_ONE(NAME, T, S, W, , true) FG_SCAN_ONE(NAME, T, S, W, _any, false)
 
 // W taps, V channels of a thread: 16 bytes of a row forward, at most four
 // channels backward; V = 1 for any stride and alignment.
@@ -43,11 +41,11 @@ using namespace fg::ssm;
 #define FG_CONV_BOTH(NAME, T, W, V) FG_CONV(NAME, T, W, V, 4) FG_CONV(NAME, T, W, 1, 1)
 
 #define FG_SSM_TYPE(NAME, T, V)                                                                                 \
-    FG_SCAN_BOTH(NAME, T, 1)                                                                                    \
-    FG_SCAN_BOTH(NAME, T, 2)                                                                                    \
-    FG_SCAN_BOTH(NAME, T, 4)                                                                                    \
-    FG_SCAN_BOTH(NAME, T, 8)                                                                                    \
-    FG_SCAN_BOTH(NAME, T, 16)                                                                                   \
+    FG_SCAN(NAME, T, 1, 1)                                                                                      \
+    FG_SCAN(NAME, T, 2, 1)                                                                                      \
+    FG_SCAN(NAME, T, 4, 1)                                                                                      \
+    FG_SCAN(NAME, T, 4, 2)                                                                                      \
+    FG_SCAN(NAME, T, 4, 4)                                                                                      \
     FG_CONV_BOTH(NAME, T, 2, V)                                                                                 \
     FG_CONV_BOTH(NAME, T, 3, V)                                                                                 \
     FG_CONV_BOTH(NAME, T, 4, V)                                                                                 \

@@ -3,19 +3,22 @@
 //   dt = softplus(delta + bias)              h_t[d,n] = exp(dt A[d,n]) h_{t-1}[d,n] + dt u B_t[n]
 //   y  = (sum_n C_t[n] h_t[d,n] + D u) silu(z)
 //
-// A wave takes 16 channels and walks along the tokens in segments of 16.  Its
+// W waves take 16 channels and walk along the tokens in segments of 16.  Their
 // lanes have two roles, between which LDS carries values:
-//   * per token and channel (time steps, gates, outputs): lane l has token l / 4
-//     of the segment and four neighbouring channels, 4 (l % 4) ...; rows are
-//     loaded and stored eight bytes a lane of a 16-bit type;
-//   * per state: lane (q, c) = (l / 16, l % 16) has the states q S ... q S + S - 1
-//     of channel c and steps through the tokens.  B and C of those states lie
-//     one token a lane in the row's 16 lanes, and reach the row as the DPP
-//     broadcast operand of the instruction that takes them; sums over a
-//     channel's states end with an exchange between the wave's four rows.
-// Nothing is worked out twice, and waves wait for each other only where the
-// backward pass adds up over channels.  The workgroup is four waves, 64
-// channels: 128-byte lines of a 16-bit type.
+//   * per token and channel (time steps, gates, outputs): each of the 64 W
+//     lanes has 4 / W neighbouring channels of one token, loaded and stored
+//     together;
+//   * per state: lane (q, c) = (lane / 16, lane % 16) of wave w has S states of
+//     channel c, from (4 w + q) S on, and steps through the tokens.  B and C of
+//     those states lie one token a lane in the row's 16 lanes, and reach the
+//     row as the DPP broadcast operand of the instruction that takes them.
+//     Sums over a channel's states go to LDS after one exchange within the wave.
+// Nothing is worked out twice.  A workgroup has 64 channels (32 for W = 4):
+// 128-byte lines of a 16-bit type.
+//
+// W is 1 up to 16 states, 2 up to 32, 4 up to 64.  (16 states on two waves, for
+// tensors that leave SIMDs with one wave, gained nothing: 4 x 2048 tokens x
+// 4096 channels in bfloat16 194 us against 177.)
 #pragma once
 
 #include "ssm_common.hpp"
@@ -23,77 +26,63 @@
 namespace fg {
 namespace ssm {
 
-// acc[i] += bcast(v[i], lane J of the row) * x[i], and acc += sum_i of it, for
-// up to four i in one statement of assembly: the compiler does not fold the
-// broadcast into a multiply-add.  The s_nop keeps the two wait states that a
-// DPP operand needs after the instruction that wrote it.
-#define FG_BC "row_newbcast:%"
-template <int J>
-__device__ __forceinline__ void fmac1(float& a, float v, float x) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 " FG_BC "3 row_mask:0xf bank_mask:0xf" : "+v"(a) : "v"(v), "v"(x), "n"(J));
-}
-template <int J>
-__device__ __forceinline__ void fmac2(float& a0, float& a1, float v0, float v1, float x) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %2, %4 " FG_BC "5 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %1, %3, %4 " FG_BC "5 row_mask:0xf bank_mask:0xf"
-        : "+&v"(a0), "+&v"(a1)
-        : "v"(v0), "v"(v1), "v"(x), "n"(J));
-}
-template <int J>
-__device__ __forceinline__ void fmac4(float& a0, float& a1, float& a2, float& a3, float v0, float v1, float v2,
-                                      float v3, float x) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %4, %8 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %1, %5, %8 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %2, %6, %8 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %3, %7, %8 " FG_BC "9 row_mask:0xf bank_mask:0xf"
-        : "+&v"(a0), "+&v"(a1), "+&v"(a2), "+&v"(a3)
-        : "v"(v0), "v"(v1), "v"(v2), "v"(v3), "v"(x), "n"(J));
-}
-template <int J>
-__device__ __forceinline__ void dot2(float& a, float v0, float v1, float x0, float x1) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %3 " FG_BC "5 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %2, %4 " FG_BC "5 row_mask:0xf bank_mask:0xf"
-        : "+&v"(a)
-        : "v"(v0), "v"(v1), "v"(x0), "v"(x1), "n"(J));
-}
-template <int J>
-__device__ __forceinline__ void dot4(float& a, float v0, float v1, float v2, float v3, float x0, float x1, float x2,
-                                     float x3) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %5 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %2, %6 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %3, %7 " FG_BC "9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %4, %8 " FG_BC "9 row_mask:0xf bank_mask:0xf"
-        : "+&v"(a)
-        : "v"(v0), "v"(v1), "v"(v2), "v"(v3), "v"(x0), "v"(x1), "v"(x2), "v"(x3), "n"(J));
-}
-#undef FG_BC
-
-// acc[s] += (token J's v[s]) * x, s < N.
+// Multiply-adds whose first factor is lane J of the row's v, in statements of
+// assembly: the compiler does not fold the broadcast into a multiply-add.  The
+// s_nop keeps the two wait states that a DPP operand needs after the
+// instruction that wrote it.
+#define FG_FMAC(acc, v, x, j) "v_fmac_f32_dpp %" #acc ", %" #v ", %" #x " row_newbcast:%" #j " row_mask:0xf bank_mask:0xf\n\t"
+// acc[s] += v[s] * x, s < N.
 template <int N, int J>
-__device__ __forceinline__ void bcast_fmac(float* acc, const float* v, float x) {
-    if constexpr (N == 1) fmac1<J>(acc[0], v[0], x);
-    else if constexpr (N == 2) fmac2<J>(acc[0], acc[1], v[0], v[1], x);
+__device__ __forceinline__ void bcast_fmac(float (&a)[N], const float (&v)[N], float x) {
+    if constexpr (N == 1)
+        asm("s_nop 1\n\t" FG_FMAC(0, 1, 2, 3) : "+v"(a[0]) : "v"(v[0]), "v"(x), "n"(J));
+    else if constexpr (N == 2)
+        asm("s_nop 1\n\t" FG_FMAC(0, 2, 4, 5) FG_FMAC(1, 3, 4, 5)
+            : "+&v"(a[0]), "+&v"(a[1])
+            : "v"(v[0]), "v"(v[1]), "v"(x), "n"(J));
     else
-        each<N / 4>([&](auto k) {
-            constexpr int i = 4 * k;
-            fmac4<J>(acc[i], acc[i + 1], acc[i + 2], acc[i + 3], v[i], v[i + 1], v[i + 2], v[i + 3], x);
-        });
+        asm("s_nop 1\n\t" FG_FMAC(0, 4, 8, 9) FG_FMAC(1, 5, 8, 9) FG_FMAC(2, 6, 8, 9) FG_FMAC(3, 7, 8, 9)
+            : "+&v"(a[0]), "+&v"(a[1]), "+&v"(a[2]), "+&v"(a[3])
+            : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(x), "n"(J));
 }
-// acc += sum_s (token J's v[s]) * x[s].
+// acc += sum_s v[s] * x[s].
 template <int N, int J>
-__device__ __forceinline__ void bcast_dot(float& acc, const float* v, const float* x) {
-    if constexpr (N == 1) fmac1<J>(acc, v[0], x[0]);
-    else if constexpr (N == 2) dot2<J>(acc, v[0], v[1], x[0], x[1]);
+__device__ __forceinline__ void bcast_dot(float& a, const float (&v)[N], const float (&x)[N]) {
+    if constexpr (N == 1)
+        asm("s_nop 1\n\t" FG_FMAC(0, 1, 2, 3) : "+&v"(a) : "v"(v[0]), "v"(x[0]), "n"(J));
+    else if constexpr (N == 2)
+        asm("s_nop 1\n\t" FG_FMAC(0, 1, 3, 5) FG_FMAC(0, 2, 4, 5)
+            : "+&v"(a)
+            : "v"(v[0]), "v"(v[1]), "v"(x[0]), "v"(x[1]), "n"(J));
     else
-        each<N / 4>([&](auto k) {
-            constexpr int i = 4 * k;
-            dot4<J>(acc, v[i], v[i + 1], v[i + 2], v[i + 3], x[i], x[i + 1], x[i + 2], x[i + 3]);
-        });
+        asm("s_nop 1\n\t" FG_FMAC(0, 1, 5, 9) FG_FMAC(0, 2, 6, 9) FG_FMAC(0, 3, 7, 9) FG_FMAC(0, 4, 8, 9)
+            : "+&v"(a)
+            : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(J));
 }
+// Two tokens' sums (lanes J and K), their instructions in turn.
+template <int N, int J, int K>
+__device__ __forceinline__ void bcast_dots(float& a, float& b, const float (&v)[N], const float (&x)[N],
+                                           const float (&y)[N]) {
+    if constexpr (N == 1)
+        asm("s_nop 1\n\t" FG_FMAC(0, 2, 3, 5) FG_FMAC(1, 2, 4, 6)
+            : "+&v"(a), "+&v"(b)
+            : "v"(v[0]), "v"(x[0]), "v"(y[0]), "n"(J), "n"(K));
+    else if constexpr (N == 2)
+        asm("s_nop 1\n\t" FG_FMAC(0, 2, 4, 8) FG_FMAC(1, 2, 6, 9) FG_FMAC(0, 3, 5, 8) FG_FMAC(1, 3, 7, 9)
+            : "+&v"(a), "+&v"(b)
+            : "v"(v[0]), "v"(v[1]), "v"(x[0]), "v"(x[1]), "v"(y[0]), "v"(y[1]), "n"(J), "n"(K));
+    else
+        asm("s_nop 1\n\t" FG_FMAC(0, 2, 6, 14) FG_FMAC(1, 2, 10, 15) FG_FMAC(0, 3, 7, 14) FG_FMAC(1, 3, 11, 15)
+            FG_FMAC(0, 4, 8, 14) FG_FMAC(1, 4, 12, 15) FG_FMAC(0, 5, 9, 14) FG_FMAC(1, 5, 13, 15)
+            : "+&v"(a), "+&v"(b)
+            : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]),
+              "v"(y[1]), "v"(y[2]), "v"(y[3]), "n"(J), "n"(K));
+}
+#undef FG_FMAC
 
-// The sum over a row's 16 channels of each of v[0 .. 4 N), N <= 4: halving the
-// values with every bit of the lane number, so that lane c ends with the sum
-// of value c (N = 4), c >> 1 (2) or c >> 2 (1) in v[0].
+// The sum over a row's 16 channels of each of v[0 .. 4 N): halving the values
+// with every bit of the lane number, so that lane c ends with the sum of value
+// c (N = 4), c >> 1 (2) or c >> 2 (1) in v[0].
 template <int N>
 __device__ __forceinline__ void channels_sum(float (&v)[4 * N], uint32_t c) {
     const bool b3 = c & 8, b2 = c & 4, b1 = c & 2, b0 = c & 1;
@@ -111,120 +100,136 @@ __device__ __forceinline__ void channels_sum(float (&v)[4 * N], uint32_t c) {
     else v[0] += dpp<kXor1>(v[0]);
 }
 
-// Where a wave works: its sequence, the tokens of its chunk, its channels.
-struct Place {
-    int64_t start;               // packed: the sequence's first row
-    uint32_t len;                // tokens of the sequence
-    uint32_t seq, chunk, group, block;
-    uint32_t t0, t1;             // the chunk's tokens
-    uint32_t wave, wblock;       // its number in the workgroup, and among all waves over channels
-    // as (q, c): the channel, within the group and among all (the group's last where it has none)
-    uint32_t q, c, ch;
-    bool valid;
-    // as (token, four channels): the first channel, how many of the four there are
-    uint32_t tok, ch4;
-    int have;
-};
-
-__device__ __forceinline__ Place place(const fg_scan_kargs& g) {
-    Place p;
-    const uint32_t lane = threadIdx.x & 63;
-    p.wave = uniform(threadIdx.x >> 6);
-    p.q = lane >> 4;
-    p.c = lane & 15;
-    p.tok = lane >> 2;
-    const uint32_t blocks = g.groups * g.group_blocks;
-    const uint32_t cb = blockIdx.x % blocks, rest = blockIdx.x / blocks;
-    p.group = cb / g.group_blocks;
-    p.block = cb % g.group_blocks;
-    p.chunk = rest % g.chunks;
-    p.seq = rest / g.chunks;
-    p.start = 0;
-    p.len = g.length;
-    if (g.offsets) {
-        // offsets out of order or beyond the rows give shorter sequences, not accesses outside
-        int64_t a = g.offsets[p.seq], b = g.offsets[p.seq + 1];
-        const int64_t all = (int64_t)g.tokens;
-        a = a < 0 ? 0 : a > all ? all : a;
-        b = b < a ? a : b > all ? all : b;
-        p.start = uniform(a);
-        p.len = uniform((uint32_t)(b - a < (int64_t)g.length ? b - a : (int64_t)g.length));
-    }
-    const uint64_t first = (uint64_t)p.chunk * g.chunk_len;
-    p.t0 = first < p.len ? (uint32_t)first : p.len;
-    p.t1 = p.len - p.t0 < g.chunk_len ? p.len : p.t0 + g.chunk_len;
-    const uint32_t base = p.block * FG_SSM_GROUP_CHANNELS + p.wave * FG_SSM_WAVE_CHANNELS;
-    const uint32_t one = base + p.c, four = base + 4 * (lane & 3);
-    p.valid = one < g.group_channels;
-    p.ch = p.group * g.group_channels + (p.valid ? one : g.group_channels - 1);
-    p.have = four >= g.group_channels ? 0 : g.group_channels - four < 4 ? (int)(g.group_channels - four) : 4;
-    p.ch4 = four;
-    p.wblock = cb * FG_SSM_WAVES + p.wave;
-    return p;
-}
-
-template <class T, int S, bool PAD>
+// WIDE: every row takes vector loads and stores, every channel has 4 S W
+// states; else any alignment and stride, and fewer states.
+template <class T, int S, int W, bool WIDE>
 struct Scan {
+    static constexpr bool PAD = !WIDE;
     using raw = typename T::raw;
-    static constexpr int SEG = FG_SSM_SEGMENT;
-    static constexpr int ES = sizeof(raw);
-    static constexpr int SP = S < 4 ? S : 4, PASSES = S / SP;  // states of a lane at a time (backward)
+    static constexpr int SEG = FG_SSM_SEGMENT, ES = sizeof(raw);
+    static constexpr int VC = 4 / W;                      // channels of a lane as (token, channels)
+    static constexpr int BLOCKS = FG_SSM_BLOCKS(W);       // of 16 channels in a workgroup
+    static constexpr int THREADS = 64 * W * BLOCKS;
 
-    // N elements as they lie in memory, in whole registers: 16-bit ones two to
-    // a register, so that a wide load needs no work that would wait for it.
+    // Where a wave works: its sequence, the tokens of its chunk, its channels.
+    struct Place {
+        int64_t start;               // packed: the sequence's first row
+        uint32_t len;                // tokens of the sequence
+        uint32_t seq, chunk, group, block;
+        uint32_t t0, t1;             // the chunk's tokens
+        uint32_t set;                // the 16 channels' number in the workgroup
+        uint32_t part;               // the wave's number among the W
+        uint32_t sets;               // the 16 channels' number among all
+        // as (q, c): channel among all (the group's last where there is none), row among 4 W
+        uint32_t q, c, ch, row;
+        bool valid;
+        // as (token, channels): first channel in the 16 and in the group, how many there are
+        uint32_t tok, sub, in_group;
+        int have;
+    };
+    static __device__ __forceinline__ Place place(const fg_scan_kargs& g) {
+        Place p;
+        const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+        p.set = wave / W;
+        p.part = wave % W;
+        p.q = lane >> 4;
+        p.c = lane & 15;
+        p.row = 4 * p.part + p.q;
+        const uint32_t e = (p.part * 64 + lane) * VC;
+        p.tok = e / 16;
+        p.sub = e % 16;
+        const uint32_t blocks = g.groups * g.group_blocks;
+        // Workgroups go to the 8 XCDs in turn; neighbouring channels, which
+        // share cache lines and B and C, go to the same one.
+        const uint32_t all_blocks = gridDim.x, per = all_blocks / 8, eighth = blockIdx.x % 8;
+        const uint32_t id = blockIdx.x < per * 8 ? eighth * per + blockIdx.x / 8 : blockIdx.x;
+        const uint32_t cb = id % blocks, rest = id / blocks;
+        p.group = cb / g.group_blocks;
+        p.block = cb % g.group_blocks;
+        p.chunk = rest % g.chunks;
+        p.seq = rest / g.chunks;
+        p.start = 0;
+        p.len = g.length;
+        if (g.offsets) {
+            // offsets out of order or beyond the rows give shorter sequences, not accesses outside
+            int64_t a = g.offsets[p.seq], b = g.offsets[p.seq + 1];
+            const int64_t all = (int64_t)g.tokens;
+            a = a < 0 ? 0 : a > all ? all : a;
+            b = b < a ? a : b > all ? all : b;
+            p.start = uniform(a);
+            p.len = uniform((uint32_t)(b - a < (int64_t)g.length ? b - a : (int64_t)g.length));
+        }
+        const uint64_t first = (uint64_t)p.chunk * g.chunk_len;
+        p.t0 = first < p.len ? (uint32_t)first : p.len;
+        p.t1 = p.len - p.t0 < g.chunk_len ? p.len : p.t0 + g.chunk_len;
+        const uint32_t base = (p.block * BLOCKS + p.set) * 16;
+        p.valid = base + p.c < g.group_channels;
+        p.ch = p.group * g.group_channels + (p.valid ? base + p.c : g.group_channels - 1);
+        p.in_group = base + p.sub;
+        p.have = p.in_group >= g.group_channels ? 0
+                 : g.group_channels - p.in_group < VC ? (int)(g.group_channels - p.in_group) : VC;
+        p.sets = cb * BLOCKS + p.set;
+        return p;
+    }
+
+    // N neighbouring elements as they lie in memory, in whole registers.  Wide:
+    // one load, 16-bit ones two to a register; else one load and register for
+    // each, at offsets of their own.  Nothing waits for a load before up().
     template <int N>
     struct Pack {
-        static constexpr int WORDS = (N * ES + 3) / 4;
+        static constexpr int WORDS = WIDE ? (N * ES + 3) / 4 : N;
         uint32_t w[WORDS];
         __device__ __forceinline__ float up(int i) const {
             if constexpr (ES == 4) return __uint_as_float(w[i]);
-            else return T::up((raw)(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
+            else if constexpr (WIDE) return T::up((raw)(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
+            else return T::up((raw)w[i]);
         }
-        __device__ __forceinline__ void load(const char* at) {
-            if constexpr (N * ES >= 4) {
-                struct __attribute__((aligned(N * ES > 16 ? 16 : N * ES))) Words {
+        __device__ __forceinline__ void load(const char* at, uint32_t row, const uint32_t (&off)[N]) {
+            if constexpr (!WIDE) {
+                each<N>([&](auto i) {
+                    const raw x = *(const raw*)(at + fresh(row + off[i]));
+                    if constexpr (ES == 4) w[i] = __builtin_bit_cast(uint32_t, x);
+                    else w[i] = x;
+                });
+            } else if constexpr (N * ES >= 4) {
+                struct __attribute__((aligned(N * ES))) Words {
                     uint32_t w[WORDS];
                 };
-                const Words x = *(const Words*)at;
+                const Words x = *(const Words*)(at + fresh(row + off[0]));
                 each<WORDS>([&](auto i) { w[i] = x.w[i]; });
             } else {
-                w[0] = *(const raw*)at;
+                w[0] = *(const raw*)(at + fresh(row + off[0]));
             }
         }
-        __device__ __forceinline__ void fill(const raw (&x)[N]) {
-            if constexpr (ES == 4) each<N>([&](auto i) { w[i] = __builtin_bit_cast(uint32_t, x[i]); });
-            else
-                each<WORDS>([&](auto i) {
-                    w[i] = (uint16_t)__builtin_bit_cast(uint16_t, (uint16_t)x[2 * i]);
-                    if constexpr (2 * i + 1 < N) w[i] |= (uint32_t)x[2 * i + 1] << 16;
-                });
-        }
     };
-    using Raw4 = Pack<4>;
+    using RawC = Pack<VC>;
     using RawS = Pack<S>;
+    struct __attribute__((aligned(4 * VC))) FloatC {
+        float v[VC];
+    };
 
     // The lane's constants.
     struct Lane {
         bool pad[S];
         float a2[S];               // A log2(e)
-        float bias[4], skip[4];
-        uint32_t off4[4];          // the four channels' offsets in a row, bytes
+        float bias[VC], skip[VC];
+        uint32_t offc[VC];         // the channels' offsets in a row, bytes
         uint32_t offs[S];          // the states' offsets in a row of B and C, bytes
     };
     static __device__ __forceinline__ Lane lane(const fg_scan_kargs& g, const Place& p) {
         Lane l;
         each<S>([&](auto s) {
-            const uint32_t n = p.q * S + s, m = n < g.states ? n : g.states - 1;
+            const uint32_t n = p.row * S + s, m = n < g.states ? n : g.states - 1;
             l.pad[s] = PAD && n >= g.states;
             l.a2[s] = n < g.states ? g.a[(uint64_t)p.ch * g.states + n] * kLog2e : 0.0f;
             l.offs[s] = (p.group * g.states + m) * ES;
         });
-        each<4>([&](auto i) {
-            // a channel that is not there: the group's last one (wide loads: its last four)
-            uint32_t c = p.ch4 + i;
-            if (c >= g.group_channels) c = p.have > 0 || !g.wide ? g.group_channels - 1 : g.group_channels - 4 + i;
+        each<VC>([&](auto i) {
+            // a channel that is not there: the group's last one (wide loads: its last ones)
+            uint32_t c = p.in_group + i;
+            if (c >= g.group_channels) c = WIDE ? g.group_channels - VC + i : g.group_channels - 1;
             c += p.group * g.group_channels;
-            l.off4[i] = c * ES;
+            l.offc[i] = c * ES;
             l.bias[i] = g.bias ? g.bias[c] : 0.0f;
             l.skip[i] = g.skip ? g.skip[c] : 0.0f;
         });
@@ -247,83 +252,129 @@ struct Scan {
     static __device__ __forceinline__ uint32_t row_of(uint32_t r, uint32_t n) {
         return TAIL && r >= n ? n - 1 : r;
     }
-    template <bool TAIL>
-    static __device__ __forceinline__ void load4(Raw4& v, const Cursor& w, const Place& p, const Lane& l, bool wide,
-                                                 uint32_t n) {
-        const uint32_t r = row_of<TAIL>(p.tok, n) * w.row;
-        if (wide) {
-            v.load(w.at + fresh(r + l.off4[0]));
-        } else {
-            raw x[4];
-            each<4>([&](auto i) { x[i] = *(const raw*)(w.at + fresh(r + l.off4[i])); });
-            v.fill(x);
-        }
+    template <bool TAIL, int N>
+    static __device__ __forceinline__ void load(Pack<N>& v, const Cursor& w, uint32_t row, const uint32_t (&off)[N],
+                                                uint32_t n) {
+        v.load(w.at, row_of<TAIL>(row, n) * w.row, off);
     }
     template <bool TAIL>
-    static __device__ __forceinline__ void store4(const Cursor& w, const Place& p, const Lane& l, bool wide, uint32_t n,
-                                                  const float (&x)[4]) {
+    static __device__ __forceinline__ void store(const Cursor& w, const Place& p, const Lane& l, uint32_t n,
+                                                 const float (&x)[VC]) {
         if (TAIL && p.tok >= n) return;
         const uint32_t r = p.tok * w.row;
         char* to = const_cast<char*>(w.at);
-        if (wide) {
-            struct __attribute__((aligned(4 * ES))) Out {
-                raw v[4];
+        if constexpr (WIDE) {
+            struct __attribute__((aligned(VC * ES))) Out {
+                raw v[VC];
             } v;
-            each<4>([&](auto i) { v.v[i] = T::down(x[i]); });
-            if (p.have > 0) *(Out*)(to + fresh(r + l.off4[0])) = v;
+            each<VC>([&](auto i) { v.v[i] = T::down(x[i]); });
+            if (p.have > 0) *(Out*)(to + fresh(r + l.offc[0])) = v;
         } else {
-            each<4>([&](auto i) {
-                if (i < p.have) *(raw*)(to + fresh(r + l.off4[i])) = T::down(x[i]);
+            each<VC>([&](auto i) {
+                if (i < p.have) *(raw*)(to + fresh(r + l.offc[i])) = T::down(x[i]);
             });
         }
     }
-    // B's or C's rows: lane (q, c) has token c's states of row q.
-    template <bool TAIL>
-    static __device__ __forceinline__ void load_states(RawS& v, const Cursor& w, const Place& p, const Lane& l,
-                                                       bool wide, uint32_t n) {
-        const uint32_t r = row_of<TAIL>(p.c, n) * w.row;
-        if (wide) {
-            v.load(w.at + fresh(r + l.offs[0]));
-        } else {
-            raw x[S];
-            each<S>([&](auto s) { x[s] = *(const raw*)(w.at + fresh(r + l.offs[s])); });
-            v.fill(x);
-        }
+    static __device__ __forceinline__ void up(float (&x)[VC], const RawC& v) {
+        each<VC>([&](auto i) { x[i] = v.up(i); });
     }
-    static __device__ __forceinline__ void up4(float (&x)[4], const Raw4& v) {
-        each<4>([&](auto i) { x[i] = v.up(i); });
-    }
-    static __device__ __forceinline__ void up_states(float (&x)[S], const RawS& v, const Lane& l) {
+    static __device__ __forceinline__ void up(float (&x)[S], const RawS& v, const Lane& l) {
         each<S>([&](auto s) { x[s] = PAD && l.pad[s] ? 0.0f : v.up(s); });
     }
 
-    // States at the start of the segment at token t: place of the wave's 64 S.
+    // Places of the wave's 64 S values: the states at the start of the segment
+    // at token t, and what chunk k adds (place `chunks`: the initial states).
+    static __device__ __forceinline__ uint64_t lanes_of(const fg_scan_kargs& g, const Place& p, uint64_t k) {
+        return ((k * (g.groups * g.group_blocks * BLOCKS) + p.sets) * W + p.part) * (64 * S) + (threadIdx.x & 63) * S;
+    }
     static __device__ __forceinline__ float* check_of(const fg_scan_kargs& g, const Place& p, uint32_t t) {
         const uint64_t seg = g.offsets ? (uint64_t)p.start / SEG + p.seq : (uint64_t)p.seq * g.check_segs;
-        return g.check + ((seg + t / SEG) * (g.groups * g.group_blocks * FG_SSM_WAVES) + p.wblock) * (64 * S) +
-               (threadIdx.x & 63) * S;
+        return g.check + lanes_of(g, p, seg + t / SEG);
     }
-    static __device__ __forceinline__ uint64_t carry_at(const fg_scan_kargs& g, const Place& p, uint32_t chunk) {
-        return (((uint64_t)p.seq * (g.chunks + 1) + chunk) * (g.groups * g.group_blocks * FG_SSM_WAVES) + p.wblock);
-    }
-    // The lane's states there; place `chunks` holds the initial states.
     static __device__ __forceinline__ float* carry_of(const fg_scan_kargs& g, const Place& p, uint32_t chunk) {
-        return g.carry + carry_at(g, p, chunk) * (64 * S) + (threadIdx.x & 63) * S;
+        return g.carry + lanes_of(g, p, (uint64_t)p.seq * (g.chunks + 1) + chunk);
+    }
+    // The 16 channels' summed time steps of chunk k.
+    static __device__ __forceinline__ float* carry_dt_of(const fg_scan_kargs& g, const Place& p, uint32_t chunk) {
+        const uint64_t k = (uint64_t)p.seq * (g.chunks + 1) + chunk;
+        return g.carry_dt + (k * (g.groups * g.group_blocks * BLOCKS) + p.sets) * 16;
     }
     static __device__ __forceinline__ uint64_t state_at(const fg_scan_kargs& g, const Place& p, int s) {
-        return ((uint64_t)p.seq * g.channels + p.ch) * g.states + p.q * S + s;
+        return ((uint64_t)p.seq * g.channels + p.ch) * g.states + p.row * S + s;
     }
     static __device__ __forceinline__ bool has_state(const fg_scan_kargs& g, const Place& p, int s) {
-        return !PAD || p.q * S + s < g.states;
+        return !PAD || p.row * S + s < g.states;
     }
-    // Orders the wave's own LDS accesses.
-    static __device__ __forceinline__ void wave_sync() {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+
+    // Takes the states h over n chunks, the i-th of them chunk at(i): four are
+    // loaded at a time.
+    template <class At>
+    static __device__ __forceinline__ void take_chunks(const fg_scan_kargs& g, const Place& p, const Lane& l,
+                                                       float (&h)[S], uint32_t n, At&& at) {
+        for (uint32_t k = 0; k < n; k += 4) {
+            float sum[4], add[4][S];
+            each<4>([&](auto j) {
+                const uint32_t i = at(k + j < n ? k + j : n - 1);
+                sum[j] = carry_dt_of(g, p, i)[p.c];
+                each<S>([&](auto s) { add[j][s] = carry_of(g, p, i)[s]; });
+            });
+            each<4>([&](auto j) {
+                if (k + j < n)
+                    each<S>([&](auto s) {
+                        h[s] = fmaf(exp2_(sum[j] * l.a2[s]), h[s], add[j][s]);
+                        if (PAD && l.pad[s]) h[s] = 0.0f;
+                    });
+            });
+        }
     }
-    // Sum over the segment's tokens of what lane (token, four channels) holds; all lanes get it.
-    static __device__ __forceinline__ float tokens_sum(float v) {
-        for (int m = 4; m < 64; m *= 2) v += __shfl_xor(v, m);
+
+    // Orders LDS accesses of the waves that share channels: the wave's own
+    // (W = 1), or the workgroup's.  Global loads on their way stay on it.
+    template <bool GROUP>
+    static __device__ __forceinline__ void sync() {
+        if constexpr (GROUP) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+    // Sums over the states of each (token, channel): 2 W parts, each the sum of
+    // two rows of a wave.
+    static constexpr int PART = SEG * 16 + 16;  // the 16 keep a wave's rows on banks of their own
+    struct Sums {
+        float v[2 * W][PART];
+        // v[j]: the lane's sum for token 4 i + j
+        __device__ __forceinline__ void put(const Place& p, int i, const float (&x)[4]) {
+            float* to = v[2 * p.part + (p.q & 1)] + (4 * i + (p.q & 2)) * 16 + p.c;
+            to[0] = swap32_add(x[0], x[2]);
+            to[16] = swap32_add(x[1], x[3]);
+        }
+        __device__ __forceinline__ void get(const Place& p, float (&x)[VC]) const {
+            FloatC f = *(const FloatC*)(v[0] + p.tok * 16 + p.sub);
+            each<VC>([&](auto i) { x[i] = f.v[i]; });
+            each<2 * W - 1>([&](auto k) {
+                f = *(const FloatC*)(v[k + 1] + p.tok * 16 + p.sub);
+                each<VC>([&](auto i) { x[i] += f.v[i]; });
+            });
+        }
+    };
+    // Sum over a segment's tokens of what each (token, channels) lane holds, to
+    // the lanes of the first token; `room`: LDS, 16 floats for each wave.
+    static __device__ __forceinline__ float tokens_sum(const Place& p, float v, float* room) {
+        for (int m = 16 / VC; m < 64; m *= 2) v += __shfl_xor(v, m);
+        if constexpr (W > 1) {
+            const uint32_t lane = threadIdx.x & 63;
+            sync<true>();
+            if (lane < 16 / VC) room[p.part * 16 + lane] = v;
+            sync<true>();
+            v = 0.0f;
+            each<W>([&](auto w) { v += room[w * 16 + lane % (16 / VC)]; });
+            sync<true>();
+        }
         return v;
     }
 
@@ -335,68 +386,99 @@ struct Scan {
 
     // ------------------------------------------------------------ forward
 
-    // LDS of a wave: per channel the tokens' (dt, dt u), twice (a segment is
-    // made ready while the one before it is worked through); the outputs.
+    // LDS of 16 channels, twice, so that one barrier a segment does: a segment
+    // is made ready, and the one before it stored, while one is worked through.
     static constexpr int XSTRIDE = 2 * SEG + 4;  // keeps the 16 channels on banks of their own
+    template <bool LOCAL>
     struct ForwardLds {
-        float x[2][16 * XSTRIDE];
-        float y[SEG * 16];
+        float x[2][16 * XSTRIDE];  // per channel the tokens' (dt, dt u)
+        std::conditional_t<LOCAL, float, Sums> y[2];
     };
+
+    // Segments whose rows are in registers or on the way: what a lane loads is
+    // small, and memory answers after one to two microseconds.
+    static constexpr int RING = ES == 2 ? 4 : 3;
 
     // A segment's time steps, to LDS.
     template <bool LOCAL, bool TAIL>
     static __device__ __forceinline__ void prepare(const fg_scan_kargs& g, const Place& p, const Lane& l, float* x,
-                                                   float (&sum_dt)[4], const float (&d)[4], const float (&u)[4],
+                                                   float (&sum_dt)[VC], const float (&d)[VC], const float (&u)[VC],
                                                    uint32_t n, bool count) {
-        each<4>([&](auto i) {
+        each<VC>([&](auto i) {
             const float dt = time_step(g, d[i] + l.bias[i]).value;
             const float2 e = {dt, dt * u[i]};
-            *(float2*)(x + (4 * (threadIdx.x & 3) + i) * XSTRIDE + 2 * p.tok) = e;
+            *(float2*)(x + (p.sub + i) * XSTRIDE + 2 * p.tok) = e;
             if constexpr (LOCAL) sum_dt[i] += count && (!TAIL || p.tok < n) ? dt : 0.0f;
         });
     }
-    template <bool LOCAL, bool TAIL>
-    static __device__ __forceinline__ void forward_segment(const Place& p, const Lane& l, const float* x, float* y,
-                                                           float (&h)[S], const float (&b)[S], const float (&c)[S],
-                                                           uint32_t n) {
-        x += p.c * XSTRIDE;
+    template <int J>
+    static __device__ __forceinline__ void advance(const Lane& l, float (&h)[S], const float (&b)[S], float dt,
+                                                   float dtu) {
+        each<S>([&](auto s) {
+            h[s] = fmaf(exp2_(dt * l.a2[s]), h[s], row_bcast<J>(b[s]) * dtu);
+            if (PAD && l.pad[s]) h[s] = 0.0f;
+        });
+    }
+    // Four tokens' (dt, dt u), read before what is worked through ahead of
+    // them: the compiler moves no LDS read above a write.
+    struct Steps {
+        float4 a, b;
+        __device__ __forceinline__ void read(const Place& p, const float* x, int i) {
+            a = *(const float4*)(x + p.c * XSTRIDE + 8 * i);
+            b = *(const float4*)(x + p.c * XSTRIDE + 8 * i + 4);
+        }
+    };
+    template <bool LOCAL, bool TAIL, class Y>
+    static __device__ __forceinline__ void forward_segment(const Place& p, const Lane& l, const float* x, Steps next,
+                                                           Y& y, float (&h)[S], const float (&b)[S],
+                                                           const float (&c)[S], uint32_t n) {
         each<SEG / 4>([&](auto i) {
-            float e[8], ys[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            *(float4*)e = *(const float4*)(x + 8 * i);
-            *(float4*)(e + 4) = *(const float4*)(x + 8 * i + 4);
-            each<4>([&](auto j) {
-                if (!TAIL || 4 * i + j < n) {
-                    each<S>([&](auto s) {
-                        h[s] = fmaf(exp2_(e[2 * j] * l.a2[s]), h[s], row_bcast<4 * i + j>(b[s]) * e[2 * j + 1]);
-                        if (PAD && l.pad[s]) h[s] = 0.0f;
-                    });
-                    if constexpr (!LOCAL) bcast_dot<S, 4 * i + j>(ys[j], c, h);
+            const float e[8] = {next.a.x, next.a.y, next.a.z, next.a.w, next.b.x, next.b.y, next.b.z, next.b.w};
+            float ys[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (i + 1 < SEG / 4) next.read(p, x, i + 1);
+            each<2>([&](auto k) {
+                constexpr int j = 2 * k, m = 4 * i + j;
+                if constexpr (TAIL) {
+                    if (m < n) {
+                        advance<m>(l, h, b, e[2 * j], e[2 * j + 1]);
+                        if constexpr (!LOCAL) bcast_dot<S, m>(ys[j], c, h);
+                    }
+                    if (m + 1 < n) {
+                        advance<m + 1>(l, h, b, e[2 * j + 2], e[2 * j + 3]);
+                        if constexpr (!LOCAL) bcast_dot<S, m + 1>(ys[j + 1], c, h);
+                    }
+                } else {
+                    float first[S];
+                    advance<m>(l, h, b, e[2 * j], e[2 * j + 1]);
+                    each<S>([&](auto s) { first[s] = h[s]; });
+                    advance<m + 1>(l, h, b, e[2 * j + 2], e[2 * j + 3]);
+                    if constexpr (!LOCAL) bcast_dots<S, m, m + 1>(ys[j], ys[j + 1], c, first, h);
                 }
             });
-            if constexpr (!LOCAL) y[(4 * i + p.q) * 16 + p.c] = rows_sum(ys);
+            if constexpr (!LOCAL) y.put(p, i, ys);
         });
     }
     template <bool TAIL>
     static __device__ __forceinline__ void outputs(const fg_scan_kargs& g, const Place& p, const Lane& l,
-                                                   const float* y, const Cursor& out, const Raw4& ru, const Raw4& rz,
+                                                   const Sums& y, const Cursor& out, const RawC& ru, const RawC& rz,
                                                    bool gated, uint32_t n) {
-        float u[4], z[4], o[4];
-        up4(u, ru);
-        up4(z, rz);
-        const float4 v = *(const float4*)(y + p.tok * 16 + 4 * (threadIdx.x & 3));
-        const float ys[4] = {v.x, v.y, v.z, v.w};
-        each<4>([&](auto i) {
+        float u[VC], z[VC], o[VC];
+        up(u, ru);
+        up(z, rz);
+        y.get(p, o);
+        each<VC>([&](auto i) {
             const float gate = z[i] * sigmoid(z[i]);
-            o[i] = fmaf(l.skip[i], u[i], ys[i]) * (gated ? gate : 1.0f);
+            o[i] = fmaf(l.skip[i], u[i], o[i]) * (gated ? gate : 1.0f);
         });
-        store4<TAIL>(out, p, l, g.wide, n, o);
+        store<TAIL>(out, p, l, n, o);
     }
 
     // LOCAL: the states that the chunk's own tokens leave, from none, and the
     // sum of its time steps; else outputs, from the states before the chunk.
     template <bool LOCAL>
     static __device__ __forceinline__ void forward(const fg_scan_kargs& g) {
-        __shared__ __attribute__((aligned(16))) ForwardLds lds[FG_SSM_WAVES];
+        __shared__ __attribute__((aligned(16))) ForwardLds<LOCAL> all[BLOCKS];
+        constexpr bool SHARED = W > 1;
         const Place p = place(g);
         if (LOCAL && p.chunk == 0) {
             // the last chunks may write the final states where the initial ones lie
@@ -408,38 +490,57 @@ struct Scan {
         if (LOCAL && p.t1 == p.len) return;                 // no chunk follows
         if (!LOCAL && p.chunk > 0 && p.t0 == p.t1) return;  // no tokens
         const Lane l = lane(g, p);
-        float(&x)[2][16 * XSTRIDE] = lds[p.wave].x;
-        float* y = lds[p.wave].y;
-        float h[S], sum_dt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        ForwardLds<LOCAL>& lds = all[p.set];
+        float h[S], sum_dt[VC];
+        each<VC>([&](auto i) { sum_dt[i] = 0.0f; });
         each<S>([&](auto s) { h[s] = 0.0f; });
         if constexpr (!LOCAL) {
             each<S>([&](auto s) {
                 if (g.chunks > 1) h[s] = carry_of(g, p, g.chunks)[s];
                 else if (g.initial && has_state(g, p, s)) h[s] = g.initial[state_at(g, p, s)];
             });
-            for (uint32_t k = 0; k < p.chunk; ++k) {
-                const float sum = g.carry_dt[carry_at(g, p, k) * 16 + p.c];
-                each<S>([&](auto s) {
-                    h[s] = fmaf(exp2_(sum * l.a2[s]), h[s], carry_of(g, p, k)[s]);
-                    if (PAD && l.pad[s]) h[s] = 0.0f;
-                });
-            }
+            take_chunks(g, p, l, h, p.chunk, [](uint32_t i) { return i; });
         }
         // Without a gate u's rows stand in for z's, which are then not used.
         const bool gated = g.z.p != nullptr;
-        Cursor cu, cd, cz, cu2, cb, cc, co;
-        cu.set(g.u, p, p.t0);
-        cd.set(g.delta, p, p.t0);
-        cb.set(g.b, p, p.t0);
-        if constexpr (!LOCAL) {
-            cc.set(g.c, p, p.t0);
-            cz.set(gated ? g.z : g.u, p, p.t0);
-            cu2.set(g.u, p, p.t0);
-            co.set(g.out, p, p.t0);
-        }
-        Raw4 rd, ru, rz, ru2;
-        RawS rb, rc;
-        float d[4], u[4], b[S], c[S];
+        struct {
+            Cursor u, d, z, b, c;
+        } at;
+        Cursor out;
+        auto set = [&](uint32_t t) {
+            at.u.set(g.u, p, t);
+            at.d.set(g.delta, p, t);
+            at.b.set(g.b, p, t);
+            if constexpr (!LOCAL) {
+                at.c.set(g.c, p, t);
+                at.z.set(gated ? g.z : g.u, p, t);
+                out.set(g.out, p, t);
+            }
+        };
+        struct Rows {
+            RawC u, d, z;
+            RawS b, c;
+        } ring[RING];
+        auto fetch = [&](Rows& r, auto tail, uint32_t n) {
+            constexpr bool TAIL = decltype(tail)::value;
+            load<TAIL>(r.d, at.d, p.tok, l.offc, n);
+            load<TAIL>(r.u, at.u, p.tok, l.offc, n);
+            load<TAIL>(r.b, at.b, p.c, l.offs, n);
+            if constexpr (!LOCAL) {
+                load<TAIL>(r.c, at.c, p.c, l.offs, n);
+                load<TAIL>(r.z, at.z, p.tok, l.offc, n);
+            }
+        };
+        auto forth = [&](int by) {
+            at.u.move(by);
+            at.d.move(by);
+            at.b.move(by);
+            if constexpr (!LOCAL) {
+                at.c.move(by);
+                at.z.move(by);
+            }
+        };
+        float d[VC], u[VC], b[S], c[S];
         auto checkpoint = [&](uint32_t t) {
             if constexpr (!LOCAL) {
                 if (g.check) {  // lanes without a channel too: the backward pass reads them
@@ -449,92 +550,67 @@ struct Scan {
             }
         };
         const uint32_t full = (p.t1 - p.t0) / SEG, rest = (p.t1 - p.t0) % SEG;
+        set(p.t0);
         if (full > 0) {
             // While segment k is worked through, k + 1 is made ready, the rows
-            // of k + 2 are loaded (at the end some once more, to no use), and
-            // the outputs of k - 1 are stored.
-            load4<false>(rd, cd, p, l, g.wide, SEG);
-            load4<false>(ru, cu, p, l, g.wide, SEG);
-            load_states<false>(rb, cb, p, l, g.wide, SEG);
-            if constexpr (!LOCAL) load_states<false>(rc, cc, p, l, g.wide, SEG);
-            up4(d, rd);
-            up4(u, ru);
-            cd.move(full > 1);
-            cu.move(full > 1);
-            load4<false>(rd, cd, p, l, g.wide, SEG);
-            load4<false>(ru, cu, p, l, g.wide, SEG);
-            prepare<LOCAL, false>(g, p, l, x[0], sum_dt, d, u, SEG, true);
-            for (uint32_t k = 0; k < full; ++k) {
-                up_states(b, rb, l);
-                up4(d, rd);
-                up4(u, ru);
-                cd.move(k + 2 < full);
-                cu.move(k + 2 < full);
-                cb.move(k + 1 < full);
-                if constexpr (!LOCAL) {
-                    up_states(c, rc, l);
-                    cc.move(k + 1 < full);
-                    if (k > 0) {
-                        outputs<false>(g, p, l, y, co, ru2, rz, gated, SEG);
-                        co.move(1);
-                    }
-                }
-                // one branch around all: loads of several branches would wait for each other
-                auto loads = [&](bool wide) {
-                    load4<false>(rd, cd, p, l, wide, SEG);
-                    load4<false>(ru, cu, p, l, wide, SEG);
-                    load_states<false>(rb, cb, p, l, wide, SEG);
+            // of k + RING - 1 are loaded (beyond the last the last, to no
+            // use), and the outputs of k - 1 are stored.
+            each<RING - 1>([&](auto j) {
+                fetch(ring[j], std::false_type{}, SEG);
+                forth(j + 1 < full);
+            });
+            up(d, ring[0].d);
+            up(u, ring[0].u);
+            prepare<LOCAL, false>(g, p, l, lds.x[0], sum_dt, d, u, SEG, true);
+            for (uint32_t k = 0; k <= full; k += RING) {
+                each<RING>([&](auto j) {
+                    const uint32_t m = k + j;
+                    if (m > full) return;
+                    Rows& last = ring[(j + RING - 1) % RING];
+                    sync<SHARED>();
                     if constexpr (!LOCAL) {
-                        load_states<false>(rc, cc, p, l, wide, SEG);
-                        load4<false>(rz, cz, p, l, wide, SEG);
-                        load4<false>(ru2, cu2, p, l, wide, SEG);
+                        if (m > 0) {
+                            outputs<false>(g, p, l, lds.y[(m - 1) & 1], out, last.u, last.z, gated, SEG);
+                            out.move(1);
+                        }
                     }
-                };
-                if (g.wide) loads(true);
-                else loads(false);
-                if constexpr (!LOCAL) {
-                    cz.move(1);
-                    cu2.move(1);
-                }
-                checkpoint(p.t0 + k * SEG);
-                wave_sync();
-                prepare<LOCAL, false>(g, p, l, x[(k + 1) & 1], sum_dt, d, u, SEG, k + 1 < full);
-                forward_segment<LOCAL, false>(p, l, x[k & 1], y, h, b, c, SEG);
-                wave_sync();
+                    if (m == full) return;
+                    fetch(last, std::false_type{}, SEG);
+                    forth(m + RING < full);
+                    up(b, ring[j].b, l);
+                    if constexpr (!LOCAL) up(c, ring[j].c, l);
+                    up(d, ring[(j + 1) % RING].d);
+                    up(u, ring[(j + 1) % RING].u);
+                    checkpoint(p.t0 + m * SEG);
+                    Steps first;
+                    first.read(p, lds.x[m & 1], 0);
+                    prepare<LOCAL, false>(g, p, l, lds.x[(m + 1) & 1], sum_dt, d, u, SEG, m + 1 < full);
+                    forward_segment<LOCAL, false>(p, l, lds.x[m & 1], first, lds.y[m & 1], h, b, c, SEG);
+                });
             }
-            if constexpr (!LOCAL) {
-                outputs<false>(g, p, l, y, co, ru2, rz, gated, SEG);
-                co.move(1);
-                cc.move(1);
-            }
-            cd.move(1);
-            cu.move(1);
-            cb.move(1);
-            wave_sync();
+            sync<SHARED>();
         }
         if (rest > 0) {
+            Rows& r = ring[0];
+            set(p.t0 + full * SEG);
             checkpoint(p.t0 + full * SEG);
-            load4<true>(rd, cd, p, l, g.wide, rest);
-            load4<true>(ru, cu, p, l, g.wide, rest);
-            load_states<true>(rb, cb, p, l, g.wide, rest);
-            if constexpr (!LOCAL) {
-                load_states<true>(rc, cc, p, l, g.wide, rest);
-                load4<true>(rz, cz, p, l, g.wide, rest);
-                up_states(c, rc, l);
-            }
-            up4(d, rd);
-            up4(u, ru);
-            up_states(b, rb, l);
-            prepare<LOCAL, true>(g, p, l, x[0], sum_dt, d, u, rest, true);
-            wave_sync();
-            forward_segment<LOCAL, true>(p, l, x[0], y, h, b, c, rest);
-            wave_sync();
-            if constexpr (!LOCAL) outputs<true>(g, p, l, y, co, ru, rz, gated, rest);
+            fetch(r, std::true_type{}, rest);
+            if constexpr (!LOCAL) up(c, r.c, l);
+            up(d, r.d);
+            up(u, r.u);
+            up(b, r.b, l);
+            prepare<LOCAL, true>(g, p, l, lds.x[0], sum_dt, d, u, rest, true);
+            sync<SHARED>();
+            Steps first;
+            first.read(p, lds.x[0], 0);
+            forward_segment<LOCAL, true>(p, l, lds.x[0], first, lds.y[0], h, b, c, rest);
+            sync<SHARED>();
+            if constexpr (!LOCAL) outputs<true>(g, p, l, lds.y[0], out, r.u, r.z, gated, rest);
         }
         if constexpr (LOCAL) {
-            each<4>([&](auto i) {
-                const float sum = tokens_sum(sum_dt[i]);
-                if (p.tok == 0) g.carry_dt[carry_at(g, p, p.chunk) * 16 + 4 * (threadIdx.x & 3) + i] = sum;
+            each<VC>([&](auto i) {
+                const float sum = tokens_sum(p, sum_dt[i], lds.x[0]);
+                if (p.tok == 0) carry_dt_of(g, p, p.chunk)[p.sub + i] = sum;
             });
             each<S>([&](auto s) { carry_of(g, p, p.chunk)[s] = h[s]; });
         } else if (g.final && p.valid && p.t1 == p.len) {
@@ -546,46 +622,52 @@ struct Scan {
 
     // ----------------------------------------------------------- backward
 
-    // LDS of a wave: per channel the tokens' time steps dt, gradients ds of the
-    // ungated outputs, and inputs dt u; per token and channel the sums over
-    // states (y, g B, g a h A); B's and C's gradients summed over the channels.
+    // LDS of 16 channels: per channel the tokens' time steps dt, gradients ds
+    // of the ungated outputs, and inputs dt u; the sums over states (y, g B,
+    // g a h A); what the (token, channels) lanes keep until the end of the
+    // segment; B's and C's gradients summed over the 16 channels.
     static constexpr int TSTRIDE = SEG + 4;
     struct BackwardLds {
         float dt[16 * TSTRIDE], ds[16 * TSTRIDE], dtu[16 * TSTRIDE];
-        float res[3][SEG * 16];
-        float4 keep[5][64];  // u, dt, its slope, ds, z's factor of each lane (token, four channels)
-        float sums[SEG * 2 * 4 * S];
+        Sums res[3];
+        FloatC keep[5][64 * W];  // u, dt, its slope, ds, z's factor
+        float bc[SEG * 2 * 4 * S * W];
     };
     struct LocalLds {
         float dt[16 * TSTRIDE], ds[16 * TSTRIDE];
     };
-
     template <bool LOCAL>
     struct BackRaws {
-        Raw4 u, d, dy, z;
+        RawC u, d, dy, z;
         RawS b, c;
         float h0[S];
     };
     template <bool LOCAL>
     struct BackCursors {
         Cursor u, d, dy, z, b, c;
+        __device__ __forceinline__ void move(int by) {
+            d.move(by);
+            dy.move(by);
+            z.move(by);
+            c.move(by);
+            if constexpr (!LOCAL) {
+                u.move(by);
+                b.move(by);
+            }
+        }
     };
     template <bool LOCAL, bool TAIL>
     static __device__ __forceinline__ void back_load(BackRaws<LOCAL>& r, const BackCursors<LOCAL>& at,
                                                      const fg_scan_kargs& g, const Place& p, const Lane& l, uint32_t t,
                                                      uint32_t n) {
-        auto loads = [&](bool wide) {
-            load4<TAIL>(r.d, at.d, p, l, wide, n);
-            load4<TAIL>(r.dy, at.dy, p, l, wide, n);
-            load4<TAIL>(r.z, at.z, p, l, wide, n);
-            load_states<TAIL>(r.c, at.c, p, l, wide, n);
-            if constexpr (!LOCAL) {
-                load4<TAIL>(r.u, at.u, p, l, wide, n);
-                load_states<TAIL>(r.b, at.b, p, l, wide, n);
-            }
-        };
-        if (g.wide) loads(true);
-        else loads(false);
+        load<TAIL>(r.d, at.d, p.tok, l.offc, n);
+        load<TAIL>(r.dy, at.dy, p.tok, l.offc, n);
+        load<TAIL>(r.z, at.z, p.tok, l.offc, n);
+        load<TAIL>(r.c, at.c, p.c, l.offs, n);
+        if constexpr (!LOCAL) {
+            load<TAIL>(r.u, at.u, p.tok, l.offc, n);
+            load<TAIL>(r.b, at.b, p.c, l.offs, n);
+        }
         if constexpr (!LOCAL) {
             const float* from = check_of(g, p, t);
             each<S>([&](auto s) { r.h0[s] = from[s]; });
@@ -594,35 +676,34 @@ struct Scan {
     // Time steps and output gradients, to LDS, with what the end of the segment needs.
     template <bool LOCAL, class L>
     static __device__ __forceinline__ void back_prepare(const BackRaws<LOCAL>& r, const fg_scan_kargs& g,
-                                                        const Place& p, const Lane& l, L& lds, float (&dt)[4],
+                                                        const Place& p, const Lane& l, L& lds, float (&dt)[VC],
                                                         bool gated) {
-        float d[4], dy[4], z[4], u[4], slope[4], ds[4], zs[4];
-        up4(d, r.d);
-        up4(dy, r.dy);
-        up4(z, r.z);
-        if constexpr (!LOCAL) up4(u, r.u);
-        each<4>([&](auto i) {
+        float d[VC], dy[VC], z[VC], u[VC];
+        FloatC k[5];
+        up(d, r.d);
+        up(dy, r.dy);
+        up(z, r.z);
+        if constexpr (!LOCAL) up(u, r.u);
+        each<VC>([&](auto i) {
             const Softplus s = time_step(g, d[i] + l.bias[i]);
             dt[i] = s.value;
-            slope[i] = s.slope;
             const float sg = sigmoid(z[i]);
-            ds[i] = gated ? dy[i] * (z[i] * sg) : dy[i];
-            zs[i] = dy[i] * (sg * fmaf(z[i], 1.0f - sg, 1.0f));
+            const float ds = gated ? dy[i] * (z[i] * sg) : dy[i];
             // a channel that is not there adds nothing to the sums over channels
             const bool here = i < p.have;
-            const uint32_t at = (4 * (threadIdx.x & 3) + i) * TSTRIDE + p.tok;
+            const uint32_t at = (p.sub + i) * TSTRIDE + p.tok;
             lds.dt[at] = dt[i];
-            lds.ds[at] = here ? ds[i] : 0.0f;
-            if constexpr (!LOCAL) lds.dtu[at] = here ? dt[i] * u[i] : 0.0f;
+            lds.ds[at] = here ? ds : 0.0f;
+            if constexpr (!LOCAL) {
+                lds.dtu[at] = here ? dt[i] * u[i] : 0.0f;
+                k[0].v[i] = u[i];
+                k[1].v[i] = dt[i];
+                k[2].v[i] = s.slope;
+                k[3].v[i] = ds;
+                k[4].v[i] = dy[i] * (sg * fmaf(z[i], 1.0f - sg, 1.0f));
+            }
         });
-        if constexpr (!LOCAL) {
-            const uint32_t lane = threadIdx.x & 63;
-            lds.keep[0][lane] = {u[0], u[1], u[2], u[3]};
-            lds.keep[1][lane] = {dt[0], dt[1], dt[2], dt[3]};
-            lds.keep[2][lane] = {slope[0], slope[1], slope[2], slope[3]};
-            lds.keep[3][lane] = {ds[0], ds[1], ds[2], ds[3]};
-            lds.keep[4][lane] = {zs[0], zs[1], zs[2], zs[3]};
-        }
+        if constexpr (!LOCAL) each<5>([&](auto i) { lds.keep[i][p.part * 64 + (threadIdx.x & 63)] = k[i]; });
     }
     template <bool TAIL>
     static __device__ __forceinline__ void back_local(const Place& p, const Lane& l, const LocalLds& lds,
@@ -644,77 +725,87 @@ struct Scan {
             });
         });
     }
-    // The gradients of one segment's tokens, SP states of the lane at a time.
-    // `midway` runs where half of the states are no longer needed: it loads
-    // the next segment's rows.
+    // The gradients of one segment's tokens.  `midway` runs where half of the
+    // states are no longer needed: it loads the next segment's rows.
     template <bool TAIL, class F>
     static __device__ __forceinline__ void back_segment(const Place& p, const Lane& l, BackwardLds& lds,
                                                         float (&carry)[S], float (&ga)[S], const float (&b)[S],
                                                         const float (&c)[S], const float (&h0)[S], uint32_t n,
                                                         F&& midway) {
-        each<PASSES>([&](auto pass) {
-            constexpr int P = pass * SP;
-            float a[SEG][SP], h[SEG][SP];
-            auto result = [&](int which, int i, float v) {
-                float* to = lds.res[which] + (4 * i + p.q) * 16 + p.c;
-                *to = P ? *to + v : v;
-            };
-            // the segment's states again
-            each<SEG / 4>([&](auto i) {
-                float dt[4], dtu[4], y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                *(float4*)dt = *(const float4*)(lds.dt + p.c * TSTRIDE + 4 * i);
-                *(float4*)dtu = *(const float4*)(lds.dtu + p.c * TSTRIDE + 4 * i);
-                each<4>([&](auto j) {
-                    constexpr int m = 4 * i + j;
-                    if (!TAIL || m < n) {
-                        each<SP>([&](auto s) {
-                            const float before = m ? h[m ? m - 1 : 0][s] : h0[P + s];
-                            a[m][s] = exp2_(dt[j] * l.a2[P + s]);
-                            h[m][s] = fmaf(a[m][s], before, row_bcast<m>(b[P + s]) * dtu[j]);
-                            if (PAD && l.pad[P + s]) h[m][s] = 0.0f;
-                        });
-                        bcast_dot<SP, m>(y[j], c + P, h[m]);
-                    }
-                });
-                result(0, i, rows_sum(y));
-            });
-            // and back
-            each<SEG / 4>([&](auto ri) {
-                constexpr int i = SEG / 4 - 1 - ri;
-                if constexpr (pass == PASSES - 1 && ri == SEG / 8) midway();
-                float dt[4], ds[4], dtu[4];
-                *(float4*)dt = *(const float4*)(lds.dt + p.c * TSTRIDE + 4 * i);
-                *(float4*)ds = *(const float4*)(lds.ds + p.c * TSTRIDE + 4 * i);
-                *(float4*)dtu = *(const float4*)(lds.dtu + p.c * TSTRIDE + 4 * i);
-                float gb[4 * SP], gc[4 * SP], gu[4] = {0.0f, 0.0f, 0.0f, 0.0f}, gd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (TAIL) each<4 * SP>([&](auto e) { gb[e] = gc[e] = 0.0f; });
-                each<4>([&](auto rj) {
-                    constexpr int j = 3 - rj, m = 4 * i + j;
-                    if (!TAIL || m < n) {
-                        bcast_fmac<SP, m>(carry + P, c + P, ds[j]);  // g_t
-                        bcast_dot<SP, m>(gu[j], b + P, carry + P);
-                        each<SP>([&](auto s) {
-                            gb[j * SP + s] = carry[P + s] * dtu[j];
-                            gc[j * SP + s] = ds[j] * h[m][s];
-                            carry[P + s] *= a[m][s];
-                            if (PAD && l.pad[P + s]) carry[P + s] = 0.0f;
-                            const float held = carry[P + s] * (m ? h[m ? m - 1 : 0][s] : h0[P + s]);
-                            gd[j] = fmaf(held, l.a2[P + s], gd[j]);
-                            ga[P + s] = fmaf(held, dt[j], ga[P + s]);
-                        });
-                    }
-                });
-                result(1, i, rows_sum(gu));
-                result(2, i, rows_sum(gd));
-                channels_sum<SP>(gb, p.c);
-                channels_sum<SP>(gc, p.c);
-                const uint32_t e = SP == 4 ? p.c : p.c >> (SP == 2 ? 1 : 2);
-                float* to = lds.sums + ((4 * i + e / SP) * 2) * (4 * S) + p.q * S + P + e % SP;
-                if (SP == 4 || (p.c & (SP == 2 ? 1 : 3)) == 0) {
-                    to[0] = gb[0];
-                    to[4 * S] = gc[0];
+        float a[SEG][S], h[SEG][S];
+        const float *xdt = lds.dt + p.c * TSTRIDE, *xds = lds.ds + p.c * TSTRIDE, *xdtu = lds.dtu + p.c * TSTRIDE;
+        // Four tokens' values, read ahead as in forward_segment.
+        struct Steps {
+            float4 dt, dtu, ds;
+        } next;
+        next.dt = *(const float4*)xdt;
+        next.dtu = *(const float4*)xdtu;
+        // the segment's states again
+        each<SEG / 4>([&](auto i) {
+            const float dt[4] = {next.dt.x, next.dt.y, next.dt.z, next.dt.w};
+            const float dtu[4] = {next.dtu.x, next.dtu.y, next.dtu.z, next.dtu.w};
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            constexpr int after = i + 1 < SEG / 4 ? i + 1 : SEG / 4 - 1;  // the last is where the way back begins
+            next.dt = *(const float4*)(xdt + 4 * after);
+            next.dtu = *(const float4*)(xdtu + 4 * after);
+            if constexpr (i + 1 == SEG / 4) next.ds = *(const float4*)(xds + 4 * after);
+            each<4>([&](auto j) {
+                constexpr int m = 4 * i + j;
+                if (!TAIL || m < n) {
+                    each<S>([&](auto s) {
+                        const float before = m ? h[m ? m - 1 : 0][s] : h0[s];
+                        a[m][s] = exp2_(dt[j] * l.a2[s]);
+                        h[m][s] = fmaf(a[m][s], before, row_bcast<m>(b[s]) * dtu[j]);
+                        if (PAD && l.pad[s]) h[m][s] = 0.0f;
+                    });
+                    if constexpr (TAIL) bcast_dot<S, m>(y[j], c, h[m]);
+                    else if constexpr (j % 2 == 1) bcast_dots<S, m - 1, m>(y[j - 1], y[j], c, h[m - 1], h[m]);
                 }
             });
+            lds.res[0].put(p, i, y);
+        });
+        // and back
+        each<SEG / 4>([&](auto ri) {
+            constexpr int i = SEG / 4 - 1 - ri;
+            if constexpr (ri == SEG / 8) midway();
+            const float dt[4] = {next.dt.x, next.dt.y, next.dt.z, next.dt.w};
+            const float dtu[4] = {next.dtu.x, next.dtu.y, next.dtu.z, next.dtu.w};
+            const float ds[4] = {next.ds.x, next.ds.y, next.ds.z, next.ds.w};
+            if constexpr (i > 0) {
+                next.dt = *(const float4*)(xdt + 4 * (i - 1));
+                next.dtu = *(const float4*)(xdtu + 4 * (i - 1));
+                next.ds = *(const float4*)(xds + 4 * (i - 1));
+            }
+            float gb[4 * S], gc[4 * S], gu[4] = {0.0f, 0.0f, 0.0f, 0.0f}, gd[4] = {0.0f, 0.0f, 0.0f, 0.0f}, later[S];
+            if constexpr (TAIL) each<4 * S>([&](auto e) { gb[e] = gc[e] = 0.0f; });
+            each<4>([&](auto rj) {
+                constexpr int j = 3 - rj, m = 4 * i + j;
+                if (!TAIL || m < n) {
+                    bcast_fmac<S, m>(carry, c, ds[j]);  // g_t
+                    if constexpr (TAIL) bcast_dot<S, m>(gu[j], b, carry);
+                    else if constexpr (j % 2 == 0) bcast_dots<S, m + 1, m>(gu[j + 1], gu[j], b, later, carry);
+                    else each<S>([&](auto s) { later[s] = carry[s]; });
+                    each<S>([&](auto s) {
+                        gb[j * S + s] = carry[s] * dtu[j];
+                        gc[j * S + s] = ds[j] * h[m][s];
+                        carry[s] *= a[m][s];
+                        if (PAD && l.pad[s]) carry[s] = 0.0f;
+                        const float held = carry[s] * (m ? h[m ? m - 1 : 0][s] : h0[s]);
+                        gd[j] = fmaf(held, l.a2[s], gd[j]);
+                        ga[s] = fmaf(held, dt[j], ga[s]);
+                    });
+                }
+            });
+            lds.res[1].put(p, i, gu);
+            lds.res[2].put(p, i, gd);
+            channels_sum<S>(gb, p.c);
+            channels_sum<S>(gc, p.c);
+            const uint32_t e = S == 4 ? p.c : p.c >> (S == 2 ? 1 : 2);
+            float* to = lds.bc + ((4 * i + e / S) * 2) * (4 * S * W) + p.row * S + e % S;
+            if (S == 4 || (p.c & (S == 2 ? 1 : 3)) == 0) {
+                to[0] = gb[0];
+                to[4 * S * W] = gc[0];
+            }
         });
     }
 
@@ -723,11 +814,12 @@ struct Scan {
     template <bool LOCAL>
     static __device__ __forceinline__ void backward(const fg_scan_kargs& g) {
         using Lds = std::conditional_t<LOCAL, LocalLds, BackwardLds>;
-        __shared__ __attribute__((aligned(16))) Lds all[FG_SSM_WAVES];
+        __shared__ __attribute__((aligned(16))) Lds all[BLOCKS];
+        constexpr bool SHARED = !LOCAL || W > 1;
         const Place p = place(g);
         if (LOCAL && (p.chunk == 0 || p.t1 == p.t0)) return;  // no chunk before it, or no tokens
         const Lane l = lane(g, p);
-        Lds& lds = all[p.wave];
+        Lds& lds = all[p.set];
         float carry[S], ga[S];
         each<S>([&](auto s) { carry[s] = ga[s] = 0.0f; });
         if constexpr (!LOCAL) {
@@ -735,17 +827,12 @@ struct Scan {
                 if (g.gfinal && has_state(g, p, s)) carry[s] = g.gfinal[state_at(g, p, s)];
             });
             const uint32_t used = p.len ? (p.len - 1) / g.chunk_len + 1 : 0;
-            for (uint32_t k = used; k-- > p.chunk + 1;) {
-                const float sum = g.carry_dt[carry_at(g, p, k) * 16 + p.c];
-                each<S>([&](auto s) {
-                    carry[s] = fmaf(exp2_(sum * l.a2[s]), carry[s], carry_of(g, p, k)[s]);
-                    if (PAD && l.pad[s]) carry[s] = 0.0f;
-                });
-            }
+            if (used > p.chunk + 1)
+                take_chunks(g, p, l, carry, used - p.chunk - 1, [&](uint32_t i) { return used - 1 - i; });
         }
         const bool gated = g.z.p != nullptr;
-        float sum_dt[4] = {0.0f, 0.0f, 0.0f, 0.0f}, gskip[4] = {0.0f, 0.0f, 0.0f, 0.0f},
-              gbias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float sum_dt[VC], gskip[VC], gbias[VC];
+        each<VC>([&](auto i) { sum_dt[i] = gskip[i] = gbias[i] = 0.0f; });
         const uint32_t full = (p.t1 - p.t0) / SEG, rest = (p.t1 - p.t0) % SEG;
         BackCursors<LOCAL> at;
         Cursor cgu, cgd, cgz;
@@ -761,78 +848,65 @@ struct Scan {
             cgd.set(g.gdelta, p, last);
             cgz.set(g.gz, p, last);
         }
-        auto move = [&](int by) {
-            at.d.move(by);
-            at.dy.move(by);
-            at.z.move(by);
-            at.c.move(by);
-            if constexpr (!LOCAL) {
-                at.u.move(by);
-                at.b.move(by);
-            }
-        };
         BackRaws<LOCAL> r;
         auto segment = [&](auto tail, uint32_t t, uint32_t n, bool more) {
             constexpr bool TAIL = decltype(tail)::value;
-            float b[S], c[S], h0[S], dt[4];
+            float b[S], c[S], h0[S], dt[VC];
             back_prepare<LOCAL>(r, g, p, l, lds, dt, gated);
-            up_states(c, r.c, l);
+            up(c, r.c, l);
             if constexpr (!LOCAL) {
-                up_states(b, r.b, l);
+                up(b, r.b, l);
                 each<S>([&](auto s) { h0[s] = r.h0[s]; });
             }
             auto midway = [&] {
                 if (more) {  // the segment before this one
-                    move(-1);
+                    at.move(-1);
                     back_load<LOCAL, false>(r, at, g, p, l, t - SEG, SEG);
                 }
             };
-            wave_sync();
+            sync<SHARED>();
             if constexpr (LOCAL) {
                 midway();
-                each<4>([&](auto i) { sum_dt[i] += !TAIL || p.tok < n ? dt[i] : 0.0f; });
+                each<VC>([&](auto i) { sum_dt[i] += !TAIL || p.tok < n ? dt[i] : 0.0f; });
                 back_local<TAIL>(p, l, lds, carry, c, n);
-                wave_sync();
+                sync<SHARED>();
             } else {
                 back_segment<TAIL>(p, l, lds, carry, ga, b, c, h0, n, midway);
-                wave_sync();
-                const uint32_t lane = threadIdx.x & 63;
-                const float* from = lds.res[0] + p.tok * 16 + 4 * (threadIdx.x & 3);
-                float y[4], gu[4], gd[4], o[4], u[4], ds[4], v[4];
-                *(float4*)u = lds.keep[0][lane];
-                *(float4*)ds = lds.keep[3][lane];
-                *(float4*)gu = *(const float4*)(from + SEG * 16);
+                sync<SHARED>();
+                const uint32_t lane = p.part * 64 + (threadIdx.x & 63);
+                float gu[VC], gd[VC], o[VC];
+                const FloatC u = lds.keep[0][lane], ds = lds.keep[3][lane];
+                lds.res[1].get(p, gu);
                 if (g.gz.p) {
-                    *(float4*)y = *(const float4*)from;
-                    *(float4*)v = lds.keep[4][lane];
-                    each<4>([&](auto i) { o[i] = v[i] * fmaf(l.skip[i], u[i], y[i]); });
-                    store4<TAIL>(cgz, p, l, g.wide, n, o);
+                    const FloatC v = lds.keep[4][lane];
+                    lds.res[0].get(p, o);
+                    each<VC>([&](auto i) { o[i] = v.v[i] * fmaf(l.skip[i], u.v[i], o[i]); });
+                    store<TAIL>(cgz, p, l, n, o);
                     cgz.move(-1);
                 }
                 if (g.gu.p) {
-                    *(float4*)v = lds.keep[1][lane];
-                    each<4>([&](auto i) { o[i] = fmaf(v[i], gu[i], l.skip[i] * ds[i]); });
-                    store4<TAIL>(cgu, p, l, g.wide, n, o);
+                    const FloatC v = lds.keep[1][lane];
+                    each<VC>([&](auto i) { o[i] = fmaf(v.v[i], gu[i], l.skip[i] * ds.v[i]); });
+                    store<TAIL>(cgu, p, l, n, o);
                     cgu.move(-1);
                 }
-                *(float4*)gd = *(const float4*)(from + 2 * SEG * 16);
-                *(float4*)v = lds.keep[2][lane];
-                each<4>([&](auto i) {
-                    o[i] = fmaf(u[i], gu[i], kLn2 * gd[i]) * v[i];
+                const FloatC slope = lds.keep[2][lane];
+                lds.res[2].get(p, gd);
+                each<VC>([&](auto i) {
+                    o[i] = fmaf(u.v[i], gu[i], kLn2 * gd[i]) * slope.v[i];
                     const bool in = !TAIL || p.tok < n;
                     gbias[i] += in ? o[i] : 0.0f;
-                    gskip[i] += in ? ds[i] * u[i] : 0.0f;
+                    gskip[i] += in ? ds.v[i] * u.v[i] : 0.0f;
                 });
                 if (g.gdelta.p) {
-                    store4<TAIL>(cgd, p, l, g.wide, n, o);
+                    store<TAIL>(cgd, p, l, n, o);
                     cgd.move(-1);
                 }
                 // B's and C's gradients of the workgroup's channels
-                __syncthreads();
-                constexpr int NS = 4 * S;
-                for (uint32_t e = threadIdx.x; e < n * 2 * NS; e += 64 * FG_SSM_WAVES) {
+                constexpr int NS = 4 * S * W;
+                for (uint32_t e = threadIdx.x; e < n * 2 * NS; e += THREADS) {
                     float sum = 0.0f;
-                    each<FG_SSM_WAVES>([&](auto w) { sum += all[w].sums[e]; });
+                    each<BLOCKS>([&](auto w) { sum += all[w].bc[e]; });
                     const uint32_t s = e % NS, m = e / (2 * NS), which = e / NS % 2;
                     if (!PAD || s < g.states) {
                         const uint64_t tok = (g.offsets ? (uint64_t)p.start : (uint64_t)p.seq * g.length) + t + m;
@@ -840,32 +914,33 @@ struct Scan {
                                   s] = sum;
                     }
                 }
-                __syncthreads();
             }
         };
         if (rest > 0) {
             back_load<LOCAL, true>(r, at, g, p, l, last, rest);
             segment(std::true_type{}, last, rest, full > 0);
         } else if (full > 0) {
-            move(-1);
-            cgu.move(-1);
-            cgd.move(-1);
-            cgz.move(-1);
+            at.move(-1);
             back_load<LOCAL, false>(r, at, g, p, l, last - SEG, SEG);
+            if constexpr (!LOCAL) {
+                cgu.move(-1);
+                cgd.move(-1);
+                cgz.move(-1);
+            }
         }
         for (uint32_t k = full; k-- > 0;) segment(std::false_type{}, p.t0 + k * SEG, SEG, k > 0);
         if constexpr (LOCAL) {
-            each<4>([&](auto i) {
-                const float sum = tokens_sum(sum_dt[i]);
-                if (p.tok == 0) g.carry_dt[carry_at(g, p, p.chunk) * 16 + 4 * (threadIdx.x & 3) + i] = sum;
+            each<VC>([&](auto i) {
+                const float sum = tokens_sum(p, sum_dt[i], lds.dt);
+                if (p.tok == 0) carry_dt_of(g, p, p.chunk)[p.sub + i] = sum;
             });
             each<S>([&](auto s) { carry_of(g, p, p.chunk)[s] = carry[s]; });
         } else {
             float* to = g.part_p + ((uint64_t)p.seq * g.chunks + p.chunk) * g.channels * (g.states + 2);
-            each<4>([&](auto i) {
-                const float s = tokens_sum(gskip[i]), v = tokens_sum(gbias[i]);
+            each<VC>([&](auto i) {
+                const float s = tokens_sum(p, gskip[i], lds.dt), v = tokens_sum(p, gbias[i], lds.dt);
                 if (i < p.have && p.tok == 0) {
-                    const uint64_t ch = p.group * g.group_channels + p.ch4 + i;
+                    const uint64_t ch = p.group * g.group_channels + p.in_group + i;
                     to[(uint64_t)g.channels * g.states + ch] = s;
                     to[(uint64_t)g.channels * (g.states + 1) + ch] = v;
                 }
@@ -873,7 +948,7 @@ struct Scan {
             if (p.valid) {
                 each<S>([&](auto s) {
                     if (has_state(g, p, s)) {
-                        to[(uint64_t)p.ch * g.states + p.q * S + s] = ga[s];
+                        to[(uint64_t)p.ch * g.states + p.row * S + s] = ga[s];
                         if (g.ginitial && p.chunk == 0) g.ginitial[state_at(g, p, s)] = carry[s];
                     }
                 });
@@ -882,15 +957,25 @@ struct Scan {
     }
 };
 
-// B's and C's gradients from the channel blocks' parts, in the order of the blocks.
+// p[0] + p[stride] + ... of n values, in this order of eight running sums.
+__device__ __forceinline__ float ordered_sum(const float* p, uint64_t stride, uint64_t n) {
+    float v[8] = {};
+    uint64_t k = 0;
+    for (; k + 8 <= n; k += 8) each<8>([&](auto j) { v[j] += p[(k + j) * stride]; });
+    each<7>([&](auto j) {
+        if (k + j < n) v[j] += p[(k + j) * stride];
+    });
+    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+}
+
+// B's and C's gradients from the channel blocks' parts, in a fixed order.
 template <class T>
 __device__ __forceinline__ void scan_reduce_bc(const fg_scan_kargs& g) {
     const uint32_t row = g.groups * 2 * g.states;
     const uint64_t n = g.tokens * row;
     const uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (e >= n) return;
-    float v = 0.0f;
-    for (uint32_t b = 0; b < g.group_blocks; ++b) v += g.part_bc[b * n + e];
+    const float v = ordered_sum(g.part_bc + e, n, g.group_blocks);
     const uint64_t tok = e / row;
     const uint32_t r = (uint32_t)(e % row), s = r % g.states, which = r / g.states % 2, grp = r / (2 * g.states);
     const uint64_t seq = g.offsets ? 0 : tok / g.length, t = g.offsets ? tok : tok % g.length;
@@ -910,13 +995,12 @@ __device__ __forceinline__ void scan_reduce_bc(const fg_scan_kargs& g) {
     }
 }
 
-// The parameters' gradients from the chunks' parts, in the order of the chunks.
+// The parameters' gradients from the chunks' parts, in a fixed order.
 __device__ __forceinline__ void scan_reduce_p(const fg_scan_kargs& g) {
     const uint64_t n = (uint64_t)g.channels * (g.states + 2);
     const uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (e >= n) return;
-    float v = 0.0f;
-    for (uint64_t k = 0; k < (uint64_t)g.seqs * g.chunks; ++k) v += g.part_p[k * n + e];
+    const float v = ordered_sum(g.part_p + e, n, (uint64_t)g.seqs * g.chunks);
     const uint64_t states = (uint64_t)g.channels * g.states;
     if (e < states) {
         if (g.ga) g.ga[e] = v;

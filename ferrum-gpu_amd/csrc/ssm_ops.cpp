@@ -383,39 +383,54 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_range(op, "groups", s.groups, 1, s.channels);
     if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
-    lane_states_ = fg_ssm_lane_states((uint32_t)s.states);
     segment_ = FG_SSM_SEGMENT;
-    group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, FG_SSM_GROUP_CHANNELS);
+    lane_states_ = s.states <= 4 ? 1 : s.states <= 8 ? 2 : 4;
+    waves_ = s.states <= 16 ? 1 : s.states <= 32 ? 2 : 4;
+    threads_ = 64 * waves_ * FG_SSM_BLOCKS(waves_);
+    group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, 16 * FG_SSM_BLOCKS(waves_));
     blocks_ = group_blocks_ * (uint32_t)s.groups;
-    chunks_forward_ = chunks_for(1024);
-    chunks_backward_ = chunks_for(1024);
-    const uint64_t waves =
-        (uint64_t)s.sequences * (std::max(chunks_forward_, chunks_backward_) + 1) * blocks_ * FG_SSM_WAVES;
+    chunks_forward_ = chunks_for(512);
+    chunks_backward_ = chunks_for(2047);
     if (chunks_forward_ > 1 || chunks_backward_ > 1) {
-        carry_ = Buffer<float, HipBackend>(dev, waves * 64 * lane_states_);
-        carry_dt_ = Buffer<float, HipBackend>(dev, waves * FG_SSM_WAVE_CHANNELS);
+        const uint64_t places = (uint64_t)s.sequences * (std::max(chunks_forward_, chunks_backward_) + 1) * blocks_ *
+                                FG_SSM_BLOCKS(waves_);
+        carry_ = Buffer<float, HipBackend>(dev, places * waves_ * 64 * lane_states_);
+        carry_dt_ = Buffer<float, HipBackend>(dev, places * 16);
     }
-    const std::string type = kTypes[s.dtype], tail = type + "_s" + std::to_string(lane_states_) +
-                                                     (4 * lane_states_ > (uint32_t)s.states ? "_pad" : "");
-    local_ = k.get((int)s.dtype, "fg_scan_local_" + tail);
-    forward_ = k.get((int)s.dtype, "fg_scan_" + tail);
-    back_local_ = k.get((int)s.dtype, "fg_scan_back_local_" + tail);
-    backward_ = k.get((int)s.dtype, "fg_scan_back_" + tail);
+    const std::string type = kTypes[s.dtype];
+    for (int wide = 0; wide < 2; ++wide) {
+        if (wide && s.states != 4 * lane_states_ * waves_) continue;
+        const std::string tail = type + "_s" + std::to_string(lane_states_) + "w" + std::to_string(waves_) +
+                                 (wide ? "" : "_any");
+        local_[wide] = k.get((int)s.dtype, "fg_scan_local_" + tail);
+        forward_[wide] = k.get((int)s.dtype, "fg_scan_" + tail);
+        back_local_[wide] = k.get((int)s.dtype, "fg_scan_back_local_" + tail);
+        backward_[wide] = k.get((int)s.dtype, "fg_scan_back_" + tail);
+    }
     reduce_bc_ = k.get((int)s.dtype, "fg_scan_reduce_bc_" + type);
     reduce_p_ = k.get(FG_DTYPE_F32, "fg_scan_reduce_p");
 }
 
-// Parts of the token axis that work at the same time, so that `target` waves do.
-uint32_t ScanPlan::chunks_for(uint32_t target) const {
-    const uint64_t waves = std::max<uint64_t>(1, (uint64_t)s_.sequences * blocks_ * FG_SSM_WAVES);
+// Parts of the token axis that are worked through at the same time.  A SIMD of
+// the GPU's 1024 takes two waves: tensors with at most `few` waves are cut
+// until there are 2048, which costs a pass over the tokens for what each part
+// adds to the states.  Measured, us for one pass of 4 sequences of 16 states in
+// bfloat16, parts 1 / 2 / 4: forward, 1024 tokens x 2048 channels (512 waves)
+// 88 / 87 / 78, 2048 x 4096 (1024 waves) 177 / 256; backward, 1024 x 2048
+// (parts 2 / 4) 204 / 157.  A part has 64 tokens or more.  Packed sequences count
+// as so many of the longest's length, which the last wave to end works through.
+uint32_t ScanPlan::chunks_for(uint32_t few) const {
+    const uint64_t seqs = s_.packed && s_.length ? ceil_div(s_.tokens, s_.length) : s_.sequences;
+    const uint64_t waves = std::max<uint64_t>(1, seqs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_);
+    if (waves > few) return 1;
     const uint64_t most = std::max<uint64_t>(1, ceil_div(s_.length, 4 * segment_));
-    return (uint32_t)std::min<uint64_t>({ceil_div(target, waves), most, 64});
+    return (uint32_t)std::min<uint64_t>({ceil_div(2048, waves), most, 64});
 }
 
 size_t ScanPlan::checkpoint_bytes() const {
     const uint64_t segs = s_.packed ? (uint64_t)s_.tokens / segment_ + s_.sequences
                                     : s_.sequences * ceil_div(s_.length, segment_);
-    return segs * blocks_ * FG_SSM_WAVES * 64 * lane_states_ * sizeof(float);
+    return segs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_ * 64 * lane_states_ * sizeof(float);
 }
 
 fg_scan_kargs ScanPlan::base(const fg_scan_inputs& in, uint32_t chunks) const {
@@ -448,14 +463,14 @@ void ScanPlan::check_inputs(const char* op, const fg_scan_inputs& in) const {
     if (!s_.packed && in.offsets) invalid(std::string(op) + ": offsets are for packed sequences");
 }
 
-// Vector accesses where every row and every lane's part of it allow them: four
-// channels, and the lane's states of a channel that has all of them.
+// Vector accesses where every row and every lane's part of it allow them: 4 /
+// waves channels, and the lane's states of a channel that has all of them.
 bool ScanPlan::wide(const fg_scan_kargs& g, std::initializer_list<const fg_ssm_view*> channels,
                     std::initializer_list<const fg_ssm_view*> states) const {
-    const uint32_t es = kBytes[s_.dtype];
-    bool yes = g.group_channels % 4 == 0 && g.states == 4 * lane_states_;
-    for (const fg_ssm_view* v : channels) yes = yes && vector_rows(*v, 4, es);
-    for (const fg_ssm_view* v : states) yes = yes && vector_rows(*v, std::min(lane_states_, 16 / es), es);
+    const uint32_t es = kBytes[s_.dtype], n = 4 / waves_;
+    bool yes = g.group_channels % n == 0 && g.states == 4 * lane_states_ * waves_;
+    for (const fg_ssm_view* v : channels) yes = yes && vector_rows(*v, n, es);
+    for (const fg_ssm_view* v : states) yes = yes && vector_rows(*v, lane_states_, es);
     return yes;
 }
 
@@ -481,11 +496,11 @@ void ScanPlan::forward(const fg_scan_forward_args& a, hipStream_t stream) const 
     all.flat("checkpoints", a.checkpoints, (int64_t)checkpoint_bytes(), true, true);
     g.final = a.final;
     g.check = (float*)a.checkpoints;
-    g.wide = wide(g, {&g.u, &g.delta, &g.z, &g.out}, {&g.b, &g.c});
+    const bool vec = wide(g, {&g.u, &g.delta, &g.z, &g.out}, {&g.b, &g.c});
     void* args[] = {&g};
     const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
-    if (g.chunks > 1) launch(dev_, stream, local_, blocks, 64 * FG_SSM_WAVES, args, op);
-    launch(dev_, stream, forward_, blocks, 64 * FG_SSM_WAVES, args, op);
+    if (g.chunks > 1) launch(dev_, stream, local_[vec], blocks, threads_, args, op);
+    launch(dev_, stream, forward_[vec], blocks, threads_, args, op);
 }
 
 void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
@@ -534,11 +549,11 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
     }
     g.part_bc = part_bc_.data();
     g.part_p = part_p_.data();
-    g.wide = wide(g, {&g.u, &g.delta, &g.z, &g.gout, &g.gu, &g.gdelta, &g.gz}, {&g.b, &g.c});
+    const bool vec = wide(g, {&g.u, &g.delta, &g.z, &g.gout, &g.gu, &g.gdelta, &g.gz}, {&g.b, &g.c});
     void* args[] = {&g};
     const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
-    if (g.chunks > 1) launch(dev_, stream, back_local_, blocks, 64 * FG_SSM_WAVES, args, op);
-    launch(dev_, stream, backward_, blocks, 64 * FG_SSM_WAVES, args, op);
+    if (g.chunks > 1) launch(dev_, stream, back_local_[vec], blocks, threads_, args, op);
+    launch(dev_, stream, backward_[vec], blocks, threads_, args, op);
     if (g.gb.p || g.gc.p) launch(dev_, stream, reduce_bc_, ceil_div(g.tokens * row, 256), 256, args, op);
     if (g.ga || g.gskip || g.gbias) launch(dev_, stream, reduce_p_, ceil_div(params, 256), 256, args, op);
 }

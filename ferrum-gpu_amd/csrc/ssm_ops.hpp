@@ -65,9 +65,11 @@ private:
     uint32_t chunks_for(uint32_t target_waves) const;
     HipBackend::DeviceHandle dev_;
     fg_scan_shape s_;
-    uint32_t lane_states_, segment_, group_blocks_, blocks_;  // blocks_: workgroups over all channels
+    uint32_t lane_states_, waves_;  // states of a lane, waves that share a channel's states
+    uint32_t segment_, threads_, group_blocks_, blocks_;  // blocks_: workgroups over all channels
     uint32_t chunks_forward_, chunks_backward_;
-    HipBackend::KernelHandle local_, forward_, back_local_, backward_, reduce_bc_, reduce_p_;
+    HipBackend::KernelHandle local_[2] = {}, forward_[2] = {}, back_local_[2] = {}, backward_[2] = {};  // [any, wide]
+    HipBackend::KernelHandle reduce_bc_, reduce_p_;
     Buffer<float, HipBackend> carry_, carry_dt_;
     std::mutex mu_;
     Buffer<float, HipBackend> part_bc_, part_p_;
