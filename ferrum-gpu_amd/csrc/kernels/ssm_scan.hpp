@@ -184,6 +184,11 @@ struct Scan {
             else if constexpr (WIDE) return T::up((raw)(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
             else return T::up((raw)w[i]);
         }
+        // The first use of what was loaded: conversions that the compiler moves
+        // up to the segment before wait for their loads there.
+        __device__ __forceinline__ void arrive() {
+            each<WORDS>([&](auto i) { asm volatile("" : "+v"(w[i])); });
+        }
         __device__ __forceinline__ void load(const char* at, uint32_t row, const uint32_t (&off)[N]) {
             if constexpr (!WIDE) {
                 each<N>([&](auto i) {
@@ -275,10 +280,12 @@ struct Scan {
             });
         }
     }
-    static __device__ __forceinline__ void up(float (&x)[VC], const RawC& v) {
+    static __device__ __forceinline__ void up(float (&x)[VC], RawC& v) {
+        v.arrive();
         each<VC>([&](auto i) { x[i] = v.up(i); });
     }
-    static __device__ __forceinline__ void up(float (&x)[S], const RawS& v, const Lane& l) {
+    static __device__ __forceinline__ void up(float (&x)[S], RawS& v, const Lane& l) {
+        v.arrive();
         each<S>([&](auto s) { x[s] = PAD && l.pad[s] ? 0.0f : v.up(s); });
     }
 
@@ -460,7 +467,7 @@ struct Scan {
     }
     template <bool TAIL>
     static __device__ __forceinline__ void outputs(const fg_scan_kargs& g, const Place& p, const Lane& l,
-                                                   const Sums& y, const Cursor& out, const RawC& ru, const RawC& rz,
+                                                   const Sums& y, const Cursor& out, RawC& ru, RawC& rz,
                                                    bool gated, uint32_t n) {
         float u[VC], z[VC], o[VC];
         up(u, ru);
@@ -562,32 +569,43 @@ struct Scan {
             up(d, ring[0].d);
             up(u, ring[0].u);
             prepare<LOCAL, false>(g, p, l, lds.x[0], sum_dt, d, u, SEG, true);
-            for (uint32_t k = 0; k <= full; k += RING) {
-                each<RING>([&](auto j) {
-                    const uint32_t m = k + j;
-                    if (m > full) return;
-                    Rows& last = ring[(j + RING - 1) % RING];
+            auto store_last = [&](auto j, uint32_t m) {  // segment m, which lies in ring[j]
+                if constexpr (!LOCAL) {
+                    outputs<false>(g, p, l, lds.y[m & 1], out, ring[j].u, ring[j].z, gated, SEG);
+                    out.move(1);
+                }
+            };
+            auto step = [&](auto j, uint32_t m) {
+                constexpr int before = (j + RING - 1) % RING;
+                sync<SHARED>();
+                if (j > 0 || m > 0) store_last(Int<before>{}, m - 1);
+                fetch(ring[before], std::false_type{}, SEG);
+                forth(m + RING < full);
+                up(b, ring[j].b, l);
+                if constexpr (!LOCAL) up(c, ring[j].c, l);
+                up(d, ring[(j + 1) % RING].d);
+                up(u, ring[(j + 1) % RING].u);
+                checkpoint(p.t0 + m * SEG);
+                Steps first;
+                first.read(p, lds.x[m & 1], 0);
+                prepare<LOCAL, false>(g, p, l, lds.x[(m + 1) & 1], sum_dt, d, u, SEG, m + 1 < full);
+                forward_segment<LOCAL, false>(p, l, lds.x[m & 1], first, lds.y[m & 1], h, b, c, SEG);
+            };
+            // Whole turns of the ring: a step that could be skipped would cost
+            // the others their count of loads on the way.
+            uint32_t k = 0;
+            for (; k + RING <= full; k += RING) each<RING>([&](auto j) { step(j, k + j); });
+            auto finish = [&](auto self, auto j) {
+                if (k + j < full) {
+                    step(j, k + j);
+                    if constexpr (j + 2 < RING) self(self, Int<j + 1>{});
+                    else sync<SHARED>(), store_last(j, k + j);
+                } else {
                     sync<SHARED>();
-                    if constexpr (!LOCAL) {
-                        if (m > 0) {
-                            outputs<false>(g, p, l, lds.y[(m - 1) & 1], out, last.u, last.z, gated, SEG);
-                            out.move(1);
-                        }
-                    }
-                    if (m == full) return;
-                    fetch(last, std::false_type{}, SEG);
-                    forth(m + RING < full);
-                    up(b, ring[j].b, l);
-                    if constexpr (!LOCAL) up(c, ring[j].c, l);
-                    up(d, ring[(j + 1) % RING].d);
-                    up(u, ring[(j + 1) % RING].u);
-                    checkpoint(p.t0 + m * SEG);
-                    Steps first;
-                    first.read(p, lds.x[m & 1], 0);
-                    prepare<LOCAL, false>(g, p, l, lds.x[(m + 1) & 1], sum_dt, d, u, SEG, m + 1 < full);
-                    forward_segment<LOCAL, false>(p, l, lds.x[m & 1], first, lds.y[m & 1], h, b, c, SEG);
-                });
-            }
+                    store_last(Int<(j + RING - 1) % RING>{}, k + j - 1);
+                }
+            };
+            finish(finish, Int<0>{});
             sync<SHARED>();
         }
         if (rest > 0) {
@@ -675,7 +693,7 @@ struct Scan {
     }
     // Time steps and output gradients, to LDS, with what the end of the segment needs.
     template <bool LOCAL, class L>
-    static __device__ __forceinline__ void back_prepare(const BackRaws<LOCAL>& r, const fg_scan_kargs& g,
+    static __device__ __forceinline__ void back_prepare(BackRaws<LOCAL>& r, const fg_scan_kargs& g,
                                                         const Place& p, const Lane& l, L& lds, float (&dt)[VC],
                                                         bool gated) {
         float d[VC], dy[VC], z[VC], u[VC];
