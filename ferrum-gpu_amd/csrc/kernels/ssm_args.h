@@ -11,6 +11,7 @@
                                     pass leaves for its backward pass */
 #define FG_SSM_MAX_STATES 64
 #define FG_CONV_MAX_WIDTH 8
+#define FG_CONV_ROWS 4            /* rows that the convolution loads at a time */
 
 /* A scan's workgroup has FG_SSM_BLOCKS(W) blocks of 16 channels with W waves
  * each; 4 W rows of 16 lanes share a channel's states. */
@@ -79,6 +80,7 @@ typedef struct {
     const int32_t* slots;
     uint64_t state_rows;
     uint32_t rows, channels, silu;
+    uint32_t each_wave; /* rows of a wave */
 } fg_conv_step_kargs;
 
 #endif

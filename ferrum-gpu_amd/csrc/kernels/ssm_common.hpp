@@ -107,5 +107,16 @@ __device__ __forceinline__ float rows_sum(const float (&v)[4]) {
     return swap16_add(swap32_add(v[0], v[2]), swap32_add(v[1], v[3]));
 }
 
+// p[0] + p[stride] + ... of n values, in this order of eight running sums.
+__device__ __forceinline__ float ordered_sum(const float* p, uint64_t stride, uint64_t n) {
+    float v[8] = {};
+    uint64_t k = 0;
+    for (; k + 8 <= n; k += 8) each<8>([&](auto j) { v[j] += p[(k + j) * stride]; });
+    each<7>([&](auto j) {
+        if (k + j < n) v[j] += p[(k + j) * stride];
+    });
+    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+}
+
 }  // namespace ssm
 }  // namespace fg

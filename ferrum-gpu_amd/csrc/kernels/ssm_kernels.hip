@@ -26,33 +26,35 @@ using namespace fg::ssm;
     }
 #define FG_SCAN(NAME, T, S, W) FG_SCAN_ONE(NAME, T, S, W, , true) FG_SCAN_ONE(NAME, T, S, W, _any, false)
 
-// W taps, V channels of a thread: 16 bytes of a row forward, at most four
-// channels backward; V = 1 for any stride and alignment.
-#define FG_CONV(NAME, T, W, V, B)                                                                               \
-    extern "C" __global__ __launch_bounds__(256) void fg_conv_##NAME##_w##W##_v##V(fg_conv_kargs g) {            \
-        Conv<T, V, W>::forward(g);                                                                             \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void fg_conv_back_##NAME##_w##W##_v##B(fg_conv_kargs g) {       \
-        Conv<T, B, W>::backward(g);                                                                            \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void fg_conv_step_##NAME##_w##W##_v##V(fg_conv_step_kargs g) {  \
-        Conv<T, V, W>::step(g);                                                                                \
-    }
-#define FG_CONV_BOTH(NAME, T, W, V) FG_CONV(NAME, T, W, V, 4) FG_CONV(NAME, T, W, 1, 1)
+// W taps, V channels of a thread: eight (16-bit rows, up to four taps, not
+// backward: more would not fit the registers), four, or one for any stride and
+// alignment.
+#define FG_CONV_KERNEL(NAME, T, W, V, CALL, ARGS)                                                               \
+    extern "C" __global__ __launch_bounds__(256) void NAME##_w##W##_v##V(ARGS g) { Conv<T, V, W>::CALL(g); }
+#define FG_CONV_FORWARD(NAME, T, W, V)                                                                          \
+    FG_CONV_KERNEL(fg_conv_##NAME, T, W, V, forward, fg_conv_kargs)                                             \
+    FG_CONV_KERNEL(fg_conv_step_##NAME, T, W, V, step, fg_conv_step_kargs)
+#define FG_CONV_BACK(NAME, T, W, V) FG_CONV_KERNEL(fg_conv_back_##NAME, T, W, V, backward, fg_conv_kargs)
+#define FG_CONV(NAME, T, W)                                                                                     \
+    FG_CONV_FORWARD(NAME, T, W, 4)                                                                              \
+    FG_CONV_FORWARD(NAME, T, W, 1)                                                                              \
+    FG_CONV_BACK(NAME, T, W, 4)                                                                                 \
+    FG_CONV_BACK(NAME, T, W, 1)
+#define FG_CONV_EIGHT(NAME, T) FG_CONV_FORWARD(NAME, T, 2, 8) FG_CONV_FORWARD(NAME, T, 3, 8) FG_CONV_FORWARD(NAME, T, 4, 8)
 
-#define FG_SSM_TYPE(NAME, T, V)                                                                                 \
+#define FG_SSM_TYPE(NAME, T)                                                                                    \
     FG_SCAN(NAME, T, 1, 1)                                                                                      \
     FG_SCAN(NAME, T, 2, 1)                                                                                      \
     FG_SCAN(NAME, T, 4, 1)                                                                                      \
     FG_SCAN(NAME, T, 4, 2)                                                                                      \
     FG_SCAN(NAME, T, 4, 4)                                                                                      \
-    FG_CONV_BOTH(NAME, T, 2, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 3, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 4, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 5, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 6, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 7, V)                                                                                 \
-    FG_CONV_BOTH(NAME, T, 8, V)                                                                                 \
+    FG_CONV(NAME, T, 2)                                                                                         \
+    FG_CONV(NAME, T, 3)                                                                                         \
+    FG_CONV(NAME, T, 4)                                                                                         \
+    FG_CONV(NAME, T, 5)                                                                                         \
+    FG_CONV(NAME, T, 6)                                                                                         \
+    FG_CONV(NAME, T, 7)                                                                                         \
+    FG_CONV(NAME, T, 8)                                                                                         \
     extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_bc_##NAME(fg_scan_kargs g) {                \
         scan_reduce_bc<T>(g);                                                                                  \
     }                                                                                                          \
@@ -62,16 +64,18 @@ using namespace fg::ssm;
 
 // One code object, three builds of this file in parallel: FG_SSM_F32, _BF16, _F16.
 #if defined(FG_SSM_F32)
-FG_SSM_TYPE(f32, F32, 4)
+FG_SSM_TYPE(f32, F32)
 extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_p(fg_scan_kargs g) { scan_reduce_p(g); }
 extern "C" __global__ __launch_bounds__(256) void fg_conv_reduce(fg_conv_kargs g, uint32_t width, float* gweight,
                                                                 float* gbias) {
     conv_reduce(g, width, gweight, gbias);
 }
 #elif defined(FG_SSM_BF16)
-FG_SSM_TYPE(bf16, BF16, 8)
+FG_SSM_TYPE(bf16, BF16)
+FG_CONV_EIGHT(bf16, BF16)
 #elif defined(FG_SSM_F16)
-FG_SSM_TYPE(f16, F16, 8)
+FG_SSM_TYPE(f16, F16)
+FG_CONV_EIGHT(f16, F16)
 #else
 #error "build with FG_SSM_F32, FG_SSM_BF16 or FG_SSM_F16"
 #endif

@@ -975,17 +975,6 @@ struct Scan {
     }
 };
 
-// p[0] + p[stride] + ... of n values, in this order of eight running sums.
-__device__ __forceinline__ float ordered_sum(const float* p, uint64_t stride, uint64_t n) {
-    float v[8] = {};
-    uint64_t k = 0;
-    for (; k + 8 <= n; k += 8) each<8>([&](auto j) { v[j] += p[(k + j) * stride]; });
-    each<7>([&](auto j) {
-        if (k + j < n) v[j] += p[(k + j) * stride];
-    });
-    return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-}
-
 // B's and C's gradients from the channel blocks' parts, in a fixed order.
 template <class T>
 __device__ __forceinline__ void scan_reduce_bc(const fg_scan_kargs& g) {

@@ -141,11 +141,30 @@ void refuse_capture(const char* op, const HipBackend::DeviceHandle& dev, hipStre
         invalid(std::string(op) + ": a plan's first backward call allocates its workspace and cannot be captured");
 }
 
+// Channels of a thread of the convolution, widest first.
+const uint32_t kVector[3] = {8, 4, 1};
+// The widest of forward calls and steps: 16 bytes, and weights that fit the registers.
+uint32_t conv_widest(uint32_t es, uint32_t width) { return es == 2 && width <= 4 ? 8 : 4; }
+
 // Device pointers and strides of `v` multiples of a vector of n elements.
 bool vector_rows(const fg_ssm_view& v, uint32_t n, uint32_t es) {
     return reinterpret_cast<uintptr_t>(v.p) % (n * es) == 0 && v.seq % n == 0 && v.row % n == 0;
 }
 bool vector_ptr(const void* p, uint32_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// The widest of kVector, at most `most`, that channels, rows and states allow,
+// as its index.
+int conv_vector(uint32_t channels, uint32_t es, std::initializer_list<const fg_ssm_view*> rows,
+                std::initializer_list<const void*> states, uint32_t most) {
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t n = kVector[i];
+        bool yes = n <= most && channels % n == 0;
+        for (const fg_ssm_view* v : rows) yes = yes && vector_rows(*v, n, es);
+        for (const void* p : states) yes = yes && vector_ptr(p, n * es);
+        if (yes) return i;
+    }
+    return 2;
+}
 
 void launch(const HipBackend::DeviceHandle& dev, hipStream_t stream, HipBackend::KernelHandle k, uint64_t blocks,
             uint32_t threads, void** args, const char* op) {
@@ -162,9 +181,10 @@ SsmKernels::SsmKernels(Device<HipBackend>& dev) {
     for (int t = 0; t < 3; ++t) {
         mod_[t] = dev.load_or_cache(ssm_code_object(t));
         for (int w = 2; w <= FG_CONV_MAX_WIDTH; ++w)
-            for (int v = 0; v < 2; ++v)
-                conv_step_[t][w][v] = get(t, std::string("fg_conv_step_") + kTypes[t] + "_w" + std::to_string(w) +
-                                                 "_v" + std::to_string(v ? 16 / kBytes[t] : 1));
+            for (int v = 0; v < 3; ++v)
+                if (kVector[v] <= conv_widest(kBytes[t], w))
+                    conv_step_[t][w][v] = get(t, std::string("fg_conv_step_") + kTypes[t] + "_w" + std::to_string(w) +
+                                                     "_v" + std::to_string(kVector[v]));
         scan_step_[t] = get(t, std::string("fg_scan_step_") + kTypes[t]);
     }
 }
@@ -181,7 +201,7 @@ void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_st
     check_range(op, "channels", a.channels, 1, kMaxCount);
     check_range(op, "width", a.width, 2, FG_CONV_MAX_WIDTH);
     check_range(op, "state_rows", a.state_rows, a.slots ? 0 : a.rows, kMaxCount);
-    const uint32_t es = kBytes[a.dtype], n = 16 / es;
+    const uint32_t es = kBytes[a.dtype];
     Arrays all(op, a.rows, 1, es);
     fg_conv_step_kargs g{};
     g.x = all.rows("x", a.x, a.channels, false);
@@ -202,11 +222,14 @@ void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_st
     g.rows = (uint32_t)a.rows;
     g.channels = (uint32_t)a.channels;
     g.silu = a.silu != 0;
-    const bool vec = a.channels % n == 0 && vector_rows(g.x, n, es) && vector_rows(g.out, n, es) &&
-                     vector_ptr(a.state, 16) && vector_ptr(a.state_out, 16);
-    const uint64_t waves = ceil_div(g.channels / (vec ? n : 1), 64) * g.rows;
+    const int v = conv_vector(g.channels, es, {&g.x, &g.out}, {a.state, a.state_out},
+                              conv_widest(es, (uint32_t)a.width));
+    // rows of a wave, at least 1024 waves: one for each SIMD
+    const uint64_t wide = ceil_div(g.channels / kVector[v], 64);
+    g.each_wave = (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, wide * g.rows / 1024));
+    const uint64_t waves = wide * ceil_div(g.rows, g.each_wave);
     void* args[] = {&g};
-    launch(dev, stream, conv_step_[a.dtype][a.width][vec], ceil_div(waves, 4), 256, args, op);
+    launch(dev, stream, conv_step_[a.dtype][a.width][v], ceil_div(waves, 4), 256, args, op);
 }
 
 void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_step_args& a,
@@ -259,6 +282,8 @@ void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_st
 
 namespace {
 
+constexpr uint32_t kConvForwardWaves = 2048, kConvBackwardWaves = 4096;
+
 // Shared by both plans' constructors: sequences, length, tokens.
 void check_sequences(const char* op, int64_t sequences, int64_t length, int64_t tokens, int64_t packed) {
     check_range(op, "sequences", sequences, 0, kMaxCount);
@@ -276,14 +301,22 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_range(op, "channels", s.channels, 1, kMaxCount);
     check_range(op, "width", s.width, 2, FG_CONV_MAX_WIDTH);
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
-    run_forward_ = 16;
-    run_backward_ = 32;
     const std::string type = kTypes[s.dtype], w = "_w" + std::to_string(s.width);
-    for (int v = 0; v < 2; ++v) {
-        forward_[v] = k.get((int)s.dtype, "fg_conv_" + type + w + "_v" + std::to_string(v ? 16 / kBytes[s.dtype] : 1));
-        backward_[v] = k.get((int)s.dtype, "fg_conv_back_" + type + w + "_v" + std::to_string(v ? 4 : 1));
+    for (int v = 0; v < 3; ++v) {
+        const std::string tail = type + w + "_v" + std::to_string(kVector[v]);
+        if (kVector[v] <= conv_widest(kBytes[s.dtype], (uint32_t)s.width)) forward_[v] = k.get((int)s.dtype, "fg_conv_" + tail);
+        if (kVector[v] <= 4) backward_[v] = k.get((int)s.dtype, "fg_conv_back_" + tail);
     }
     reduce_ = k.get(FG_DTYPE_F32, "fg_conv_reduce");
+}
+
+// Tokens of a thread: as many as leave `waves` waves, each of 64 threads of n
+// channels, between FG_CONV_ROWS * 2 and 64.
+uint32_t ConvPlan::run_for(uint32_t n, uint32_t waves) const {
+    const uint64_t all = ceil_div(s_.channels / n, 64) * (uint64_t)s_.tokens;
+    uint32_t run = 2 * FG_CONV_ROWS;
+    while (run < 64 && all / (2 * run) >= waves) run *= 2;
+    return run;
 }
 
 fg_conv_kargs ConvPlan::base(const int32_t* offsets) const {
@@ -301,7 +334,7 @@ fg_conv_kargs ConvPlan::base(const int32_t* offsets) const {
 
 void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const {
     const char* op = "conv forward";
-    const uint32_t es = kBytes[s_.dtype], n = 16 / es;
+    const uint32_t es = kBytes[s_.dtype];
     fg_conv_kargs g = base(a.offsets);
     Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, es);
     g.x = all.rows("x", a.x, s_.channels, false);
@@ -317,13 +350,13 @@ void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const 
     g.bias = a.bias;
     g.initial = a.initial;
     g.final = a.final;
-    g.run = run_forward_;
+    const int v = conv_vector(g.channels, es, {&g.x, &g.out}, {a.initial, a.final},
+                              conv_widest(es, (uint32_t)s_.width));
+    g.run = run_for(kVector[v], kConvForwardWaves);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
-    const bool vec = s_.channels % n == 0 && vector_rows(g.x, n, es) && vector_rows(g.out, n, es) &&
-                     vector_ptr(a.initial, 16) && vector_ptr(a.final, 16);
-    const uint64_t waves = ceil_div(g.channels / (vec ? n : 1), 64) * g.runs * g.seqs;
+    const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
     void* args[] = {&g};
-    launch(dev_, stream, forward_[vec], ceil_div(waves, 4), 256, args, op);
+    launch(dev_, stream, forward_[v], ceil_div(waves, 4), 256, args, op);
 }
 
 void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
@@ -348,7 +381,9 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
     g.initial = a.initial;
     g.gfinal = a.grad_final;
     g.ginitial = a.grad_initial;
-    g.run = run_backward_;
+    const int v = conv_vector(g.channels, es, {&g.x, &g.out, &g.gx}, {a.initial, a.grad_final, a.grad_initial}, 4);
+    // the run, and with it the workspace, is that of four channels for any call
+    g.run = run_for(std::min<uint32_t>(4, (uint32_t)s_.channels), kConvBackwardWaves);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const uint64_t n = (uint64_t)s_.channels * (s_.width + 1);
     {
@@ -359,16 +394,13 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
         }
     }
     g.part = part_.data();
-    const bool vec = s_.channels % 4 == 0 && vector_rows(g.x, 4, es) && vector_rows(g.out, 4, es) &&
-                     vector_rows(g.gx, 4, es) && vector_ptr(a.initial, 4 * es) && vector_ptr(a.grad_final, 4 * es) &&
-                     vector_ptr(a.grad_initial, 4 * es);
-    const uint64_t waves = ceil_div(g.channels / (vec ? 4 : 1), 64) * g.runs * g.seqs;
+    const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
     void* args[] = {&g};
-    launch(dev_, stream, backward_[vec], ceil_div(waves, 4), 256, args, op);
+    launch(dev_, stream, backward_[v], ceil_div(waves, 4), 256, args, op);
     uint32_t width = (uint32_t)s_.width;
     float *gw = a.grad_weight, *gb = a.grad_bias;
     void* rargs[] = {&g, &width, &gw, &gb};
-    if (gw || gb) launch(dev_, stream, reduce_, ceil_div(n, 256), 256, rargs, op);
+    if (gw || gb) launch(dev_, stream, reduce_, ceil_div(n, 64), 256, rargs, op);
 }
 
 // -------------------------------------------------------------------- scan

@@ -30,7 +30,7 @@ public:
 
 private:
     HipBackend::Module mod_[3];
-    HipBackend::KernelHandle conv_step_[3][FG_CONV_MAX_WIDTH + 1][2] = {};  // [dtype][width][any alignment, 16 bytes]
+    HipBackend::KernelHandle conv_step_[3][FG_CONV_MAX_WIDTH + 1][3] = {};  // [dtype][width][8, 4, 1 channels]
     HipBackend::KernelHandle scan_step_[3] = {};
 };
 
@@ -44,8 +44,8 @@ private:
     fg_conv_kargs base(const int32_t* offsets) const;
     HipBackend::DeviceHandle dev_;
     fg_conv_shape s_;
-    uint32_t run_forward_, run_backward_;
-    HipBackend::KernelHandle forward_[2], backward_[2], reduce_;  // [any alignment, vectors]
+    uint32_t run_for(uint32_t n, uint32_t waves) const;
+    HipBackend::KernelHandle forward_[3] = {}, backward_[3] = {}, reduce_;  // [8, 4, 1 channels of a thread]
     std::mutex mu_;
     Buffer<float, HipBackend> part_;
 };

@@ -121,12 +121,13 @@ def test_every_kernel_that_the_host_looks_up_is_instantiated():
     """Names composed in ssm_ops.cpp against the code objects' symbols in the library."""
     blob = open(N.LIB_PATH, "rb").read()
     names = ["fg_scan_reduce_p", "fg_conv_reduce"]
-    for t, v in (("f32", 4), ("bf16", 8), ("f16", 8)):
+    for t, most in (("f32", 4), ("bf16", 8), ("f16", 8)):
         for s, tail in itertools.product(("s1w1", "s2w1", "s4w1", "s4w2", "s4w4"), ("", "_any")):
             names += [f"fg_scan_{k}{t}_{s}{tail}" for k in ("", "local_", "back_", "back_local_")]
         names += [f"fg_scan_reduce_bc_{t}", f"fg_scan_step_{t}"]
         for w in range(2, ssm.MAX_WIDTH + 1):
-            names += [f"fg_conv_{t}_w{w}_v{n}" for n in (1, v)] + [f"fg_conv_step_{t}_w{w}_v{n}" for n in (1, v)]
+            names += [f"fg_conv_{k}{t}_w{w}_v{n}" for k in ("", "step_")
+                      for n in {1, 4, most if w <= 4 else 4}]
             names += [f"fg_conv_back_{t}_w{w}_v{n}" for n in (1, 4)]
     missing = [n for n in names if b"\0" + n.encode() + b"\0" not in blob]
     assert not missing, missing
