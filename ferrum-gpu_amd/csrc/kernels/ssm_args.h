@@ -52,8 +52,8 @@ typedef struct {
     const int32_t* slots;
     uint64_t state_rows;
     uint32_t rows, channels, states, groups, group_channels;
-    uint32_t lanes; /* lanes of a channel */
     uint32_t softplus;
+    uint32_t each_wave; /* rows of a wave */
 } fg_scan_step_kargs;
 
 typedef struct {

@@ -42,6 +42,15 @@ using namespace fg::ssm;
     FG_CONV_BACK(NAME, T, W, 1)
 #define FG_CONV_EIGHT(NAME, T) FG_CONV_FORWARD(NAME, T, 2, 8) FG_CONV_FORWARD(NAME, T, 3, 8) FG_CONV_FORWARD(NAME, T, 4, 8)
 
+// L: lanes of a channel, four states each; _any as for the scan.
+#define FG_SCAN_STEP(NAME, T, L)                                                                                \
+    extern "C" __global__ __launch_bounds__(256) void fg_scan_step_##NAME##_l##L(fg_scan_step_kargs g) {        \
+        scan_step_body<T, L, true>(g);                                                                         \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void fg_scan_step_##NAME##_l##L##_any(fg_scan_step_kargs g) {  \
+        scan_step_body<T, L, false>(g);                                                                        \
+    }
+
 #define FG_SSM_TYPE(NAME, T)                                                                                    \
     FG_SCAN(NAME, T, 1, 1)                                                                                      \
     FG_SCAN(NAME, T, 2, 1)                                                                                      \
@@ -58,9 +67,11 @@ using namespace fg::ssm;
     extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_bc_##NAME(fg_scan_kargs g) {                \
         scan_reduce_bc<T>(g);                                                                                  \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void fg_scan_step_##NAME(fg_scan_step_kargs g) {                \
-        scan_step_body<T>(g);                                                                                  \
-    }
+    FG_SCAN_STEP(NAME, T, 1)                                                                                    \
+    FG_SCAN_STEP(NAME, T, 2)                                                                                    \
+    FG_SCAN_STEP(NAME, T, 4)                                                                                    \
+    FG_SCAN_STEP(NAME, T, 8)                                                                                    \
+    FG_SCAN_STEP(NAME, T, 16)
 
 // One code object, three builds of this file in parallel: FG_SSM_F32, _BF16, _F16.
 #if defined(FG_SSM_F32)

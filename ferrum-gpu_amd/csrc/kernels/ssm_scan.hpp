@@ -1019,47 +1019,88 @@ __device__ __forceinline__ void scan_reduce_p(const fg_scan_kargs& g) {
 }
 
 // One token of each row, the states in a cache of slots: a lane takes four
-// states of a channel, `lanes` neighbouring lanes (a power of two) a channel.
-template <class T>
+// states of a channel, LANES neighbouring lanes a channel, and walks through
+// g.each_wave rows, the next row's loads on their way.  Bound by the states,
+// read and written once.  WIDE: four states and their A, B and C load together
+// and every channel has 4 LANES states; else any alignment and number.
+template <class T, int LANES, bool WIDE>
 __device__ __forceinline__ void scan_step_body(const fg_scan_step_kargs& g) {
     using raw = typename T::raw;
-    const uint64_t id = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const uint32_t part = (uint32_t)(id % g.lanes);
-    const uint64_t of = id / g.lanes;
-    const bool valid = of < (uint64_t)g.rows * g.channels;
-    const uint32_t row = valid ? (uint32_t)(of / g.channels) : 0, ch = valid ? (uint32_t)(of % g.channels) : 0;
-    const int64_t slot = g.slots ? g.slots[row] : (int64_t)row;
-    const bool live = valid && slot >= 0 && (uint64_t)slot < g.state_rows;  // a row without a slot: zeros out
-    float acc = 0.0f, u = 0.0f;
-    if (live) {
-        auto in = [&](const fg_ssm_view& v, uint32_t i) { return T::up(((const raw*)v.p)[(int64_t)row * v.seq + i]); };
-        u = in(g.u, ch);
-        const float x = in(g.delta, ch) + (g.bias ? g.bias[ch] : 0.0f);
-        const float dt = g.softplus ? softplus(x).value : x;
-        const uint32_t grp = ch / g.group_channels;
-        const uint64_t at = ((uint64_t)slot * g.channels + ch) * g.states;
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t n = part * 4 + k;
-            if (n < g.states) {
-                float h = exp2_(dt * (g.a[(uint64_t)ch * g.states + n] * kLog2e)) * g.state[at + n];
-                h = fmaf(dt * u, in(g.b, grp * g.states + n), h);
-                g.state_out[at + n] = h;
-                acc = fmaf(in(g.c, grp * g.states + n), h, acc);
-            }
-        }
+    struct __attribute__((aligned(4 * sizeof(raw)))) Raw4 {
+        raw v[4];
+    };
+    const uint32_t per_row = (g.channels * LANES + 63) / 64;  // waves
+    const uint32_t wave = uniform(blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64);
+    const uint32_t row0 = wave / per_row * g.each_wave;
+    if (row0 >= g.rows) return;
+    const uint32_t rows = g.rows - row0 < g.each_wave ? g.rows - row0 : g.each_wave;
+    const uint32_t id = wave % per_row * 64 + (threadIdx.x & 63), part = id % LANES, n0 = 4 * part;
+    const bool valid = id / LANES < g.channels;  // the others take part in the sums of none
+    const uint32_t ch = valid ? id / LANES : g.channels - 1;
+    const uint32_t bc = ch / g.group_channels * g.states + n0;
+    auto has = [&](int k) { return WIDE || n0 + k < g.states; };
+
+    float a2[4];
+    if constexpr (WIDE) {
+        *(float4*)a2 = *(const float4*)(g.a + (uint64_t)ch * g.states + n0);
+        each<4>([&](auto k) { a2[k] *= kLog2e; });
+    } else {
+        each<4>([&](auto k) { a2[k] = has(k) ? g.a[(uint64_t)ch * g.states + n0 + k] * kLog2e : 0.0f; });
     }
-    for (uint32_t m = 1; m < g.lanes; m *= 2) acc += __shfl_xor(acc, m);
-    if (valid && part == 0) {
-        if (live) {
-            if (g.skip) acc = fmaf(g.skip[ch], u, acc);
-            if (g.z.p) {
-                const float z = T::up(((const raw*)g.z.p)[(int64_t)row * g.z.seq + ch]);
-                acc *= z * sigmoid(z);
+    const float bias = g.bias ? g.bias[ch] : 0.0f, skip = g.skip ? g.skip[ch] : 0.0f;
+
+    struct Row {
+        float h[4], b[4], c[4], u, delta, z;
+        int64_t slot;
+    };
+    auto fetch = [&](Row& r, uint32_t row) {
+        const int64_t slot = g.slots ? g.slots[row] : (int64_t)row;
+        r.slot = slot >= 0 && (uint64_t)slot < g.state_rows ? slot : -1;
+        auto in = [&](const fg_ssm_view& v, uint32_t i) { return T::up(((const raw*)v.p)[(int64_t)row * v.seq + i]); };
+        auto four = [&](float(&x)[4], const fg_ssm_view& v) {
+            if constexpr (WIDE) {
+                const Raw4 q = *(const Raw4*)((const raw*)v.p + (int64_t)row * v.seq + bc);
+                each<4>([&](auto k) { x[k] = T::up(q.v[k]); });
+            } else {
+                each<4>([&](auto k) { x[k] = has(k) ? in(v, bc + k) : 0.0f; });
             }
-        } else {
-            acc = 0.0f;
-        }
-        ((raw*)g.out.p)[(int64_t)row * g.out.seq + ch] = T::down(acc);
+        };
+        if (r.slot < 0) return;
+        const float* from = g.state + ((uint64_t)r.slot * g.channels + ch) * g.states + n0;
+        if constexpr (WIDE) *(float4*)r.h = *(const float4*)from;
+        else each<4>([&](auto k) { r.h[k] = has(k) ? from[k] : 0.0f; });
+        r.u = in(g.u, ch);
+        r.delta = in(g.delta, ch);
+        if (g.z.p) r.z = in(g.z, ch);
+        four(r.b, g.b);
+        four(r.c, g.c);
+    };
+    Row next;
+    fetch(next, row0);
+    for (uint32_t i = 0; i < rows; ++i) {
+        const Row r = next;
+        if (i + 1 < rows) fetch(next, row0 + i + 1);
+        float y = 0.0f;
+        if (r.slot >= 0) {
+            const float x = r.delta + bias, dt = g.softplus ? softplus(x).value : x;
+            float h[4];
+            each<4>([&](auto k) {
+                h[k] = fmaf(exp2_(dt * a2[k]), r.h[k], dt * r.u * r.b[k]);
+                y = has(k) ? fmaf(r.c[k], h[k], y) : y;
+            });
+            float* to = g.state_out + ((uint64_t)r.slot * g.channels + ch) * g.states + n0;
+            if constexpr (WIDE) {
+                if (valid) *(float4*)to = {h[0], h[1], h[2], h[3]};
+            } else {
+                each<4>([&](auto k) {
+                    if (valid && has(k)) to[k] = h[k];
+                });
+            }
+            for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
+            y = fmaf(skip, r.u, y);
+            if (g.z.p) y *= r.z * sigmoid(r.z);
+        }  // a row without a slot: zeros out
+        if (valid && part == 0) ((raw*)g.out.p)[(int64_t)(row0 + i) * g.out.seq + ch] = T::down(y);
     }
 }
 

@@ -31,7 +31,7 @@ public:
 private:
     HipBackend::Module mod_[3];
     HipBackend::KernelHandle conv_step_[3][FG_CONV_MAX_WIDTH + 1][3] = {};  // [dtype][width][8, 4, 1 channels]
-    HipBackend::KernelHandle scan_step_[3] = {};
+    HipBackend::KernelHandle scan_step_[3][5][2] = {};  // [dtype][log2 of a channel's lanes][any, wide]
 };
 
 class ConvPlan {

@@ -53,18 +53,31 @@ MAX_STATES, MAX_WIDTH = 64, 8
 _DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
 _BYTES = {"float32": 4, "bfloat16": 2, "float16": 2}
 _ACTIVATIONS = {"silu": 1, None: 0}
-_dtype_names: dict = {}  # torch dtypes by name, as they come
+_torch_types: dict = {}  # name -> torch dtype, filled when the first tensor comes
+
+
+def _torch_type(dtype: str):
+    t = _torch_types.get(dtype)
+    if t is None:
+        import torch  # a tensor has come, so it is there
+
+        for name in (*_DTYPES, "int32"):
+            _torch_types[name] = getattr(torch, name)
+        t = _torch_types[dtype]
+    return t
 
 
 def _dtype_of(x) -> str:
     d = x.dtype
-    name = _dtype_names.get(d)
-    if name is None:
-        name = _dtype_names[d] = str(d).rpartition(".")[2]
-    return name
+    for name, t in _torch_types.items():
+        if t is d:
+            return name
+    return str(d).rpartition(".")[2]
 
 
 def _check_dtype(dtype) -> str:
+    if dtype in _DTYPES:
+        return dtype
     name = dtype if isinstance(dtype, str) else str(dtype).rpartition(".")[2]
     if name not in _DTYPES:
         raise ValueError(f"dtype must be one of {list(_DTYPES)}, got {dtype}")
@@ -86,9 +99,15 @@ def _address(x, nbytes: int, what: str) -> int:
     return int(x)
 
 
-def _on(x, ordinal: int, what: str) -> None:
+def _wrong(x, what: str, shapes, dtype, ordinal: int):
+    """Why a tensor is refused; called when one of the checks has failed."""
+    if shapes is not None and x.shape not in shapes:
+        return ValueError(f"{what}: shape {tuple(x.shape)}, expected {shapes[0]}")
+    if dtype is not None and _dtype_of(x) != dtype:
+        return ValueError(f"{what}: {_dtype_of(x)}, expected {dtype}")
     if x.get_device() != ordinal:
-        raise ValueError(f"{what}: tensor on {x.device}, the call runs on GPU {ordinal}")
+        return ValueError(f"{what}: tensor on {x.device}, the call runs on GPU {ordinal}")
+    return None
 
 
 def _flat(x, shape: tuple, dtype: str, nbytes: int, ordinal: int, what: str) -> int:
@@ -96,13 +115,10 @@ def _flat(x, shape: tuple, dtype: str, nbytes: int, ordinal: int, what: str) -> 
     if x is None:
         return 0
     if hasattr(x, "data_ptr"):
-        if tuple(x.shape) != shape:
-            raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {shape}")
-        if _dtype_of(x) != dtype:
-            raise ValueError(f"{what}: {_dtype_of(x)}, expected {dtype}")
+        if x.shape != shape or x.dtype is not _torch_type(dtype) or x.get_device() != ordinal:
+            raise _wrong(x, what, (shape,), dtype, ordinal)
         if not x.is_contiguous():
             raise ValueError(f"{what}: tensor is not contiguous")
-        _on(x, ordinal, what)
         return x.data_ptr()
     return _address(x, nbytes, what)
 
@@ -115,7 +131,8 @@ def _bytes(x, nbytes: int, ordinal: int, what: str) -> int:
         if x.numel() * x.element_size() < nbytes or not x.is_contiguous():
             raise ValueError(f"{what}: tensor of {x.numel() * x.element_size()} bytes (contiguous: "
                              f"{x.is_contiguous()}), the call reads or writes {nbytes} contiguous bytes")
-        _on(x, ordinal, what)
+        if x.get_device() != ordinal:
+            raise _wrong(x, what, None, None, ordinal)
         return x.data_ptr()
     return _address(x, nbytes, what)
 
@@ -127,19 +144,19 @@ def _rows(x, lead: tuple, width: int, inner: tuple, dtype: str, ordinal: int, wh
         return 0, 0, 0
     n = len(lead)
     if hasattr(x, "data_ptr"):
-        shape = tuple(x.shape)
         st = x.stride()
-        if shape == lead + (width,):
-            fine = width == 1 or st[n] == 1
-        elif shape == lead + inner:
+        if x.dtype is not _torch_type(dtype) or x.get_device() != ordinal:
+            fine = None
+        elif x.shape == (*lead, width):
+            fine = st[n] == 1 or width == 1
+        elif inner and x.shape == lead + inner:
             fine = (inner[1] == 1 or st[n + 1] == 1) and (inner[0] == 1 or st[n] == inner[1])
         else:
-            raise ValueError(f"{what}: shape {shape}, expected {lead + (width,)}")
+            fine = None
+        if fine is None:
+            raise _wrong(x, what, (lead + (width,), lead + inner), dtype, ordinal)
         if not fine:
             raise ValueError(f"{what}: the elements of a row must be adjacent (strides {tuple(st)})")
-        if _dtype_of(x) != dtype:
-            raise ValueError(f"{what}: {_dtype_of(x)}, expected {dtype}")
-        _on(x, ordinal, what)
         return (x.data_ptr(), st[0], st[1]) if n == 2 else (x.data_ptr(), 0, st[0])
     rows = lead[0] * lead[1] if n == 2 else lead[0]
     p = _address(x, rows * width * _BYTES[dtype], what)

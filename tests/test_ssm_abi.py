@@ -124,7 +124,8 @@ def test_every_kernel_that_the_host_looks_up_is_instantiated():
     for t, most in (("f32", 4), ("bf16", 8), ("f16", 8)):
         for s, tail in itertools.product(("s1w1", "s2w1", "s4w1", "s4w2", "s4w4"), ("", "_any")):
             names += [f"fg_scan_{k}{t}_{s}{tail}" for k in ("", "local_", "back_", "back_local_")]
-        names += [f"fg_scan_reduce_bc_{t}", f"fg_scan_step_{t}"]
+        names += [f"fg_scan_reduce_bc_{t}"]
+        names += [f"fg_scan_step_{t}_l{n}{tail}" for n in (1, 2, 4, 8, 16) for tail in ("", "_any")]
         for w in range(2, ssm.MAX_WIDTH + 1):
             names += [f"fg_conv_{k}{t}_w{w}_v{n}" for k in ("", "step_")
                       for n in {1, 4, most if w <= 4 else 4}]
