@@ -139,11 +139,9 @@ struct Scan {
         p.tok = e / 16;
         p.sub = e % 16;
         const uint32_t blocks = g.groups * g.group_blocks;
-        // Workgroups go to the 8 XCDs in turn; neighbouring channels, which
-        // share cache lines and B and C, go to the same one.
-        const uint32_t all_blocks = gridDim.x, per = all_blocks / 8, eighth = blockIdx.x % 8;
-        const uint32_t id = blockIdx.x < per * 8 ? eighth * per + blockIdx.x / 8 : blockIdx.x;
-        const uint32_t cb = id % blocks, rest = id / blocks;
+        // Workgroups go to the 8 XCDs in turn, which spreads packed sequences'
+        // unequal parts; in whole lines, neighbours share only B and C.
+        const uint32_t cb = blockIdx.x % blocks, rest = blockIdx.x / blocks;
         p.group = cb / g.group_blocks;
         p.block = cb % g.group_blocks;
         p.chunk = rest % g.chunks;

@@ -115,11 +115,12 @@ public:
 private:
     static bool apart(const Extent& a, const Extent& b) {
         if (a.p + a.bytes <= b.p || b.p + b.bytes <= a.p) return true;
-        // column windows of one array: the same strides, and the windows apart within a row
-        if (a.row <= 0 || a.row != b.row || a.seq != b.seq || a.seq % a.row) return false;
-        int64_t off = (b.p - a.p) % a.row;
-        if (off < 0) off += a.row;
-        return off >= a.width && off + b.width <= a.row;
+        // column windows of one array: the same strides, and the windows apart within the smaller one
+        const int64_t step = a.row > 0 ? a.row : a.seq;
+        if (step <= 0 || a.row != b.row || a.seq != b.seq || a.seq % step) return false;
+        int64_t off = (b.p - a.p) % step;
+        if (off < 0) off += step;
+        return off >= a.width && off + b.width <= step;
     }
     void add(const Extent& e) {
         for (int i = 0; i < n_; ++i) {
@@ -425,10 +426,11 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     const char* op = "scan plan";
     check_dtype(op, s.dtype);
     check_sequences(op, s.sequences, s.length, s.tokens, s.packed);
-    check_range(op, "channels", s.channels, 1, kMaxCount);
+    check_range(op, "channels", s.channels, 1, kMaxRowStride);
     check_range(op, "states", s.states, 1, FG_SSM_MAX_STATES);
     check_range(op, "groups", s.groups, 1, s.channels);
     if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
+    check_range(op, "groups * states", s.groups * s.states, 1, kMaxRowStride);
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     segment_ = FG_SSM_SEGMENT;
     lane_states_ = s.states <= 4 ? 1 : s.states <= 8 ? 2 : 4;
@@ -465,13 +467,15 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
 // bfloat16, parts 1 / 2 / 4: forward, 1024 tokens x 2048 channels (512 waves)
 // 88 / 87 / 78, 2048 x 4096 (1024 waves) 177 / 256; backward, 1024 x 2048
 // (parts 2 / 4) 204 / 157.  A part has 64 tokens or more.  Packed sequences count
-// as so many of the longest's length, which the last wave to end works through.
+// as so many of the longest's length, which the last wave to end works through,
+// and are cut into twice the parts, which evens them out (7 sequences, 9001
+// tokens x 1536 channels x 8 states in float16: 136 us, twice the parts 97).
 uint32_t ScanPlan::chunks_for(uint32_t few) const {
     const uint64_t seqs = s_.packed && s_.length ? ceil_div(s_.tokens, s_.length) : s_.sequences;
     const uint64_t waves = std::max<uint64_t>(1, seqs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_);
     if (waves > few) return 1;
     const uint64_t most = std::max<uint64_t>(1, ceil_div(s_.length, 4 * segment_));
-    return (uint32_t)std::min<uint64_t>({ceil_div(2048, waves), most, 64});
+    return (uint32_t)std::min<uint64_t>({ceil_div(s_.packed ? 4096 : 2048, waves), most, 64});
 }
 
 size_t ScanPlan::checkpoint_bytes() const {

@@ -215,6 +215,53 @@ def test_step(gpu_device, batch, channels, width, dtype):
             assert torch.equal(dst.cpu(), st)
 
 
+def test_long_runs_and_many_rows(gpu_device):
+    """Tokens enough for a thread's longest run forward, and rows enough for a
+    wave to walk through several."""
+    import ferrum_gpu
+    rng = np.random.default_rng(31)
+    length, channels, width = 270001, 8, 4
+    x, gy = (_rounded(rng, (1, length, channels), "float32") for _ in range(2))
+    w = torch.from_numpy(rng.standard_normal((channels, width))).float()
+    out, gx, gw = _fill(x.shape, "float32"), _fill(x.shape, "float32"), _fill(w.shape, "float32")
+    dx, dgy, dw = x.cuda(), gy.cuda(), w.cuda()
+    plan = ferrum_gpu.ssm.ConvPlan(1, length, channels, width, gpu_device, dtype="float32")
+    rows = torch.empty(length, channels, device="cuda")
+    state = _rounded(rng, (length, width - 1, channels), "float32").cuda()
+    before, new = state.clone(), torch.empty_like(state)
+    torch.cuda.synchronize()
+    plan.forward(dx, dw, out)
+    plan.backward(dx, dw, dgy, grad_x=gx, grad_weight=gw)
+    ferrum_gpu.ssm.conv_step(gpu_device, dx[0], dw, state, rows, state_out=new)
+    _done(gpu_device)
+    r, m = (o.conv(_np(x[0]), _np(w), grad=_np(gy[0]), magnitude=q) for q in (False, True))
+    o.within(_np(out[0]), r["out"], m["out"], _rounds(width), "float32", "out")
+    o.within(_np(gx[0]), r["x"], m["x"], _rounds(width), "float32", "grad_x")
+    # the sums run in parts: at most 64 tokens, then eight running sums of the parts in each of four waves
+    o.within(_np(gw), r["weight"], m["weight"], _rounds(width, length), "float32", "grad_weight")
+    win = np.concatenate([_np(before), _np(x[0])[:, None]], 1)
+    p, mp = ((q(win) * q(_np(w)).T).sum(1) for q in (lambda v: v, np.abs))
+    o.within(_np(rows), p * o.sigmoid(p), mp, _rounds(width), "float32", "step")
+    assert np.array_equal(_np(new), win[:, 1:]) and torch.equal(state, before)
+
+
+def test_windows_of_one_array(gpu_device):
+    """One token of each row: input and output that are columns of one array."""
+    import ferrum_gpu
+    big = torch.randn(3, 1, 64, device="cuda")
+    w, st = torch.randn(32, 4, device="cuda"), torch.randn(3, 3, 32, device="cuda")
+    want, new = torch.empty(3, 1, 32, device="cuda"), torch.empty_like(st)
+    plan = ferrum_gpu.ssm.ConvPlan(3, 1, 32, 4, gpu_device, dtype="float32")
+    torch.cuda.synchronize()
+    plan.forward(big[..., :32].contiguous(), w, want, initial=st)
+    plan.forward(big[..., :32], w, big[..., 32:], initial=st)
+    _done(gpu_device)
+    assert torch.equal(big[..., 32:], want)
+    ferrum_gpu.ssm.conv_step(gpu_device, big[:, 0, :32], w, st, big[:, 0, 32:], state_out=new)
+    _done(gpu_device)
+    assert torch.equal(big[..., 32:], want)
+
+
 def test_prompt_then_tokens(gpu_device):
     """A prompt and single tokens after it are the whole sequence."""
     import ferrum_gpu

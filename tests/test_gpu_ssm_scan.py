@@ -131,7 +131,8 @@ def _check(dev, rng, batch, length, channels, states, groups, dtype, use_softplu
 @pytest.mark.parametrize("batch,length,channels,states,groups", [
     (1, 1, 16, 16, 1), (2, 2, 64, 16, 1), (1, 3, 1, 1, 1), (3, 15, 15, 3, 1), (2, 16, 17, 4, 1), (1, 17, 70, 5, 1),
     (2, 33, 130, 8, 2), (1, 64, 48, 13, 3), (2, 65, 64, 16, 2), (1, 100, 20, 17, 1), (2, 29, 24, 24, 2),
-    (1, 37, 33, 33, 1), (2, 23, 70, 64, 1), (1, 300, 32, 16, 1), (1, 517, 16, 2, 1), (5, 9, 80, 16, 5)])
+    (1, 37, 33, 33, 1), (2, 23, 70, 64, 1), (1, 300, 32, 16, 1), (1, 517, 16, 2, 1), (5, 9, 80, 16, 5),
+    (1, 300, 16, 40, 1), (2, 210, 36, 24, 2), (1, 260, 48, 32, 1), (1, 145, 8, 4, 1)])
 def test_sizes(gpu_device, batch, length, channels, states, groups, dtype):
     print(f"[case] scan {batch}x{length}x{channels}x{states} groups={groups} {dtype}", flush=True)
     _check(gpu_device, np.random.default_rng(length * 100 + states), batch, length, channels, states, groups, dtype)
@@ -145,7 +146,7 @@ def test_layouts_and_options(gpu_device, layout, use_softplus, without):
     _check(gpu_device, np.random.default_rng(8), 3, 45, 40, 16, 2, "float32", use_softplus, without, layout)
 
 
-@pytest.mark.parametrize("states,longest", [(16, 70), (6, 70), (24, 70), (16, 400)])
+@pytest.mark.parametrize("states,longest", [(16, 70), (6, 70), (24, 70), (16, 400), (33, 400), (8, 400)])
 def test_packed(gpu_device, states, longest):
     """Empty, one-token and longer sequences that end inside a segment, rows
     that belong to none (NaN there reaches nothing; outputs stay as they were)."""
@@ -399,6 +400,66 @@ def test_step(gpu_device, batch, channels, states, groups, dtype):
             assert torch.equal(state.cpu(), st)
 
 
+def test_step_many_rows(gpu_device):
+    """Rows enough for a wave to walk through several, the last wave fewer."""
+    import ferrum_gpu
+    rng = np.random.default_rng(21)
+    batch, channels, states = 33001, 16, 16
+    i = _inputs(rng, (batch,), channels, states, 1, "float32", batch)
+    d = {k: v.cuda() for k, v in i.items()}
+    out, slots = _fill((batch, channels)), torch.from_numpy(rng.permutation(batch).astype(np.int32)).cuda()
+    slots[5], slots[batch - 1] = -1, batch
+    state = d["initial"].clone()
+    torch.cuda.synchronize()
+    ferrum_gpu.ssm.scan_step(gpu_device, d["u"], d["delta"], d["A"], d["B"], d["C"], state, out, D=d["D"], z=d["z"],
+                             delta_bias=d["delta_bias"], slots=slots)
+    _done(gpu_device)
+    n = {k: _np(v) for k, v in i.items()}
+    s = slots.cpu().numpy()
+    on = (s >= 0) & (s < batch)
+    dt = o.softplus(n["delta"] + n["delta_bias"])
+    a = np.exp(dt[:, :, None] * n["A"])
+    prior = n["initial"][np.where(on, s, 0)]
+    want, m = ((f(a * prior) if f is np.abs else a * prior) + f((dt * n["u"])[:, :, None] * n["B"][:, 0][:, None])
+               for f in (lambda v: v, np.abs))
+    rounds = o.scan_rounds(1, n["A"], float(dt.max()), states)
+    after = _np(state)
+    o.within(after[s[on]], want[on], m[on], rounds, "float32", "state")
+    untouched = np.ones(batch, bool)
+    untouched[s[on]] = False
+    assert np.array_equal(after[untouched], n["initial"][untouched])
+    gate = n["z"] * o.sigmoid(n["z"])
+    y = ((want * n["C"][:, 0][:, None]).sum(-1) + n["D"] * n["u"]) * gate
+    my = ((m * np.abs(n["C"][:, 0][:, None])).sum(-1) + np.abs(n["D"] * n["u"])) * np.abs(gate)
+    o.within(_np(out)[on], y[on], my[on], rounds, "float32", "out")
+    assert (_np(out)[~on] == 0).all()
+
+
+def test_windows_of_one_array(gpu_device):
+    """One token of each row: inputs and outputs that are columns of one array."""
+    import ferrum_gpu
+    d, n = 32, 16
+    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(2), (3, 1), d, n, 1, "float32", 3).items()}
+    big = torch.zeros(3, 1, 4 * d + 2 * n, device="cuda")
+    big[..., :d], big[..., d:2 * d], big[..., 2 * d:3 * d] = i["u"], i["delta"], i["z"]
+    big[..., 4 * d:4 * d + n], big[..., 4 * d + n:] = i["B"][:, :, 0], i["C"][:, :, 0]
+    plan = ferrum_gpu.ssm.ScanPlan(3, 1, d, n, gpu_device, dtype="float32")
+    want, state = torch.empty_like(i["u"]), i["initial"].clone()
+    cols = [big[..., k * d:(k + 1) * d] for k in range(4)]
+    b, c = big[..., 4 * d:4 * d + n], big[..., 4 * d + n:]
+    torch.cuda.synchronize()
+    plan.forward(i["u"], i["delta"], i["A"], i["B"], i["C"], want, z=i["z"], initial=i["initial"])
+    plan.forward(cols[0], cols[1], i["A"], b, c, cols[3], z=cols[2], initial=i["initial"])
+    _done(gpu_device)
+    assert torch.equal(cols[3], want)
+    cols[3].zero_()
+    torch.cuda.synchronize()
+    ferrum_gpu.ssm.scan_step(gpu_device, cols[0][:, 0], cols[1][:, 0], i["A"], b[:, 0], c[:, 0], state, cols[3][:, 0],
+                             z=cols[2][:, 0])
+    _done(gpu_device)
+    assert torch.allclose(cols[3], want, rtol=1e-5, atol=1e-5)
+
+
 def test_prompt_then_tokens(gpu_device):
     """A prompt and single tokens after it are the whole sequence, within what
     32 bits leave."""
@@ -526,6 +587,9 @@ def test_refusals(gpu_device):
             make(**bad)
     with pytest.raises(E, match="groups must divide"):
         make(groups=3)
+    for bad in (dict(channels=(1 << 25) + 8), dict(channels=1 << 25, groups=1 << 24)):
+        with pytest.raises(E, match="must be in"):
+            make(length=1, batch=1, **bad)
     plan = make()
     x, out = torch.zeros(2, 8, 16, device="cuda"), torch.zeros(2, 8, 16, device="cuda")
     A, D = torch.zeros(16, 4, device="cuda"), torch.zeros(16, device="cuda")
