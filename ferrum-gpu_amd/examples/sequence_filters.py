@@ -108,6 +108,7 @@ class Block:
 def main(device=None) -> dict:
     """Runs the block all three ways and returns how far they are apart."""
     device = device or ferrum_gpu.hip.Device(0)
+    torch.manual_seed(0)
     block = Block(device)
     batch, length, more, rows = 3, 50, 8, 5
     x = torch.randn(batch, length + more, block.channels, device="cuda")

@@ -12,6 +12,14 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+import gpu_tensor  # noqa: E402
+from gpu_tensor import Far, fill, like, same, up, values  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def _on_gpu(gpu_device):
+    yield from gpu_tensor.use(gpu_device)
+
 
 def _type(dtype):
     return getattr(torch, dtype)
@@ -21,22 +29,9 @@ def _rounded(rng, shape, dtype, scale=1.0):
     return (torch.from_numpy(rng.standard_normal(shape)) * scale).to(_type(dtype))
 
 
-def _np(x):
-    return x.detach().double().cpu().numpy()
-
-
 def _rounds(width, summed=1):
     # products and sums of the taps, the bias, the activation and its slope (at most 30 between them)
     return 2 * width + summed + 32
-
-
-def _fill(shape, dtype, value=7.0):
-    return torch.full(shape, value, dtype=_type(dtype), device="cuda")
-
-
-def _done(dev):
-    dev.sync()
-    torch.cuda.synchronize()
 
 
 def _check(dev, rng, batch, length, channels, width, dtype, silu=True, bias=True, state=True, layout="plain"):
@@ -48,41 +43,39 @@ def _check(dev, rng, batch, length, channels, width, dtype, silu=True, bias=True
     ini, gf = ((_rounded(rng, (batch, width - 1, channels), dtype) if state else None) for _ in range(2))
 
     def laid(v, room=False):
-        v = v.cuda() if not room else _fill(v.shape, dtype)
+        v = torch.full_like(v, 7) if room else v
         if layout == "window":    # a column window of a wider array
-            big = _fill(v.shape[:2] + (2 * channels + 3,), dtype)
+            big = torch.full(v.shape[:2] + (2 * channels + 3,), 7.0, dtype=v.dtype)
             big[..., channels + 1:2 * channels + 1] = v
-            return big[..., channels + 1:2 * channels + 1]
+            return up(big[..., channels + 1:2 * channels + 1])
         if layout == "tokens":    # tokens before sequences
-            return v.transpose(0, 1).contiguous().transpose(0, 1)
-        return v
+            return up(v.transpose(0, 1).contiguous().transpose(0, 1))
+        return up(v)
 
     dx, dgy, out, gx = laid(x), laid(gy), laid(x, True), laid(x, True)
-    fin, gini = (_fill((batch, width - 1, channels), dtype) if state else None for _ in range(2))
-    gw, gb = _fill((channels, width), "float32"), _fill((channels,), "float32")
-    cuda = lambda v: None if v is None else v.cuda()  # noqa: E731
-    dw, db, dini, dgf = cuda(w), cuda(b), cuda(ini), cuda(gf)
+    fin, gini = (fill((batch, width - 1, channels), dtype) if state else None for _ in range(2))
+    gw, gb = fill((channels, width), "float32"), fill((channels,), "float32")
+    dw, db, dini, dgf = up(w), up(b), up(ini), up(gf)
     plan = ferrum_gpu.ssm.ConvPlan(batch, length, channels, width, dev, dtype=dtype,
                                    activation="silu" if silu else None)
-    torch.cuda.synchronize()
     plan.forward(dx, dw, out, bias=db, initial=dini, final=fin)
     plan.backward(dx, dw, dgy, grad_x=gx, grad_weight=gw, grad_bias=gb, bias=db, initial=dini, grad_initial=gini,
                   grad_final=dgf)
-    _done(dev)
+    dev.sync()
     tw, tb = np.zeros((channels, width)), np.zeros(channels)
     mw, mb = tw.copy(), tb.copy()
     for s in range(batch):
-        args = dict(x=_np(x[s]), w=_np(w), bias=None if b is None else _np(b), initial=None if ini is None else
-                    _np(ini[s]), silu=silu, grad=_np(gy[s]), grad_final=None if gf is None else _np(gf[s]))
+        args = dict(x=values(x[s]), w=values(w), bias=None if b is None else values(b), initial=None if ini is None else
+                    values(ini[s]), silu=silu, grad=values(gy[s]), grad_final=None if gf is None else values(gf[s]))
         r, m = o.conv(**args), o.conv(**args, magnitude=True)
-        o.within(_np(out[s]), r["out"], m["out"], _rounds(width), dtype, "out")
-        o.within(_np(gx[s]), r["x"], m["x"], _rounds(width), dtype, "grad_x")
+        o.within(values(out[s]), r["out"], m["out"], _rounds(width), dtype, "out")
+        o.within(values(gx[s]), r["x"], m["x"], _rounds(width), dtype, "grad_x")
         if state:
-            assert np.array_equal(_np(fin[s]), r["final"])
-            o.within(_np(gini[s]), r["initial"], m["initial"], _rounds(width), dtype, "grad_initial")
+            assert np.array_equal(values(fin[s]), r["final"])
+            o.within(values(gini[s]), r["initial"], m["initial"], _rounds(width), dtype, "grad_initial")
         tw, tb, mw, mb = tw + r["weight"], tb + r["bias"], mw + m["weight"], mb + m["bias"]
-    o.within(_np(gw), tw, mw, _rounds(width, batch * length), "float32", "grad_weight")
-    o.within(_np(gb), tb, mb, _rounds(width, batch * length), "float32", "grad_bias")
+    o.within(values(gw), tw, mw, _rounds(width, batch * length), "float32", "grad_weight")
+    o.within(values(gb), tb, mb, _rounds(width, batch * length), "float32", "grad_bias")
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
@@ -117,64 +110,60 @@ def test_packed(gpu_device, channels):
     w, b = torch.from_numpy(rng.standard_normal((channels, width))).float(), torch.zeros(channels)
     ini = _rounded(rng, (len(used), width - 1, channels), "float32")
     plan = ferrum_gpu.ssm.ConvPlan(len(used), longest, channels, width, gpu_device, dtype="float32", tokens=tokens)
-    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
-    out, gx, fin = _fill(x.shape, "float32"), _fill(x.shape, "float32"), _fill(ini.shape, "float32")
-    gw = _fill(w.shape, "float32")
-    dx, dgy, dw, db, dini = x.cuda(), gy.cuda(), w.cuda(), b.cuda(), ini.cuda()
-    torch.cuda.synchronize()
+    off = up(torch.tensor(offsets, dtype=torch.int32))
+    out, gx, fin = fill(x.shape, "float32"), fill(x.shape, "float32"), fill(ini.shape, "float32")
+    gw = fill(w.shape, "float32")
+    dx, dgy, dw, db, dini = up(x), up(gy), up(w), up(b), up(ini)
     plan.forward(dx, dw, out, bias=db, initial=dini, final=fin, offsets=off)
     plan.backward(dx, dw, dgy, grad_x=gx, grad_weight=gw, bias=db, initial=dini, offsets=off)
-    _done(gpu_device)
+    gpu_device.sync()
     tw, mw = 0, 0
     touched = np.zeros(tokens, bool)
     for s, (i, j) in enumerate(used):
         touched[i:j] = True
-        args = dict(x=_np(x[i:j]), w=_np(w), bias=_np(b), initial=_np(ini[s]), grad=_np(gy[i:j]))
+        args = dict(x=values(x[i:j]), w=values(w), bias=values(b), initial=values(ini[s]), grad=values(gy[i:j]))
         r, m = o.conv(**args), o.conv(**args, magnitude=True)
-        o.within(_np(out[i:j]), r["out"], m["out"], _rounds(width), "float32", "out")
-        o.within(_np(gx[i:j]), r["x"], m["x"], _rounds(width), "float32", "grad_x")
-        assert np.array_equal(_np(fin[s]), r["final"])
+        o.within(values(out[i:j]), r["out"], m["out"], _rounds(width), "float32", "out")
+        o.within(values(gx[i:j]), r["x"], m["x"], _rounds(width), "float32", "grad_x")
+        assert np.array_equal(values(fin[s]), r["final"])
         tw, mw = tw + r["weight"], mw + m["weight"]
-    o.within(_np(gw), tw, mw, _rounds(width, tokens), "float32", "grad_weight")
-    assert (out[~torch.from_numpy(touched).cuda()] == 7).all() and (gx[~torch.from_numpy(touched).cuda()] == 7).all()
+    o.within(values(gw), tw, mw, _rounds(width, tokens), "float32", "grad_weight")
+    assert all((v.get()[torch.from_numpy(~touched)] == 7).all() for v in (out, gx))
     # taken as the nearest valid ones: rows -5 .. 4 are 0 .. 4, 60 .. 500 are 60 .. 90, and 500 .. 60 are none
     off.copy_(torch.tensor([-5, 4, 60, 500, 60, 60, 60], dtype=torch.int32))
     out.fill_(7)
-    torch.cuda.synchronize()
     plan.forward(dx, dw, out, bias=db, initial=dini, offsets=off)
-    _done(gpu_device)
-    want = o.conv(_np(x[4:60][:longest]), _np(w), _np(b), _np(ini[1]))["out"]
-    assert np.allclose(_np(out[4:4 + longest]), want, rtol=1e-4, atol=1e-4)
+    gpu_device.sync()
+    want = o.conv(values(x[4:60][:longest]), values(w), values(b), values(ini[1]))["out"]
+    assert np.allclose(values(out[4:4 + longest]), want, rtol=1e-4, atol=1e-4)
     assert (out[4 + longest:60] == 7).all()
 
 
 def test_no_tokens(gpu_device):
     """No sequences, or sequences without tokens: states pass through, parameter gradients are zeros."""
     import ferrum_gpu
-    w = torch.ones(8, 3, device="cuda")
+    w = up(torch.ones(8, 3))
     for batch, length in ((0, 5), (2, 0)):
-        x = torch.empty(batch, length, 8, device="cuda")
-        ini = torch.randn(batch, 2, 8, device="cuda")
-        fin, gini, gw = _fill((batch, 2, 8), "float32"), _fill((batch, 2, 8), "float32"), _fill((8, 3), "float32")
+        x = fill((batch, length, 8))
+        ini = up(torch.randn(batch, 2, 8))
+        fin, gini, gw = fill((batch, 2, 8), "float32"), fill((batch, 2, 8), "float32"), fill((8, 3), "float32")
         plan = ferrum_gpu.ssm.ConvPlan(batch, length, 8, 3, gpu_device, dtype="float32")
-        torch.cuda.synchronize()
-        plan.forward(x, w, torch.empty_like(x), initial=ini, final=fin)
-        plan.backward(x, w, torch.empty_like(x), grad_weight=gw, initial=ini, grad_initial=gini, grad_final=ini)
-        _done(gpu_device)
-        assert torch.equal(fin, ini) and torch.equal(gini, ini) and (gw == 0).all()
+        plan.forward(x, w, like(x), initial=ini, final=fin)
+        plan.backward(x, w, like(x), grad_weight=gw, initial=ini, grad_initial=gini, grad_final=ini)
+        gpu_device.sync()
+        assert same(fin, ini) and same(gini, ini) and (gw == 0).all()
 
 
 def test_final_may_be_initial(gpu_device):
     import ferrum_gpu
-    x = torch.randn(2, 1, 64, device="cuda")
-    state = torch.randn(2, 4, 64, device="cuda")
-    want = torch.cat([state, x], 1)[:, 1:]
-    w, out = torch.randn(64, 5, device="cuda"), torch.empty_like(x)
+    x = up(torch.randn(2, 1, 64))
+    state = up(torch.randn(2, 4, 64))
+    want = torch.cat([state.get(), x.get()], 1)[:, 1:]
+    w, out = up(torch.randn(64, 5)), like(x)
     plan = ferrum_gpu.ssm.ConvPlan(2, 1, 64, 5, gpu_device, dtype="float32")
-    torch.cuda.synchronize()
     plan.forward(x, w, out, initial=state, final=state)
-    _done(gpu_device)
-    assert torch.equal(state, want)
+    gpu_device.sync()
+    assert same(state, want)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
@@ -192,27 +181,26 @@ def test_step(gpu_device, batch, channels, width, dtype):
     if batch > 2:
         slots[0], slots[1] = -1, rows
     for in_place in (True, False):
-        dst, out = st.cuda(), _fill((batch, channels), dtype)
+        dst, out = up(st), fill((batch, channels), dtype)
         new = None if in_place else dst.clone()
-        wide = _fill((batch, 2 * channels), dtype)
+        wide = fill((batch, 2 * channels), dtype)
         wide[:, channels:] = x
-        args = w.cuda(), b.cuda(), torch.from_numpy(slots).cuda()
-        torch.cuda.synchronize()
+        args = up(w), up(b), up(torch.from_numpy(slots))
         ferrum_gpu.ssm.conv_step(gpu_device, wide[:, channels:], args[0], dst, out, bias=args[1], slots=args[2],
                                  state_out=new)
-        _done(gpu_device)
-        want_state = _np(st)
+        gpu_device.sync()
+        want_state = values(st)
         for i, s in enumerate(slots):
             if s < 0 or s >= rows:
                 assert (out[i] == 0).all()
                 continue
-            a = dict(x=_np(x[i])[None], w=_np(w), bias=_np(b), initial=_np(st[s]))
+            a = dict(x=values(x[i])[None], w=values(w), bias=values(b), initial=values(st[s]))
             r, m = o.conv(**a), o.conv(**a, magnitude=True)
-            o.within(_np(out[i]), r["out"][0], m["out"][0], _rounds(width), dtype, "out")
+            o.within(values(out[i]), r["out"][0], m["out"][0], _rounds(width), dtype, "out")
             want_state[s] = r["final"]
-        assert np.array_equal(_np(dst if in_place else new), want_state)
+        assert np.array_equal(values(dst if in_place else new), want_state)
         if not in_place:
-            assert torch.equal(dst.cpu(), st)
+            assert same(dst, st)
 
 
 def test_long_runs_and_many_rows(gpu_device):
@@ -223,62 +211,60 @@ def test_long_runs_and_many_rows(gpu_device):
     length, channels, width = 270001, 8, 4
     x, gy = (_rounded(rng, (1, length, channels), "float32") for _ in range(2))
     w = torch.from_numpy(rng.standard_normal((channels, width))).float()
-    out, gx, gw = _fill(x.shape, "float32"), _fill(x.shape, "float32"), _fill(w.shape, "float32")
-    dx, dgy, dw = x.cuda(), gy.cuda(), w.cuda()
+    out, gx, gw = fill(x.shape, "float32"), fill(x.shape, "float32"), fill(w.shape, "float32")
+    dx, dgy, dw = up(x), up(gy), up(w)
     plan = ferrum_gpu.ssm.ConvPlan(1, length, channels, width, gpu_device, dtype="float32")
-    rows = torch.empty(length, channels, device="cuda")
-    state = _rounded(rng, (length, width - 1, channels), "float32").cuda()
-    before, new = state.clone(), torch.empty_like(state)
-    torch.cuda.synchronize()
+    rows = fill((length, channels))
+    state = _rounded(rng, (length, width - 1, channels), "float32")
+    before, state = state, up(state)
+    new = like(state)
     plan.forward(dx, dw, out)
     plan.backward(dx, dw, dgy, grad_x=gx, grad_weight=gw)
     ferrum_gpu.ssm.conv_step(gpu_device, dx[0], dw, state, rows, state_out=new)
-    _done(gpu_device)
-    r, m = (o.conv(_np(x[0]), _np(w), grad=_np(gy[0]), magnitude=q) for q in (False, True))
-    o.within(_np(out[0]), r["out"], m["out"], _rounds(width), "float32", "out")
-    o.within(_np(gx[0]), r["x"], m["x"], _rounds(width), "float32", "grad_x")
+    gpu_device.sync()
+    r, m = (o.conv(values(x[0]), values(w), grad=values(gy[0]), magnitude=q) for q in (False, True))
+    o.within(values(out[0]), r["out"], m["out"], _rounds(width), "float32", "out")
+    o.within(values(gx[0]), r["x"], m["x"], _rounds(width), "float32", "grad_x")
     # the sums run in parts: at most 64 tokens, then eight running sums of the parts in each of four waves
-    o.within(_np(gw), r["weight"], m["weight"], _rounds(width, length), "float32", "grad_weight")
-    win = np.concatenate([_np(before), _np(x[0])[:, None]], 1)
-    p, mp = ((q(win) * q(_np(w)).T).sum(1) for q in (lambda v: v, np.abs))
-    o.within(_np(rows), p * o.sigmoid(p), mp, _rounds(width), "float32", "step")
-    assert np.array_equal(_np(new), win[:, 1:]) and torch.equal(state, before)
+    o.within(values(gw), r["weight"], m["weight"], _rounds(width, length), "float32", "grad_weight")
+    win = np.concatenate([values(before), values(x[0])[:, None]], 1)
+    p, mp = ((q(win) * q(values(w)).T).sum(1) for q in (lambda v: v, np.abs))
+    o.within(values(rows), p * o.sigmoid(p), mp, _rounds(width), "float32", "step")
+    assert np.array_equal(values(new), win[:, 1:]) and same(state, before)
 
 
 def test_windows_of_one_array(gpu_device):
     """One token of each row: input and output that are columns of one array."""
     import ferrum_gpu
-    big = torch.randn(3, 1, 64, device="cuda")
-    w, st = torch.randn(32, 4, device="cuda"), torch.randn(3, 3, 32, device="cuda")
-    want, new = torch.empty(3, 1, 32, device="cuda"), torch.empty_like(st)
+    big = up(torch.randn(3, 1, 64))
+    w, st = up(torch.randn(32, 4)), up(torch.randn(3, 3, 32))
+    want, new = fill((3, 1, 32)), like(st)
     plan = ferrum_gpu.ssm.ConvPlan(3, 1, 32, 4, gpu_device, dtype="float32")
-    torch.cuda.synchronize()
-    plan.forward(big[..., :32].contiguous(), w, want, initial=st)
+    plan.forward(up(big.get()[..., :32].contiguous()), w, want, initial=st)
     plan.forward(big[..., :32], w, big[..., 32:], initial=st)
-    _done(gpu_device)
-    assert torch.equal(big[..., 32:], want)
+    gpu_device.sync()
+    assert same(big[..., 32:], want)
     ferrum_gpu.ssm.conv_step(gpu_device, big[:, 0, :32], w, st, big[:, 0, 32:], state_out=new)
-    _done(gpu_device)
-    assert torch.equal(big[..., 32:], want)
+    gpu_device.sync()
+    assert same(big[..., 32:], want)
 
 
 def test_prompt_then_tokens(gpu_device):
     """A prompt and single tokens after it are the whole sequence."""
     import ferrum_gpu
     batch, length, channels, width, more = 2, 9, 48, 4, 5
-    x = torch.randn(batch, length + more, channels, device="cuda")
-    w = torch.randn(channels, width, device="cuda")
-    whole, out = torch.empty_like(x), torch.empty_like(x)
-    state = torch.empty(batch, width - 1, channels, device="cuda")
+    x = up(torch.randn(batch, length + more, channels))
+    w = up(torch.randn(channels, width))
+    whole, out = like(x), like(x)
+    state = fill((batch, width - 1, channels))
     ssm = ferrum_gpu.ssm
-    torch.cuda.synchronize()
     ssm.ConvPlan(batch, length + more, channels, width, gpu_device, dtype="float32").forward(x, w, whole)
     plan = ssm.ConvPlan(batch, length, channels, width, gpu_device, dtype="float32")
     plan.forward(x[:, :length], w, out[:, :length], final=state)
     for t in range(length, length + more):
         ssm.conv_step(gpu_device, x[:, t], w, state, out[:, t])
-    _done(gpu_device)
-    assert torch.equal(out, whole)
+    gpu_device.sync()
+    assert same(out, whole)
 
 
 def test_refusals(gpu_device):
@@ -293,16 +279,16 @@ def test_refusals(gpu_device):
     with pytest.raises(ValueError, match="dtype"):
         make(dtype="float64")
     plan = make()
-    x, out = torch.zeros(2, 8, 16, device="cuda"), torch.zeros(2, 8, 16, device="cuda")
-    w, b = torch.zeros(16, 4, device="cuda"), torch.zeros(16, device="cuda")
-    st = torch.zeros(2, 3, 16, device="cuda")
-    big = torch.zeros(2, 8, 32, device="cuda")
+    x, out = up(torch.zeros(2, 8, 16)), up(torch.zeros(2, 8, 16))
+    w, b = up(torch.zeros(16, 4)), up(torch.zeros(16))
+    st = up(torch.zeros(2, 3, 16))
+    big = up(torch.zeros(2, 8, 32))
     with pytest.raises(ValueError, match="shape"):
         plan.forward(x[:, :7], w, out)
     with pytest.raises(ValueError, match="runs on GPU"):
-        plan.forward(x.cpu(), w, out)
+        plan.forward(x.get(), w, out)
     with pytest.raises(ValueError, match="only packed"):
-        plan.forward(x, w, out, offsets=torch.zeros(3, dtype=torch.int32, device="cuda"))
+        plan.forward(x, w, out, offsets=up(torch.zeros(3, dtype=torch.int32)))
     with pytest.raises(ValueError, match="packed sequences need them"):
         make(tokens=16).forward(x.view(16, 16), w, out.view(16, 16))
     with pytest.raises(E, match="overlap"):
@@ -315,7 +301,7 @@ def test_refusals(gpu_device):
     with pytest.raises(E, match="overlap"):
         plan.backward(x, w, out, grad_x=big[..., :16], grad_weight=w)
     with pytest.raises(ValueError, match="float32"):
-        plan.forward(x, w.half(), out)
+        plan.forward(x, up(w.get().half()), out)
     with pytest.raises(E, match="null buffer"):
         plan.forward(0, w, out)
     with pytest.raises(E, match="not aligned"):
@@ -333,7 +319,7 @@ def test_refusals(gpu_device):
     plan.destroy()
     with pytest.raises(ValueError, match="destroyed"):
         plan.forward(x, w, out)
-    _done(gpu_device)
+    gpu_device.sync()
 
 
 def test_device_buffers_and_addresses(gpu_device):
@@ -366,10 +352,10 @@ def test_captured_calls_replay(gpu_device):
     from ferrum_gpu.hip import Capture
     from ferrum_gpu._native import FerrumGpuError
     ssm = ferrum_gpu.ssm
-    x, gy = torch.randn(2, 40, 64, device="cuda"), torch.randn(2, 40, 64, device="cuda")
-    w, st = torch.randn(64, 4, device="cuda"), torch.randn(2, 3, 64, device="cuda")
-    out, gx, gw = torch.empty_like(x), torch.empty_like(x), torch.empty_like(w)
-    so, new = torch.empty(2, 64, device="cuda"), torch.empty_like(st)
+    x, gy = up(torch.randn(2, 40, 64)), up(torch.randn(2, 40, 64))
+    w, st = up(torch.randn(64, 4)), up(torch.randn(2, 3, 64))
+    out, gx, gw = like(x), like(x), like(w)
+    so, new = fill((2, 64)), like(st)
     plan = ssm.ConvPlan(2, 40, 64, 4, gpu_device, dtype="float32")
 
     def calls(stream=0):
@@ -377,7 +363,6 @@ def test_captured_calls_replay(gpu_device):
         plan.backward(x, w, gy, grad_x=gx, grad_weight=gw, initial=st, stream=stream)
         ssm.conv_step(gpu_device, x[:, 0], w, st, so, state_out=new, stream=stream)
 
-    torch.cuda.synchronize()
     with pytest.raises(FerrumGpuError, match="cannot be captured"):
         with Capture(gpu_device) as cap:
             calls(cap.stream)
@@ -387,31 +372,28 @@ def test_captured_calls_replay(gpu_device):
     for k in range(4):
         x.normal_()
         gy.normal_()
-        torch.cuda.synchronize()
         calls()
-        _done(gpu_device)
+        gpu_device.sync()
         want = [v.clone() for v in (out, gx, gw, so, new)]
         for v in (out, gx, gw, so, new):
             v.fill_(7)
-        torch.cuda.synchronize()
         cap.graph.launch()
-        _done(gpu_device)
-        assert all(torch.equal(a, b) for a, b in zip(want, (out, gx, gw, so, new))), k
+        gpu_device.sync()
+        assert all(same(a, b) for a, b in zip(want, (out, gx, gw, so, new))), k
 
 
 def test_rows_far_apart(gpu_device):
     """Rows whose distance from the first passes 2^32 bytes."""
     import ferrum_gpu
+    from ferrum_gpu.hip import DeviceBuffer
     row, length = 1 << 25, 70
-    far = torch.empty(length * row, dtype=torch.float16, device="cuda").as_strided((1, length, 64), (0, row, 1))
-    near = torch.randn(1, length, 64, device="cuda").half()
-    far.copy_(near)
-    w = torch.randn(64, 4, device="cuda")
-    a, b = torch.empty_like(near), torch.empty_like(near)
+    x = torch.randn(1, length, 64).half()
+    far, near = Far(DeviceBuffer(gpu_device, 2 * length * row), x, row, 0), up(x)
+    w = up(torch.randn(64, 4))
+    a, b = like(near), like(near)
     plan = ferrum_gpu.ssm.ConvPlan(1, length, 64, 4, gpu_device, dtype="float16")
-    torch.cuda.synchronize()
     plan.forward(far, w, a)
     plan.forward(near, w, b)
     plan.forward(near, w, far)
-    _done(gpu_device)
-    assert torch.equal(a, b) and torch.equal(far.contiguous(), b)
+    gpu_device.sync()
+    assert same(a, b) and same(far, b)

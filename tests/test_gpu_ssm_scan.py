@@ -12,24 +12,19 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+import gpu_tensor  # noqa: E402
+from gpu_tensor import Far, fill, like, room, same, up, values  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def _on_gpu(gpu_device):
+    yield from gpu_tensor.use(gpu_device)
+
 GRADS = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
 
 
 def _type(dtype):
     return getattr(torch, dtype)
-
-
-def _np(x):
-    return x.detach().double().cpu().numpy()
-
-
-def _fill(shape, dtype="float32", value=7.0):
-    return torch.full(tuple(shape), value, dtype=_type(dtype), device="cuda")
-
-
-def _done(dev):
-    dev.sync()
-    torch.cuda.synchronize()
 
 
 def _inputs(rng, lead, channels, states, groups, dtype, batch):
@@ -44,13 +39,13 @@ def _inputs(rng, lead, channels, states, groups, dtype, batch):
 
 
 def _oracle_args(i, at, s, use_softplus, without):
-    a = {k: _np(i[k][at]) for k in ("u", "delta", "B", "C")}
-    a.update(A=_np(i["A"]), use_softplus=use_softplus, grad=_np(i["gy"][at]))
+    a = {k: values(i[k][at]) for k in ("u", "delta", "B", "C")}
+    a.update(A=values(i["A"]), use_softplus=use_softplus, grad=values(i["gy"][at]))
     for name, key in (("D", "D"), ("delta_bias", "bias")):
-        a[key] = None if name in without else _np(i[name])
-    a["z"] = None if "z" in without else _np(i["z"][at])
+        a[key] = None if name in without else values(i[name])
+    a["z"] = None if "z" in without else values(i["z"][at])
     for name, key in (("initial", "initial"), ("gfinal", "grad_final")):
-        a[key] = None if name in without else _np(i[name][s])
+        a[key] = None if name in without else values(i[name][s])
     return a
 
 
@@ -67,24 +62,24 @@ def _compare(got, i, spans, channels, groups, states, dtype, use_softplus=True, 
         per_token = channels // groups
         rounds = o.scan_rounds(raw.shape[0], a["A"], most, states)
         summed = o.scan_rounds(raw.shape[0], a["A"], most, states, per_token)
-        o.within(_np(got["out"][at]), r["out"], m["out"], rounds, dtype, "out")
+        o.within(values(got["out"][at]), r["out"], m["out"], rounds, dtype, "out")
         if "final" in got:
-            o.within(_np(got["final"][s]), r["final"], m["final"], rounds, "float32", "final")
+            o.within(values(got["final"][s]), r["final"], m["final"], rounds, "float32", "final")
         if "u" not in got:
             continue
         for k in ("u", "delta", "z"):
             if k in got:
-                o.within(_np(got[k][at]), r[k], m[k], 2 * rounds, dtype, "grad_" + k)
+                o.within(values(got[k][at]), r[k], m[k], 2 * rounds, dtype, "grad_" + k)
         for k in ("B", "C"):
-            o.within(_np(got[k][at]).reshape(r[k].shape), r[k], m[k], 2 * summed, dtype, "grad_" + k)
+            o.within(values(got[k][at]).reshape(r[k].shape), r[k], m[k], 2 * summed, dtype, "grad_" + k)
         if "initial" in got:
-            o.within(_np(got["initial"][s]), r["initial"], m["initial"], rounds, "float32", "grad_initial")
+            o.within(values(got["initial"][s]), r["initial"], m["initial"], rounds, "float32", "grad_initial")
         for k, name in (("A", "A"), ("D", "D"), ("bias", "delta_bias")):
             x, y = total.get(name, (0, 0))
             total[name] = x + r[k], y + m[k]
             rounds_of[name] = max(rounds_of.get(name, 0), 2 * rounds)
     for name, (x, y) in total.items():
-        o.within(_np(got[name]), x, y, rounds_of[name] + tokens + sum(i["u"].shape[:-1]), "float32", "grad_" + name)
+        o.within(values(got[name]), x, y, rounds_of[name] + tokens + sum(i["u"].shape[:-1]), "float32", "grad_" + name)
 
 
 def _check(dev, rng, batch, length, channels, states, groups, dtype, use_softplus=True, without=(), layout="plain"):
@@ -95,34 +90,33 @@ def _check(dev, rng, batch, length, channels, states, groups, dtype, use_softplu
         i["delta_bias"] = i["delta_bias"].abs() * 0.1
 
     def laid(v, room=False):
-        v = v.cuda() if not room else _fill(v.shape, dtype)
+        v = torch.full_like(v, 7) if room else v
         if v.dim() == 4 and layout != "plain":
             v = v.flatten(2)
         if layout == "window":
             n = v.shape[-1]
-            big = _fill(v.shape[:2] + (2 * n + 5,), dtype)
+            big = torch.full(v.shape[:2] + (2 * n + 5,), 7.0, dtype=v.dtype)
             big[..., n + 3:2 * n + 3] = v
-            return big[..., n + 3:2 * n + 3]
+            return up(big[..., n + 3:2 * n + 3])
         if layout == "tokens":
-            return v.transpose(0, 1).contiguous().transpose(0, 1)
-        return v
+            return up(v.transpose(0, 1).contiguous().transpose(0, 1))
+        return up(v)
 
-    d = {k: laid(v) if k in ("u", "delta", "z", "B", "C", "gy") else v.cuda() for k, v in i.items()}
-    got = {"out": laid(i["u"], True), "final": _fill(i["initial"].shape), "initial": _fill(i["initial"].shape)}
-    got.update({k: laid(i[k], True) if k in ("u", "delta", "z", "B", "C") else _fill(i[k].shape) for k in GRADS})
+    d = {k: laid(v) if k in ("u", "delta", "z", "B", "C", "gy") else up(v) for k, v in i.items()}
+    got = {"out": laid(i["u"], True), "final": fill(i["initial"].shape), "initial": fill(i["initial"].shape)}
+    got.update({k: laid(i[k], True) if k in ("u", "delta", "z", "B", "C") else fill(i[k].shape) for k in GRADS})
     opt = {k: d[k] for k in ("D", "z", "delta_bias") if k not in without}
     if "z" in without:
         del got["z"]
     plan = ferrum_gpu.ssm.ScanPlan(batch, length, channels, states, dev, groups=groups, dtype=dtype,
                                    softplus=use_softplus)
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
-    torch.cuda.synchronize()
+    check = room(plan.checkpoint_bytes)
     main = [d[k] for k in ("u", "delta", "A", "B", "C")]
     plan.forward(*main, got["out"], **opt, initial=None if "initial" in without else d["initial"],
                  final=got["final"], checkpoints=check)
     plan.backward(*main, d["gy"], check, **opt, **{"grad_" + k: got[k] for k in GRADS if k in got},
                   grad_initial=got["initial"], grad_final=None if "gfinal" in without else d["gfinal"])
-    _done(dev)
+    dev.sync()
     at = [((s, slice(0, length)), s) for s in range(batch)]
     _compare(got, i, at, channels, groups, states, dtype, use_softplus, without)
 
@@ -160,20 +154,19 @@ def test_packed(gpu_device, states, longest):
     i = _inputs(rng, (tokens,), channels, states, groups, "float32", n)
     for k in ("u", "delta", "z", "B", "C", "gy"):
         i[k][:3] = i[k][offsets[-1]:] = float("nan")
-    d = {k: v.cuda() for k, v in i.items()}
-    got = {"out": _fill(i["u"].shape), "final": _fill(i["initial"].shape), "initial": _fill(i["initial"].shape)}
-    got.update({k: _fill(i[k].shape) for k in GRADS})
-    off = torch.from_numpy(offsets.astype(np.int32)).cuda()
+    d = {k: up(v) for k, v in i.items()}
+    got = {"out": fill(i["u"].shape), "final": fill(i["initial"].shape), "initial": fill(i["initial"].shape)}
+    got.update({k: fill(i[k].shape) for k in GRADS})
+    off = up(torch.from_numpy(offsets.astype(np.int32)))
     plan = ferrum_gpu.ssm.ScanPlan(n, longest, channels, states, gpu_device, groups=groups, dtype="float32",
                                    tokens=tokens)
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
+    check = room(plan.checkpoint_bytes)
     opt = {k: d[k] for k in ("D", "z", "delta_bias")}
     main = [d[k] for k in ("u", "delta", "A", "B", "C")]
-    torch.cuda.synchronize()
     plan.forward(*main, got["out"], **opt, initial=d["initial"], final=got["final"], offsets=off, checkpoints=check)
     plan.backward(*main, d["gy"], check, **opt, **{"grad_" + k: got[k] for k in GRADS}, grad_initial=got["initial"],
                   grad_final=d["gfinal"], offsets=off)
-    _done(gpu_device)
+    gpu_device.sync()
     _compare(got, i, [((slice(int(offsets[s]), int(offsets[s + 1])),), s) for s in range(n)], channels, groups,
              states, "float32")
     for k in ("out", "u", "delta", "z", "B", "C"):
@@ -181,62 +174,58 @@ def test_packed(gpu_device, states, longest):
     # offsets out of order or beyond the rows touch nothing outside them
     got["out"].fill_(7)
     off.copy_(torch.tensor([-4, 2, 9, 5, 2 ** 31 - 1, 1, 1, 1][:n + 1], dtype=torch.int32))
-    torch.cuda.synchronize()
     plan.forward(*main, got["out"], **opt, initial=d["initial"], final=got["final"], offsets=off, checkpoints=check)
     plan.backward(*main, d["gy"], check, **opt, **{"grad_" + k: got[k] for k in GRADS}, offsets=off)
-    _done(gpu_device)
+    gpu_device.sync()
 
 
 def test_no_tokens(gpu_device):
     """No sequences, or sequences without tokens: states pass through, parameter gradients are zeros."""
     import ferrum_gpu
     for batch, length in ((0, 5), (2, 0)):
-        i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(0), (batch, length), 16, 8, 1, "float32",
+        i = {k: up(v) for k, v in _inputs(np.random.default_rng(0), (batch, length), 16, 8, 1, "float32",
                                              batch).items()}
-        fin, gini, gA = _fill((batch, 16, 8)), _fill((batch, 16, 8)), _fill((16, 8))
+        fin, gini, gA = fill((batch, 16, 8)), fill((batch, 16, 8)), fill((16, 8))
         plan = ferrum_gpu.ssm.ScanPlan(batch, length, 16, 8, gpu_device, dtype="float32")
-        check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
+        check = room(plan.checkpoint_bytes)
         main = [i[k] for k in ("u", "delta", "A", "B", "C")]
-        torch.cuda.synchronize()
-        plan.forward(*main, torch.empty_like(i["u"]), initial=i["initial"], final=fin, checkpoints=check)
+        plan.forward(*main, like(i["u"]), initial=i["initial"], final=fin, checkpoints=check)
         plan.backward(*main, i["gy"], check, grad_A=gA, grad_initial=gini, grad_final=i["gfinal"])
-        _done(gpu_device)
-        assert torch.equal(fin, i["initial"]) and torch.equal(gini, i["gfinal"]) and (gA == 0).all()
+        gpu_device.sync()
+        assert same(fin, i["initial"]) and same(gini, i["gfinal"]) and (gA == 0).all()
 
 
 @pytest.mark.parametrize("length", [5, 900])
 def test_final_may_be_initial(gpu_device, length):
     """Also where the token axis is split: no part reads what another has written."""
     import ferrum_gpu
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(1), (1, length), 32, 16, 1, "float32", 1).items()}
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(1), (1, length), 32, 16, 1, "float32", 1).items()}
     plan = ferrum_gpu.ssm.ScanPlan(1, length, 32, 16, gpu_device, dtype="float32")
     main = [i[k] for k in ("u", "delta", "A", "B", "C")]
-    a, b, fin, state = torch.empty_like(i["u"]), torch.empty_like(i["u"]), _fill((1, 32, 16)), i["initial"].clone()
-    torch.cuda.synchronize()
+    a, b, fin, state = like(i["u"]), like(i["u"]), fill((1, 32, 16)), i["initial"].clone()
     plan.forward(*main, a, initial=i["initial"], final=fin)
     plan.forward(*main, b, initial=state, final=state)
-    _done(gpu_device)
-    assert torch.equal(a, b) and torch.equal(fin, state)
+    gpu_device.sync()
+    assert same(a, b) and same(fin, state)
 
 
 def test_same_bits_again(gpu_device):
     """Sums over channels and tokens do not depend on timing."""
     import ferrum_gpu
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(4), (2, 333), 200, 16, 1, "bfloat16", 2).items()}
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(4), (2, 333), 200, 16, 1, "bfloat16", 2).items()}
     plan = ferrum_gpu.ssm.ScanPlan(2, 333, 200, 16, gpu_device)
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
+    check = room(plan.checkpoint_bytes)
     main, opt = [i[k] for k in ("u", "delta", "A", "B", "C")], {k: i[k] for k in ("D", "z", "delta_bias")}
-    torch.cuda.synchronize()
     runs = []
     for _ in range(3):
-        got = {k: torch.empty_like(i[k]) for k in GRADS}
-        out = torch.empty_like(i["u"])
+        got = {k: like(i[k]) for k in GRADS}
+        out = like(i["u"])
         plan.forward(*main, out, **opt, checkpoints=check)
         plan.backward(*main, i["gy"], check, **opt, **{"grad_" + k: v for k, v in got.items()})
-        _done(gpu_device)
+        gpu_device.sync()
         runs.append([out, *got.values()])
     for other in runs[1:]:
-        assert all(torch.equal(x, y) for x, y in zip(runs[0], other))
+        assert all(same(x, y) for x, y in zip(runs[0], other))
 
 
 def test_gradient_is_the_difference(gpu_device):
@@ -248,30 +237,29 @@ def test_gradient_is_the_difference(gpu_device):
     import ferrum_gpu
     rng = np.random.default_rng(6)
     batch, length, channels, states = 2, 40, 24, 16
-    i = {k: v.cuda() for k, v in _inputs(rng, (batch, length), channels, states, 1, "float32", batch).items()}
+    i = {k: up(v) for k, v in _inputs(rng, (batch, length), channels, states, 1, "float32", batch).items()}
     plan = ferrum_gpu.ssm.ScanPlan(batch, length, channels, states, gpu_device, dtype="float32")
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
+    check = room(plan.checkpoint_bytes)
 
     def loss(j):
-        out, fin = torch.empty_like(j["u"]), torch.empty_like(j["initial"])
-        torch.cuda.synchronize()
+        out, fin = like(j["u"]), like(j["initial"])
         plan.forward(*(j[k] for k in ("u", "delta", "A", "B", "C")), out, D=j["D"], z=j["z"],
                      delta_bias=j["delta_bias"], initial=j["initial"], final=fin, checkpoints=check)
-        _done(gpu_device)
-        return (out.double() * i["gy"]).sum().item() + (fin.double() * i["gfinal"]).sum().item()
+        gpu_device.sync()
+        return float((values(out) * values(i["gy"])).sum() + (values(fin) * values(i["gfinal"])).sum())
 
     loss(i)
-    got = {k: torch.empty_like(i[k]) for k in GRADS + ("initial",)}
+    got = {k: like(i[k]) for k in GRADS + ("initial",)}
     plan.backward(*(i[k] for k in ("u", "delta", "A", "B", "C")), i["gy"], check, D=i["D"], z=i["z"],
                   delta_bias=i["delta_bias"], **{"grad_" + k: v for k, v in got.items()}, grad_final=i["gfinal"])
-    _done(gpu_device)
+    gpu_device.sync()
     for k, g in got.items():
-        v = torch.from_numpy(rng.standard_normal(tuple(g.shape))).float().cuda()
+        v = torch.from_numpy(rng.standard_normal(tuple(g.shape))).float()
         v /= v.norm()
         h = 2.0 ** -6
-        want = (loss({**i, k: i[k] + h * v}) - loss({**i, k: i[k] - h * v})) / (2 * h)
-        scale = g.double().norm().item()
-        assert abs((g.double() * v).sum().item() - want) <= 2e-3 * scale, k
+        want = (loss({**i, k: up(i[k].get() + h * v)}) - loss({**i, k: up(i[k].get() - h * v)})) / (2 * h)
+        g = g.get().double()
+        assert abs((g * v).sum().item() - want) <= 2e-3 * g.norm().item(), k
 
 
 @pytest.mark.parametrize("states", [16, 13, 6, 33])
@@ -280,16 +268,15 @@ def test_nothing_leaks(gpu_device, states):
     all others as they are; an infinite time step forgets (its own channel
     only), whatever the number of states."""
     import ferrum_gpu
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(3), (2, 50), 40, states, 1, "float32", 2).items()}
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(3), (2, 50), 40, states, 1, "float32", 2).items()}
     plan = ferrum_gpu.ssm.ScanPlan(2, 50, 40, states, gpu_device, dtype="float32")
 
     def run(j):
-        out, fin = torch.empty_like(j["u"]), _fill((2, 40, states))
-        torch.cuda.synchronize()
+        out, fin = like(j["u"]), fill((2, 40, states))
         plan.forward(*(j[k] for k in ("u", "delta", "A", "B", "C")), out, D=j["D"], z=j["z"],
                      delta_bias=j["delta_bias"], initial=j["initial"], final=fin)
-        _done(gpu_device)
-        return out, fin
+        gpu_device.sync()
+        return out.get(), fin.get()
 
     good, good_fin = run(i)
     j = {k: v.clone() for k, v in i.items()}
@@ -300,27 +287,27 @@ def test_nothing_leaks(gpu_device, states):
     out, fin = run(j)
     touched = torch.zeros_like(out, dtype=torch.bool)
     touched[0, 30:, 5] = touched[0, 20, 9] = touched[1, :, 7] = touched[1, 49] = True
-    assert torch.equal(out[~touched], good[~touched])
+    assert same(out[~touched], good[~touched])
     assert torch.isnan(out[0, 30:, 5]).all() and torch.isinf(out[0, 20, 9]) and torch.isnan(out[1, :, 7]).all()
     keep = [c for c in range(40) if c != 5]
-    assert torch.equal(fin[0, keep], good_fin[0, keep])
+    assert same(fin[0, keep], good_fin[0, keep])
     # delta = inf with u = 0 at a token: the decay is 0, the input inf * 0 = NaN
     # for this channel; delta = inf and u > 0: infinite states of B's signs
     k = {n: v.clone() for n, v in i.items()}
     k["delta"][0, 10, 3] = float("inf")
     k["u"][0, 10, 3] = 1.0
     out, fin = run(k)
-    b = i["B"][0, 10, 0]
-    assert torch.isinf(fin[0, 3]).all() and torch.equal(fin[0, 3] > 0, b > 0)
+    b = i["B"].get()[0, 10, 0]
+    assert torch.isinf(fin[0, 3]).all() and same(fin[0, 3] > 0, b > 0)
     keep = [c for c in range(40) if c != 3]
-    assert torch.equal(out[0][:, keep], good[0][:, keep]) and torch.equal(out[1], good[1])
+    assert same(out[0][:, keep], good[0][:, keep]) and same(out[1], good[1])
     # A = -inf: such a state holds only its own token's input
     m = {n: v.clone() for n, v in i.items()}
     m["A"][11] = float("-inf")
     out, fin = run(m)
-    raw = (i["delta"] + i["delta_bias"])[:, -1, 11].double()
-    want = (o.softplus(raw.cpu().numpy()) * _np(i["u"][:, -1, 11]))[:, None] * _np(i["B"][:, -1, 0])
-    assert np.allclose(_np(fin[:, 11]), want, rtol=1e-5, atol=1e-30)
+    raw = values((i["delta"].get() + i["delta_bias"].get())[:, -1, 11])
+    want = (o.softplus(raw) * values(i["u"][:, -1, 11]))[:, None] * values(i["B"][:, -1, 0])
+    assert np.allclose(values(fin[:, 11]), want, rtol=1e-5, atol=1e-30)
 
 
 @pytest.mark.parametrize("length", [30, 700])
@@ -333,29 +320,29 @@ def test_a_constant_scan_is_the_ffts_filter(gpu_device, length):
     from ferrum_gpu import pointwise
     rng = np.random.default_rng(12)
     channels, states = 8, 16
-    i = {k: v.cuda() for k, v in _inputs(rng, (1, length), channels, states, 1, "float32", 1).items()}
+    i = _inputs(rng, (1, length), channels, states, 1, "float32", 1)
     i["delta"].zero_()
     i["B"][:], i["C"][:] = i["B"][:, :1].clone(), i["C"][:, :1].clone()
-    out = torch.empty_like(i["u"])
+    u = i["u"][0].t()
+    i = {k: up(v) for k, v in i.items()}
+    out = like(i["u"])
     plan = ferrum_gpu.ssm.ScanPlan(1, length, channels, states, gpu_device, dtype="float32")
-    torch.cuda.synchronize()
     plan.forward(*(i[k] for k in ("u", "delta", "A", "B", "C")), out, delta_bias=i["delta_bias"])
     log_n = (2 * length - 1).bit_length()
-    dt = o.softplus(_np(i["delta_bias"]))
+    dt = o.softplus(values(i["delta_bias"]))
     t = np.arange(length)
-    kernel = np.einsum("n,tdn,n,d->dt", _np(i["C"])[0, 0, 0], np.exp(t[:, None, None] * dt[:, None] * _np(i["A"])),
-                       _np(i["B"])[0, 0, 0], dt)
-    both = torch.zeros(2, channels, 1 << log_n, dtype=torch.complex64, device="cuda")
-    both[0, :, :length] = i["u"][0].t()
-    both[1, :, :length] = torch.from_numpy(kernel).cuda()
+    kernel = np.einsum("n,tdn,n,d->dt", values(i["C"])[0, 0, 0], np.exp(t[:, None, None] * dt[:, None] * values(i["A"])),
+                       values(i["B"])[0, 0, 0], dt)
+    both = torch.zeros(2, channels, 1 << log_n, dtype=torch.complex64)
+    both[0, :, :length], both[1, :, :length] = u, torch.from_numpy(kernel)
+    both = up(both)
     fft, back = (ferrum_gpu.fft.Plan1D(log_n, n, gpu_device) for n in (2 * channels, channels))
-    torch.cuda.synchronize()
     fft.execute(both, both, "forward")
     pointwise.cmul(gpu_device, both[0], both[1], both[0], channels << log_n)
     back.execute(both[0], both[0], "inverse", normalize=True)
-    _done(gpu_device)
-    want = both[0, :, :length].real.t()
-    assert (out[0] - want).abs().max().item() <= 1e-4 * want.abs().max().item()
+    gpu_device.sync()
+    want = both.get()[0, :, :length].real.t()
+    assert (out.get()[0] - want).abs().max().item() <= 1e-4 * want.abs().max().item()
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
@@ -372,16 +359,15 @@ def test_step(gpu_device, batch, channels, states, groups, dtype):
     slots = rng.permutation(rows)[:batch].astype(np.int32)
     if batch > 2:
         slots[0], slots[1] = -1, rows
-    d = {k: v.cuda() for k, v in i.items()}
+    d = {k: up(v) for k, v in i.items()}
     for in_place, without in ((True, ()), (False, ("z", "D", "delta_bias"))):
-        state, out = st.cuda(), _fill((batch, channels), dtype)
+        state, out = up(st), fill((batch, channels), dtype)
         new = None if in_place else state.clone()
         opt = {k: d[k] for k in ("D", "z", "delta_bias") if k not in without}
-        ds = torch.from_numpy(slots).cuda()
-        torch.cuda.synchronize()
+        ds = up(torch.from_numpy(slots))
         ferrum_gpu.ssm.scan_step(gpu_device, d["u"], d["delta"], d["A"], d["B"], d["C"], state, out, slots=ds,
                                  state_out=new, **opt)
-        _done(gpu_device)
+        gpu_device.sync()
         after = state if in_place else new
         free = np.ones(rows, bool)
         for r, s in enumerate(slots):
@@ -393,11 +379,11 @@ def test_step(gpu_device, batch, channels, states, groups, dtype):
                              without + ("gfinal",))
             want, m = o.scan(**a), o.scan(**a, magnitude=True)
             rounds = o.scan_rounds(1, a["A"], 5.0, states)
-            o.within(_np(out[r]), want["out"][0], m["out"][0], rounds, dtype, "out")
-            o.within(_np(after[int(s)]), want["final"], m["final"], rounds, "float32", "state")
-        assert torch.equal(after.cpu()[torch.from_numpy(free)], st[torch.from_numpy(free)])
+            o.within(values(out[r]), want["out"][0], m["out"][0], rounds, dtype, "out")
+            o.within(values(after[int(s)]), want["final"], m["final"], rounds, "float32", "state")
+        assert same(after.get()[torch.from_numpy(free)], st[torch.from_numpy(free)])
         if not in_place:
-            assert torch.equal(state.cpu(), st)
+            assert same(state, st)
 
 
 def test_step_many_rows(gpu_device):
@@ -406,16 +392,15 @@ def test_step_many_rows(gpu_device):
     rng = np.random.default_rng(21)
     batch, channels, states = 33001, 16, 16
     i = _inputs(rng, (batch,), channels, states, 1, "float32", batch)
-    d = {k: v.cuda() for k, v in i.items()}
-    out, slots = _fill((batch, channels)), torch.from_numpy(rng.permutation(batch).astype(np.int32)).cuda()
+    d = {k: up(v) for k, v in i.items()}
+    out, slots = fill((batch, channels)), up(torch.from_numpy(rng.permutation(batch).astype(np.int32)))
     slots[5], slots[batch - 1] = -1, batch
     state = d["initial"].clone()
-    torch.cuda.synchronize()
     ferrum_gpu.ssm.scan_step(gpu_device, d["u"], d["delta"], d["A"], d["B"], d["C"], state, out, D=d["D"], z=d["z"],
                              delta_bias=d["delta_bias"], slots=slots)
-    _done(gpu_device)
-    n = {k: _np(v) for k, v in i.items()}
-    s = slots.cpu().numpy()
+    gpu_device.sync()
+    n = {k: values(v) for k, v in i.items()}
+    s = slots.get().numpy()
     on = (s >= 0) & (s < batch)
     dt = o.softplus(n["delta"] + n["delta_bias"])
     a = np.exp(dt[:, :, None] * n["A"])
@@ -423,7 +408,7 @@ def test_step_many_rows(gpu_device):
     want, m = ((f(a * prior) if f is np.abs else a * prior) + f((dt * n["u"])[:, :, None] * n["B"][:, 0][:, None])
                for f in (lambda v: v, np.abs))
     rounds = o.scan_rounds(1, n["A"], float(dt.max()), states)
-    after = _np(state)
+    after = values(state)
     o.within(after[s[on]], want[on], m[on], rounds, "float32", "state")
     untouched = np.ones(batch, bool)
     untouched[s[on]] = False
@@ -431,33 +416,31 @@ def test_step_many_rows(gpu_device):
     gate = n["z"] * o.sigmoid(n["z"])
     y = ((want * n["C"][:, 0][:, None]).sum(-1) + n["D"] * n["u"]) * gate
     my = ((m * np.abs(n["C"][:, 0][:, None])).sum(-1) + np.abs(n["D"] * n["u"])) * np.abs(gate)
-    o.within(_np(out)[on], y[on], my[on], rounds, "float32", "out")
-    assert (_np(out)[~on] == 0).all()
+    o.within(values(out)[on], y[on], my[on], rounds, "float32", "out")
+    assert (values(out)[~on] == 0).all()
 
 
 def test_windows_of_one_array(gpu_device):
     """One token of each row: inputs and outputs that are columns of one array."""
     import ferrum_gpu
     d, n = 32, 16
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(2), (3, 1), d, n, 1, "float32", 3).items()}
-    big = torch.zeros(3, 1, 4 * d + 2 * n, device="cuda")
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(2), (3, 1), d, n, 1, "float32", 3).items()}
+    big = up(torch.zeros(3, 1, 4 * d + 2 * n))
     big[..., :d], big[..., d:2 * d], big[..., 2 * d:3 * d] = i["u"], i["delta"], i["z"]
     big[..., 4 * d:4 * d + n], big[..., 4 * d + n:] = i["B"][:, :, 0], i["C"][:, :, 0]
     plan = ferrum_gpu.ssm.ScanPlan(3, 1, d, n, gpu_device, dtype="float32")
-    want, state = torch.empty_like(i["u"]), i["initial"].clone()
+    want, state = like(i["u"]), i["initial"].clone()
     cols = [big[..., k * d:(k + 1) * d] for k in range(4)]
     b, c = big[..., 4 * d:4 * d + n], big[..., 4 * d + n:]
-    torch.cuda.synchronize()
     plan.forward(i["u"], i["delta"], i["A"], i["B"], i["C"], want, z=i["z"], initial=i["initial"])
     plan.forward(cols[0], cols[1], i["A"], b, c, cols[3], z=cols[2], initial=i["initial"])
-    _done(gpu_device)
-    assert torch.equal(cols[3], want)
-    cols[3].zero_()
-    torch.cuda.synchronize()
+    gpu_device.sync()
+    assert same(cols[3], want)
+    cols[3].fill_(0)
     ferrum_gpu.ssm.scan_step(gpu_device, cols[0][:, 0], cols[1][:, 0], i["A"], b[:, 0], c[:, 0], state, cols[3][:, 0],
                              z=cols[2][:, 0])
-    _done(gpu_device)
-    assert torch.allclose(cols[3], want, rtol=1e-5, atol=1e-5)
+    gpu_device.sync()
+    assert torch.allclose(cols[3].get(), want.get(), rtol=1e-5, atol=1e-5)
 
 
 def test_prompt_then_tokens(gpu_device):
@@ -466,12 +449,11 @@ def test_prompt_then_tokens(gpu_device):
     import ferrum_gpu
     ssm = ferrum_gpu.ssm
     batch, length, more, channels, states = 2, 21, 6, 48, 16
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(7), (batch, length + more), channels, states, 1,
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(7), (batch, length + more), channels, states, 1,
                                          "float32", batch).items()}
     rows, opt = ("u", "delta", "B", "C", "z"), {k: i[k] for k in ("D", "delta_bias")}
-    whole, out, state, fin = torch.empty_like(i["u"]), torch.empty_like(i["u"]), i["initial"].clone(), \
-        torch.empty_like(i["initial"])
-    torch.cuda.synchronize()
+    whole, out, state, fin = like(i["u"]), like(i["u"]), i["initial"].clone(), \
+        like(i["initial"])
 
     def forward(n, to, **k):
         r = {x: i[x][:, :n] for x in rows}
@@ -484,8 +466,8 @@ def test_prompt_then_tokens(gpu_device):
     for t in range(length, length + more):
         r = {x: i[x][:, t] for x in rows}
         ssm.scan_step(gpu_device, r["u"], r["delta"], i["A"], r["B"], r["C"], state, out[:, t], z=r["z"], **opt)
-    _done(gpu_device)
-    assert torch.allclose(out, whole, rtol=1e-5, atol=1e-5) and torch.allclose(state, fin, rtol=1e-5, atol=1e-5)
+    gpu_device.sync()
+    assert all(torch.allclose(x.get(), y.get(), rtol=1e-5, atol=1e-5) for x, y in ((out, whole), (state, fin)))
 
 
 def test_broadcast_inputs(gpu_device):
@@ -496,16 +478,16 @@ def test_broadcast_inputs(gpu_device):
     i = _inputs(np.random.default_rng(8), (batch, length), channels, states, 1, "float32", batch)
     for k in ("B", "C"):
         i[k] = i[k][:1].expand(batch, -1, -1, -1)
-    d = {k: (v[:1].cuda().expand(v.shape) if k in ("B", "C") else v.cuda()) for k, v in i.items()}
+    d = {k: up(v) for k, v in i.items()}
+    assert d["B"].stride()[0] == 0
     plan = ferrum_gpu.ssm.ScanPlan(batch, length, channels, states, gpu_device, dtype="float32")
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
-    got = {k: _fill(i[k].shape) for k in GRADS}
-    got["out"] = _fill(i["u"].shape)
+    check = room(plan.checkpoint_bytes)
+    got = {k: fill(i[k].shape) for k in GRADS}
+    got["out"] = fill(i["u"].shape)
     main, opt = [d[k] for k in ("u", "delta", "A", "B", "C")], {k: d[k] for k in ("D", "z", "delta_bias")}
-    torch.cuda.synchronize()
     plan.forward(*main, got["out"], **opt, checkpoints=check)
     plan.backward(*main, d["gy"], check, **opt, **{"grad_" + k: got[k] for k in GRADS})
-    _done(gpu_device)
+    gpu_device.sync()
     _compare(got, i, [((s, slice(0, length)), s) for s in range(batch)], channels, 1, states, "float32",
              without=("initial", "gfinal"))
 
@@ -516,11 +498,11 @@ def test_another_stream_and_captured_calls(gpu_device):
     from ferrum_gpu.hip import Capture, Stream
     from ferrum_gpu._native import FerrumGpuError
     ssm = ferrum_gpu.ssm
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(9), (1, 600), 64, 16, 1, "float32", 1).items()}
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(9), (1, 600), 64, 16, 1, "float32", 1).items()}
     plan = ssm.ScanPlan(1, 600, 64, 16, gpu_device, dtype="float32")
-    check = torch.empty(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
-    got = {k: torch.empty_like(i[k]) for k in GRADS}
-    out, so, new = torch.empty_like(i["u"]), torch.empty(1, 64, device="cuda"), torch.empty(1, 64, 16, device="cuda")
+    check = room(plan.checkpoint_bytes)
+    got = {k: like(i[k]) for k in GRADS}
+    out, so, new = like(i["u"]), fill((1, 64)), fill((1, 64, 16))
     main, opt = [i[k] for k in ("u", "delta", "A", "B", "C")], {k: i[k] for k in ("D", "z", "delta_bias")}
 
     def calls(stream):
@@ -530,7 +512,6 @@ def test_another_stream_and_captured_calls(gpu_device):
                       so, state_out=new, stream=stream)
 
     every = [out, so, new, *got.values()]
-    torch.cuda.synchronize()
     with pytest.raises(FerrumGpuError, match="cannot be captured"):
         with Capture(gpu_device) as cap:
             calls(cap.stream)
@@ -541,38 +522,33 @@ def test_another_stream_and_captured_calls(gpu_device):
     for k in range(4):
         for n in ("u", "delta", "gy", "B", "C"):
             i[n].normal_()
-        torch.cuda.synchronize()
         calls(0)
-        _done(gpu_device)
+        gpu_device.sync()
         want = [v.clone() for v in every]
         for run in (lambda: calls(stream.handle), cap.graph.launch):
             for v in every:
                 v.fill_(7)
-            torch.cuda.synchronize()
             run()
             stream.sync()
-            _done(gpu_device)
-            assert all(torch.equal(a, b) for a, b in zip(want, every)), k
+            gpu_device.sync()
+            assert all(same(a, b) for a, b in zip(want, every)), k
 
 
 def test_rows_far_apart(gpu_device):
     """Rows whose distance from the first passes 2^32 bytes."""
     import ferrum_gpu
+    from ferrum_gpu.hip import DeviceBuffer
     row, length = 1 << 25, 70
-    i = {k: v.cuda() for k, v in _inputs(np.random.default_rng(5), (1, length), 64, 16, 1, "float16", 1).items()}
-    big = torch.empty(length * row, dtype=torch.float16, device="cuda")
-    far = lambda v, at: big.as_strided(tuple(v.shape), (0, row) + ((16, 1) if v.dim() == 4 else (1,)), at)  # noqa: E731
-    f = dict(i)
-    for at, k in enumerate(("u", "delta", "z", "B", "C")):
-        f[k] = far(i[k], 100 * at)
-        f[k].copy_(i[k])
+    host = _inputs(np.random.default_rng(5), (1, length), 64, 16, 1, "float16", 1)
+    i = {k: up(v) for k, v in host.items()}
+    big = DeviceBuffer(gpu_device, 2 * length * row)
+    f = {**i, **{k: Far(big, host[k], row, 100 * at) for at, k in enumerate(("u", "delta", "z", "B", "C"))}}
     plan = ferrum_gpu.ssm.ScanPlan(1, length, 64, 16, gpu_device, dtype="float16")
-    outs = [torch.empty_like(i["u"]), far(i["u"], 1000)]
-    torch.cuda.synchronize()
+    outs = [like(i["u"]), Far(big, torch.zeros(1, length, 64, dtype=torch.float16), row, 1000)]
     for j, out in zip((i, f), outs):
         plan.forward(*(j[k] for k in ("u", "delta", "A", "B", "C")), out, z=j["z"])
-    _done(gpu_device)
-    assert torch.equal(outs[0], outs[1].contiguous())
+    gpu_device.sync()
+    assert same(*outs)
 
 
 def test_refusals(gpu_device):
@@ -591,23 +567,23 @@ def test_refusals(gpu_device):
         with pytest.raises(E, match="must be in"):
             make(length=1, batch=1, **bad)
     plan = make()
-    x, out = torch.zeros(2, 8, 16, device="cuda"), torch.zeros(2, 8, 16, device="cuda")
-    A, D = torch.zeros(16, 4, device="cuda"), torch.zeros(16, device="cuda")
-    B, C = torch.zeros(2, 8, 2, 4, device="cuda"), torch.zeros(2, 8, 8, device="cuda")
-    st = torch.zeros(2, 16, 4, device="cuda")
-    check = torch.zeros(plan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
-    delta = torch.zeros_like(x)
+    x, out = up(torch.zeros(2, 8, 16)), up(torch.zeros(2, 8, 16))
+    A, D = up(torch.zeros(16, 4)), up(torch.zeros(16))
+    B, C = up(torch.zeros(2, 8, 2, 4)), up(torch.zeros(2, 8, 8))
+    st = up(torch.zeros(2, 16, 4))
+    check = room(plan.checkpoint_bytes)
+    delta = like(x)
     plan.forward(x, delta, A, B, C, out, checkpoints=check)
     with pytest.raises(ValueError, match="shape"):
-        plan.forward(x, delta, A.t().contiguous(), B, C, out)
+        plan.forward(x, delta, up(A.get().t().contiguous()), B, C, out)
     with pytest.raises(ValueError, match="shape"):
         plan.forward(x, delta, A, B[..., :3], C, out)
     with pytest.raises(ValueError, match="bfloat16"):
-        plan.forward(x.bfloat16(), delta, A, B, C, out)
+        plan.forward(up(x.get().bfloat16()), delta, A, B, C, out)
     with pytest.raises(ValueError, match="float64"):
-        plan.forward(x, delta, A, B, C, out, D=D.double())
+        plan.forward(x, delta, A, B, C, out, D=up(D.get().double()))
     with pytest.raises(ValueError, match="runs on GPU"):
-        plan.forward(x, delta, A.cpu(), B, C, out)
+        plan.forward(x, delta, A.get(), B, C, out)
     with pytest.raises(ValueError, match="checkpoints"):
         plan.forward(x, delta, A, B, C, out, checkpoints=check[:-1])
     with pytest.raises(ValueError, match="shape"):
@@ -623,20 +599,20 @@ def test_refusals(gpu_device):
     with pytest.raises(E, match="overlap"):
         plan.backward(x, delta, A, B, C, out, check, grad_u=delta)
     with pytest.raises(E, match="grad_z without z"):
-        plan.backward(x, delta, A, B, C, out, check, grad_z=torch.zeros_like(x))
+        plan.backward(x, delta, A, B, C, out, check, grad_z=like(x))
     with pytest.raises(ValueError, match="only packed"):
-        plan.forward(x, delta, A, B, C, out, offsets=torch.zeros(3, dtype=torch.int32, device="cuda"))
+        plan.forward(x, delta, A, B, C, out, offsets=up(torch.zeros(3, dtype=torch.int32)))
     with pytest.raises(ValueError, match="int32"):
         make(tokens=16).forward(x.view(16, 16), delta.view(16, 16), A, B.view(16, 2, 4), C.view(16, 8),
-                                out.view(16, 16), offsets=torch.zeros(3, dtype=torch.int64, device="cuda"))
+                                out.view(16, 16), offsets=up(torch.zeros(3, dtype=torch.int64)))
     with pytest.raises(E, match="state_rows"):
         ssm.scan_step(gpu_device, x[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], st[:1], out[:, 0])
     with pytest.raises(ValueError, match="slots"):
         ssm.scan_step(gpu_device, x[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], st, out[:, 0],
-                      slots=torch.zeros(3, dtype=torch.int32, device="cuda"))
+                      slots=up(torch.zeros(3, dtype=torch.int32)))
     with pytest.raises(ValueError, match="B: shape"):
         ssm.scan_step(gpu_device, x[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], st, out[:, 0], groups=0)
     plan.destroy()
     with pytest.raises(ValueError, match="destroyed"):
         plan.forward(x, delta, A, B, C, out)
-    _done(gpu_device)
+    gpu_device.sync()
