@@ -96,16 +96,6 @@ __device__ __forceinline__ float swap32_add(float a, float b) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(a), __float_as_int(b), false, false);
     return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
-__device__ __forceinline__ float swap16_add(float a, float b) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(a), __float_as_int(b), false, false);
-    return __int_as_float(r[0]) + __int_as_float(r[1]);
-}
-// Sums over the four rows of a wave (lanes l, l + 16, l + 32, l + 48): row i
-// gets the sum of v[i].  Swapping the upper half of one register with the
-// lower half of another and adding the two sums both at once.
-__device__ __forceinline__ float rows_sum(const float (&v)[4]) {
-    return swap16_add(swap32_add(v[0], v[2]), swap32_add(v[1], v[3]));
-}
 
 // p[0] + p[stride] + ... of n values, in this order of eight running sums.
 __device__ __forceinline__ float ordered_sum(const float* p, uint64_t stride, uint64_t n) {

@@ -66,6 +66,12 @@ __device__ __forceinline__ ConvPlace conv_place(const fg_conv_kargs& g) {
     return p;
 }
 
+// The first place of packed sequence `seq` among the runs' parts.
+__device__ __forceinline__ uint64_t conv_places_before(const fg_conv_kargs& g, uint32_t seq) {
+    const int64_t a = g.offsets[seq], all = (int64_t)g.tokens;
+    return (uint64_t)(a < 0 ? 0 : a > all ? all : a) / g.run + seq;
+}
+
 template <class T, int V, int W>
 struct Conv {
     using Io = Vec<T, V>;
@@ -189,11 +195,27 @@ struct Conv {
         });
         if (!p.past) backward_run(g, p, turn, gw, gbias);
         if (!p.any) return;
-        float* to = g.part + ((uint64_t)p.seq * g.runs + p.run) * g.channels * (W + 1);
+        const auto put = [&](uint64_t k) {
+            float* to = g.part + k * g.channels * (W + 1);
+            each<V>([&](auto i) {
+                each<W>([&](auto k) { to[(uint64_t)(p.ch + i) * W + k] = gw[k][i]; });
+                to[(uint64_t)g.channels * W + p.ch + i] = gbias[i];
+            });
+        };
+        if (!g.offsets) return put((uint64_t)p.seq * g.runs + p.run);
+        // Packed: a place for every run's length of rows and one more for each
+        // sequence, not for each sequence's longest.  What is left before the
+        // next sequence's first is zeros; that sequence begins where this one
+        // ends, or later where this one is cut.
+        const uint64_t first = (uint64_t)p.start / g.run + p.seq, end = conv_places_before(g, p.seq + 1);
+        uint64_t k = first + p.run;
+        if (k < end) put(k);
+        if (p.run + 1 < g.runs) return;
         each<V>([&](auto i) {
-            each<W>([&](auto k) { to[(uint64_t)(p.ch + i) * W + k] = gw[k][i]; });
-            to[(uint64_t)g.channels * W + p.ch + i] = gbias[i];
+            gbias[i] = 0.0f;
+            each<W>([&](auto k) { gw[k][i] = 0.0f; });
         });
+        while (++k < end) put(k);
     }
     static __device__ __forceinline__ void backward_run(const fg_conv_kargs& g, const ConvPlace& p, Turn& turn,
                                                         float (&gw)[W][V], float (&gbias)[V]) {
@@ -317,16 +339,21 @@ struct Conv {
 };
 
 // The parameters' gradients from the runs' parts, in a fixed order: four waves
-// of a workgroup take 64 values and a quarter of the parts each.  Runs beyond
-// the end of a packed sequence have written zeros.
+// of a workgroup take 64 values and a quarter of the parts each.
 __device__ __forceinline__ void conv_reduce(const fg_conv_kargs& g, uint32_t width, float* gweight, float* gbias) {
     __shared__ float parts[4][64];
-    const uint64_t n = (uint64_t)g.channels * (width + 1), count = (uint64_t)g.seqs * g.runs;
+    const uint64_t n = (uint64_t)g.channels * (width + 1);
+    uint64_t start = 0, count = (uint64_t)g.seqs * g.runs;
+    if (g.offsets) {
+        const uint64_t end = conv_places_before(g, g.seqs);
+        start = conv_places_before(g, 0);
+        count = end > start ? end - start : 0;
+    }
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t e = (uint64_t)blockIdx.x * 64 + lane, each_wave = (count + 3) / 4, first = wave * each_wave;
     float v = 0.0f;
     if (e < n && first < count)
-        v = ordered_sum(g.part + first * n + e, n, count - first < each_wave ? count - first : each_wave);
+        v = ordered_sum(g.part + (start + first) * n + e, n, count - first < each_wave ? count - first : each_wave);
     parts[wave][lane] = v;
     __syncthreads();
     if (wave > 0 || e >= n) return;

@@ -19,6 +19,7 @@ const char* const kTypes[3] = {"f32", "bf16", "f16"};
 const uint32_t kBytes[3] = {4, 2, 2};
 constexpr int64_t kMaxRowStride = 1 << 25;   // 32-bit offsets within a segment's rows
 constexpr int64_t kMaxCount = 0x7fffffff;
+constexpr int64_t kMaxBytes = int64_t(1) << 46;
 
 KernelArtifact ssm_code_object(int dtype) {
     static const unsigned char* const start[3] = {fg_ssm_f32_code_object_start, fg_ssm_bf16_code_object_start,
@@ -44,6 +45,16 @@ void check_range(const char* op, const char* what, int64_t v, int64_t lo, int64_
     if (v < lo || v > hi)
         invalid(std::string(op) + ": " + what + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) +
                 "], got " + std::to_string(v));
+}
+
+// The product of an array's sizes, refused where no memory holds as many bytes.
+int64_t size_of(const char* op, const char* what, std::initializer_list<int64_t> sizes) {
+    int64_t n = 1;
+    for (int64_t k : sizes) {
+        if (k > 0 && n > kMaxBytes / k) invalid(std::string(op) + ": " + what + ": too large");
+        n *= k;
+    }
+    return n;
 }
 
 // The extent of an array of rows, in bytes from its first element.
@@ -78,6 +89,8 @@ public:
             invalid(std::string(op_) + ": " + name + ": row stride " + std::to_string(v.row) + " exceeds " +
                     std::to_string(kMaxRowStride));
         if (seqs_ == 0 || rows_ == 0) return v;
+        const __int128 last = (__int128)(seqs_ - 1) * v.seq + (__int128)(rows_ - 1) * v.row + width;
+        if (last > kMaxBytes / es_) invalid(std::string(op_) + ": " + name + ": too large");
         if (out) {
             // rows of all sequences apart: the larger stride steps over all that the smaller one covers
             int64_t small = v.row, small_n = rows_, large = v.seq, large_n = seqs_;
@@ -210,13 +223,13 @@ void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_st
     check_range(op, "width", a.width, 2, FG_CONV_MAX_WIDTH);
     check_range(op, "state_rows", a.state_rows, a.slots ? 0 : a.rows, kMaxCount);
     const uint32_t es = kBytes[a.dtype];
+    const int64_t state = size_of(op, "state", {a.state_rows, a.width - 1, a.channels, es});
     Arrays all(op, a.rows, 1, es);
     fg_conv_step_kargs g{};
     g.x = all.rows("x", a.x, a.channels, false);
     g.out = all.rows("out", a.out, a.channels, true);
     all.flat("weight", a.weight, 4 * a.channels * a.width, false, false);
     all.flat("bias", a.bias, 4 * a.channels, false, true);
-    const int64_t state = a.state_rows * (a.width - 1) * a.channels * es;
     all.flat("state", a.state, state, a.state_out == a.state, false, es);
     if (a.state_out != a.state || !a.state_out) all.flat("state_out", a.state_out, state, true, false, es);
     all.flat("slots", a.slots, 4 * a.rows, false, true);
@@ -246,11 +259,12 @@ void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_st
     const char* op = "scan_step";
     check_dtype(op, a.dtype);
     check_range(op, "rows", a.rows, 0, kMaxCount);
-    check_range(op, "channels", a.channels, 1, kMaxCount);
+    check_range(op, "channels", a.channels, 1, kMaxRowStride);
     check_range(op, "states", a.states, 1, FG_SSM_MAX_STATES);
     check_range(op, "groups", a.groups, 1, a.channels);
     if (a.channels % a.groups) invalid("scan_step: groups must divide channels");
     check_range(op, "state_rows", a.state_rows, a.slots ? 0 : a.rows, kMaxCount);
+    const int64_t state = size_of(op, "state", {4, a.state_rows, a.channels, a.states});
     Arrays all(op, a.rows, 1, kBytes[a.dtype]);
     fg_scan_step_kargs g{};
     g.u = all.rows("u", a.u, a.channels, false);
@@ -262,7 +276,6 @@ void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_st
     all.flat("A", a.a, 4 * a.channels * a.states, false, false);
     all.flat("D", a.d, 4 * a.channels, false, true);
     all.flat("delta_bias", a.delta_bias, 4 * a.channels, false, true);
-    const int64_t state = 4 * a.state_rows * a.channels * a.states;
     all.flat("state", a.state, state, a.state_out == a.state, false);
     if (a.state_out != a.state || !a.state_out) all.flat("state_out", a.state_out, state, true, false);
     all.flat("slots", a.slots, 4 * a.rows, false, true);
@@ -316,6 +329,7 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_sequences(op, s.sequences, s.length, s.tokens, s.packed);
     check_range(op, "channels", s.channels, 1, kMaxCount);
     check_range(op, "width", s.width, 2, FG_CONV_MAX_WIDTH);
+    size_of(op, "states", {s.sequences, s.width - 1, s.channels, kBytes[s.dtype]});
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     const std::string type = kTypes[s.dtype], w = "_w" + std::to_string(s.width);
     for (int v = 0; v < 3; ++v) {
@@ -406,7 +420,8 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
         std::lock_guard<std::mutex> lock(mu_);
         if (!part_.data() && g.seqs) {
             refuse_capture(op, dev_, stream);
-            part_ = Buffer<float, HipBackend>(dev_, n * g.runs * g.seqs);
+            const uint64_t places = s_.packed ? g.tokens / g.run + g.seqs : (uint64_t)g.runs * g.seqs;
+            part_ = Buffer<float, HipBackend>(dev_, n * places);
         }
     }
     g.part = part_.data();
@@ -431,6 +446,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_range(op, "groups", s.groups, 1, s.channels);
     if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
     check_range(op, "groups * states", s.groups * s.states, 1, kMaxRowStride);
+    size_of(op, "states", {4, s.sequences, s.channels, s.states});
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     segment_ = FG_SSM_SEGMENT;
     lane_states_ = s.states <= 4 ? 1 : s.states <= 8 ? 2 : 4;

@@ -139,6 +139,32 @@ def test_packed(gpu_device, channels):
     assert (out[4 + longest:60] == 7).all()
 
 
+@pytest.mark.parametrize("longest", [700, 21])
+def test_packed_parameter_gradients(gpu_device, longest):
+    """Many short sequences and a plan for much longer ones, or for shorter
+    ones (which cuts them): nothing of an earlier call's other sequences, rows
+    before, between or after is in the sums."""
+    import ferrum_gpu
+    rng = np.random.default_rng(23)
+    width, tokens, channels, n = 4, 700, 24, 30
+    x, gy = (_rounded(rng, (tokens, channels), "float32") for _ in range(2))
+    w = torch.from_numpy(rng.standard_normal((channels, width))).float()
+    plan = ferrum_gpu.ssm.ConvPlan(n, longest, channels, width, gpu_device, dtype="float32", tokens=tokens)
+    gw, gb, dx, dgy, dw = fill(w.shape), fill((channels,)), up(x), up(gy), up(w)
+    for start, most in ((0, 46), (17, 30), (300, 3)):
+        lengths = np.minimum(rng.integers(0, most, n), tokens)
+        offsets = np.minimum(start + np.concatenate([[0], np.cumsum(lengths)]), tokens).astype(np.int32)
+        plan.backward(dx, dw, dgy, grad_weight=gw, grad_bias=gb, offsets=up(torch.from_numpy(offsets)))
+        gpu_device.sync()
+        want, size = [0, 0], [0, 0]
+        for i, j in zip(offsets[:-1], np.minimum(offsets[1:], offsets[:-1] + longest)):
+            r, m = (o.conv(values(x[i:j]), values(w), grad=values(gy[i:j]), magnitude=q) for q in (False, True))
+            want = [want[0] + r["weight"], want[1] + r["bias"]]
+            size = [size[0] + m["weight"], size[1] + m["bias"]]
+        o.within(values(gw), want[0], size[0], _rounds(width, tokens), "float32", "grad_weight")
+        o.within(values(gb), want[1], size[1], _rounds(width, tokens), "float32", "grad_bias")
+
+
 def test_no_tokens(gpu_device):
     """No sequences, or sequences without tokens: states pass through, parameter gradients are zeros."""
     import ferrum_gpu
@@ -308,6 +334,11 @@ def test_refusals(gpu_device):
         plan.forward(x.data_ptr() + 2, w, out)
     with pytest.raises(E, match="exceeds"):
         make(batch=1, length=2, channels=(1 << 25) + 8, width=2).forward(x.data_ptr(), w.data_ptr(), out.data_ptr())
+    with pytest.raises(E, match="too large"):
+        make(batch=(1 << 31) - 1, channels=1 << 25, width=8)
+    with pytest.raises(E, match="too large"):
+        ssm.conv_step(gpu_device, x.data_ptr(), w.data_ptr(), st.data_ptr(), out.data_ptr(), batch=2,
+                      channels=(1 << 31) - 1, width=8, state_rows=(1 << 31) - 1, dtype="float32")
     with pytest.raises(ValueError, match="bytes"):
         plan.forward(ferrum_gpu.hip.DeviceBuffer(gpu_device, 64), w, out)
     with pytest.raises(E, match="state_rows"):

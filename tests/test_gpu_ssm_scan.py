@@ -566,6 +566,8 @@ def test_refusals(gpu_device):
     for bad in (dict(channels=(1 << 25) + 8), dict(channels=1 << 25, groups=1 << 24)):
         with pytest.raises(E, match="must be in"):
             make(length=1, batch=1, **bad)
+    with pytest.raises(E, match="too large"):
+        make(batch=(1 << 31) - 1, length=1, channels=1 << 25, groups=1)
     plan = make()
     x, out = up(torch.zeros(2, 8, 16)), up(torch.zeros(2, 8, 16))
     A, D = up(torch.zeros(16, 4)), up(torch.zeros(16))
