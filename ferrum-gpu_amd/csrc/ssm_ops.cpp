@@ -311,6 +311,12 @@ void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_st
 
 namespace {
 
+// Waves that a thread's run of tokens may leave: longer runs read fewer rows
+// twice and bring fewer parts to sum, shorter ones keep more loads on their way.
+// Measured, us for 1024 / 2048 / 4096 waves: forward, 9 packed sequences, 9001
+// tokens x 1536 channels in float16 18.2 / 14.4 / 14.9, 8 x 2048 tokens x 4096
+// channels in bfloat16 (runs of 64 and 64 / 32) - / 50.6 / 55.0.  Backward, the
+// last with 4096 / 8192 waves: 104 and 8.0 for the sums / 120 and 13.6.
 constexpr uint32_t kConvForwardWaves = 2048, kConvBackwardWaves = 4096;
 
 // Shared by both plans' constructors: sequences, length, tokens.
@@ -341,10 +347,12 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
 }
 
 // Tokens of a thread: as many as leave `waves` waves, each of 64 threads of n
-// channels, between FG_CONV_ROWS * 2 and 64.
-uint32_t ConvPlan::run_for(uint32_t n, uint32_t waves) const {
+// channels, up to 64 and `least` or more.  Forward that is one group of rows (2
+// x 1001 tokens x 2048 channels in bfloat16: 8.2 us, two groups 8.6), backward
+// two, for which half as many parts are summed.
+uint32_t ConvPlan::run_for(uint32_t n, uint32_t waves, uint32_t least) const {
     const uint64_t all = ceil_div(s_.channels / n, 64) * (uint64_t)s_.tokens;
-    uint32_t run = 2 * FG_CONV_ROWS;
+    uint32_t run = least;
     while (run < 64 && all / (2 * run) >= waves) run *= 2;
     return run;
 }
@@ -382,7 +390,7 @@ void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const 
     g.final = a.final;
     const int v = conv_vector(g.channels, es, {&g.x, &g.out}, {a.initial, a.final},
                               conv_widest(es, (uint32_t)s_.width));
-    g.run = run_for(kVector[v], kConvForwardWaves);
+    g.run = run_for(kVector[v], kConvForwardWaves, FG_CONV_ROWS);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
     void* args[] = {&g};
@@ -413,7 +421,7 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
     g.ginitial = a.grad_initial;
     const int v = conv_vector(g.channels, es, {&g.x, &g.out, &g.gx}, {a.initial, a.grad_final, a.grad_initial}, 4);
     // the run, and with it the workspace, is that of four channels for any call
-    g.run = run_for(std::min<uint32_t>(4, (uint32_t)s_.channels), kConvBackwardWaves);
+    g.run = run_for(std::min<uint32_t>(4, (uint32_t)s_.channels), kConvBackwardWaves, 2 * FG_CONV_ROWS);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const uint64_t n = (uint64_t)s_.channels * (s_.width + 1);
     {

@@ -44,7 +44,7 @@ private:
     fg_conv_kargs base(const int32_t* offsets) const;
     HipBackend::DeviceHandle dev_;
     fg_conv_shape s_;
-    uint32_t run_for(uint32_t n, uint32_t waves) const;
+    uint32_t run_for(uint32_t n, uint32_t waves, uint32_t least) const;
     HipBackend::KernelHandle forward_[3] = {}, backward_[3] = {}, reduce_;  // [8, 4, 1 channels of a thread]
     std::mutex mu_;
     Buffer<float, HipBackend> part_;
