@@ -90,7 +90,7 @@ template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kXor1 = 0xb1, kXor2 = 0x4e;
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e;
 
 __device__ __forceinline__ float swap32_add(float a, float b) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(a), __float_as_int(b), false, false);

@@ -80,20 +80,54 @@ __device__ __forceinline__ void bcast_dots(float& a, float& b, const float (&v)[
 }
 #undef FG_FMAC
 
+// For i < N: low[i] + low[i] of the lane that MOVE names, in the banks of four
+// lanes of BANKS high[i] + high[i] of it, to low[i].  In assembly: the compiler
+// makes two selections of this and one sum.
+#define FG_FOLD(i, move) "v_add_f32_dpp %" #i ", %" #i ", %" #i " " move " row_mask:0xf bank_mask:0xf\n\t"
+#define FG_OVER(i, n, move, banks) "v_add_f32_dpp %" #i ", %" #n ", %" #n " " move " row_mask:0xf bank_mask:" banks "\n\t"
+#define FG_HALVE(NAME, MOVE, BANKS)                                                                             \
+    template <int N>                                                                                            \
+    __device__ __forceinline__ void NAME(float* low, const float* high) {                                       \
+        if constexpr (N == 8) {                                                                                 \
+            NAME<4>(low, high);                                                                                 \
+            NAME<4>(low + 4, high + 4);                                                                         \
+        } else if constexpr (N == 4) {                                                                          \
+            asm("s_nop 1\n\t" FG_FOLD(0, MOVE) FG_FOLD(1, MOVE) FG_FOLD(2, MOVE)  \
+                FG_FOLD(3, MOVE) FG_OVER(0, 4, MOVE, BANKS) FG_OVER(1, 5, MOVE, BANKS)                \
+                FG_OVER(2, 6, MOVE, BANKS) FG_OVER(3, 7, MOVE, BANKS)                                           \
+                : "+&v"(low[0]), "+&v"(low[1]), "+&v"(low[2]), "+&v"(low[3])                                    \
+                : "v"(high[0]), "v"(high[1]), "v"(high[2]), "v"(high[3]));                                      \
+        } else if constexpr (N == 2) {                                                                          \
+            asm("s_nop 1\n\t" FG_FOLD(0, MOVE) FG_FOLD(1, MOVE) FG_OVER(0, 2, MOVE, BANKS)  \
+                FG_OVER(1, 3, MOVE, BANKS)                                                                      \
+                : "+&v"(low[0]), "+&v"(low[1])                                                                  \
+                : "v"(high[0]), "v"(high[1]));                                                                  \
+        } else {                                                                                                \
+            asm("s_nop 1\n\t" FG_FOLD(0, MOVE) FG_OVER(0, 1, MOVE, BANKS)                             \
+                : "+&v"(low[0])                                                                                 \
+                : "v"(high[0]));                                                                                \
+        }                                                                                                       \
+    }
+FG_HALVE(halve8, "row_ror:8", "0xc")
+FG_HALVE(halve4, "row_half_mirror", "0xa")
+#undef FG_HALVE
+#undef FG_OVER
+#undef FG_FOLD
+
 // The sum over a row's 16 channels of each of v[0 .. 4 N): halving the values
 // with every bit of the lane number, so that lane c ends with the sum of value
 // c (N = 4), c >> 1 (2) or c >> 2 (1) in v[0].
 template <int N>
 __device__ __forceinline__ void channels_sum(float (&v)[4 * N], uint32_t c) {
-    const bool b3 = c & 8, b2 = c & 4, b1 = c & 2, b0 = c & 1;
+    const bool b1 = c & 2, b0 = c & 1;
     auto level = [&](auto half, bool upper, auto ctrl) {
         each<half>([&](auto i) {
             const float low = v[i], high = v[i + half];
             v[i] = (upper ? high : low) + dpp<ctrl>(upper ? low : high);
         });
     };
-    level(Int<2 * N>{}, b3, Int<kRor8>{});
-    level(Int<N>{}, b2, Int<kHalfMirror>{});
+    halve8<2 * N>(v, v + 2 * N);
+    halve4<N>(v, v + N);
     if constexpr (N >= 2) level(Int<N / 2>{}, b1, Int<kXor2>{});
     else v[0] += dpp<kXor2>(v[0]);
     if constexpr (N >= 4) level(Int<1>{}, b0, Int<kXor1>{});
