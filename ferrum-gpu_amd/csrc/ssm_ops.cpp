@@ -348,8 +348,8 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
 
 // Tokens of a thread: as many as leave `waves` waves, each of 64 threads of n
 // channels, up to 64 and `least` or more.  Forward that is one group of rows (2
-// x 1001 tokens x 2048 channels in bfloat16: 8.2 us, two groups 8.6), backward
-// two, for which half as many parts are summed.
+// x 1001 tokens x 2048 channels in bfloat16: 8.2 us, two groups 8.6) or the two
+// that hold a wider window, backward two, for which half as many parts are summed.
 uint32_t ConvPlan::run_for(uint32_t n, uint32_t waves, uint32_t least) const {
     const uint64_t all = ceil_div(s_.channels / n, 64) * (uint64_t)s_.tokens;
     uint32_t run = least;
@@ -390,7 +390,9 @@ void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const 
     g.final = a.final;
     const int v = conv_vector(g.channels, es, {&g.x, &g.out}, {a.initial, a.final},
                               conv_widest(es, (uint32_t)s_.width));
-    g.run = run_for(kVector[v], kConvForwardWaves, FG_CONV_ROWS);
+    // no shorter than the window: only a sequence's first run, which writes the
+    // final state, reads the initial one, which may be the same array
+    g.run = run_for(kVector[v], kConvForwardWaves, s_.width - 1 > FG_CONV_ROWS ? 2 * FG_CONV_ROWS : FG_CONV_ROWS);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
     void* args[] = {&g};

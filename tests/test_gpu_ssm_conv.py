@@ -192,6 +192,26 @@ def test_final_may_be_initial(gpu_device):
     assert same(state, want)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("width", [2, 5, 6, 7, 8])
+def test_final_may_be_initial_over_runs(gpu_device, width, packed):
+    """Several runs to a sequence: none but the first may read the state."""
+    import ferrum_gpu
+    batch, length, channels = 16, 61, 200
+    tokens = batch * length
+    x = up(torch.randn(*((tokens,) if packed else (batch, length)), channels))
+    state = up(torch.randn(batch, width - 1, channels))
+    kept, fin, w = state.clone(), fill((batch, width - 1, channels), "float32"), up(torch.randn(channels, width))
+    a, b = like(x), like(x)
+    off = {"offsets": up(torch.arange(0, tokens + 1, length, dtype=torch.int32))} if packed else {}
+    plan = ferrum_gpu.ssm.ConvPlan(batch, length, channels, width, gpu_device, dtype="float32",
+                                   tokens=tokens if packed else None)
+    plan.forward(x, w, a, initial=kept, final=fin, **off)
+    plan.forward(x, w, b, initial=state, final=state, **off)
+    gpu_device.sync()
+    assert same(a, b) and same(fin, state)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("batch,channels,width", [(1, 8, 4), (5, 1000, 4), (3, 65, 3), (2, 2048, 8), (7, 16, 2)])
 def test_step(gpu_device, batch, channels, width, dtype):
