@@ -631,7 +631,7 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
     const uint64_t blocks = (uint64_t)g.seqs * g.chunks * blocks_;
     if (g.chunks > 1) launch(dev_, stream, back_local_[vec], blocks, threads_, args, op);
     launch(dev_, stream, backward_[vec], blocks, threads_, args, op);
-    if (g.gb.p || g.gc.p) launch(dev_, stream, reduce_bc_, ceil_div(g.tokens * row, 256), 256, args, op);
+    if ((g.gb.p || g.gc.p) && g.seqs) launch(dev_, stream, reduce_bc_, ceil_div(g.tokens * row, 256), 256, args, op);
     if (g.ga || g.gskip || g.gbias) launch(dev_, stream, reduce_p_, ceil_div(params, 256), 256, args, op);
 }
 

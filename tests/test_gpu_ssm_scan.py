@@ -195,6 +195,21 @@ def test_no_tokens(gpu_device):
         assert same(fin, i["initial"]) and same(gini, i["gfinal"]) and (gA == 0).all()
 
 
+def test_rows_of_no_sequence(gpu_device):
+    """Packed rows without any sequence: nothing is read or written, parameter gradients are zeros."""
+    import ferrum_gpu
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(0), (9,), 16, 8, 1, "float32", 0).items()}
+    off = up(torch.zeros(1, dtype=torch.int32))
+    out, gB, gC, gA = fill((9, 16)), fill((9, 1, 8)), fill((9, 1, 8)), fill((16, 8))
+    plan = ferrum_gpu.ssm.ScanPlan(0, 5, 16, 8, gpu_device, dtype="float32", tokens=9)
+    check = room(plan.checkpoint_bytes)
+    main = [i[k] for k in ("u", "delta", "A", "B", "C")]
+    plan.forward(*main, out, offsets=off, checkpoints=check)
+    plan.backward(*main, i["gy"], check, grad_A=gA, grad_B=gB, grad_C=gC, offsets=off)
+    gpu_device.sync()
+    assert all((v.get() == 7).all() for v in (out, gB, gC)) and (gA == 0).all()
+
+
 @pytest.mark.parametrize("length", [5, 900])
 def test_final_may_be_initial(gpu_device, length):
     """Also where the token axis is split: no part reads what another has written."""
