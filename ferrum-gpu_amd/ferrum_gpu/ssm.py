@@ -54,6 +54,7 @@ _DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
 _BYTES = {"float32": 4, "bfloat16": 2, "float16": 2}
 _ACTIVATIONS = {"silu": 1, None: 0}
 _torch_types: dict = {}  # name -> torch dtype, filled when the first tensor comes
+_type_names: dict = {}  # the other way round
 
 
 def _torch_type(dtype: str):
@@ -63,16 +64,14 @@ def _torch_type(dtype: str):
 
         for name in (*_DTYPES, "int32"):
             _torch_types[name] = getattr(torch, name)
+            _type_names[_torch_types[name]] = name
         t = _torch_types[dtype]
     return t
 
 
 def _dtype_of(x) -> str:
     d = x.dtype
-    for name, t in _torch_types.items():
-        if t is d:
-            return name
-    return str(d).rpartition(".")[2]
+    return _type_names.get(d) or str(d).rpartition(".")[2]
 
 
 def _check_dtype(dtype) -> str:
@@ -114,6 +113,12 @@ def _flat(x, shape: tuple, dtype: str, nbytes: int, ordinal: int, what: str) -> 
     """The address of a contiguous array, 0 for None."""
     if x is None:
         return 0
+    # What a tensor passes in most calls; a one-token call is bound by the host.
+    try:
+        if x.shape == shape and x.dtype is _torch_types[dtype] and x.get_device() == ordinal and x.is_contiguous():
+            return x.data_ptr()
+    except (AttributeError, KeyError):  # no tensor, or the first one
+        pass
     if hasattr(x, "data_ptr"):
         if x.shape != shape or x.dtype is not _torch_type(dtype) or x.get_device() != ordinal:
             raise _wrong(x, what, (shape,), dtype, ordinal)
@@ -353,17 +358,31 @@ class ScanPlan(_Plan):
             _n.check(rc)
 
 
-def _size(given, x, axis: int, what: str) -> int:
+def _shape(x) -> tuple:
+    return x.shape if hasattr(x, "data_ptr") else ()
+
+
+def _size(given, shape: tuple, axis: int, what: str) -> int:
     """A size: what the caller gave, else the tensor's."""
     if given is not None:
         return int(given)
-    if hasattr(x, "data_ptr") and x.dim() > axis:
-        return x.shape[axis]
+    if len(shape) > axis:
+        return shape[axis]
     raise ValueError(f"{what} is needed where the array is not a tensor that has it")
 
 
-def _step_row(x, batch: int, width: int, inner: tuple, dtype: str, ordinal: int, what: str) -> tuple:
-    p, _, row = _rows(x, (batch,), width, inner, dtype, ordinal, what)
+def _step_row(x, shape: tuple, inner: tuple, dtype: str, ordinal: int, what: str) -> tuple:
+    """_rows() of one token of each row: ``shape`` is (batch, width)."""
+    if x is None:
+        return 0, 0, 0
+    try:  # as in _flat()
+        if x.shape == shape and x.dtype is _torch_types[dtype] and x.get_device() == ordinal:
+            row, element = x.stride()
+            if element == 1:
+                return x.data_ptr(), row, 0
+    except (AttributeError, KeyError):
+        pass
+    p, _, row = _rows(x, shape[:1], shape[1], inner, dtype, ordinal, what)
     return p, row, 0
 
 
@@ -377,17 +396,19 @@ def conv_step(device: Device, x, weight, state, out, bias=None, slots=None, stat
     two rows may share a slot.  ``state_out``: where the moved windows go
     (None: ``state`` itself).  Sizes and ``dtype`` come from tensors; they are
     given where the arrays are DeviceBuffers or addresses."""
-    batch, channels = _size(batch, x, 0, "batch"), _size(channels, x, 1, "channels")
-    width = _size(width, weight, 1, "width")
-    state_rows = _size(state_rows, state, 0, "state_rows")
+    lead = _shape(x)
+    batch, channels = _size(batch, lead, 0, "batch"), _size(channels, lead, 1, "channels")
+    width = _size(width, _shape(weight), 1, "width")
+    state_rows = _size(state_rows, _shape(state), 0, "state_rows")
     dtype = _check_dtype(dtype or (_dtype_of(x) if hasattr(x, "data_ptr") else "bfloat16"))
     at = device.ordinal
+    row = (batch, channels)
     shape = (state_rows, width - 1, channels)
     nbytes = state_rows * (width - 1) * channels * _BYTES[dtype]
     s = _flat(state, shape, dtype, nbytes, at, "state")
     args = _conv_step_pack(batch, channels, width, _DTYPES[dtype], _check_activation(activation), state_rows,
-                           *_step_row(x, batch, channels, (), dtype, at, "x"),
-                           *_step_row(out, batch, channels, (), dtype, at, "out"),
+                           *_step_row(x, row, (), dtype, at, "x"),
+                           *_step_row(out, row, (), dtype, at, "out"),
                            _flat(weight, (channels, width), "float32", 4 * channels * width, at, "weight"),
                            _flat(bias, (channels,), "float32", 4 * channels, at, "bias"), s,
                            s if state_out is None else _flat(state_out, shape, dtype, nbytes, at, "state_out"),
@@ -406,25 +427,26 @@ def scan_step(device: Device, u, delta, A, B, C, state, out, D=None, z=None, del
     ``state_out`` as for conv_step().  Sizes and ``dtype`` come from tensors
     (``groups`` from B's); they are given where the arrays are DeviceBuffers or
     addresses."""
-    batch, channels = _size(batch, u, 0, "batch"), _size(channels, u, 1, "channels")
-    states = _size(states, A, 1, "states")
-    state_rows = _size(state_rows, state, 0, "state_rows")
+    lead = _shape(u)
+    batch, channels = _size(batch, lead, 0, "batch"), _size(channels, lead, 1, "channels")
+    states = _size(states, _shape(A), 1, "states")
+    state_rows = _size(state_rows, _shape(state), 0, "state_rows")
     dtype = _check_dtype(dtype or (_dtype_of(u) if hasattr(u, "data_ptr") else "bfloat16"))
     if groups is None:
         groups = 1 if not hasattr(B, "data_ptr") or states < 1 else B.shape[1] if B.dim() == 3 \
             else B.shape[-1] // states
     at = device.ordinal
-    inner = (groups, states)
+    row, bc, inner = (batch, channels), (batch, groups * states), (groups, states)
     shape = (state_rows, channels, states)
     nbytes = 4 * state_rows * channels * states
     s = _flat(state, shape, "float32", nbytes, at, "state")
     args = _scan_step_pack(batch, channels, states, groups, _DTYPES[dtype], bool(softplus), state_rows,
-                           *_step_row(u, batch, channels, (), dtype, at, "u"),
-                           *_step_row(delta, batch, channels, (), dtype, at, "delta"),
-                           *_step_row(B, batch, groups * states, inner, dtype, at, "B"),
-                           *_step_row(C, batch, groups * states, inner, dtype, at, "C"),
-                           *_step_row(z, batch, channels, (), dtype, at, "z"),
-                           *_step_row(out, batch, channels, (), dtype, at, "out"),
+                           *_step_row(u, row, (), dtype, at, "u"),
+                           *_step_row(delta, row, (), dtype, at, "delta"),
+                           *_step_row(B, bc, inner, dtype, at, "B"),
+                           *_step_row(C, bc, inner, dtype, at, "C"),
+                           *_step_row(z, row, (), dtype, at, "z"),
+                           *_step_row(out, row, (), dtype, at, "out"),
                            _flat(A, (channels, states), "float32", 4 * channels * states, at, "A"),
                            _flat(D, (channels,), "float32", 4 * channels, at, "D"),
                            _flat(delta_bias, (channels,), "float32", 4 * channels, at, "delta_bias"), s,
