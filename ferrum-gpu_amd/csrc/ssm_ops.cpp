@@ -492,7 +492,9 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
 // adds to the states.  Measured, us for one pass of 4 sequences of 16 states in
 // bfloat16, parts 1 / 2 / 4: forward, 1024 tokens x 2048 channels (512 waves)
 // 88 / 87 / 78, 2048 x 4096 (1024 waves) 177 / 256; backward, 1024 x 2048
-// (parts 2 / 4) 204 / 157.  A part has 64 tokens or more.  Packed sequences count
+// (parts 2 / 4) 204 / 157.  A part has 32 tokens or more (16 / 32 / 64: forward, 300 x
+// 1024 15.5 / 14.2 / 17.9, training step 128 x 1024 34 / 41 / 56, 1024 x 512 59 / 51 /
+// 61; 16 states in bfloat16).  Packed sequences count
 // as so many of the longest's length, which the last wave to end works through,
 // and are cut into twice the parts, which evens them out (7 sequences, 9001
 // tokens x 1536 channels x 8 states in float16: 136 us, twice the parts 97).
@@ -500,7 +502,7 @@ uint32_t ScanPlan::chunks_for(uint32_t few) const {
     const uint64_t seqs = s_.packed && s_.length ? ceil_div(s_.tokens, s_.length) : s_.sequences;
     const uint64_t waves = std::max<uint64_t>(1, seqs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_);
     if (waves > few) return 1;
-    const uint64_t most = std::max<uint64_t>(1, ceil_div(s_.length, 4 * segment_));
+    const uint64_t most = std::max<uint64_t>(1, ceil_div(s_.length, 2 * segment_));
     return (uint32_t)std::min<uint64_t>({ceil_div(s_.packed ? 4096 : 2048, waves), most, 64});
 }
 
