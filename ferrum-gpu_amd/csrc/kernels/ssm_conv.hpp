@@ -7,6 +7,11 @@
 // or are zero.  A thread takes V neighbouring channels through a run of
 // tokens with the last W - 1 rows in registers, so each row is read once, plus
 // W - 1 rows at the start of a run (backward: also at its end).
+//
+// Bound by memory where there are many rows, else by the chain of loads of one
+// run.  Measured (4 taps, bfloat16): 8 x 2048 tokens x 4096 channels forward 48
+// to 51 us (5.4 TB/s), backward 105 (3.8 TB/s) and 7 for the sums over the
+// runs; 2 x 1001 x 2048 forward 8 us; a step of 256 rows x 4096 channels 6 us.
 #pragma once
 
 #include "ssm_common.hpp"
