@@ -20,7 +20,7 @@
 // forward (5 of them the formula's), 22.8 in the gradients' pass, issued in 73
 // to 81 % of the cycles (counters of 4 x 1024 tokens x 2048 channels x 16 states
 // in bfloat16).  Measured: 4 x 2048 tokens x 4096 channels forward 165 us; 4 x
-// 1024 x 2048 forward and backward 234 us; steps of 256 rows x 4096 channels 33
+// 1024 x 2048 forward and backward 233 us; steps of 256 rows x 4096 channels 33
 // us, 4.3 TB/s of states.
 //
 // W is 1 up to 16 states, 2 up to 32, 4 up to 64.  (16 states on two waves, for
