@@ -92,6 +92,15 @@ __device__ __forceinline__ float dpp(float x) {
 }
 constexpr int kXor1 = 0xb1, kXor2 = 0x4e;
 
+// Two wait states behind the instructions that wrote v, which lane exchanges
+// need.  The compiler keeps them by itself, but not for what a statement of
+// assembly wrote.
+__device__ __forceinline__ void settle(float& a) { asm("s_nop 1" : "+v"(a)); }
+__device__ __forceinline__ void settle(float& a, float& b, float& c, float& d) {
+    asm("s_nop 1" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+
+// Both values settled.
 __device__ __forceinline__ float swap32_add(float a, float b) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(a), __float_as_int(b), false, false);
     return __int_as_float(r[0]) + __int_as_float(r[1]);

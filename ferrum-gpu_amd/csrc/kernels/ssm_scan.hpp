@@ -36,7 +36,8 @@ namespace ssm {
 // Multiply-adds whose first factor is lane J of the row's v, in statements of
 // assembly: the compiler does not fold the broadcast into a multiply-add.  The
 // s_nop keeps the two wait states that a DPP operand needs after the
-// instruction that wrote it.
+// instruction that wrote it; who takes a result into a lane exchange settles it
+// first (settle()).
 #define FG_FMAC(acc, v, x, j) "v_fmac_f32_dpp %" #acc ", %" #v ", %" #x " row_newbcast:%" #j " row_mask:0xf bank_mask:0xf\n\t"
 // acc[s] += v[s] * x, s < N.
 template <int N, int J>
@@ -136,7 +137,7 @@ __device__ __forceinline__ void channels_sum(float (&v)[4 * N], uint32_t c) {
     halve8<2 * N>(v, v + 2 * N);
     halve4<N>(v, v + N);
     if constexpr (N >= 2) level(Int<N / 2>{}, b1, Int<kXor2>{});
-    else v[0] += dpp<kXor2>(v[0]);
+    else settle(v[0]), v[0] += dpp<kXor2>(v[0]);  // written in assembly (halve4)
     if constexpr (N >= 4) level(Int<1>{}, b0, Int<kXor1>{});
     else v[0] += dpp<kXor1>(v[0]);
 }
@@ -394,7 +395,8 @@ struct Scan {
     struct Sums {
         float v[2 * W][PART];
         // v[j]: the lane's sum for token 4 i + j
-        __device__ __forceinline__ void put(const Place& p, int i, const float (&x)[4]) {
+        __device__ __forceinline__ void put(const Place& p, int i, float (&x)[4]) {
+            settle(x[0], x[1], x[2], x[3]);  // written in assembly (bcast_dot)
             float* to = v[2 * p.part + (p.q & 1)] + (4 * i + (p.q & 2)) * 16 + p.c;
             to[0] = swap32_add(x[0], x[2]);
             to[16] = swap32_add(x[1], x[3]);
