@@ -159,7 +159,7 @@ def _rows(x, lead: tuple, width: int, inner: tuple, dtype: str, ordinal: int, wh
         else:
             fine = None
         if fine is None:
-            raise _wrong(x, what, (lead + (width,), lead + inner), dtype, ordinal)
+            raise _wrong(x, what, (lead + (width,), lead + inner) if inner else (lead + (width,),), dtype, ordinal)
         if not fine:
             raise ValueError(f"{what}: the elements of a row must be adjacent (strides {tuple(st)})")
         return (x.data_ptr(), st[0], st[1]) if n == 2 else (x.data_ptr(), 0, st[0])

@@ -178,5 +178,16 @@ def test_tensors_are_checked_on_the_host():
             flat(bad)
 
 
+@pytest.mark.parametrize("lead,width", [((2, 8), 16), ((8,), 16)])
+def test_rows_without_their_last_axis_are_refused(lead, width):
+    """A dense plan's (batch, length), a packed plan's (tokens), a step's (batch)."""
+    torch = pytest.importorskip("torch")
+    for bad in (torch.zeros(lead), torch.zeros(*lead, width, 1), torch.zeros(width)):
+        with pytest.raises(ValueError, match="shape"):
+            ssm._rows(bad, lead, width, (), "float32", -1, "x")
+        with pytest.raises(ValueError, match="shape"):
+            ssm._step_row(bad, (lead[0], width), (), "float32", -1, "x")
+
+
 def test_package_exports_the_module():
     assert ferrum_gpu.ssm is ssm and "ssm" in ferrum_gpu.__all__
