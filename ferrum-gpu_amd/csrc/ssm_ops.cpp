@@ -326,6 +326,15 @@ void check_sequences(const char* op, int64_t sequences, int64_t length, int64_t 
     if (packed) check_range(op, "tokens", tokens, 0, int64_t(1) << 40);
 }
 
+// Rows of `width` elements: what is worked out from their number (launches,
+// workspaces, checkpoints) stays within 64 bits, also for inputs whose stride of
+// 0 lets a small array stand for any number of rows.
+template <class Shape>
+void check_rows(const char* op, const Shape& s, int64_t width) {
+    if (s.packed) size_of(op, "rows", {s.tokens, width, kBytes[s.dtype]});
+    else size_of(op, "rows", {s.sequences, s.length, width, kBytes[s.dtype]});
+}
+
 }  // namespace
 
 ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_conv_shape& s)
@@ -335,6 +344,7 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_sequences(op, s.sequences, s.length, s.tokens, s.packed);
     check_range(op, "channels", s.channels, 1, kMaxCount);
     check_range(op, "width", s.width, 2, FG_CONV_MAX_WIDTH);
+    check_rows(op, s, s.channels);
     size_of(op, "states", {s.sequences, s.width - 1, s.channels, kBytes[s.dtype]});
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     const std::string type = kTypes[s.dtype], w = "_w" + std::to_string(s.width);
@@ -394,7 +404,7 @@ void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const 
     // final state, reads the initial one, which may be the same array
     g.run = run_for(kVector[v], kConvForwardWaves, s_.width - 1 > FG_CONV_ROWS ? 2 * FG_CONV_ROWS : FG_CONV_ROWS);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
-    const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
+    const int64_t waves = size_of(op, "launch", {(int64_t)ceil_div(g.channels / kVector[v], 64), g.runs, g.seqs});
     void* args[] = {&g};
     launch(dev_, stream, forward_[v], ceil_div(waves, 4), 256, args, op);
 }
@@ -431,11 +441,12 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
         if (!part_.data() && g.seqs) {
             refuse_capture(op, dev_, stream);
             const uint64_t places = s_.packed ? g.tokens / g.run + g.seqs : (uint64_t)g.runs * g.seqs;
+            size_of(op, "workspace", {4, (int64_t)n, (int64_t)places});
             part_ = Buffer<float, HipBackend>(dev_, n * places);
         }
     }
     g.part = part_.data();
-    const uint64_t waves = ceil_div(g.channels / kVector[v], 64) * g.runs * g.seqs;
+    const int64_t waves = size_of(op, "launch", {(int64_t)ceil_div(g.channels / kVector[v], 64), g.runs, g.seqs});
     void* args[] = {&g};
     launch(dev_, stream, backward_[v], ceil_div(waves, 4), 256, args, op);
     uint32_t width = (uint32_t)s_.width;
@@ -456,6 +467,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     check_range(op, "groups", s.groups, 1, s.channels);
     if (s.channels % s.groups) invalid("scan plan: groups must divide channels");
     check_range(op, "groups * states", s.groups * s.states, 1, kMaxRowStride);
+    check_rows(op, s, std::max(s.channels, s.groups * s.states));
     size_of(op, "states", {4, s.sequences, s.channels, s.states});
     if (!s_.packed) s_.tokens = s_.sequences * s_.length;
     segment_ = FG_SSM_SEGMENT;
@@ -469,6 +481,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     if (chunks_forward_ > 1 || chunks_backward_ > 1) {
         const uint64_t places = (uint64_t)s.sequences * (std::max(chunks_forward_, chunks_backward_) + 1) * blocks_ *
                                 FG_SSM_BLOCKS(waves_);
+        size_of(op, "workspace", {4, (int64_t)places, waves_, 64, lane_states_});
         carry_ = Buffer<float, HipBackend>(dev, places * waves_ * 64 * lane_states_);
         carry_dt_ = Buffer<float, HipBackend>(dev, places * 16);
     }
@@ -622,6 +635,8 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
         std::lock_guard<std::mutex> lock(mu_);
         if (!part_p_.data() && g.seqs) {
             refuse_capture(op, dev_, stream);
+            size_of(op, "workspace", {4, group_blocks_, s_.tokens, (int64_t)row});
+            size_of(op, "workspace", {4, (int64_t)params, g.seqs, g.chunks});
             part_bc_ = Buffer<float, HipBackend>(dev_, group_blocks_ * (uint64_t)s_.tokens * row);
             part_p_ = Buffer<float, HipBackend>(dev_, params * g.seqs * g.chunks);
         }

@@ -448,3 +448,23 @@ def test_rows_far_apart(gpu_device):
     plan.forward(near, w, far)
     gpu_device.sync()
     assert same(a, b) and same(far, b)
+
+
+def test_sizes_that_pass_64_bits(gpu_device):
+    """Rows of stride 0 can stand for any number of them: no size worked out from it wraps around."""
+    import ferrum_gpu
+    from ferrum_gpu import _native as N
+    ssm, E, most = ferrum_gpu.ssm, N.FerrumGpuError, (1 << 31) - 1
+    for make in (lambda **k: ssm.ConvPlan(width=2, **k), lambda **k: ssm.ScanPlan(states=4, **k)):
+        with pytest.raises(E, match="rows: too large"):
+            make(batch=most, length=most, channels=1024, device=gpu_device)
+        with pytest.raises(E, match="rows: too large"):
+            make(batch=1, length=most, channels=1 << 25, tokens=1 << 40, device=gpu_device)
+    # a workspace that no memory holds: 2^24 sequences' parts of 3 * 2^21 sums
+    tokens, channels = 1 << 24, 1 << 21
+    plan = ssm.ConvPlan(tokens, most, channels, 2, gpu_device, tokens=tokens)
+    row = up(torch.zeros(1, channels, dtype=torch.bfloat16)).expand(tokens, channels)
+    off = up(torch.zeros(tokens + 1, dtype=torch.int32))
+    with pytest.raises(E, match="workspace: too large"):
+        plan.backward(row, up(torch.zeros(channels, 2)), row, offsets=off)
+    gpu_device.sync()
