@@ -45,6 +45,13 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// h 2^(2 x) + add, also where 2^(2 x) alone passes the type's range: by 2^x
+// twice.  The largest number stands for an infinite 2^x, which takes no 0 to NaN.
+__device__ __forceinline__ float times_exp2_twice(float h, float x, float add) {
+    const float f = fminf(exp2_(x), 3.402823466e38f);
+    return fmaf(h * f, f, add);
+}
+
 // 1 / (1 + exp(-x)).
 __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + exp2_(-kLog2e * x));

@@ -354,7 +354,8 @@ struct Scan {
     }
 
     // Takes the states h over n chunks, the i-th of them chunk at(i): four are
-    // loaded at a time.
+    // loaded at a time.  A chunk's factor can pass the range that the states keep
+    // token by token (growing ones, of positive A or negative steps).
     template <class At>
     static __device__ __forceinline__ void take_chunks(const fg_scan_kargs& g, const Place& p, const Lane& l,
                                                        float (&h)[S], uint32_t n, At&& at) {
@@ -366,9 +367,10 @@ struct Scan {
                 each<S>([&](auto s) { add[j][s] = carry_of(g, p, i)[s]; });
             });
             each<4>([&](auto j) {
+                const float half = 0.5f * sum[j];
                 if (k + j < n)
                     each<S>([&](auto s) {
-                        h[s] = fmaf(exp2_(sum[j] * l.a2[s]), h[s], add[j][s]);
+                        h[s] = times_exp2_twice(h[s], half * l.a2[s], add[j][s]);
                         if (PAD && l.pad[s]) h[s] = 0.0f;
                     });
             });

@@ -633,3 +633,49 @@ def test_refusals(gpu_device):
     with pytest.raises(ValueError, match="destroyed"):
         plan.forward(x, delta, A, B, C, out)
     gpu_device.sync()
+
+
+@pytest.mark.parametrize("states", [16, 5])
+def test_parts_of_growing_and_shrinking_states(gpu_device, states):
+    """States that are 0, or so small or large, that they stay finite token by
+    token, under factors of a part of the tokens (here e^96 and e^-96) that
+    32 bits do not hold; forward and backward."""
+    import ferrum_gpu
+    length, channels = 300, 16
+    i = _inputs(np.random.default_rng(13), (1, length), channels, states, 1, "float32", 1)
+    i["A"].fill_(3.0)
+    i["delta"].fill_(1.0)
+    i["delta_bias"].zero_()
+    # channels 0 .. 7: nothing comes in before the last tokens, no gradient after the first
+    i["u"][:, :-5] = i["gy"][:, 5:] = 0
+    i["initial"][:, :8] = i["gfinal"][:, :8] = 0
+    # the others: 32 tokens up, 32 down, four times; or down, then up
+    turns = torch.arange(length) // 32 % 2 == 1
+    i["delta"][0, turns, 8:] = -1
+    i["delta"][0, 256:, 8:] = 0
+    i["delta"][:, :, 12:] *= -1
+    i["initial"][:, 8:12], i["initial"][:, 12:] = 1e-30, 1e30
+    i["gfinal"][:, 8:12], i["gfinal"][:, 12:] = 1e30, 1e-30
+    i["u"][:, :, 8:] = i["gy"][:, :, 8:] = 0
+    d = {k: up(v) for k, v in i.items()}
+    plan = ferrum_gpu.ssm.ScanPlan(1, length, channels, states, gpu_device, dtype="float32", softplus=False)
+    check = room(plan.checkpoint_bytes)
+    got = {"out": fill(i["u"].shape), "final": fill(i["initial"].shape), "initial": fill(i["initial"].shape)}
+    grads = ("u", "delta", "A")
+    got.update({k: fill(i[k].shape) for k in grads})
+    main = [d[k] for k in ("u", "delta", "A", "B", "C")]
+    plan.forward(*main, got["out"], initial=d["initial"], final=got["final"], checkpoints=check)
+    plan.backward(*main, d["gy"], check, **{"grad_" + k: got[k] for k in grads}, grad_initial=got["initial"],
+                  grad_final=d["gfinal"])
+    gpu_device.sync()
+    a = _oracle_args(i, (0, slice(0, length)), 0, False, ("z", "D"))
+    r, m = o.scan(**a), o.scan(**a, magnitude=True)
+    # as _compare(), with a sum of the time steps and its product in each of ten parts
+    rounds = o.scan_rounds(length, a["A"], 1.0, states) + 10 * (34 + 3 * 32)
+    o.within(values(got["out"][0]), r["out"], m["out"], rounds, "float32", "out")
+    o.within(values(got["final"][0]), r["final"], m["final"], rounds, "float32", "final")
+    o.within(values(got["initial"][0]), r["initial"], m["initial"], rounds, "float32", "grad_initial")
+    for k in ("u", "delta"):
+        o.within(values(got[k][0]), r[k], m[k], 2 * rounds, "float32", "grad_" + k)
+    o.within(values(got["A"]), r["A"], m["A"], 2 * rounds + length, "float32", "grad_A")
+    assert (values(got["final"])[0, 8:] != 0).all() and (values(got["initial"])[0, 8:] != 0).all()
