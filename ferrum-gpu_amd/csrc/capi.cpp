@@ -903,6 +903,14 @@ int fg_conv_plan_destroy(fg_conv_plan_t plan) {
     });
 }
 
+int fg_conv_plan_get_info(fg_conv_plan_t plan, fg_conv_plan_info* out) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(out, "out");
+        plan->plan->info(out);
+    });
+}
+
 int fg_conv_forward(fg_conv_plan_t plan, const fg_conv_forward_args* args, fg_stream_t stream) {
     return guarded([&] {
         need(plan, "plan");
@@ -954,6 +962,14 @@ int fg_scan_checkpoint_bytes(fg_scan_plan_t plan, size_t* bytes) {
         need(plan, "plan");
         need(bytes, "bytes");
         *bytes = plan->plan->checkpoint_bytes();
+    });
+}
+
+int fg_scan_plan_get_info(fg_scan_plan_t plan, fg_scan_plan_info* out) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(out, "out");
+        plan->plan->info(out);
     });
 }
 

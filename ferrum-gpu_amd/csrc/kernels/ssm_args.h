@@ -32,12 +32,13 @@ typedef struct {
     float *ga, *gskip, *gbias, *ginitial;
     const int32_t* offsets; /* packed: sequences + 1 of them; null: dense */
     float* check;           /* states at segment starts */
-    float* carry;           /* [sequences][chunks + 1][blocks of 16 channels][16 * 4 W S]: what a chunk adds;
-                               the last place: the initial states */
-    float* carry_dt;        /* [sequences][chunks + 1][blocks of 16 channels][16]: its summed time steps */
+    float* carry;           /* [places + sequences][blocks of 16 channels][16 * 4 W S]: what a chunk adds;
+                               behind the chunks' places: each sequence's initial states */
+    float* carry_dt;        /* [places][blocks of 16 channels][16]: its summed time steps */
     float* part_bc;         /* [channel blocks of a group][tokens][groups][2][states] */
-    float* part_p;          /* [sequences * chunks][channels * (states + 2)] */
+    float* part_p;          /* [places][channels * (states + 2)] */
     uint64_t tokens;        /* packed: of all sequences */
+    uint64_t places;        /* of chunks, over all sequences */
     uint32_t seqs, length, channels, states, groups;
     uint32_t group_channels, group_blocks; /* channels of a group, workgroups over them */
     uint32_t chunks, chunk_len;            /* chunk_len: a multiple of the segment */

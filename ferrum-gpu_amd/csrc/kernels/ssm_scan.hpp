@@ -142,6 +142,19 @@ __device__ __forceinline__ void channels_sum(float (&v)[4 * N], uint32_t c) {
     else v[0] += dpp<kXor1>(v[0]);
 }
 
+// A sequence's first row, packed; offsets beyond the rows are taken as the nearest.
+__device__ __forceinline__ int64_t scan_row_of(const fg_scan_kargs& g, uint32_t seq) {
+    const int64_t a = g.offsets[seq], all = (int64_t)g.tokens;
+    return a < 0 ? 0 : a > all ? all : a;
+}
+
+// The first place of sequence `seq` among the chunks of all.  Packed: one for
+// every chunk's length of rows and one more for each sequence, not for each
+// sequence's longest.
+__device__ __forceinline__ uint64_t scan_places_before(const fg_scan_kargs& g, uint32_t seq) {
+    return g.offsets ? (uint64_t)((uint32_t)scan_row_of(g, seq) / g.chunk_len) + seq : (uint64_t)seq * g.chunks;
+}
+
 // WIDE: every row takes vector loads and stores, every channel has 4 S W
 // states; else any alignment and stride, and fewer states.
 template <class T, int S, int W, bool WIDE>
@@ -156,6 +169,7 @@ struct Scan {
     // Where a wave works: its sequence, the tokens of its chunk, its channels.
     struct Place {
         int64_t start;               // packed: the sequence's first row
+        uint64_t first;              // its first place among the chunks of all
         uint32_t len;                // tokens of the sequence
         uint32_t seq, chunk, group, block;
         uint32_t t0, t1;             // the chunk's tokens
@@ -189,14 +203,15 @@ struct Scan {
         p.chunk = rest % g.chunks;
         p.seq = rest / g.chunks;
         p.start = 0;
+        p.first = (uint64_t)p.seq * g.chunks;
         p.len = g.length;
         if (g.offsets) {
             // offsets out of order or beyond the rows give shorter sequences, not accesses outside
-            int64_t a = g.offsets[p.seq], b = g.offsets[p.seq + 1];
-            const int64_t all = (int64_t)g.tokens;
-            a = a < 0 ? 0 : a > all ? all : a;
-            b = b < a ? a : b > all ? all : b;
+            const int64_t a = scan_row_of(g, p.seq);
+            int64_t b = scan_row_of(g, p.seq + 1);
+            b = b < a ? a : b;
             p.start = uniform(a);
+            p.first = (uint64_t)((uint32_t)p.start / g.chunk_len) + p.seq;
             p.len = uniform((uint32_t)(b - a < (int64_t)g.length ? b - a : (int64_t)g.length));
         }
         const uint64_t first = (uint64_t)p.chunk * g.chunk_len;
@@ -330,7 +345,7 @@ struct Scan {
     }
 
     // Places of the wave's 64 S values: the states at the start of the segment
-    // at token t, and what chunk k adds (place `chunks`: the initial states).
+    // at token t, what a chunk adds, and the initial states.
     static __device__ __forceinline__ uint64_t lanes_of(const fg_scan_kargs& g, const Place& p, uint64_t k) {
         return ((k * (g.groups * g.group_blocks * BLOCKS) + p.sets) * W + p.part) * (64 * S) + (threadIdx.x & 63) * S;
     }
@@ -339,12 +354,14 @@ struct Scan {
         return g.check + lanes_of(g, p, seg + t / SEG);
     }
     static __device__ __forceinline__ float* carry_of(const fg_scan_kargs& g, const Place& p, uint32_t chunk) {
-        return g.carry + lanes_of(g, p, (uint64_t)p.seq * (g.chunks + 1) + chunk);
+        return g.carry + lanes_of(g, p, p.first + chunk);
+    }
+    static __device__ __forceinline__ float* initial_of(const fg_scan_kargs& g, const Place& p) {
+        return g.carry + lanes_of(g, p, g.places + p.seq);
     }
     // The 16 channels' summed time steps of chunk k.
     static __device__ __forceinline__ float* carry_dt_of(const fg_scan_kargs& g, const Place& p, uint32_t chunk) {
-        const uint64_t k = (uint64_t)p.seq * (g.chunks + 1) + chunk;
-        return g.carry_dt + (k * (g.groups * g.group_blocks * BLOCKS) + p.sets) * 16;
+        return g.carry_dt + ((p.first + chunk) * (g.groups * g.group_blocks * BLOCKS) + p.sets) * 16;
     }
     static __device__ __forceinline__ uint64_t state_at(const fg_scan_kargs& g, const Place& p, int s) {
         return ((uint64_t)p.seq * g.channels + p.ch) * g.states + p.row * S + s;
@@ -534,7 +551,7 @@ struct Scan {
             // the last chunks may write the final states where the initial ones lie
             each<S>([&](auto s) {
                 const bool has = g.initial && has_state(g, p, s);
-                carry_of(g, p, g.chunks)[s] = has ? g.initial[state_at(g, p, s)] : 0.0f;
+                initial_of(g, p)[s] = has ? g.initial[state_at(g, p, s)] : 0.0f;
             });
         }
         if (LOCAL && p.t1 == p.len) return;                 // no chunk follows
@@ -546,7 +563,7 @@ struct Scan {
         each<S>([&](auto s) { h[s] = 0.0f; });
         if constexpr (!LOCAL) {
             each<S>([&](auto s) {
-                if (g.chunks > 1) h[s] = carry_of(g, p, g.chunks)[s];
+                if (g.chunks > 1) h[s] = initial_of(g, p)[s];
                 else if (g.initial && has_state(g, p, s)) h[s] = g.initial[state_at(g, p, s)];
             });
             take_chunks(g, p, l, h, p.chunk, [](uint32_t i) { return i; });
@@ -879,6 +896,8 @@ struct Scan {
         constexpr bool SHARED = !LOCAL || W > 1;
         const Place p = place(g);
         if (LOCAL && (p.chunk == 0 || p.t1 == p.t0)) return;  // no chunk before it, or no tokens
+        // packed chunks without tokens may have no place for the parameters' parts
+        if (!LOCAL && p.chunk > 0 && p.t1 == p.t0 && p.first + p.chunk >= scan_places_before(g, p.seq + 1)) return;
         const Lane l = lane(g, p);
         Lds& lds = all[p.set];
         float carry[S], ga[S];
@@ -997,21 +1016,34 @@ struct Scan {
             });
             each<S>([&](auto s) { carry_of(g, p, p.chunk)[s] = carry[s]; });
         } else {
-            float* to = g.part_p + ((uint64_t)p.seq * g.chunks + p.chunk) * g.channels * (g.states + 2);
             each<VC>([&](auto i) {
-                const float s = tokens_sum(p, gskip[i], lds.dt), v = tokens_sum(p, gbias[i], lds.dt);
-                if (i < p.have && p.tok == 0) {
-                    const uint64_t ch = p.group * g.group_channels + p.in_group + i;
-                    to[(uint64_t)g.channels * g.states + ch] = s;
-                    to[(uint64_t)g.channels * (g.states + 1) + ch] = v;
-                }
+                gskip[i] = tokens_sum(p, gskip[i], lds.dt);
+                gbias[i] = tokens_sum(p, gbias[i], lds.dt);
             });
-            if (p.valid) {
-                each<S>([&](auto s) {
-                    if (has_state(g, p, s)) {
-                        to[(uint64_t)p.ch * g.states + p.row * S + s] = ga[s];
-                        if (g.ginitial && p.chunk == 0) g.ginitial[state_at(g, p, s)] = carry[s];
+            auto put = [&](uint64_t k) {
+                float* to = g.part_p + k * g.channels * (g.states + 2);
+                each<VC>([&](auto i) {
+                    if (i < p.have && p.tok == 0) {
+                        const uint64_t ch = p.group * g.group_channels + p.in_group + i;
+                        to[(uint64_t)g.channels * g.states + ch] = gskip[i];
+                        to[(uint64_t)g.channels * (g.states + 1) + ch] = gbias[i];
                     }
+                });
+                each<S>([&](auto s) {
+                    if (p.valid && has_state(g, p, s)) to[(uint64_t)p.ch * g.states + p.row * S + s] = ga[s];
+                });
+            };
+            const uint64_t place = p.first + p.chunk, end = scan_places_before(g, p.seq + 1);
+            if (place < end) put(place);
+            if (g.offsets && p.chunk + 1 == g.chunks) {
+                // what is left before the next sequence's first place: zeros
+                each<VC>([&](auto i) { gskip[i] = gbias[i] = 0.0f; });
+                each<S>([&](auto s) { ga[s] = 0.0f; });
+                for (uint64_t k = place + 1; k < end; ++k) put(k);
+            }
+            if (g.ginitial && p.chunk == 0 && p.valid) {
+                each<S>([&](auto s) {
+                    if (has_state(g, p, s)) g.ginitial[state_at(g, p, s)] = carry[s];
                 });
             }
         }
@@ -1050,7 +1082,9 @@ __device__ __forceinline__ void scan_reduce_p(const fg_scan_kargs& g) {
     const uint64_t n = (uint64_t)g.channels * (g.states + 2);
     const uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (e >= n) return;
-    const float v = ordered_sum(g.part_p + e, n, (uint64_t)g.seqs * g.chunks);
+    // without sequences there are no places (and packed, no first one to begin at)
+    const uint64_t first = g.seqs ? scan_places_before(g, 0) : 0, end = g.seqs ? scan_places_before(g, g.seqs) : 0;
+    const float v = ordered_sum(g.part_p + first * n + e, n, end > first ? end - first : 0);
     const uint64_t states = (uint64_t)g.channels * g.states;
     if (e < states) {
         if (g.ga) g.ga[e] = v;

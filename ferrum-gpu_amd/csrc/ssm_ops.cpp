@@ -367,6 +367,25 @@ uint32_t ConvPlan::run_for(uint32_t n, uint32_t waves, uint32_t least) const {
     return run;
 }
 
+// No shorter than the window: only a sequence's first run, which writes the
+// final state, reads the initial one, which may be the same array.
+uint32_t ConvPlan::forward_run(uint32_t n) const {
+    return run_for(n, kConvForwardWaves, s_.width - 1 > FG_CONV_ROWS ? 2 * FG_CONV_ROWS : FG_CONV_ROWS);
+}
+
+// The run, and with it the workspace, is that of four channels for any call.
+uint32_t ConvPlan::backward_run() const {
+    return run_for(std::min<uint32_t>(4, (uint32_t)s_.channels), kConvBackwardWaves, 2 * FG_CONV_ROWS);
+}
+
+void ConvPlan::info(fg_conv_plan_info* out) {
+    std::lock_guard<std::mutex> lock(mu_);
+    const int v = conv_vector((uint32_t)s_.channels, 1, {}, {}, conv_widest(kBytes[s_.dtype], (uint32_t)s_.width));
+    out->forward_tokens = forward_run(kVector[v]);
+    out->backward_tokens = backward_run();
+    out->workspace_bytes = (int64_t)part_.bytes();
+}
+
 fg_conv_kargs ConvPlan::base(const int32_t* offsets) const {
     if (s_.packed && !offsets) invalid("conv: packed sequences need offsets");
     if (!s_.packed && offsets) invalid("conv: offsets are for packed sequences");
@@ -400,9 +419,7 @@ void ConvPlan::forward(const fg_conv_forward_args& a, hipStream_t stream) const 
     g.final = a.final;
     const int v = conv_vector(g.channels, es, {&g.x, &g.out}, {a.initial, a.final},
                               conv_widest(es, (uint32_t)s_.width));
-    // no shorter than the window: only a sequence's first run, which writes the
-    // final state, reads the initial one, which may be the same array
-    g.run = run_for(kVector[v], kConvForwardWaves, s_.width - 1 > FG_CONV_ROWS ? 2 * FG_CONV_ROWS : FG_CONV_ROWS);
+    g.run = forward_run(kVector[v]);
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const int64_t waves = size_of(op, "launch", {(int64_t)ceil_div(g.channels / kVector[v], 64), g.runs, g.seqs});
     void* args[] = {&g};
@@ -432,8 +449,7 @@ void ConvPlan::backward(const fg_conv_backward_args& a, hipStream_t stream) {
     g.gfinal = a.grad_final;
     g.ginitial = a.grad_initial;
     const int v = conv_vector(g.channels, es, {&g.x, &g.out, &g.gx}, {a.initial, a.grad_final, a.grad_initial}, 4);
-    // the run, and with it the workspace, is that of four channels for any call
-    g.run = run_for(std::min<uint32_t>(4, (uint32_t)s_.channels), kConvBackwardWaves, 2 * FG_CONV_ROWS);
+    g.run = backward_run();
     g.runs = (uint32_t)std::max<uint64_t>(1, ceil_div(g.length, g.run));
     const uint64_t n = (uint64_t)s_.channels * (s_.width + 1);
     {
@@ -476,15 +492,9 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     threads_ = 64 * waves_ * FG_SSM_BLOCKS(waves_);
     group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, 16 * FG_SSM_BLOCKS(waves_));
     blocks_ = group_blocks_ * (uint32_t)s.groups;
-    chunks_forward_ = chunks_for(512);
-    chunks_backward_ = chunks_for(2047);
-    if (chunks_forward_ > 1 || chunks_backward_ > 1) {
-        const uint64_t places = (uint64_t)s.sequences * (std::max(chunks_forward_, chunks_backward_) + 1) * blocks_ *
-                                FG_SSM_BLOCKS(waves_);
-        size_of(op, "workspace", {4, (int64_t)places, waves_, 64, lane_states_});
-        carry_ = Buffer<float, HipBackend>(dev, places * waves_ * 64 * lane_states_);
-        carry_dt_ = Buffer<float, HipBackend>(dev, places * 16);
-    }
+    cut(ahead_, chunks_for(512));
+    cut(back_, chunks_for(2047));
+    allocate(ahead_);
     const std::string type = kTypes[s.dtype];
     for (int wide = 0; wide < 2; ++wide) {
         if (wide && s.states != 4 * lane_states_ * waves_) continue;
@@ -519,21 +529,47 @@ uint32_t ScanPlan::chunks_for(uint32_t few) const {
     return (uint32_t)std::min<uint64_t>({ceil_div(s_.packed ? 4096 : 2048, waves), most, 64});
 }
 
+// Chunks of whole segments, at most `chunks` of a sequence, and their places:
+// packed, one for every chunk's length of rows and one more for each sequence.
+void ScanPlan::cut(Carry& c, uint32_t chunks) const {
+    c.chunk_len = (uint32_t)std::max<uint64_t>(1, ceil_div(ceil_div(s_.length, chunks), segment_)) * segment_;
+    c.chunks = (uint32_t)std::max<uint64_t>(1, ceil_div(s_.length, c.chunk_len));
+    c.places = s_.packed ? (uint64_t)s_.tokens / c.chunk_len + s_.sequences : (uint64_t)s_.sequences * c.chunks;
+}
+
+void ScanPlan::allocate(Carry& c) const {
+    if (c.chunks == 1) return;
+    const int64_t sets = (int64_t)blocks_ * FG_SSM_BLOCKS(waves_);
+    size_of("scan", "workspace", {4, (int64_t)c.places + s_.sequences, sets, waves_, 64, lane_states_});
+    c.states = Buffer<float, HipBackend>(dev_, (c.places + s_.sequences) * sets * waves_ * 64 * lane_states_);
+    c.dt = Buffer<float, HipBackend>(dev_, c.places * sets * 16);
+}
+
+void ScanPlan::info(fg_scan_plan_info* out) {
+    std::lock_guard<std::mutex> lock(mu_);
+    out->forward_parts = ahead_.chunks;
+    out->forward_tokens = ahead_.chunk_len;
+    out->backward_parts = back_.chunks;
+    out->backward_tokens = back_.chunk_len;
+    out->workspace_bytes = (int64_t)(ahead_.states.bytes() + ahead_.dt.bytes() + back_.states.bytes() +
+                                     back_.dt.bytes() + part_bc_.bytes() + part_p_.bytes());
+}
+
 size_t ScanPlan::checkpoint_bytes() const {
     const uint64_t segs = s_.packed ? (uint64_t)s_.tokens / segment_ + s_.sequences
                                     : s_.sequences * ceil_div(s_.length, segment_);
     return segs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_ * 64 * lane_states_ * sizeof(float);
 }
 
-fg_scan_kargs ScanPlan::base(const fg_scan_inputs& in, uint32_t chunks) const {
+fg_scan_kargs ScanPlan::base(const fg_scan_inputs& in, const Carry& c) const {
     fg_scan_kargs g{};
     g.a = in.a;
     g.skip = in.d;
     g.bias = in.delta_bias;
     g.initial = in.initial;
     g.offsets = in.offsets;
-    g.carry = carry_.data();
-    g.carry_dt = carry_dt_.data();
+    g.carry = c.states.data();
+    g.carry_dt = c.dt.data();
     g.tokens = (uint64_t)s_.tokens;
     g.seqs = (uint32_t)s_.sequences;
     g.length = (uint32_t)s_.length;
@@ -542,9 +578,9 @@ fg_scan_kargs ScanPlan::base(const fg_scan_inputs& in, uint32_t chunks) const {
     g.groups = (uint32_t)s_.groups;
     g.group_channels = g.channels / g.groups;
     g.group_blocks = group_blocks_;
-    g.chunk_len = (uint32_t)ceil_div(ceil_div(s_.length, chunks), segment_) * segment_;
-    if (g.chunk_len == 0) g.chunk_len = segment_;
-    g.chunks = (uint32_t)std::max<uint64_t>(1, ceil_div(s_.length, g.chunk_len));
+    g.chunk_len = c.chunk_len;
+    g.chunks = c.chunks;
+    g.places = c.places;
     g.check_segs = (uint32_t)ceil_div(s_.length, segment_);
     g.softplus = s_.softplus != 0;
     return g;
@@ -570,7 +606,7 @@ void ScanPlan::forward(const fg_scan_forward_args& a, hipStream_t stream) const 
     const char* op = "scan forward";
     const fg_scan_inputs& in = a.in;
     check_inputs(op, in);
-    fg_scan_kargs g = base(in, chunks_forward_);
+    fg_scan_kargs g = base(in, ahead_);
     Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, kBytes[s_.dtype]);
     const int64_t state = 4 * s_.sequences * s_.channels * s_.states;
     g.u = all.rows("u", in.u, s_.channels, false);
@@ -600,7 +636,7 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
     const fg_scan_inputs& in = a.in;
     check_inputs(op, in);
     if (a.grad_z.ptr && !in.z.ptr) invalid("scan backward: grad_z without z");
-    fg_scan_kargs g = base(in, chunks_backward_);
+    fg_scan_kargs g = base(in, back_);
     Arrays all(op, s_.packed ? 1 : s_.sequences, s_.packed ? s_.tokens : s_.length, kBytes[s_.dtype]);
     const int64_t state = 4 * s_.sequences * s_.channels * s_.states;
     g.u = all.rows("u", in.u, s_.channels, false);
@@ -636,11 +672,14 @@ void ScanPlan::backward(const fg_scan_backward_args& a, hipStream_t stream) {
         if (!part_p_.data() && g.seqs) {
             refuse_capture(op, dev_, stream);
             size_of(op, "workspace", {4, group_blocks_, s_.tokens, (int64_t)row});
-            size_of(op, "workspace", {4, (int64_t)params, g.seqs, g.chunks});
+            size_of(op, "workspace", {4, (int64_t)params, (int64_t)back_.places});
+            allocate(back_);
             part_bc_ = Buffer<float, HipBackend>(dev_, group_blocks_ * (uint64_t)s_.tokens * row);
-            part_p_ = Buffer<float, HipBackend>(dev_, params * g.seqs * g.chunks);
+            part_p_ = Buffer<float, HipBackend>(dev_, params * back_.places);
         }
     }
+    g.carry = back_.states.data();
+    g.carry_dt = back_.dt.data();
     g.part_bc = part_bc_.data();
     g.part_p = part_p_.data();
     const bool vec = wide(g, {&g.u, &g.delta, &g.z, &g.gout, &g.gu, &g.gdelta, &g.gz}, {&g.b, &g.c});

@@ -37,6 +37,7 @@ private:
 class ConvPlan {
 public:
     ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_conv_shape& s);
+    void info(fg_conv_plan_info* out);
     void forward(const fg_conv_forward_args& a, hipStream_t stream) const;
     void backward(const fg_conv_backward_args& a, hipStream_t stream);
 
@@ -45,6 +46,8 @@ private:
     HipBackend::DeviceHandle dev_;
     fg_conv_shape s_;
     uint32_t run_for(uint32_t n, uint32_t waves, uint32_t least) const;
+    uint32_t forward_run(uint32_t n) const;
+    uint32_t backward_run() const;
     HipBackend::KernelHandle forward_[3] = {}, backward_[3] = {}, reduce_;  // [8, 4, 1 channels of a thread]
     std::mutex mu_;
     Buffer<float, HipBackend> part_;
@@ -54,23 +57,31 @@ class ScanPlan {
 public:
     ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, const fg_scan_shape& s);
     size_t checkpoint_bytes() const;
+    void info(fg_scan_plan_info* out);
     void forward(const fg_scan_forward_args& a, hipStream_t stream) const;
     void backward(const fg_scan_backward_args& a, hipStream_t stream);
 
 private:
-    fg_scan_kargs base(const fg_scan_inputs& in, uint32_t chunks) const;
+    // What the chunks of a pass add to the states that pass through them.
+    struct Carry {
+        uint32_t chunks = 1, chunk_len = 0;  // of a sequence; tokens of a chunk
+        uint64_t places = 0;                 // over all sequences
+        Buffer<float, HipBackend> states, dt;
+    };
+    void cut(Carry& c, uint32_t chunks) const;
+    void allocate(Carry& c) const;
+    fg_scan_kargs base(const fg_scan_inputs& in, const Carry& c) const;
     void check_inputs(const char* op, const fg_scan_inputs& in) const;
     bool wide(const fg_scan_kargs& g, std::initializer_list<const fg_ssm_view*> channels,
               std::initializer_list<const fg_ssm_view*> states) const;
-    uint32_t chunks_for(uint32_t target_waves) const;
+    uint32_t chunks_for(uint32_t few) const;
     HipBackend::DeviceHandle dev_;
     fg_scan_shape s_;
     uint32_t lane_states_, waves_;  // states of a lane, waves that share a channel's states
     uint32_t segment_, threads_, group_blocks_, blocks_;  // blocks_: workgroups over all channels
-    uint32_t chunks_forward_, chunks_backward_;
     HipBackend::KernelHandle local_[2] = {}, forward_[2] = {}, back_local_[2] = {}, backward_[2] = {};  // [any, wide]
     HipBackend::KernelHandle reduce_bc_, reduce_p_;
-    Buffer<float, HipBackend> carry_, carry_dt_;
+    Carry ahead_, back_;  // back_'s buffers from the first backward call on
     std::mutex mu_;
     Buffer<float, HipBackend> part_bc_, part_p_;
 };

@@ -138,6 +138,8 @@ for _name in ("fg_conv_forward", "fg_conv_backward", "fg_conv_step", "fg_scan_fo
               "fg_scan_step"):
     _sig(_name, _vp, ctypes.c_char_p, _vp)  # the argument struct, packed
 _sig("fg_conv_plan_destroy", _vp)
+_sig("fg_conv_plan_get_info", _vp, _vp)
+_sig("fg_scan_plan_get_info", _vp, _vp)
 _sig("fg_scan_plan_destroy", _vp)
 _sig("fg_scan_checkpoint_bytes", _vp, _P(_sz))
 

@@ -210,6 +210,13 @@ class _Plan:
             raise ValueError("plan is destroyed")
         return self._p
 
+    def describe(self) -> dict:
+        """How the calls run, and the GPU memory that the plan holds (the
+        backward pass's from its first call on)."""
+        out = (ctypes.c_int64 * len(self._info))()
+        _n.check(self._get_info(self._handle(), out))
+        return dict(zip(self._info, out))
+
     def destroy(self) -> None:
         """Free the plan and its workspaces; no call of it may be in flight."""
         if getattr(self, "_p", None) is not None and self._p.value:
@@ -236,7 +243,8 @@ class ConvPlan(_Plan):
     and ``length`` is the longest one's.
     """
 
-    _destroy = _n.lib.fg_conv_plan_destroy
+    _destroy, _get_info = _n.lib.fg_conv_plan_destroy, _n.lib.fg_conv_plan_get_info
+    _info = ("forward_tokens", "backward_tokens", "workspace_bytes")
 
     def __init__(self, batch: int, length: int, channels: int, width: int, device: Device, dtype="bfloat16",
                  activation: str | None = "silu", tokens: int | None = None):
@@ -295,7 +303,8 @@ class ScanPlan(_Plan):
     one's.
     """
 
-    _destroy = _n.lib.fg_scan_plan_destroy
+    _destroy, _get_info = _n.lib.fg_scan_plan_destroy, _n.lib.fg_scan_plan_get_info
+    _info = ("forward_parts", "forward_tokens", "backward_parts", "backward_tokens", "workspace_bytes")
 
     def __init__(self, batch: int, length: int, channels: int, states: int, device: Device, groups: int = 1,
                  dtype="bfloat16", softplus: bool = True, tokens: int | None = None):

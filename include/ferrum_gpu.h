@@ -445,6 +445,14 @@ typedef struct fg_conv_backward_args {
 
 FG_API int fg_conv_plan_create(fg_device_t dev, const fg_conv_shape *shape, fg_conv_plan_t *out);
 FG_API int fg_conv_plan_destroy(fg_conv_plan_t plan);
+/* How a plan's calls run: tokens of a thread (forward: of contiguous rows), and
+ * the GPU memory that the plan holds (the backward pass's from its first call
+ * on: (width + 1) * channels floats for every backward_tokens rows, packed also
+ * for every sequence). */
+typedef struct fg_conv_plan_info {
+    int64_t forward_tokens, backward_tokens, workspace_bytes;
+} fg_conv_plan_info;
+FG_API int fg_conv_plan_get_info(fg_conv_plan_t plan, fg_conv_plan_info *out);
 FG_API int fg_conv_forward(fg_conv_plan_t plan, const fg_conv_forward_args *args, fg_stream_t stream);
 /* The first call allocates the plan's workspace for the parameters' gradients,
  * so it cannot be captured into a graph; later ones can. */
@@ -506,6 +514,17 @@ typedef struct fg_scan_backward_args {
 FG_API int fg_scan_plan_create(fg_device_t dev, const fg_scan_shape *shape, fg_scan_plan_t *out);
 FG_API int fg_scan_plan_destroy(fg_scan_plan_t plan);
 FG_API int fg_scan_checkpoint_bytes(fg_scan_plan_t plan, size_t *bytes);
+/* How a plan's calls cut the token axis: at most so many parts of a sequence (1:
+ * not cut), of so many tokens.  And the GPU memory that the plan holds: where
+ * the axis is cut, a state for every part, packed one for every forward_tokens
+ * (backward_tokens) rows and two for each sequence; from the first backward call
+ * on also (states + 2) * channels floats for every such part, and, whatever
+ * gradients are asked for, 2 * groups * states floats of every token for each 64
+ * channels of a group (32 above 16 states). */
+typedef struct fg_scan_plan_info {
+    int64_t forward_parts, forward_tokens, backward_parts, backward_tokens, workspace_bytes;
+} fg_scan_plan_info;
+FG_API int fg_scan_plan_get_info(fg_scan_plan_t plan, fg_scan_plan_info *out);
 FG_API int fg_scan_forward(fg_scan_plan_t plan, const fg_scan_forward_args *args, fg_stream_t stream);
 /* The first call allocates the plan's workspace for the gradients' sums, so it
  * cannot be captured into a graph; later ones can. */

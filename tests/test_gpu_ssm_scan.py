@@ -679,3 +679,59 @@ def test_parts_of_growing_and_shrinking_states(gpu_device, states):
         o.within(values(got[k][0]), r[k], m[k], 2 * rounds, "float32", "grad_" + k)
     o.within(values(got["A"]), r["A"], m["A"], 2 * rounds + length, "float32", "grad_A")
     assert (values(got["final"])[0, 8:] != 0).all() and (values(got["initial"])[0, 8:] != 0).all()
+
+
+@pytest.mark.parametrize("longest", [1000, 21])
+@pytest.mark.parametrize("states", [16, 24])
+def test_packed_parameter_gradients(gpu_device, states, longest):
+    """Many short sequences and a plan for much longer ones, or for shorter
+    ones (which cuts them): nothing of an earlier call's other sequences, rows
+    before, between or after is in the sums."""
+    import ferrum_gpu
+    rng = np.random.default_rng(17 + states)
+    tokens, channels, n = 700, 24, 30
+    i = _inputs(rng, (tokens,), channels, states, 1, "float32", n)
+    d = {k: up(v) for k, v in i.items()}
+    plan = ferrum_gpu.ssm.ScanPlan(n, longest, channels, states, gpu_device, dtype="float32", tokens=tokens)
+    assert plan.describe()["backward_parts"] > (10 if longest == 1000 else 0)
+    check = room(plan.checkpoint_bytes)
+    opt = {k: d[k] for k in ("D", "z", "delta_bias")}
+    main = [d[k] for k in ("u", "delta", "A", "B", "C")]
+    for start, most in ((0, 46), (17, 30), (300, 3)):
+        lengths = rng.integers(0, most, n)
+        offsets = np.minimum(start + np.concatenate([[0], np.cumsum(lengths)]), tokens)
+        off = up(torch.from_numpy(offsets.astype(np.int32)))
+        got = {"out": fill(i["u"].shape), "final": fill(i["initial"].shape), "initial": fill(i["initial"].shape)}
+        got.update({k: fill(i[k].shape) for k in GRADS})
+        plan.forward(*main, got["out"], **opt, initial=d["initial"], final=got["final"], offsets=off,
+                     checkpoints=check)
+        plan.backward(*main, d["gy"], check, **opt, **{"grad_" + k: got[k] for k in GRADS},
+                      grad_initial=got["initial"], grad_final=d["gfinal"], offsets=off)
+        gpu_device.sync()
+        spans = [((slice(int(a), int(min(b, a + longest))),), s) for s, (a, b) in enumerate(zip(offsets, offsets[1:]))]
+        _compare(got, i, spans, channels, 1, states, "float32")
+
+
+def test_workspaces_go_by_rows(gpu_device):
+    """Packed: not by as many tokens for every sequence as the longest has, and
+    the backward pass's from its first call on."""
+    import ferrum_gpu
+    n, longest, tokens, channels, states = 1024, 4096, 4096, 64, 16
+    plan = ferrum_gpu.ssm.ScanPlan(n, longest, channels, states, gpu_device, dtype="float32", tokens=tokens)
+    before = plan.describe()
+    assert before["forward_parts"] > 10
+    # a state of each channel, and its time step, for every part; a state for each sequence's initial ones
+    parts = tokens // before["forward_tokens"] + n
+    assert before["workspace_bytes"] == 4 * channels * (states * (parts + n) + parts)
+    i = {k: up(v) for k, v in _inputs(np.random.default_rng(0), (tokens,), channels, states, 1, "float32", 0).items()}
+    off = up(torch.arange(0, tokens + 1, 4, dtype=torch.int32))
+    check, gA = room(plan.checkpoint_bytes), fill((channels, states))
+    main = [i[k] for k in ("u", "delta", "A", "B", "C")]
+    plan.forward(*main, like(i["u"]), offsets=off, checkpoints=check)
+    plan.backward(*main, i["gy"], check, grad_A=gA, offsets=off)
+    gpu_device.sync()
+    after, parts = plan.describe(), tokens // before["backward_tokens"] + n
+    assert after["workspace_bytes"] - before["workspace_bytes"] == \
+        4 * channels * (states * (parts + n) + parts) + 4 * channels * (states + 2) * parts + 4 * tokens * 2 * states
+    one = ferrum_gpu.ssm.ScanPlan(64, 100, 512, states, gpu_device, dtype="float32")
+    assert one.describe()["forward_parts"] == 1 and one.describe()["workspace_bytes"] == 0
