@@ -1068,7 +1068,7 @@ __device__ __forceinline__ void scan_reduce_bc(const fg_scan_kargs& g) {
             if (g.offsets[mid] <= (int64_t)tok) lo = mid;
             else hi = mid;
         }
-        const int64_t start = g.offsets[lo];
+        const int64_t start = scan_row_of(g, lo);
         if ((int64_t)tok < start || (int64_t)tok >= g.offsets[lo + 1] || (int64_t)tok - start >= g.length) return;
     }
     const fg_ssm_view& w = which ? g.gc : g.gb;

@@ -28,8 +28,9 @@ cannot be checked.
 
 Packed sequences lie one after another in ``tokens`` rows: rows ``offsets[s]``
 up to ``offsets[s + 1]`` are sequence ``s``, at most ``length`` of them;
-``offsets`` holds ``batch + 1`` int32 on the GPU.  Rows outside every sequence
-are not written.
+``offsets`` holds ``batch + 1`` int32 on the GPU that do not fall (outputs are
+undefined where they do); values beyond the rows are taken as the nearest.  Rows
+outside every sequence are not written.
 
 Arithmetic is float32 whatever the type of the rows.  Results do not depend on
 timing: sums over channels and tokens are added in a fixed order.  All calls

@@ -395,9 +395,10 @@ FG_API int fg_stream_copy(fg_device_t dev, const void *d_in, void *d_out, size_t
  * Dense calls (packed = 0) have `sequences` sequences of `length` tokens.
  * Packed ones have the rows of all sequences one after another, `tokens` rows
  * in all; seq_stride is not used.  offsets[s] <= row < offsets[s + 1] are
- * sequence s's, at most `length` of them; `offsets` is on the device, and its
- * values are taken as the nearest valid ones (no row outside `tokens` is
- * touched whatever they are).  Rows outside every sequence are not written.
+ * sequence s's, at most `length` of them; `offsets` is on the device, and values
+ * beyond the rows are taken as the nearest.  They must not fall: where they do,
+ * outputs and gradients are undefined (no row outside `tokens` is touched
+ * whatever they are).  Rows outside every sequence are not written.
  *
  * All calls are stream-ordered and asynchronous (stream NULL: the device's
  * default stream).  A plan's workspaces serve one call at a time.  The structs

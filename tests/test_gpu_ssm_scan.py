@@ -735,3 +735,32 @@ def test_workspaces_go_by_rows(gpu_device):
         4 * channels * (states * (parts + n) + parts) + 4 * channels * (states + 2) * parts + 4 * tokens * 2 * states
     one = ferrum_gpu.ssm.ScanPlan(64, 100, 512, states, gpu_device, dtype="float32")
     assert one.describe()["forward_parts"] == 1 and one.describe()["workspace_bytes"] == 0
+
+
+def test_gradients_of_offsets_beyond_the_rows(gpu_device):
+    """Offsets before the first row or behind the last are taken as those, by
+    every gradient alike; the sequences are cut at the plan's length."""
+    import ferrum_gpu
+    rng = np.random.default_rng(19)
+    tokens, channels, states, longest = 60, 24, 16, 33
+    i = _inputs(rng, (tokens,), channels, states, 1, "float32", 3)
+    d = {k: up(v) for k, v in i.items()}
+    plan = ferrum_gpu.ssm.ScanPlan(3, longest, channels, states, gpu_device, dtype="float32", tokens=tokens)
+    check = room(plan.checkpoint_bytes)
+    main = [d[k] for k in ("u", "delta", "A", "B", "C")]
+    for beyond, nearest in (([-5, 33, 40, 90], [0, 33, 40, 60]), ([-9, -3, 50, 70], [0, 0, 50, 60])):
+        runs = []
+        for offsets in (beyond, nearest):
+            off = up(torch.tensor(offsets, dtype=torch.int32))
+            got = [fill(i[k].shape) for k in ("u", "u", "A", "B", "C")]
+            plan.forward(*main, got[0], offsets=off, checkpoints=check)
+            plan.backward(*main, d["gy"], check, grad_u=got[1], grad_A=got[2], grad_B=got[3], grad_C=got[4],
+                          offsets=off)
+            gpu_device.sync()
+            runs.append(got)
+        assert all(same(a, b) for a, b in zip(*runs))
+        rows = torch.zeros(tokens, dtype=torch.bool)
+        for a, b in zip(nearest, nearest[1:]):
+            rows[a:min(b, a + longest)] = True
+        for g in runs[0][3:]:
+            assert (g.get()[rows] != 7).all() and (g.get()[~rows] == 7).all()
