@@ -128,9 +128,10 @@ public:
 private:
     static bool apart(const Extent& a, const Extent& b) {
         if (a.p + a.bytes <= b.p || b.p + b.bytes <= a.p) return true;
-        // column windows of one array: the same strides, and the windows apart within the smaller one
-        const int64_t step = a.row > 0 ? a.row : a.seq;
-        if (step <= 0 || a.row != b.row || a.seq != b.seq || a.seq % step) return false;
+        // column windows of one array, whichever of its axes comes first: the same
+        // strides, the larger a multiple of the smaller one, and the windows apart within that
+        const int64_t least = std::min(a.row, a.seq), most = std::max(a.row, a.seq), step = least > 0 ? least : most;
+        if (step <= 0 || a.row != b.row || a.seq != b.seq || most % step) return false;
         int64_t off = (b.p - a.p) % step;
         if (off < 0) off += step;
         return off >= a.width && off + b.width <= step;

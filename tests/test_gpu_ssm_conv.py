@@ -468,3 +468,39 @@ def test_sizes_that_pass_64_bits(gpu_device):
     with pytest.raises(E, match="workspace: too large"):
         plan.backward(row, up(torch.zeros(channels, 2)), row, offsets=off)
     gpu_device.sync()
+
+
+@pytest.mark.parametrize("lead", [(4, 9), (9, 4), (1, 9), (4, 1)])
+def test_windows_of_an_array_with_tokens_first(gpu_device, lead):
+    """Input and output, and two gradients, as columns of one (tokens,
+    sequences, channels) array; windows that share a column are refused."""
+    import ferrum_gpu
+    from ferrum_gpu._native import FerrumGpuError
+    batch, length = lead
+    big = up(torch.randn(length, batch, 80).transpose(0, 1))
+    a, b, shared = big[..., :32], big[..., 40:72], big[..., 71:]
+    x, w, gy = up(a.get().contiguous()), up(torch.randn(32, 4)), up(torch.randn(batch, length, 32))
+    want, out, gx = like(x), like(x), like(x)
+    plan = ferrum_gpu.ssm.ConvPlan(batch, length, 32, 4, gpu_device, dtype="float32")
+    plan.forward(x, w, want)
+    plan.forward(a, w, b)
+    gpu_device.sync()
+    assert same(b, want)
+    plan.backward(x, w, gy, grad_x=want)
+    plan.backward(a, w, gy, grad_x=b)
+    gpu_device.sync()
+    assert same(b, want)
+    small = ferrum_gpu.ssm.ConvPlan(batch, length, 9, 4, gpu_device, dtype="float32")
+    for bad in (big[..., 63:72], big[..., 70:79]):
+        with pytest.raises(FerrumGpuError, match="overlap"):
+            small.forward(shared, up(torch.randn(9, 4)), bad)
+    small.forward(shared, up(torch.randn(9, 4)), big[..., 62:71])
+    scan = ferrum_gpu.ssm.ScanPlan(batch, length, 8, 4, gpu_device, dtype="float32")
+    check = gpu_tensor.room(scan.checkpoint_bytes)
+    u, B, C, A = big[..., :8], big[..., 8:12], big[..., 12:16], up(-torch.ones(8, 4))
+    scan.forward(u, u, A, B, C, big[..., 16:24], checkpoints=check)
+    scan.backward(u, u, A, B, C, big[..., 16:24], check, grad_u=big[..., 24:32], grad_delta=big[..., 32:40],
+                  grad_B=big[..., 40:44], grad_C=big[..., 44:48])
+    with pytest.raises(FerrumGpuError, match="grad_u and grad_delta overlap"):
+        scan.backward(u, u, A, B, C, big[..., 16:24], check, grad_u=big[..., 24:32], grad_delta=big[..., 31:39])
+    gpu_device.sync()
