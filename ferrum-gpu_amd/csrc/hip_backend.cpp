@@ -169,12 +169,17 @@ void check_launch(HipBackend::KernelHandle k, Dim3 grid, Dim3 block) {
 
 }  // namespace
 
+HipBackend::Stream HipBackend::stream_of(const DeviceHandle& dev, Stream stream) {
+    if (stream == (Stream)FG_STREAM_NULL) return nullptr;
+    return stream ? stream : dev->stream;
+}
+
 void HipBackend::launch(const DeviceHandle& dev, Stream stream, KernelHandle k, Dim3 grid, Dim3 block,
                         uint32_t shared_bytes, void** args) {
     check_launch(k, grid, block);
     bind(dev);
     hip_check(hipModuleLaunchKernel(k, grid.x, grid.y, grid.z, block.x, block.y, block.z, shared_bytes,
-                                    stream ? stream : dev->stream, args, nullptr),
+                                    stream_of(dev, stream), args, nullptr),
               "hipModuleLaunchKernel");
 }
 

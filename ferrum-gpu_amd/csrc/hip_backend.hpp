@@ -79,6 +79,9 @@ struct HipBackend {
     // Backend::get_kernel (backend.rs:56-59).
     static KernelHandle get_kernel(const Module& mod, const char* name);
     // Backend::launch (backend.rs:62-70): args[i] points at argument i's bytes.
+    // The HIP stream of a call's argument: null is the device's default stream,
+    // FG_STREAM_NULL HIP's null stream (launch() only).
+    static Stream stream_of(const DeviceHandle& dev, Stream stream);
     static void launch(const DeviceHandle& dev, Stream stream, KernelHandle k, Dim3 grid, Dim3 block,
                        uint32_t shared_bytes, void** args);
 

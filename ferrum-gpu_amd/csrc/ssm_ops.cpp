@@ -155,7 +155,7 @@ private:
 void refuse_capture(const char* op, const HipBackend::DeviceHandle& dev, hipStream_t stream) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     HipBackend::bind(dev);
-    hip_check(hipStreamIsCapturing(stream ? stream : dev->stream, &cap), "hipStreamIsCapturing");
+    hip_check(hipStreamIsCapturing(HipBackend::stream_of(dev, stream), &cap), "hipStreamIsCapturing");
     if (cap != hipStreamCaptureStatusNone)
         invalid(std::string(op) + ": a plan's first backward call allocates its workspace and cannot be captured");
 }

@@ -4,9 +4,9 @@ then token by token with its states in a cache, and trained.
 
     python ferrum-gpu_amd/examples/sequence_filters.py
 
-The block's projections are torch products on the device's default stream; the
-filters run on the package's stream, so the two wait for each other where one
-takes what the other made.
+The block's projections are torch products, and the filters run on torch's current
+stream between them, so the host waits for nothing.  torch is imported before
+the package, as it has to be.
 """
 
 from __future__ import annotations
@@ -29,18 +29,20 @@ class Block:
         g = torch.Generator(device="cuda").manual_seed(seed)
         rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
         self.device, self.channels, self.states, self.width, self.rank = device, channels, states, width, rank
-        self.dtype, self.name = dtype, str(dtype).rpartition(".")[2]
+        self.dtype, self.name, self.plans = dtype, str(dtype).rpartition(".")[2], {}
         self.weight, self.bias = 0.5 * rand(channels, width), 0.1 * rand(channels)
         self.project = (rand(channels, rank + 2 * states) / channels ** 0.5).to(dtype)
         self.widen = (rand(rank, channels) / rank ** 0.5).to(dtype)
         self.A = -torch.arange(1, states + 1, device="cuda", dtype=torch.float32).repeat(channels, 1)
         self.D, self.delta_bias = torch.ones(channels, device="cuda"), torch.full((channels,), -3.0, device="cuda")
 
-    def _torch_then_package(self):
-        torch.cuda.current_stream().synchronize()
-
-    def _package_then_torch(self):
-        self.device.sync()
+    def _plans(self, batch, length):
+        """Both filters' plans for sequences of this shape, made once."""
+        if (batch, length) not in self.plans:
+            self.plans[batch, length] = (
+                ssm.ConvPlan(batch, length, self.channels, self.width, self.device, dtype=self.name),
+                ssm.ScanPlan(batch, length, self.channels, self.states, self.device, dtype=self.name))
+        return self.plans[batch, length]
 
     def _split(self, u):
         p = u @ self.project
@@ -49,59 +51,45 @@ class Block:
 
     def prompt(self, x, z, conv_state, scan_state):
         """Outputs for whole sequences; the states are left for what follows."""
-        batch, length, channels = x.shape
         u, out = torch.empty_like(x), torch.empty_like(x)
-        conv = ssm.ConvPlan(batch, length, channels, self.width, self.device, dtype=self.name)
-        scan = ssm.ScanPlan(batch, length, channels, self.states, self.device, dtype=self.name)
-        self._torch_then_package()
-        conv.forward(x, self.weight, u, bias=self.bias, initial=conv_state, final=conv_state)
-        self._package_then_torch()
+        conv, scan = self._plans(*x.shape[:2])
+        here = torch.cuda.current_stream()
+        conv.forward(x, self.weight, u, bias=self.bias, initial=conv_state, final=conv_state, stream=here)
         delta, b, c = self._split(u)
-        self._torch_then_package()
         scan.forward(u, delta, self.A, b, c, out, D=self.D, z=z, delta_bias=self.delta_bias, initial=scan_state,
-                     final=scan_state)
-        self._package_then_torch()
+                     final=scan_state, stream=here)
         return out
 
     def token(self, x, z, conv_state, scan_state, slots):
         """Outputs for one token of each row, whose states lie in cache slots."""
         u, out = torch.empty_like(x), torch.empty_like(x)
-        self._torch_then_package()
-        ssm.conv_step(self.device, x, self.weight, conv_state, u, bias=self.bias, slots=slots)
-        self._package_then_torch()
+        here = torch.cuda.current_stream()
+        ssm.conv_step(self.device, x, self.weight, conv_state, u, bias=self.bias, slots=slots, stream=here)
         delta, b, c = self._split(u)
-        self._torch_then_package()
         ssm.scan_step(self.device, u, delta, self.A, b, c, scan_state, out, D=self.D, z=z,
-                      delta_bias=self.delta_bias, slots=slots)
-        self._package_then_torch()
+                      delta_bias=self.delta_bias, slots=slots, stream=here)
         return out
 
     def gradients(self, x, z, grad):
         """Gradients of the convolution's and the scan's parameters and of x and z."""
-        batch, length, channels = x.shape
         u, out = torch.empty_like(x), torch.empty_like(x)
-        conv = ssm.ConvPlan(batch, length, channels, self.width, self.device, dtype=self.name)
-        scan = ssm.ScanPlan(batch, length, channels, self.states, self.device, dtype=self.name)
+        conv, scan = self._plans(*x.shape[:2])
         check = torch.empty(scan.checkpoint_bytes, dtype=torch.uint8, device="cuda")
-        self._torch_then_package()
-        conv.forward(x, self.weight, u, bias=self.bias)
-        self._package_then_torch()
+        here = torch.cuda.current_stream()
+        conv.forward(x, self.weight, u, bias=self.bias, stream=here)
         delta, b, c = self._split(u)
         g = {k: torch.empty_like(v) for k, v in dict(u=u, delta=delta, A=self.A, B=b, C=c, D=self.D, z=z,
                                                      delta_bias=self.delta_bias).items()}
-        self._torch_then_package()
-        scan.forward(u, delta, self.A, b, c, out, D=self.D, z=z, delta_bias=self.delta_bias, checkpoints=check)
+        scan.forward(u, delta, self.A, b, c, out, D=self.D, z=z, delta_bias=self.delta_bias, checkpoints=check,
+                     stream=here)
         scan.backward(u, delta, self.A, b, c, grad, check, D=self.D, z=z, delta_bias=self.delta_bias,
-                      **{"grad_" + k: v for k, v in g.items()})
-        self._package_then_torch()
+                      **{"grad_" + k: v for k, v in g.items()}, stream=here)
         r, n = self.rank, self.states
         p = torch.cat([g["delta"] @ self.widen.t().contiguous(), g["B"], g["C"]], -1)
         g["u"] += p @ self.project.t().contiguous()
         g["x"], g["weight"], g["bias"] = torch.empty_like(x), torch.empty_like(self.weight), torch.empty_like(self.bias)
-        self._torch_then_package()
         conv.backward(x, self.weight, g["u"], grad_x=g["x"], grad_weight=g["weight"], grad_bias=g["bias"],
-                      bias=self.bias)
-        self._package_then_torch()
+                      bias=self.bias, stream=here)
         return out, g
 
 

@@ -33,10 +33,17 @@ undefined where they do); values beyond the rows are taken as the nearest.  Rows
 outside every sequence are not written.
 
 Arithmetic is float32 whatever the type of the rows.  Results do not depend on
-timing: sums over channels and tokens are added in a fixed order.  All calls
-are stream-ordered and asynchronous (``stream=0``: the device's default
-stream).  A plan's workspaces serve one call at a time; its first ``backward``
-allocates, so it cannot be captured into a graph, later calls can.
+timing: sums over channels and tokens are added in a fixed order.
+
+All calls are stream-ordered and asynchronous.  ``stream`` takes a
+``torch.cuda.Stream``, and with torch tensors it should: ``stream=
+torch.cuda.current_stream()`` runs the call behind the torch operations that made
+its tensors and ahead of those that take its outputs or get their memory.  The
+default, ``stream=0``, is the device's own default stream, which waits for none
+of torch's and none of them for it: there the caller synchronizes both, or
+passes arrays that nothing else is working on.  Stream handles are taken too.  A
+plan's workspaces serve one call at a time; its first ``backward`` allocates, so
+it cannot be captured into a graph, later calls can.
 """
 
 from __future__ import annotations
@@ -97,6 +104,21 @@ def _address(x, nbytes: int, what: str) -> int:
             raise ValueError(f"{what}: buffer of {x.nbytes} bytes, the call reads or writes {nbytes}")
         return x.ptr
     return int(x)
+
+
+_NULL_STREAM = 1  # FG_STREAM_NULL: torch's default stream, whose handle is 0
+
+
+def _stream(stream, ordinal: int):
+    """What the library takes as its stream: a handle, or None for the device's default stream."""
+    if stream.__class__ is int or stream is None:
+        return stream or None
+    handle = getattr(stream, "cuda_stream", None)
+    if handle is None:
+        return int(stream) or None
+    if stream.device_index != ordinal:
+        raise ValueError(f"stream: of GPU {stream.device_index}, the call runs on GPU {ordinal}")
+    return handle or _NULL_STREAM
 
 
 def _wrong(x, what: str, shapes, dtype, ordinal: int):
@@ -260,7 +282,7 @@ class ConvPlan(_Plan):
     def _state(self, x, what: str) -> int:
         return _flat(x, self._state_shape, self.dtype, self._state_bytes, self.device.ordinal, what)
 
-    def forward(self, x, weight, out, bias=None, initial=None, final=None, offsets=None, stream: int = 0) -> None:
+    def forward(self, x, weight, out, bias=None, initial=None, final=None, offsets=None, stream=0) -> None:
         """``weight`` (channels, width) and ``bias`` (channels) float32.
         ``initial``: the (batch, width - 1, channels) rows before each sequence
         (None: zeros); ``final``: room for the last width - 1 rows of (initial,
@@ -269,12 +291,12 @@ class ConvPlan(_Plan):
                                   self._param(weight, (self.channels, self.width), "weight"),
                                   self._param(bias, (self.channels,), "bias"), self._state(initial, "initial"),
                                   self._state(final, "final"), self._offsets(offsets))
-        rc = _n.lib.fg_conv_forward(self._handle(), args, stream or None)
+        rc = _n.lib.fg_conv_forward(self._handle(), args, _stream(stream, self.device.ordinal))
         if rc:
             _n.check(rc)
 
     def backward(self, x, weight, grad_out, grad_x=None, grad_weight=None, grad_bias=None, bias=None, initial=None,
-                 grad_initial=None, grad_final=None, offsets=None, stream: int = 0) -> None:
+                 grad_initial=None, grad_final=None, offsets=None, stream=0) -> None:
         """Gradients from ``grad_out``, that of ``out``, and ``grad_final``,
         that of ``final`` (None: zeros), given forward's inputs; each is
         written where room for it is given."""
@@ -286,7 +308,7 @@ class ConvPlan(_Plan):
                                    self._param(grad_weight, (self.channels, self.width), "grad_weight"),
                                    self._param(grad_bias, (self.channels,), "grad_bias"),
                                    self._state(grad_initial, "grad_initial"), self._offsets(offsets))
-        rc = _n.lib.fg_conv_backward(self._handle(), args, stream or None)
+        rc = _n.lib.fg_conv_backward(self._handle(), args, _stream(stream, self.device.ordinal))
         if rc:
             _n.check(rc)
 
@@ -333,7 +355,7 @@ class ScanPlan(_Plan):
                 self._param(delta_bias, d, "delta_bias"), self._state(initial, "initial"), self._offsets(offsets))
 
     def forward(self, u, delta, A, B, C, out, D=None, z=None, delta_bias=None, initial=None, final=None, offsets=None,
-                checkpoints=None, stream: int = 0) -> None:
+                checkpoints=None, stream=0) -> None:
         """``A`` (channels, states), ``D`` and ``delta_bias`` (channels)
         float32; without ``z`` no gate.  ``initial``: the (batch, channels,
         states) states before each sequence (None: zeros); ``final``: room for
@@ -342,13 +364,13 @@ class ScanPlan(_Plan):
         args = _scan_forward_pack(*self._inputs(u, delta, A, B, C, D, z, delta_bias, initial, offsets),
                                   *self._row(out, "out"), self._state(final, "final"),
                                   _bytes(checkpoints, self.checkpoint_bytes, self.device.ordinal, "checkpoints"))
-        rc = _n.lib.fg_scan_forward(self._handle(), args, stream or None)
+        rc = _n.lib.fg_scan_forward(self._handle(), args, _stream(stream, self.device.ordinal))
         if rc:
             _n.check(rc)
 
     def backward(self, u, delta, A, B, C, grad_out, checkpoints, grad_u=None, grad_delta=None, grad_A=None,
                  grad_B=None, grad_C=None, D=None, z=None, delta_bias=None, grad_D=None, grad_z=None,
-                 grad_delta_bias=None, grad_initial=None, grad_final=None, offsets=None, stream: int = 0) -> None:
+                 grad_delta_bias=None, grad_initial=None, grad_final=None, offsets=None, stream=0) -> None:
         """Gradients from ``grad_out``, that of ``out``, and ``grad_final``,
         that of ``final`` (None: zeros), given forward's inputs and the
         ``checkpoints`` it left; each is written where room for it is given."""
@@ -363,7 +385,7 @@ class ScanPlan(_Plan):
                                    self._param(grad_D, d, "grad_D"),
                                    self._param(grad_delta_bias, d, "grad_delta_bias"),
                                    self._state(grad_initial, "grad_initial"))
-        rc = _n.lib.fg_scan_backward(self._handle(), args, stream or None)
+        rc = _n.lib.fg_scan_backward(self._handle(), args, _stream(stream, self.device.ordinal))
         if rc:
             _n.check(rc)
 
@@ -397,7 +419,7 @@ def _step_row(x, shape: tuple, inner: tuple, dtype: str, ordinal: int, what: str
 
 
 def conv_step(device: Device, x, weight, state, out, bias=None, slots=None, state_out=None, activation="silu",
-              batch=None, channels=None, width=None, state_rows=None, dtype=None, stream: int = 0) -> None:
+              batch=None, channels=None, width=None, state_rows=None, dtype=None, stream=0) -> None:
     """ConvPlan's convolution of one token of each of ``batch`` rows.
 
     ``state``: the (state_rows, width - 1, channels) windows before the token;
@@ -423,14 +445,14 @@ def conv_step(device: Device, x, weight, state, out, bias=None, slots=None, stat
                            _flat(bias, (channels,), "float32", 4 * channels, at, "bias"), s,
                            s if state_out is None else _flat(state_out, shape, dtype, nbytes, at, "state_out"),
                            _flat(slots, (batch,), "int32", 4 * batch, at, "slots"))
-    rc = _n.lib.fg_conv_step(device.handle, args, stream or None)
+    rc = _n.lib.fg_conv_step(device.handle, args, _stream(stream, at))
     if rc:
         _n.check(rc)
 
 
 def scan_step(device: Device, u, delta, A, B, C, state, out, D=None, z=None, delta_bias=None, slots=None,
               state_out=None, softplus: bool = True, groups: int | None = None, batch=None, channels=None,
-              states=None, state_rows=None, dtype=None, stream: int = 0) -> None:
+              states=None, state_rows=None, dtype=None, stream=0) -> None:
     """ScanPlan's scan of one token of each of ``batch`` rows.
 
     ``state``: (state_rows, channels, states) float32; ``slots`` and
@@ -462,6 +484,6 @@ def scan_step(device: Device, u, delta, A, B, C, state, out, D=None, z=None, del
                            _flat(delta_bias, (channels,), "float32", 4 * channels, at, "delta_bias"), s,
                            s if state_out is None else _flat(state_out, shape, "float32", nbytes, at, "state_out"),
                            _flat(slots, (batch,), "int32", 4 * batch, at, "slots"))
-    rc = _n.lib.fg_scan_step(device.handle, args, stream or None)
+    rc = _n.lib.fg_scan_step(device.handle, args, _stream(stream, at))
     if rc:
         _n.check(rc)

@@ -400,9 +400,12 @@ FG_API int fg_stream_copy(fg_device_t dev, const void *d_in, void *d_out, size_t
  * outputs and gradients are undefined (no row outside `tokens` is touched
  * whatever they are).  Rows outside every sequence are not written.
  *
- * All calls are stream-ordered and asynchronous (stream NULL: the device's
- * default stream).  A plan's workspaces serve one call at a time.  The structs
- * hold 8-byte members only. */
+ * All calls are stream-ordered and asynchronous.  stream NULL is the device's
+ * default stream, which does not wait for HIP's null stream, nor that for it;
+ * these calls also take the null stream itself, as FG_STREAM_NULL, for callers
+ * whose other work runs there.  A plan's workspaces serve one call at a time.
+ * The structs hold 8-byte members only. */
+#define FG_STREAM_NULL ((fg_stream_t)1)
 #define FG_DTYPE_F32 0
 #define FG_DTYPE_BF16 1
 #define FG_DTYPE_F16 2

@@ -191,3 +191,17 @@ def test_rows_without_their_last_axis_are_refused(lead, width):
 
 def test_package_exports_the_module():
     assert ferrum_gpu.ssm is ssm and "ssm" in ferrum_gpu.__all__
+
+
+def test_streams_that_calls_take():
+    """Handles, torch's streams (its default one has the handle 0), nothing of another GPU."""
+    class Stream:
+        def __init__(self, handle, index=0):
+            self.cuda_stream, self.device_index = handle, index
+
+    assert ssm._stream(0, 0) is None and ssm._stream(None, 0) is None and ssm._stream(77, 0) == 77
+    assert ssm._stream(Stream(0), 0) == 1 and ssm._stream(Stream(5), 0) == 5
+    with pytest.raises(ValueError, match="GPU 1"):
+        ssm._stream(Stream(5, 1), 0)
+    text = open(HEADER).read()
+    assert re.search(r"#define FG_STREAM_NULL \(\(fg_stream_t\)1\)", text)
