@@ -44,6 +44,9 @@ of torch's and none of them for it: there the caller synchronizes both, or
 passes arrays that nothing else is working on.  Stream handles are taken too.  A
 plan's workspaces serve one call at a time; its first ``backward`` allocates, so
 it cannot be captured into a graph, later calls can.
+
+Import torch before this package: torch finds no GPU in a process that loaded
+the package, and with it the system's HIP runtime, first.
 """
 
 from __future__ import annotations
@@ -128,7 +131,8 @@ def _wrong(x, what: str, shapes, dtype, ordinal: int):
     if dtype is not None and _dtype_of(x) != dtype:
         return ValueError(f"{what}: {_dtype_of(x)}, expected {dtype}")
     if x.get_device() != ordinal:
-        return ValueError(f"{what}: tensor on {x.device}, the call runs on GPU {ordinal}")
+        hint = "; torch finds no GPU where this package was imported first" if x.get_device() < 0 else ""
+        return ValueError(f"{what}: tensor on {x.device}, the call runs on GPU {ordinal}{hint}")
     return None
 
 

@@ -205,3 +205,9 @@ def test_streams_that_calls_take():
         ssm._stream(Stream(5, 1), 0)
     text = open(HEADER).read()
     assert re.search(r"#define FG_STREAM_NULL \(\(fg_stream_t\)1\)", text)
+
+
+def test_a_tensor_without_a_gpu_says_why():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="runs on GPU 0; torch finds no GPU where this package was imported first"):
+        ssm._rows(torch.zeros(2, 8, 16), (2, 8), 16, (), "float32", 0, "x")
