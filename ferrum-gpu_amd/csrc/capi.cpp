@@ -48,7 +48,7 @@ struct fg_device {
     Buffer<Cf32, HipBackend> staging;
     Buffer<Cf32, HipBackend> staging_out;  // out-of-place outputs (plans whose in-place form differs)
     fg::Pointwise pointwise;  // elementwise kernels of fft_module
-    fg::SsmKernels ssm;       // the sequence filters' code objects
+    std::unique_ptr<fg::SsmKernels> ssm;  // the sequence filters' code objects
     std::atomic<int> dependents{0};  // live plans and captured graphs made on this device
     std::unique_ptr<fg::HostStager> stager;  // pinned pieces of the host path (first large call)
     // fg_fft_exec_split_noalloc: calls on this device take turns at the
@@ -141,7 +141,7 @@ fg_device* open_device(int ordinal) {
     d->dev.reset(new HipDevice(h));
     d->fft_module = d->dev->load_or_cache(fg::fft_code_object());
     d->pointwise = fg::Pointwise(d->fft_module);
-    d->ssm = fg::SsmKernels(*d->dev);
+    d->ssm.reset(new fg::SsmKernels(*d->dev));
     // The allocation-free entry point's scratch area: its address on this
     // device, resolved once with the device current (scratch.hip).
     HipBackend::bind(h);
@@ -889,7 +889,7 @@ int fg_conv_plan_create(fg_device_t dev, const fg_conv_shape* shape, fg_conv_pla
         need(shape, "shape");
         std::unique_ptr<fg_conv_plan> p(new fg_conv_plan);
         p->dev = dev;
-        p->plan.reset(new fg::ConvPlan(dev->dev->handle(), dev->ssm, *shape));
+        p->plan.reset(new fg::ConvPlan(dev->dev->handle(), *dev->ssm, *shape));
         dev->dependents.fetch_add(1);
         *out = p.release();
     });
@@ -931,7 +931,7 @@ int fg_conv_step(fg_device_t dev, const fg_conv_step_args* args, fg_stream_t str
     return guarded([&] {
         need(dev, "device");
         need(args, "args");
-        dev->ssm.conv_step(dev->dev->handle(), *args, (hipStream_t)stream);
+        dev->ssm->conv_step(dev->dev->handle(), *args, (hipStream_t)stream);
     });
 }
 
@@ -943,7 +943,7 @@ int fg_scan_plan_create(fg_device_t dev, const fg_scan_shape* shape, fg_scan_pla
         need(shape, "shape");
         std::unique_ptr<fg_scan_plan> p(new fg_scan_plan);
         p->dev = dev;
-        p->plan.reset(new fg::ScanPlan(dev->dev->handle(), dev->ssm, *shape));
+        p->plan.reset(new fg::ScanPlan(dev->dev->handle(), *dev->ssm, *shape));
         dev->dependents.fetch_add(1);
         *out = p.release();
     });
@@ -993,7 +993,7 @@ int fg_scan_step(fg_device_t dev, const fg_scan_step_args* args, fg_stream_t str
     return guarded([&] {
         need(dev, "device");
         need(args, "args");
-        dev->ssm.scan_step(dev->dev->handle(), *args, (hipStream_t)stream);
+        dev->ssm->scan_step(dev->dev->handle(), *args, (hipStream_t)stream);
     });
 }
 

@@ -73,14 +73,16 @@ using namespace fg::ssm;
     FG_SCAN_STEP(NAME, T, 8)                                                                                    \
     FG_SCAN_STEP(NAME, T, 16)
 
-// One code object, three builds of this file in parallel: FG_SSM_F32, _BF16, _F16.
-#if defined(FG_SSM_F32)
-FG_SSM_TYPE(f32, F32)
+// The sums that are float32 whatever the rows' type, in each code object.
 extern "C" __global__ __launch_bounds__(256) void fg_scan_reduce_p(fg_scan_kargs g) { scan_reduce_p(g); }
 extern "C" __global__ __launch_bounds__(256) void fg_conv_reduce(fg_conv_kargs g, uint32_t width, float* gweight,
                                                                 float* gbias) {
     conv_reduce(g, width, gweight, gbias);
 }
+
+// One code object, three builds of this file in parallel: FG_SSM_F32, _BF16, _F16.
+#if defined(FG_SSM_F32)
+FG_SSM_TYPE(f32, F32)
 #elif defined(FG_SSM_BF16)
 FG_SSM_TYPE(bf16, BF16)
 FG_CONV_EIGHT(bf16, BF16)

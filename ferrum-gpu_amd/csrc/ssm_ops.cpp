@@ -194,25 +194,42 @@ void launch(const HipBackend::DeviceHandle& dev, hipStream_t stream, HipBackend:
 
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// A call that is being captured may be the first of its type: loading a code
+// object is no work of the stream's, and the thread's capture mode allows it meanwhile.
+class CaptureAllows {
+public:
+    CaptureAllows() { hip_check(hipThreadExchangeStreamCaptureMode(&mode_), "hipThreadExchangeStreamCaptureMode"); }
+    ~CaptureAllows() { (void)hipThreadExchangeStreamCaptureMode(&mode_); }
+
+private:
+    hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
+};
+
 }  // namespace
 
-SsmKernels::SsmKernels(Device<HipBackend>& dev) {
-    for (int t = 0; t < 3; ++t) {
-        mod_[t] = dev.load_or_cache(ssm_code_object(t));
-        for (int w = 2; w <= FG_CONV_MAX_WIDTH; ++w)
-            for (int v = 0; v < 3; ++v)
-                if (kVector[v] <= conv_widest(kBytes[t], w))
-                    conv_step_[t][w][v] = get(t, std::string("fg_conv_step_") + kTypes[t] + "_w" + std::to_string(w) +
-                                                     "_v" + std::to_string(kVector[v]));
-        for (int l = 0; l < 5; ++l)
-            for (int wide = 0; wide < 2; ++wide)
-                scan_step_[t][l][wide] = get(t, std::string("fg_scan_step_") + kTypes[t] + "_l" +
-                                                    std::to_string(1 << l) + (wide ? "" : "_any"));
-    }
+const SsmKernels::Type& SsmKernels::type(int t) const {
+    std::lock_guard<std::mutex> lock(mu_);
+    if (types_[t]) return *types_[t];
+    HipBackend::bind(dev_.handle());
+    const CaptureAllows allows;
+    std::unique_ptr<Type> k(new Type);
+    k->mod = dev_.load_or_cache(ssm_code_object(t));
+    const auto find = [&](const std::string& name) { return HipBackend::get_kernel(k->mod, name.c_str()); };
+    for (int w = 2; w <= FG_CONV_MAX_WIDTH; ++w)
+        for (int v = 0; v < 3; ++v)
+            if (kVector[v] <= conv_widest(kBytes[t], w))
+                k->conv_step[w][v] = find(std::string("fg_conv_step_") + kTypes[t] + "_w" + std::to_string(w) + "_v" +
+                                          std::to_string(kVector[v]));
+    for (int l = 0; l < 5; ++l)
+        for (int wide = 0; wide < 2; ++wide)
+            k->scan_step[l][wide] = find(std::string("fg_scan_step_") + kTypes[t] + "_l" + std::to_string(1 << l) +
+                                         (wide ? "" : "_any"));
+    types_[t] = std::move(k);
+    return *types_[t];
 }
 
 HipBackend::KernelHandle SsmKernels::get(int dtype, const std::string& name) const {
-    return HipBackend::get_kernel(mod_[dtype], name.c_str());
+    return HipBackend::get_kernel(type(dtype).mod, name.c_str());
 }
 
 void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_step_args& a,
@@ -252,7 +269,7 @@ void SsmKernels::conv_step(const HipBackend::DeviceHandle& dev, const fg_conv_st
     g.each_wave = (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, wide * g.rows / 2048));
     const uint64_t waves = wide * ceil_div(g.rows, g.each_wave);
     void* args[] = {&g};
-    launch(dev, stream, conv_step_[a.dtype][a.width][v], ceil_div(waves, 4), 256, args, op);
+    launch(dev, stream, type((int)a.dtype).conv_step[a.width][v], ceil_div(waves, 4), 256, args, op);
 }
 
 void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_step_args& a,
@@ -305,7 +322,7 @@ void SsmKernels::scan_step(const HipBackend::DeviceHandle& dev, const fg_scan_st
     g.each_wave = (uint32_t)std::min<uint64_t>(16, std::max<uint64_t>(1, per_row * g.rows / 8192));
     const uint64_t waves = per_row * ceil_div(g.rows, g.each_wave);
     void* args[] = {&g};
-    launch(dev, stream, scan_step_[a.dtype][lanes][wide], ceil_div(waves, 4), 256, args, op);
+    launch(dev, stream, type((int)a.dtype).scan_step[lanes][wide], ceil_div(waves, 4), 256, args, op);
 }
 
 // ------------------------------------------------------------- convolution
@@ -354,7 +371,7 @@ ConvPlan::ConvPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
         if (kVector[v] <= conv_widest(kBytes[s.dtype], (uint32_t)s.width)) forward_[v] = k.get((int)s.dtype, "fg_conv_" + tail);
         if (kVector[v] <= 4) backward_[v] = k.get((int)s.dtype, "fg_conv_back_" + tail);
     }
-    reduce_ = k.get(FG_DTYPE_F32, "fg_conv_reduce");
+    reduce_ = k.get((int)s.dtype, "fg_conv_reduce");
 }
 
 // Tokens of a thread: as many as leave `waves` waves, each of 64 threads of n
@@ -507,7 +524,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
         backward_[wide] = k.get((int)s.dtype, "fg_scan_back_" + tail);
     }
     reduce_bc_ = k.get((int)s.dtype, "fg_scan_reduce_bc_" + type);
-    reduce_p_ = k.get(FG_DTYPE_F32, "fg_scan_reduce_p");
+    reduce_p_ = k.get((int)s.dtype, "fg_scan_reduce_p");
 }
 
 // Parts of the token axis that are worked through at the same time.  A SIMD of
