@@ -511,7 +511,7 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
     group_blocks_ = (uint32_t)ceil_div(s.channels / s.groups, 16 * FG_SSM_BLOCKS(waves_));
     blocks_ = group_blocks_ * (uint32_t)s.groups;
     cut(ahead_, chunks_for(512));
-    cut(back_, chunks_for(2047));
+    cut(back_, chunks_for(s.packed ? 1536 : 1024));
     allocate(ahead_);
     const std::string type = kTypes[s.dtype];
     for (int wide = 0; wide < 2; ++wide) {
@@ -529,16 +529,19 @@ ScanPlan::ScanPlan(const HipBackend::DeviceHandle& dev, const SsmKernels& k, con
 
 // Parts of the token axis that are worked through at the same time.  A SIMD of
 // the GPU's 1024 takes two waves: tensors with at most `few` waves are cut
-// until there are 2048, which costs a pass over the tokens for what each part
-// adds to the states.  Measured, us for one pass of 4 sequences of 16 states in
-// bfloat16, parts 1 / 2 / 4: forward, 1024 tokens x 2048 channels (512 waves)
-// 88 / 87 / 78, 2048 x 4096 (1024 waves) 177 / 256; backward, 1024 x 2048
-// (parts 2 / 4) 204 / 157.  A part has 32 tokens or more (16 / 32 / 64: forward, 300 x
-// 1024 15.5 / 14.2 / 17.9, training step 128 x 1024 34 / 41 / 56, 1024 x 512 59 / 51 /
-// 61; 16 states in bfloat16).  Packed sequences count
-// as so many of the longest's length, which the last wave to end works through,
-// and are cut into twice the parts, which evens them out (7 sequences, 9001
-// tokens x 1536 channels x 8 states in float16: 136 us, twice the parts 97).
+// until there are 2048 (packed ones, which count as so many of the longest's
+// length, 4096: that evens unequal sequences out), into 64 parts at most, of 32
+// tokens or more.  That costs a pass over the tokens for what each part adds to
+// the states.  Measured, us not cut / cut so, 1024 tokens x 2048 channels x 16
+// states in bfloat16 for each sequence:
+//   waves              512       640       768       1024      1280      1536      1792
+//   forward            83 / 71   83 / 97   84 / 111  84 / 129  -         -         -
+//   backward           307 / 155 309 / 227 310 / 278 314 / 293 440 / 434 443 / 440 450 / 523
+//   backward, packed   307 / 178 -         -         385 / 305 434 / 389 473 / 466 501 / 520
+// Packed, 2048 / 4096: 7 sequences, 9001 tokens x 1536 channels x 8 states in
+// float16, forward 136 / 97 (of an earlier kernel).  float32 backward 1152 waves 451 / 468, 300 tokens 1536 waves 141 / 149.  A part's
+// least tokens, 16 / 32 / 64: forward, 300 x 1024 15.5 / 14.2 / 17.9, training step
+// 128 x 1024 34 / 41 / 56, 1024 x 512 59 / 51 / 61.
 uint32_t ScanPlan::chunks_for(uint32_t few) const {
     const uint64_t seqs = s_.packed && s_.length ? ceil_div(s_.tokens, s_.length) : s_.sequences;
     const uint64_t waves = std::max<uint64_t>(1, seqs * blocks_ * FG_SSM_BLOCKS(waves_) * waves_);

@@ -313,3 +313,13 @@ def test_steps_of_nan(gpu_device, states, dtype):
     j["initial"][r, c, 1] = bad[r, 1, c] = float("nan")
     m["scan"][r, c] = m["state"][r, c, 1] = m["conv"][r, c] = m["window"][r, 0, c] = True
     _untouched(run(j, bad), good, m)
+
+
+@pytest.mark.parametrize("batch,tokens,forward,backward", [
+    (4, None, 4, 4), (5, None, 1, 4), (8, None, 1, 2), (9, None, 1, 1), (10, None, 1, 1), (15, None, 1, 1),
+    (20, 4096, 8, 8), (20, 8192, 1, 4), (20, 12288, 1, 3), (20, 14336, 1, 1)])
+def test_scan_parts_by_waves(gpu_device, batch, tokens, forward, backward):
+    """Sequences of 128 waves each: the axis is cut where that was measured to gain."""
+    import ferrum_gpu
+    d = ferrum_gpu.ssm.ScanPlan(batch, 1024, 2048, 16, gpu_device, tokens=tokens).describe()
+    assert (d["forward_parts"], d["backward_parts"]) == (forward, backward), d
