@@ -10,8 +10,13 @@
 //
 // Bound by memory where there are many rows, else by the chain of loads of one
 // run.  Measured (4 taps, bfloat16): 8 x 2048 tokens x 4096 channels forward 48
-// to 51 us (5.4 TB/s), backward 105 (3.8 TB/s) and 7 for the sums over the
-// runs; 2 x 1001 x 2048 forward 8 us; a step of 256 rows x 4096 channels 6 us.
+// us over the same rows again and again (5.6 TB/s, partly from the Infinity
+// Cache), 65 behind a backward pass (4.1 TB/s), backward 105 (3.8 TB/s) and 7 for
+// the sums over the runs; 2 x 1001 x 2048 forward 8 us; a step of 256 rows x 4096
+// channels 6 us.
+// Widths of 4 / 5 / 6 / 7 / 8 taps, 8 x 2048 x 4096 backward with its sums, us:
+// bfloat16 110 / 105 / 128 / 121 / 221, float32 168 / 169 / 176 / 186 / 191.  Eight
+// taps take more than 256 registers backward (264 to 279), so that a SIMD has one wave.
 #pragma once
 
 #include "ssm_common.hpp"

@@ -10,7 +10,9 @@ using namespace fg::ssm;
 
 // S: states of a lane, W: waves that share a channel's states; _any: for any
 // alignment, and channels with fewer than 4 S W states.  The backward kernel holds two states
-// and decays for each of its 16 S, so S = 4 is held to two waves per SIMD.
+// and decays for each of its 16 S, so S = 4 is held to two waves per SIMD.  That takes
+// all 256 registers and leaves a few in scratch memory: 27 of a lane (_any 65), 2 (26)
+// on two waves, none (4) on four.
 #define FG_SCAN_KERNEL(NAME, T, S, W, WIDE, CALL)                                                               \
     extern "C" __global__ __launch_bounds__((Scan<T, S, W, WIDE>::THREADS))                                     \
     __attribute__((amdgpu_waves_per_eu(2, 3))) void NAME(fg_scan_kargs g) {                                    \

@@ -13,19 +13,22 @@
 //     those states lie one token a lane in the row's 16 lanes, and reach the
 //     row as the DPP broadcast operand of the instruction that takes them.
 //     Sums over a channel's states go to LDS after one exchange within the wave.
-// Nothing is worked out twice.  A workgroup has 64 channels (32 for W = 4):
-// 128-byte lines of a 16-bit type.
+// Within a pass nothing is worked out twice.  (Where the token axis is cut, the
+// pass before it works out the time steps and decays too, and the backward pass
+// works the states out again.)  A workgroup has 64 channels, 128-byte lines of a
+// 16-bit type, above 16 states 32.
 //
 // Bound by the issue of VALU instructions: 7.8 for each state of a token
-// forward (5 of them the formula's), 22.8 in the gradients' pass, issued in 73
+// forward (5 of them the formula's), 22.7 in the gradients' pass, issued in 74
 // to 81 % of the cycles (counters of 4 x 1024 tokens x 2048 channels x 16 states
-// in bfloat16).  Measured: 4 x 2048 tokens x 4096 channels forward 165 us; 4 x
+// in bfloat16).  Measured: 4 x 2048 tokens x 4096 channels forward 166 us; 4 x
 // 1024 x 2048 forward and backward 233 us; steps of 256 rows x 4096 channels 33
 // us, 4.3 TB/s of states.
 //
-// W is 1 up to 16 states, 2 up to 32, 4 up to 64.  (16 states on two waves, for
-// tensors that leave SIMDs with one wave, gained nothing: 4 x 2048 tokens x
-// 4096 channels in bfloat16 194 us against 177.)
+// W is 1 up to 16 states, 2 up to 32, 4 up to 64.  (16 states on two waves were
+// tried where every SIMD has a wave without: 4 x 2048 tokens x 4096 channels in
+// bfloat16 194 us, when one took 177.  For tensors of fewer waves they are not
+// measured.)
 #pragma once
 
 #include "ssm_common.hpp"
