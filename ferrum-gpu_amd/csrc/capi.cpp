@@ -21,6 +21,7 @@
 #include "hip_backend.hpp"
 #include "host_stage.hpp"
 #include "scratch.hpp"
+#include "rec_ops.hpp"
 #include "ssm_ops.hpp"
 
 using fg::Buffer;
@@ -49,6 +50,7 @@ struct fg_device {
     Buffer<Cf32, HipBackend> staging_out;  // out-of-place outputs (plans whose in-place form differs)
     fg::Pointwise pointwise;  // elementwise kernels of fft_module
     std::unique_ptr<fg::SsmKernels> ssm;  // the sequence filters' code objects
+    std::unique_ptr<fg::RecurrenceKernels> rec;
     std::atomic<int> dependents{0};  // live plans and captured graphs made on this device
     std::unique_ptr<fg::HostStager> stager;  // pinned pieces of the host path (first large call)
     // fg_fft_exec_split_noalloc: calls on this device take turns at the
@@ -100,6 +102,11 @@ struct fg_scan_plan {
     fg_device* dev = nullptr;
 };
 
+struct fg_recurrence_plan {
+    std::unique_ptr<fg::RecurrencePlan> plan;
+    fg_device* dev = nullptr;
+};
+
 struct fg_graph {
     HipBackend::Graph g;
     fg_device* dev = nullptr;
@@ -142,6 +149,7 @@ fg_device* open_device(int ordinal) {
     d->fft_module = d->dev->load_or_cache(fg::fft_code_object());
     d->pointwise = fg::Pointwise(d->fft_module);
     d->ssm.reset(new fg::SsmKernels(*d->dev));
+    d->rec.reset(new fg::RecurrenceKernels(*d->dev));
     // The allocation-free entry point's scratch area: its address on this
     // device, resolved once with the device current (scratch.hip).
     HipBackend::bind(h);
@@ -994,6 +1002,68 @@ int fg_scan_step(fg_device_t dev, const fg_scan_step_args* args, fg_stream_t str
         need(dev, "device");
         need(args, "args");
         dev->ssm->scan_step(dev->dev->handle(), *args, (hipStream_t)stream);
+    });
+}
+
+int fg_recurrence_plan_create(fg_device_t dev, const fg_recurrence_shape* shape, fg_recurrence_plan_t* out) {
+    return guarded([&] {
+        need(out, "out");
+        *out = nullptr;
+        need(dev, "device");
+        need(shape, "shape");
+        std::unique_ptr<fg_recurrence_plan> p(new fg_recurrence_plan);
+        p->dev = dev;
+        p->plan.reset(new fg::RecurrencePlan(dev->dev->handle(), *dev->rec, *shape));
+        dev->dependents.fetch_add(1);
+        *out = p.release();
+    });
+}
+
+int fg_recurrence_plan_destroy(fg_recurrence_plan_t plan) {
+    return guarded([&] {
+        if (!plan) return;
+        plan->dev->dependents.fetch_sub(1);
+        delete plan;
+    });
+}
+
+int fg_recurrence_checkpoint_bytes(fg_recurrence_plan_t plan, size_t* bytes) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(bytes, "bytes");
+        *bytes = plan->plan->checkpoint_bytes();
+    });
+}
+
+int fg_recurrence_plan_get_info(fg_recurrence_plan_t plan, fg_recurrence_plan_info* out) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(out, "out");
+        plan->plan->info(out);
+    });
+}
+
+int fg_recurrence_forward(fg_recurrence_plan_t plan, const fg_recurrence_forward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->forward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_recurrence_backward(fg_recurrence_plan_t plan, const fg_recurrence_backward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->backward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(dev, "device");
+        need(args, "args");
+        dev->rec->step(dev->dev->handle(), *args, (hipStream_t)stream);
     });
 }
 

@@ -1,0 +1,45 @@
+/* rec_args.h -- kernel arguments and tile sizes of the gated linear recurrence
+ * (rec_scan.hpp), shared by the kernels and their host launchers (rec_ops.cpp). */
+#ifndef FG_REC_ARGS_H
+#define FG_REC_ARGS_H
+
+#include "ssm_args.h"
+
+#define FG_REC_CHANNELS 64                        /* of a workgroup */
+#define FG_REC_WAVES 8                            /* of a workgroup, at most */
+#define FG_REC_SEGMENT(bytes) ((bytes) == 2 ? 8 : 4) /* tokens of a lane, forward */
+#define FG_REC_BACK_SEGMENT 4                     /* backward */
+#define FG_REC_CHECK (4 * FG_REC_BACK_SEGMENT * FG_REC_WAVES) /* tokens between the states that a
+                                                    forward pass leaves for its backward pass */
+
+typedef struct {
+    fg_ssm_view x, ga, gx, out; /* backward: out is the output's gradient */
+    fg_ssm_view dx, dga, dgx;   /* gradients; may be null */
+    const float *decay, *bias_a, *bias_x, *initial;
+    float* final;
+    const float* gfinal;
+    float *ginitial, *gdecay, *gbias_a, *gbias_x;
+    const int32_t* offsets; /* packed: sequences + 1 of them; null: dense */
+    float* check;           /* [chains][checks][channels], states before each FG_REC_CHECK tokens;
+                               packed, behind them: [sequences][channels] initial states */
+    float* part;            /* [parts][3][channels] */
+    uint64_t tokens;        /* of a chain: a dense sequence's, packed those of all */
+    uint64_t checks;        /* of a chain */
+    uint64_t parts;
+    uint32_t seqs, chains, channels;
+    uint32_t blocks;        /* workgroups over the channels */
+    uint32_t tiles;         /* of a chain */
+    float rate;
+} fg_rec_kargs;
+
+typedef struct {
+    fg_ssm_view x, ga, gx, out; /* .seq: of rows; .row unused */
+    const float *decay, *bias_a, *bias_x, *state;
+    float* state_out;
+    const int32_t* slots;
+    uint64_t state_rows;
+    uint32_t rows, channels;
+    float rate;
+} fg_rec_step_kargs;
+
+#endif

@@ -1,5 +1,5 @@
-"""ferrum_gpu.ssm -- sequence filters: the short causal convolution and the
-selective state space scan.
+"""ferrum_gpu.ssm -- sequence filters: the short causal convolution, the
+selective state space scan and the gated linear recurrence.
 
 They stand beside the FFT's filters (``fft`` -> ``pointwise.cmul`` -> inverse),
 which cover long filters that stay the same over time: the convolution is for
@@ -13,6 +13,8 @@ FFT computes too.
 ``conv_step``          one token of each row, windows in a cache of slots
 ``ScanPlan``           selective scan of whole sequences, and its gradients
 ``scan_step``          one token of each row, states in a cache of slots
+``RecurrencePlan``     gated linear recurrence of whole sequences, and its gradients
+``recurrence_step``    one token of each row, states in a cache of slots
 =====================  =====================================================
 
 Arrays of rows (one row of ``channels``, for B and C ``groups * states``
@@ -21,7 +23,7 @@ elements a token) are GPU torch tensors of shape ``(batch, length, n)``, packed
 any strides but 1 between the elements of a row: slices of a projection's
 output need no copy.  DeviceBuffers and raw device addresses are taken as
 contiguous.  Everything else is contiguous: parameters and their gradients,
-scan states (float32), convolution states (``dtype``), ``offsets`` and
+scan and recurrence states (float32), convolution states (``dtype``), ``offsets`` and
 ``slots`` (int32).  A tensor of another shape, type or device and a DeviceBuffer
 that is too small raise ValueError before anything is launched; a raw address
 cannot be checked.
@@ -57,7 +59,8 @@ import struct
 from ferrum_gpu import _native as _n
 from ferrum_gpu.hip import Device, DeviceBuffer, _release
 
-__all__ = ["ConvPlan", "ScanPlan", "conv_step", "scan_step", "MAX_STATES", "MAX_WIDTH"]
+__all__ = ["ConvPlan", "ScanPlan", "RecurrencePlan", "conv_step", "scan_step", "recurrence_step", "MAX_STATES",
+           "MAX_WIDTH"]
 
 MAX_STATES, MAX_WIDTH = 64, 8
 
@@ -201,8 +204,12 @@ _conv_step_pack = struct.Struct("=6q" + "Qqq" * 2 + "Q" * 5).pack
 _scan_forward_pack = struct.Struct("=" + "Qqq" * 5 + "Q" * 5 + "Qqq" + "QQ").pack
 _scan_backward_pack = struct.Struct("=" + "Qqq" * 5 + "Q" * 5 + "Qqq" + "QQ" + "Qqq" * 5 + "Q" * 4).pack
 _scan_step_pack = struct.Struct("=7q" + "Qqq" * 6 + "Q" * 6).pack
+_recurrence_forward_pack = struct.Struct("=" + "Qqq" * 3 + "Q" * 4 + "Qqq" + "QQQ").pack
+_recurrence_backward_pack = struct.Struct("=" + "Qqq" * 3 + "Q" * 4 + "Qqq" + "QQ" + "Qqq" * 3 + "Q" * 4).pack
+_recurrence_step_pack = struct.Struct("=4qd" + "Qqq" * 4 + "Q" * 6).pack
 _shape_pack = struct.Struct("=8q").pack
 _scan_shape_pack = struct.Struct("=9q").pack
+_recurrence_shape_pack = struct.Struct("=6qd").pack
 
 
 class _Plan:
@@ -394,6 +401,80 @@ class ScanPlan(_Plan):
             _n.check(rc)
 
 
+class RecurrencePlan(_Plan):
+    """Gated linear recurrence of ``batch`` sequences, one state for each of
+    ``channels`` channels::
+
+        r = sigmoid(gate_a + bias_a),  i = sigmoid(gate_x + bias_x)
+        a = exp(-rate softplus(decay) r)
+        h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
+
+    With ``tokens`` the sequences are packed; ``length`` is not used then.
+    """
+
+    _destroy, _get_info = _n.lib.fg_recurrence_plan_destroy, _n.lib.fg_recurrence_plan_get_info
+    _info = ("forward_tokens", "backward_tokens", "workspace_bytes")
+
+    def __init__(self, batch: int, length: int, channels: int, device: Device, dtype="bfloat16", rate: float = 8.0,
+                 tokens: int | None = None):
+        self._setup(batch, length, tokens, channels, device, dtype)
+        self.rate = float(rate)
+        shape = _recurrence_shape_pack(self.batch, self.length, self.tokens, self.channels, _DTYPES[self.dtype],
+                                       self.packed, self.rate)
+        _n.check(_n.lib.fg_recurrence_plan_create(device.handle, shape, ctypes.byref(self._p)))
+        n = ctypes.c_size_t()
+        _n.check(_n.lib.fg_recurrence_checkpoint_bytes(self._p, ctypes.byref(n)))
+        #: Bytes of the ``checkpoints`` that a backward pass takes.
+        self.checkpoint_bytes = n.value
+
+    def _state(self, x, what: str) -> int:
+        return self._param(x, (self.batch, self.channels), what)
+
+    def _inputs(self, x, gate_a, gate_x, decay, bias_a, bias_x, offsets) -> tuple:
+        d = (self.channels,)
+        return (*self._row(x, "x"), *self._row(gate_a, "gate_a"), *self._row(gate_x, "gate_x"),
+                self._param(decay, d, "decay"), self._param(bias_a, d, "bias_a"), self._param(bias_x, d, "bias_x"),
+                self._offsets(offsets))
+
+    def forward(self, x, gate_a, gate_x, decay, out, bias_a=None, bias_x=None, initial=None, final=None,
+                offsets=None, checkpoints=None, stream=0) -> None:
+        """``decay``, ``bias_a`` and ``bias_x`` (channels) float32.  ``initial``:
+        the (batch, channels) states before each sequence (None: zeros);
+        ``final``: room for those after its last token, may be ``initial``.
+        ``checkpoints``: ``checkpoint_bytes`` of room, where backward()
+        follows."""
+        args = _recurrence_forward_pack(*self._inputs(x, gate_a, gate_x, decay, bias_a, bias_x, offsets),
+                                        *self._row(out, "out"), self._state(initial, "initial"),
+                                        self._state(final, "final"),
+                                        _bytes(checkpoints, self.checkpoint_bytes, self.device.ordinal,
+                                               "checkpoints"))
+        rc = _n.lib.fg_recurrence_forward(self._handle(), args, _stream(stream, self.device.ordinal))
+        if rc:
+            _n.check(rc)
+
+    def backward(self, x, gate_a, gate_x, decay, grad_out, checkpoints, grad_x=None, grad_gate_a=None,
+                 grad_gate_x=None, grad_decay=None, bias_a=None, bias_x=None, grad_bias_a=None, grad_bias_x=None,
+                 grad_initial=None, grad_final=None, offsets=None, stream=0) -> None:
+        """Gradients from ``grad_out``, that of ``out``, and ``grad_final``,
+        that of ``final`` (None: zeros), given forward's inputs and the
+        ``checkpoints`` it left; each is written where room for it is given."""
+        d = (self.channels,)
+        args = _recurrence_backward_pack(*self._inputs(x, gate_a, gate_x, decay, bias_a, bias_x, offsets),
+                                         *self._row(grad_out, "grad_out"),
+                                         _bytes(checkpoints, self.checkpoint_bytes, self.device.ordinal,
+                                                "checkpoints"),
+                                         self._state(grad_final, "grad_final"), *self._row(grad_x, "grad_x"),
+                                         *self._row(grad_gate_a, "grad_gate_a"),
+                                         *self._row(grad_gate_x, "grad_gate_x"),
+                                         self._param(grad_decay, d, "grad_decay"),
+                                         self._param(grad_bias_a, d, "grad_bias_a"),
+                                         self._param(grad_bias_x, d, "grad_bias_x"),
+                                         self._state(grad_initial, "grad_initial"))
+        rc = _n.lib.fg_recurrence_backward(self._handle(), args, _stream(stream, self.device.ordinal))
+        if rc:
+            _n.check(rc)
+
+
 def _shape(x) -> tuple:
     return x.shape if hasattr(x, "data_ptr") else ()
 
@@ -489,5 +570,36 @@ def scan_step(device: Device, u, delta, A, B, C, state, out, D=None, z=None, del
                            s if state_out is None else _flat(state_out, shape, "float32", nbytes, at, "state_out"),
                            _flat(slots, (batch,), "int32", 4 * batch, at, "slots"))
     rc = _n.lib.fg_scan_step(device.handle, args, _stream(stream, at))
+    if rc:
+        _n.check(rc)
+
+
+def recurrence_step(device: Device, x, gate_a, gate_x, decay, state, out, bias_a=None, bias_x=None, slots=None,
+                    state_out=None, rate: float = 8.0, batch=None, channels=None, state_rows=None, dtype=None,
+                    stream=0) -> None:
+    """RecurrencePlan's recurrence of one token of each of ``batch`` rows.
+
+    ``state``: (state_rows, channels) float32; ``slots`` and ``state_out`` as
+    for conv_step().  Sizes and ``dtype`` come from tensors; they are given where
+    the arrays are DeviceBuffers or addresses."""
+    lead = _shape(x)
+    batch, channels = _size(batch, lead, 0, "batch"), _size(channels, lead, 1, "channels")
+    state_rows = _size(state_rows, _shape(state), 0, "state_rows")
+    dtype = _check_dtype(dtype or (_dtype_of(x) if hasattr(x, "data_ptr") else "bfloat16"))
+    at = device.ordinal
+    row, param, shape, nbytes = (batch, channels), (channels,), (state_rows, channels), 4 * state_rows * channels
+    s = _flat(state, shape, "float32", nbytes, at, "state")
+    args = _recurrence_step_pack(batch, channels, _DTYPES[dtype], state_rows, rate,
+                                 *_step_row(x, row, (), dtype, at, "x"),
+                                 *_step_row(gate_a, row, (), dtype, at, "gate_a"),
+                                 *_step_row(gate_x, row, (), dtype, at, "gate_x"),
+                                 *_step_row(out, row, (), dtype, at, "out"),
+                                 _flat(decay, param, "float32", 4 * channels, at, "decay"),
+                                 _flat(bias_a, param, "float32", 4 * channels, at, "bias_a"),
+                                 _flat(bias_x, param, "float32", 4 * channels, at, "bias_x"), s,
+                                 s if state_out is None else _flat(state_out, shape, "float32", nbytes, at,
+                                                                   "state_out"),
+                                 _flat(slots, (batch,), "int32", 4 * batch, at, "slots"))
+    rc = _n.lib.fg_recurrence_step(device.handle, args, _stream(stream, at))
     if rc:
         _n.check(rc)

@@ -546,6 +546,79 @@ typedef struct fg_scan_step_args {
 } fg_scan_step_args;
 FG_API int fg_scan_step(fg_device_t dev, const fg_scan_step_args *args, fg_stream_t stream);
 
+/* The gated linear recurrence: one state for each channel, which a gate of the
+ * token lets decay.
+ *   r = sigmoid(gate_a + bias_a[d]), i = sigmoid(gate_x + bias_x[d])
+ *   a = exp(-rate softplus(decay[d]) r)
+ *   h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
+ * Rows, packed sequences (their number of tokens is not held against `length`),
+ * states and workspaces as for the scan. */
+typedef struct fg_recurrence_plan *fg_recurrence_plan_t;
+
+typedef struct fg_recurrence_shape {
+    int64_t sequences, length, tokens; /* tokens: packed only */
+    int64_t channels, dtype, packed;
+    double rate; /* finite, 0 or more */
+} fg_recurrence_shape;
+
+/* Optional (NULL): bias_a, bias_x (zeros); offsets unless packed. */
+typedef struct fg_recurrence_inputs {
+    fg_rows x, gate_a, gate_x;
+    const float *decay, *bias_a, *bias_x; /* [channels] */
+    const int32_t *offsets;
+} fg_recurrence_inputs;
+
+/* initial (NULL: zeros): the [sequences][channels] states before each sequence;
+ * final (NULL: not wanted): those after its last token, may be initial.
+ * checkpoints (NULL: no backward pass follows): fg_recurrence_checkpoint_bytes()
+ * that the backward pass of the same inputs takes. */
+typedef struct fg_recurrence_forward_args {
+    fg_recurrence_inputs in;
+    fg_rows out;
+    const float *initial;
+    float *final;
+    void *checkpoints;
+} fg_recurrence_forward_args;
+
+/* Gradients from grad_out, that of out, and grad_final (NULL: zeros), that of
+ * final.  Each output may be NULL. */
+typedef struct fg_recurrence_backward_args {
+    fg_recurrence_inputs in;
+    fg_rows grad_out;
+    const void *checkpoints;
+    const float *grad_final;
+    fg_rows grad_x, grad_gate_a, grad_gate_x;
+    float *grad_decay, *grad_bias_a, *grad_bias_x, *grad_initial;
+} fg_recurrence_backward_args;
+
+FG_API int fg_recurrence_plan_create(fg_device_t dev, const fg_recurrence_shape *shape, fg_recurrence_plan_t *out);
+FG_API int fg_recurrence_plan_destroy(fg_recurrence_plan_t plan);
+FG_API int fg_recurrence_checkpoint_bytes(fg_recurrence_plan_t plan, size_t *bytes);
+/* Tokens that a workgroup works through at a time, and the GPU memory that the
+ * plan holds (the backward pass's from its first call on). */
+typedef struct fg_recurrence_plan_info {
+    int64_t forward_tokens, backward_tokens, workspace_bytes;
+} fg_recurrence_plan_info;
+FG_API int fg_recurrence_plan_get_info(fg_recurrence_plan_t plan, fg_recurrence_plan_info *out);
+FG_API int fg_recurrence_forward(fg_recurrence_plan_t plan, const fg_recurrence_forward_args *args, fg_stream_t stream);
+/* The first call allocates the plan's workspace for the parameters' gradients, so
+ * it cannot be captured into a graph; later ones can. */
+FG_API int fg_recurrence_backward(fg_recurrence_plan_t plan, const fg_recurrence_backward_args *args,
+                                  fg_stream_t stream);
+
+/* One token of each row; slots as for fg_conv_step, over the state_rows
+ * [channels] states.  state_out may be state. */
+typedef struct fg_recurrence_step_args {
+    int64_t rows, channels, dtype, state_rows;
+    double rate;
+    fg_rows x, gate_a, gate_x, out; /* row i: seq_stride * i; row_stride is not used */
+    const float *decay, *bias_a, *bias_x;
+    const float *state;
+    float *state_out;
+    const int32_t *slots;
+} fg_recurrence_step_args;
+FG_API int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args *args, fg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
