@@ -12,6 +12,13 @@
 #define FG_REC_CHECK (4 * FG_REC_BACK_SEGMENT * FG_REC_WAVES) /* tokens between the states that a
                                                     forward pass leaves for its backward pass */
 
+/* Tiles whose pairs a workgroup composes itself, see rec_scan.hpp. */
+#define FG_REC_GROUP 8
+/* What a plan's tiles pass on: 8-byte words, first the tickets drawn, behind them for
+ * each tile FG_REC_WORDS of FG_REC_CHANNELS words. */
+#define FG_REC_WORDS 3
+#define FG_REC_CHAIN_BYTES(places) (64 + 8ull * FG_REC_WORDS * FG_REC_CHANNELS * (places))
+
 typedef struct {
     fg_ssm_view x, ga, gx, out; /* backward: out is the output's gradient */
     fg_ssm_view dx, dga, dgx;   /* gradients; may be null */
@@ -23,6 +30,8 @@ typedef struct {
     float* check;           /* [chains][checks][channels], states before each FG_REC_CHECK tokens;
                                packed, behind them: [sequences][channels] initial states */
     float* part;            /* [parts][3][channels] */
+    unsigned long long* chain; /* FG_REC_CHAIN_BYTES(tiles * chains * blocks); null where a chain is one tile */
+    uint64_t over_places;   /* (2^64 - 1) / (tiles * chains * blocks) */
     uint64_t tokens;        /* of a chain: a dense sequence's, packed those of all */
     uint64_t checks;        /* of a chain */
     uint64_t parts;

@@ -14,6 +14,18 @@
 // row by lane exchanges and from wave to wave through LDS, and each lane runs over
 // its tokens again from the state that then enters them.
 //
+// From tile to tile of a chain they pass through memory, in one launch.  A word of 8
+// bytes holds a float and the launch's tag, so that what is read with the tag is
+// whole and of this launch, and no order of memory has to be kept.  Every tile writes
+// its pair; a tile composes those of the tiles before it in its group of
+// FG_REC_GROUP and the state that leaves the group before, which that group's last
+// tile writes: from left to right, so that a result does not depend on who was
+// first.  Workgroups take their tiles by a ticket, first tiles first: who waits does
+// so for workgroups that hold earlier tickets, and of those that hold one the
+// earliest waits for nobody, so every wait ends.  The tickets count on from launch
+// to launch, and their number gives the tag: nothing has to be cleared between
+// launches, also when a graph replays them.
+//
 // Packed sequences are one chain of rows: a sequence's first token takes its
 // initial state in place of the one before it.
 #pragma once
@@ -58,6 +70,92 @@ template <bool PACKED>
 __device__ __forceinline__ float through(float p1, float p2) {
     const float v = fmaxf(p1 * p2, kLeast);
     return PACKED && fminf(p1, p2) < 0.0f ? -1.0f : v;
+}
+
+// A workgroup's tile, counted from the end that its chain begins at, and its launch's tag.
+struct Place {
+    uint32_t block, chain, tile, tag;
+};
+__device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
+    const uint32_t across = g.blocks * g.chains;
+    uint32_t at = blockIdx.x, tag = 0;
+    if (g.chain) {
+        __shared__ unsigned long long ticket;
+        if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(g.chain, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const uint64_t mine = ticket, places = (uint64_t)across * g.tiles;
+        uint64_t launch = __umul64hi(mine, g.over_places);  // mine / places, or one less
+        uint64_t rest = mine - launch * places;
+        if (rest >= places) {
+            rest -= places;
+            ++launch;
+        }
+        at = uniform((uint32_t)rest);
+        tag = uniform((uint32_t)(launch % 0xffffffffull) + 1);  // never 0, which memory starts with
+    }
+    Place p;
+    p.tile = at / across;
+    const uint32_t rest = at - p.tile * across;
+    p.chain = rest / g.blocks;
+    p.block = rest - p.chain * g.blocks;
+    p.tag = tag;
+    return p;
+}
+
+__device__ __forceinline__ unsigned long long* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
+    return g.chain + 8 +
+           (((uint64_t)tile * g.chains + p.chain) * g.blocks + p.block) * (FG_REC_WORDS * FG_REC_CHANNELS);
+}
+__device__ __forceinline__ void tell(unsigned long long* to, uint32_t tag, float v) {
+    __hip_atomic_store(to, (unsigned long long)tag << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long ask(const unsigned long long* from) {
+    return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// For the first wave, a lane for each channel: tells the tile's pair p, q and returns
+// the state that enters the tile, `first` for a chain's first one.
+template <bool PACKED>
+__device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at, float p, float q, float first) {
+    const uint32_t lane = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
+    const bool last = at.tile + 1 == g.tiles;
+    unsigned long long* mine = words(g, at, at.tile) + lane;
+    if (!last) {
+        tell(mine, at.tag, p);
+        tell(mine + FG_REC_CHANNELS, at.tag, q);
+    }
+    unsigned long long w[2 * FG_REC_GROUP];
+    float state = first;
+    // Waits end, as above; the count bounds them all the same, with NaN for what has not come.
+    for (uint32_t tries = 0;; ++tries) {
+        bool all = true;
+        each<FG_REC_GROUP - 1>([&](auto k) {
+            if (k < in_group) {
+                const unsigned long long* from = words(g, at, at.tile - in_group + k) + lane;
+                w[2 * k] = ask(from);
+                w[2 * k + 1] = ask(from + FG_REC_CHANNELS);
+            }
+        });
+        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask(words(g, at, at.tile - in_group - 1) + lane + 2 * FG_REC_CHANNELS);
+        each<FG_REC_GROUP - 1>([&](auto k) {
+            if (k < in_group) all = all && w[2 * k] >> 32 == at.tag && w[2 * k + 1] >> 32 == at.tag;
+        });
+        if (at.tile >= FG_REC_GROUP) all = all && w[2 * FG_REC_GROUP - 1] >> 32 == at.tag;
+        if (__all(all)) break;
+        if (tries == 1u << 22) {
+            each<2 * FG_REC_GROUP>([&](auto k) { w[k] = 0x7fc00000; });
+            q = __uint_as_float(0x7fc00000);
+            break;
+        }
+        __builtin_amdgcn_s_sleep(1);
+    }
+    if (at.tile >= FG_REC_GROUP) state = __uint_as_float((uint32_t)w[2 * FG_REC_GROUP - 1]);
+    each<FG_REC_GROUP - 1>([&](auto k) {
+        if (k < in_group)
+            state = enter<PACKED>(__uint_as_float((uint32_t)w[2 * k]), __uint_as_float((uint32_t)w[2 * k + 1]), state);
+    });
+    if (!last && in_group == FG_REC_GROUP - 1) tell(mine + 2 * FG_REC_CHANNELS, at.tag, enter<PACKED>(p, q, state));
+    return state;
 }
 
 template <class T, bool WIDE, bool PACKED>
@@ -213,19 +311,45 @@ struct Rec {
             *(float4*)&t.v[wave][1][l.ch] = make_float4(q[0], q[1], q[2], q[3]);
         }
     }
-    // From the state that enters the tile: the one that enters the wave, and the one that leaves the tile.
+    // From the state that enters the tile to the one that enters the wave.
     template <bool BACK>
     static __device__ __forceinline__ void pass(const Totals& t, uint32_t wave, uint32_t waves, const Lane& l,
-                                                float (&carry)[V], float (&mine)[V]) {
-        for (uint32_t k = 0; k < waves; ++k) {
+                                                float (&h)[V]) {
+        const uint32_t before = BACK ? waves - 1 - wave : wave;
+        for (uint32_t k = 0; k < before; ++k) {
             const uint32_t w = BACK ? waves - 1 - k : k;
-            if (w == wave) each<V>([&](auto c) { mine[c] = carry[c]; });
             const float4 p = *(const float4*)&t.v[w][0][l.ch], q = *(const float4*)&t.v[w][1][l.ch];
-            carry[0] = enter<PACKED>(p.x, q.x, carry[0]);
-            carry[1] = enter<PACKED>(p.y, q.y, carry[1]);
-            carry[2] = enter<PACKED>(p.z, q.z, carry[2]);
-            carry[3] = enter<PACKED>(p.w, q.w, carry[3]);
+            h[0] = enter<PACKED>(p.x, q.x, h[0]);
+            h[1] = enter<PACKED>(p.y, q.y, h[1]);
+            h[2] = enter<PACKED>(p.z, q.z, h[2]);
+            h[3] = enter<PACKED>(p.w, q.w, h[3]);
         }
+    }
+
+    // The state that enters the tile, at the lane's channels.  `first`: a chain's
+    // first one, [channels of the workgroup] or null.
+    template <bool BACK>
+    static __device__ __forceinline__ void enter_tile(const fg_rec_kargs& g, const Place& at, const Totals& t, float* lds,
+                                                      const float* first, uint32_t wave, uint32_t waves, const Lane& l,
+                                                      float (&h)[V]) {
+        if (g.tiles == 1) {
+            params(h, first, l);
+            return;
+        }
+        if (wave == 0) {
+            float p = 1.0f, q = 0.0f;
+            for (uint32_t k = 0; k < waves; ++k) {
+                const uint32_t w = BACK ? waves - 1 - k : k;
+                const float p2 = t.v[w][0][l.lane], q2 = t.v[w][1][l.lane];
+                q = enter<PACKED>(p2, q2, q);
+                p = through<PACKED>(p, p2);
+            }
+            const bool some = first && at.block * FG_REC_CHANNELS + l.lane < g.channels;
+            lds[l.lane] = entering<PACKED>(g, at, p, q, some ? first[l.lane] : 0.0f);
+        }
+        __syncthreads();
+        const float4 v = *(const float4*)&lds[l.ch];
+        h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
     }
 
     // A packed sequence's row of [sequences][channels].
@@ -270,16 +394,16 @@ struct Rec {
 
     static __device__ __forceinline__ void forward(const fg_rec_kargs& g) {
         constexpr int S = FG_REC_SEGMENT(sizeof(raw));
-        __shared__ Totals totals[2];
-        const uint32_t block = blockIdx.x % g.blocks, chain = blockIdx.x / g.blocks;
+        __shared__ Totals totals;
+        __shared__ float4 entered[FG_REC_CHANNELS / 4];
+        const Place at = place_of(g);
+        const uint32_t block = at.block, chain = at.chain, tile = at.tile;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
         Params w;
         w.load(g, block, l);
         const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
-        float carry[V] = {};
-        if constexpr (!PACKED) params(carry, of(g.initial, g, chain, block), l);
-        for (uint32_t tile = 0; tile < g.tiles; ++tile) {
+        {
             const int64_t t0 = ((int64_t)tile * waves + wave) * (4 * S);
             const Marks<S> m = marks<S>(g, t0 + l.row * S);
             float a[S][V], b[S][V], p[V], q[V];
@@ -319,10 +443,11 @@ struct Rec {
             each<V>([&](auto c) { p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast); });
             float ep[V], eq[V], h[V];
             rows<false>(p, q, ep, eq, l);
-            Totals& t = totals[tile & 1];
-            publish<false>(t, wave, l, p, q);
+            publish<false>(totals, wave, l, p, q);
             __syncthreads();
-            pass<false>(t, wave, waves, l, carry, h);
+            enter_tile<false>(g, at, totals, &entered[0].x, PACKED ? nullptr : of(g.initial, g, chain, block), wave,
+                              waves, l, h);
+            pass<false>(totals, wave, waves, l, h);
             if (g.check && t0 % FG_REC_CHECK == 0 && l.row == 0 && t0 < (int64_t)g.tokens)
                 put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + at0, l, h);
             each<V>([&](auto c) { h[c] = enter<PACKED>(ep[c], eq[c], h[c]); });
@@ -340,23 +465,24 @@ struct Rec {
                     }
                 }
             });
-            if constexpr (PACKED) empty(g, g.initial, g.final, block, chain, tile);
+            empty(g, g.initial, g.final, block, chain, tile);
         }
-        if constexpr (!PACKED) empty(g, g.initial, g.final, block, chain, 0);
     }
 
     static __device__ __forceinline__ void backward(const fg_rec_kargs& g) {
         constexpr int S = FG_REC_BACK_SEGMENT;
-        __shared__ Totals ahead[2], behind[2];
-        const uint32_t block = blockIdx.x % g.blocks, chain = blockIdx.x / g.blocks;
+        __shared__ Totals both[2];
+        __shared__ float4 entered[FG_REC_CHANNELS / 4];
+        Totals &ta = both[0], &tb = both[1];
+        const Place at = place_of(g);
+        const uint32_t block = at.block, chain = at.chain, tile = g.tiles - 1 - at.tile;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
         Params w;
         w.load(g, block, l);
         const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
-        float back[V] = {}, sums[3][V] = {};
-        if constexpr (!PACKED) params(back, of(g.gfinal, g, chain, block), l);
-        for (uint32_t tile = g.tiles; tile-- > 0;) {
+        float sums[3][V] = {};
+        {
             const int64_t t0 = ((int64_t)tile * waves + wave) * (4 * S);
             const Marks<S> m = marks<S>(g, t0 + l.row * S);
             float a[S][V], b[S][V], p[V], q[V], rp[V], rq[V];
@@ -404,18 +530,19 @@ struct Rec {
                 rp[c] = PACKED && m.last ? -1.0f : fmaxf(p[c], kLeast);
                 p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast);
             });
-            float ep[V], eq[V], rep[V], req[V], h[V], d[V], state[V] = {};
+            float ep[V], eq[V], rep[V], req[V], h[V] = {}, d[V];
             rows<false>(p, q, ep, eq, l);
             rows<true>(rp, rq, rep, req, l);
-            Totals &ta = ahead[tile & 1], &tb = behind[tile & 1];
             publish<false>(ta, wave, l, p, q);
             publish<true>(tb, wave, l, rp, rq);
             const int64_t first_token = (int64_t)tile * waves * (4 * S);
             if (first_token < (int64_t)g.tokens)
-                params(state, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
+                params(h, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
             __syncthreads();
-            pass<false>(ta, wave, waves, l, state, h);
-            pass<true>(tb, wave, waves, l, back, d);
+            pass<false>(ta, wave, waves, l, h);
+            enter_tile<true>(g, at, tb, &entered[0].x, PACKED ? nullptr : of(g.gfinal, g, chain, block), wave, waves, l,
+                             d);
+            pass<true>(tb, wave, waves, l, d);
             each<V>([&](auto c) {
                 h[c] = enter<PACKED>(ep[c], eq[c], h[c]);
                 d[c] = enter<PACKED>(rep[c], req[c], d[c]);
@@ -467,13 +594,12 @@ struct Rec {
                     }
                 }
             });
-            if constexpr (PACKED) empty(g, g.gfinal, g.ginitial, block, chain, tile);
+            empty(g, g.gfinal, g.ginitial, block, chain, tile);
         }
-        if constexpr (!PACKED) empty(g, g.gfinal, g.ginitial, block, chain, 0);
         // the parameters' sums: over the rows of a wave, then over the waves
         __syncthreads();
-        float* to = &ahead[0].v[0][0][0];  // [wave][3][channel]
-        static_assert(sizeof(ahead) >= 4 * 3 * FG_REC_WAVES * FG_REC_CHANNELS, "the sums fit");
+        float* to = &both[0].v[0][0][0];  // [wave][3][channel]
+        static_assert(sizeof(both) >= 4 * 3 * FG_REC_WAVES * FG_REC_CHANNELS, "the sums fit");
         each<3>([&](auto k) {
             each<V>([&](auto c) {
                 float v = sums[k][c];
@@ -487,7 +613,7 @@ struct Rec {
             const uint32_t k = e / FG_REC_CHANNELS, ch = e % FG_REC_CHANNELS;
             float v = 0.0f;
             for (uint32_t u = 0; u < waves; ++u) v += to[(u * 3 + k) * FG_REC_CHANNELS + ch];
-            if (at0 + ch < g.channels) g.part[((uint64_t)chain * 3 + k) * g.channels + at0 + ch] = v;
+            if (at0 + ch < g.channels) g.part[(((uint64_t)chain * g.tiles + tile) * 3 + k) * g.channels + at0 + ch] = v;
         }
     }
 };

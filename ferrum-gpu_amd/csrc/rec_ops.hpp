@@ -39,11 +39,15 @@ public:
 
 private:
     uint32_t waves(uint32_t segment) const;
-    fg_rec_kargs base(const char* op, const fg_recurrence_inputs& in, uint32_t segment) const;
+    uint64_t places(uint32_t segment) const;
+    Buffer<char, HipBackend> chain(uint32_t segment) const;
+    fg_rec_kargs base(const char* op, const fg_recurrence_inputs& in, uint32_t segment,
+                      const Buffer<char, HipBackend>& chain) const;
     HipBackend::DeviceHandle dev_;
     fg_recurrence_shape s_;
     uint64_t chains_, rows_;  // chains of so many rows: dense, the sequences; packed, one
     HipBackend::KernelHandle forward_[2] = {}, backward_[2] = {}, reduce_;  // [any, wide]
+    Buffer<char, HipBackend> ahead_, back_;  // what the tiles pass on, back_ from the first backward call on
     std::mutex mu_;
     Buffer<float, HipBackend> part_;
 };

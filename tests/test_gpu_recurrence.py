@@ -150,7 +150,8 @@ def run(dev, lead, channels, dtype, rate=8.0, layout="plain", offsets=None, bias
     (1, 1, 1, "float32"), (2, 3, 5, "bfloat16"), (1, 7, 64, "float16"), (3, 8, 68, "bfloat16"),
     (1, 31, 130, "float32"), (2, 33, 64, "bfloat16"), (1, 127, 66, "float16"), (1, 128, 64, "float32"),
     (1, 129, 192, "bfloat16"), (2, 255, 100, "float16"), (1, 256, 64, "bfloat16"), (1, 257, 61, "bfloat16"),
-    (5, 513, 64, "bfloat16"), (1, 1025, 70, "float16"), (2, 1000, 128, "float32"), (1, 2049, 260, "bfloat16")])
+    (5, 513, 64, "bfloat16"), (1, 1025, 70, "float16"), (2, 1000, 128, "float32"), (1, 2049, 260, "bfloat16"),
+    (1, 5003, 64, "bfloat16"), (3, 2600, 130, "float32")])
 def test_sizes(gpu_device, batch, length, channels, dtype):
     run(gpu_device, (batch, length), channels, dtype)
 
