@@ -21,6 +21,7 @@
 #include "hip_backend.hpp"
 #include "host_stage.hpp"
 #include "scratch.hpp"
+#include "norm_ops.hpp"
 #include "rec_ops.hpp"
 #include "ssm_ops.hpp"
 
@@ -51,6 +52,7 @@ struct fg_device {
     fg::Pointwise pointwise;  // elementwise kernels of fft_module
     std::unique_ptr<fg::SsmKernels> ssm;  // the sequence filters' code objects
     std::unique_ptr<fg::RecurrenceKernels> rec;
+    std::unique_ptr<fg::NormKernels> norm;
     std::atomic<int> dependents{0};  // live plans and captured graphs made on this device
     std::unique_ptr<fg::HostStager> stager;  // pinned pieces of the host path (first large call)
     // fg_fft_exec_split_noalloc: calls on this device take turns at the
@@ -107,6 +109,11 @@ struct fg_recurrence_plan {
     fg_device* dev = nullptr;
 };
 
+struct fg_norm_plan {
+    std::unique_ptr<fg::NormPlan> plan;
+    fg_device* dev = nullptr;
+};
+
 struct fg_graph {
     HipBackend::Graph g;
     fg_device* dev = nullptr;
@@ -150,6 +157,7 @@ fg_device* open_device(int ordinal) {
     d->pointwise = fg::Pointwise(d->fft_module);
     d->ssm.reset(new fg::SsmKernels(*d->dev));
     d->rec.reset(new fg::RecurrenceKernels(*d->dev));
+    d->norm.reset(new fg::NormKernels(*d->dev));
     // The allocation-free entry point's scratch area: its address on this
     // device, resolved once with the device current (scratch.hip).
     HipBackend::bind(h);
@@ -1064,6 +1072,60 @@ int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args* args, fg_
         need(dev, "device");
         need(args, "args");
         dev->rec->step(dev->dev->handle(), *args, (hipStream_t)stream);
+    });
+}
+
+int fg_norm_plan_create(fg_device_t dev, const fg_norm_shape* shape, fg_norm_plan_t* out) {
+    return guarded([&] {
+        need(out, "out");
+        *out = nullptr;
+        need(dev, "device");
+        need(shape, "shape");
+        std::unique_ptr<fg_norm_plan> p(new fg_norm_plan);
+        p->dev = dev;
+        p->plan.reset(new fg::NormPlan(dev->dev->handle(), *dev->norm, *shape));
+        dev->dependents.fetch_add(1);
+        *out = p.release();
+    });
+}
+
+int fg_norm_plan_destroy(fg_norm_plan_t plan) {
+    return guarded([&] {
+        if (!plan) return;
+        plan->dev->dependents.fetch_sub(1);
+        delete plan;
+    });
+}
+
+int fg_norm_plan_get_info(fg_norm_plan_t plan, fg_norm_plan_info* out) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(out, "out");
+        plan->plan->info(out);
+    });
+}
+
+int fg_norm_forward(fg_norm_plan_t plan, const fg_norm_forward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->forward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_norm_backward(fg_norm_plan_t plan, const fg_norm_backward_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(plan, "plan");
+        need(args, "args");
+        plan->plan->backward(*args, (hipStream_t)stream);
+    });
+}
+
+int fg_dropout(fg_device_t dev, const fg_dropout_args* args, fg_stream_t stream) {
+    return guarded([&] {
+        need(dev, "device");
+        need(args, "args");
+        dev->norm->dropout(dev->dev->handle(), *args, (hipStream_t)stream);
     });
 }
 

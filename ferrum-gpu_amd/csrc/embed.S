@@ -1,7 +1,7 @@
-/* embed.S -- places the gfx950 code objects (FFT, and the sequence filters and
- * the recurrence for each element type) inside libferrum_gpu.so so the HIP backend can hand them
+/* embed.S -- places the gfx950 code objects (FFT, and the sequence filters, the
+ * recurrence, the norm and dropout for each element type) inside libferrum_gpu.so so the HIP backend can hand them
  * to hipModuleLoadData without touching the file system (FG_HSACO_PATH and
- * FG_SSM_*_PATH, FG_REC_*_PATH are set by the Makefile). */
+ * FG_SSM_*_PATH, FG_REC_*_PATH, FG_NORM_*_PATH are set by the Makefile). */
     .section .rodata.fg_fft_code_object,"a",@progbits
     .p2align 12
     .globl fg_fft_code_object_start
@@ -30,4 +30,7 @@ FG_EMBED(ssm_f16, FG_SSM_F16_PATH)
 FG_EMBED(rec_f32, FG_REC_F32_PATH)
 FG_EMBED(rec_bf16, FG_REC_BF16_PATH)
 FG_EMBED(rec_f16, FG_REC_F16_PATH)
+FG_EMBED(norm_f32, FG_NORM_F32_PATH)
+FG_EMBED(norm_bf16, FG_NORM_BF16_PATH)
+FG_EMBED(norm_f16, FG_NORM_F16_PATH)
     .section .note.GNU-stack,"",@progbits

@@ -18,11 +18,16 @@
 
 namespace fg {
 
-__host__ __device__ __forceinline__ uint64_t splitmix64_at(uint64_t seed, uint64_t j) {
-    uint64_t z = seed + (j + 1) * 0x9E3779B97F4A7C15ull;
+constexpr uint64_t kSplitmixStep = 0x9E3779B97F4A7C15ull;
+
+__host__ __device__ __forceinline__ uint64_t splitmix64_mix(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
     return z ^ (z >> 31);
+}
+
+__host__ __device__ __forceinline__ uint64_t splitmix64_at(uint64_t seed, uint64_t j) {
+    return splitmix64_mix(seed + (j + 1) * kSplitmixStep);
 }
 
 __device__ __forceinline__ float uniform_at(uint64_t seed, uint64_t j) {

@@ -1,0 +1,322 @@
+// norm_rows.hpp -- the root-mean-square norm of rows with what stands before it
+// on a residual stream, its gradient, and dropout on its own:
+//
+//   v = dropout(x) + residual,  s = 1 / sqrt(mean(v^2) + eps),  out = v s weight
+//   sum = v, rounded to the rows' type
+//
+// out in 8 bits (e4m3): out / scale, scale = max |out| / 448 over a row or a group of
+// its elements.  With w = v weight and its largest m, both are w 448 / m and m s /
+// 448, so that one pass finds all that the other needs.
+//
+// Backward, from the stored sum u: with s of u and g = grad_out weight,
+//   dv = s (g - u s^2 mean(g u)) + grad_sum,  dx = dropout(dv),  dresidual = dv
+//   dweight = sum over rows of grad_out u s
+//
+// A team of threads takes a row, each thread chunks of 16 bytes of it: the row is
+// read once and stays in registers.  Rows that do not fit are read again (C = 0).
+//
+// Dropout keeps element e (row-major) where 32 bits are at least p 2^32: half e % 2 of
+// the seed's splitmix64 number offset + e / 2 (fill.hpp), so no mask is stored.
+#pragma once
+
+#include "norm_args.h"
+#include "ssm_common.hpp"
+
+#include "fill.hpp"
+
+namespace fg {
+namespace norm {
+
+using namespace ssm;
+
+constexpr float kMost = 448.0f;            // e4m3's largest
+constexpr float kLeast = 7.888609e-31f;    // 2^-100: what 448 / m is taken of at least
+
+// Chunks of 16 bytes at any address of their elements: the GPU's loads and stores take them.
+template <class T>
+struct Chunk {
+    using raw = typename T::raw;
+    static constexpr int E = 16 / sizeof(raw);
+    struct __attribute__((packed, aligned(sizeof(raw)))) Raw {
+        raw v[E];
+    };
+    struct __attribute__((packed, aligned(4))) Floats {
+        float v[E];
+    };
+    struct __attribute__((packed, aligned(1))) Bytes {
+        uint32_t v[E / 4];
+    };
+    // n of E elements, 0 for the others.
+    static __device__ __forceinline__ Raw load(const void* p, int64_t at, uint32_t n) {
+        const raw* from = (const raw*)p + at;
+        Raw r;
+        if (n >= E) return *(const Raw*)from;
+        each<E>([&](auto i) { r.v[i] = i < n ? from[i] : raw(0); });
+        return r;
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t at, uint32_t n, const float (&x)[E]) {
+        raw* to = (raw*)p + at;
+        Raw r;
+        each<E>([&](auto i) { r.v[i] = T::down(x[i]); });
+        if (n >= E) {
+            *(Raw*)to = r;
+        } else {
+            each<E>([&](auto i) {
+                if (i < n) to[i] = r.v[i];
+            });
+        }
+    }
+    static __device__ __forceinline__ void floats(float (&x)[E], const float* p, uint32_t at, uint32_t n) {
+        if (!p) {
+            each<E>([&](auto i) { x[i] = 1.0f; });
+        } else if (n >= E) {
+            const Floats f = *(const Floats*)(p + at);
+            each<E>([&](auto i) { x[i] = f.v[i]; });
+        } else {
+            each<E>([&](auto i) { x[i] = i < n ? p[at + i] : 0.0f; });
+        }
+    }
+    static __device__ __forceinline__ void store8(void* p, int64_t at, uint32_t n, const float (&x)[E]) {
+        uint8_t* to = (uint8_t*)p + at;
+        Bytes b;
+        each<E / 4>([&](auto i) {
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+            b.v[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
+        });
+        if (n >= E) {
+            *(Bytes*)to = b;
+        } else {
+            each<E>([&](auto i) {
+                if (i < n) to[i] = (uint8_t)(b.v[i / 4] >> (8 * (i % 4)));
+            });
+        }
+    }
+    // x where it is kept times 1 / (1 - p), else 0, of elements e, e + 1, ...
+    static __device__ __forceinline__ void drop(float (&x)[E], uint64_t seed, uint64_t first, uint64_t e, uint32_t drop,
+                                                uint32_t all, float keep) {
+        const auto one = [&](float& v, uint32_t bits) { v = !all && bits >= drop ? v * keep : 0.0f; };
+        if (e & 1) {
+            each<E>([&](auto i) {
+                const uint64_t z = splitmix64_at(seed, first + (e + i) / 2);
+                one(x[i], (uint32_t)((e + i) & 1 ? z >> 32 : z));
+            });
+        } else {
+            const uint64_t state = seed + (first + e / 2 + 1) * kSplitmixStep;
+            each<E / 2>([&](auto i) {
+                const uint64_t z = splitmix64_mix(state + i * kSplitmixStep);
+                one(x[2 * i], (uint32_t)z);
+                one(x[2 * i + 1], (uint32_t)(z >> 32));
+            });
+        }
+    }
+};
+
+// Two sums, or a sum and a largest value, over a team's threads.
+template <int TEAM, bool MAX>
+__device__ __forceinline__ void over_team(float& a, float& b, float2 (&lds)[FG_NORM_THREADS / 64]) {
+    each<6>([&](auto i) {
+        a += __shfl_xor(a, 1 << i);
+        const float o = __shfl_xor(b, 1 << i);
+        b = MAX ? fmaxf(b, o) : b + o;
+    });
+    if constexpr (TEAM > 64) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.0f;
+        each<TEAM / 64>([&](auto w) {
+            const float2 v = lds[w];
+            a += v.x;
+            b = MAX ? fmaxf(b, v.y) : b + v.y;
+        });
+    }
+}
+
+// C: chunks of a thread; 0: any number of them, read again.
+template <class T, int C, int TEAM>
+struct Rows {
+    using Io = Chunk<T>;
+    using Raw = typename Io::Raw;
+    static constexpr int E = Io::E, TEAMS = FG_NORM_THREADS / TEAM, KEPT = C ? C : 1;
+
+    static __device__ __forceinline__ uint32_t count(const fg_norm_kargs& g, uint32_t col) {
+        return col >= g.width ? 0 : g.width - col;
+    }
+    template <class F>
+    static __device__ __forceinline__ void chunks(const fg_norm_kargs& g, F&& f) {
+        const uint32_t first = (threadIdx.x % TEAM) * E;
+        if constexpr (C > 0) {
+            each<C>([&](auto k) {
+                const uint32_t col = first + k * (TEAM * E);
+                f(k, col, count(g, col));
+            });
+        } else {
+            // every thread of the team passes as often: lanes exchange values within
+            for (uint32_t at = 0; at < g.width; at += TEAM * E) f(Int<0>{}, at + first, count(g, at + first));
+        }
+    }
+
+    static __device__ __forceinline__ void value(const fg_norm_kargs& g, uint64_t row, uint32_t col, uint32_t n,
+                                                 uint64_t numbers, float (&v)[E]) {
+        const Raw x = Io::load(g.x.p, (int64_t)row * g.x.row + col, n);
+        each<E>([&](auto i) { v[i] = T::up(x.v[i]); });
+        if (g.drop) Io::drop(v, g.seed, numbers, row * g.width + col, g.drop, g.drop_all, g.keep);
+        if (g.residual.p) {
+            const Raw r = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
+            each<E>([&](auto i) { v[i] += T::up(r.v[i]); });
+        }
+    }
+
+    static __device__ __forceinline__ void forward(const fg_norm_kargs& g) {
+        __shared__ float2 lds[2][FG_NORM_THREADS / 64];
+        const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
+        float w[KEPT][E], v[KEPT][E];
+        if constexpr (C > 0) chunks(g, [&](auto k, uint32_t col, uint32_t n) { Io::floats(w[k], g.weight, col, n); });
+        uint32_t turn = 0;
+        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += (uint64_t)gridDim.x * TEAMS, turn ^= 1) {
+            const uint64_t row = at + threadIdx.x / TEAM;
+            const bool some = row < g.rows;  // a whole team's
+            float squares = 0.0f, most = 0.0f;
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                each<E>([&](auto i) { v[k][i] = 0.0f; });
+                if (!some || !n) return;
+                if constexpr (C == 0) Io::floats(w[k], g.weight, col, n);
+                value(g, row, col, n, numbers, v[k]);
+                each<E>([&](auto i) {
+                    if (i >= n) v[k][i] = 0.0f;  // a dropped place beyond the row holds nothing else
+                    squares = fmaf(v[k][i], v[k][i], squares);
+                    most = fmaxf(most, fabsf(v[k][i] * w[k][i]));
+                });
+                if (g.sum.p && C) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k]);
+            });
+            over_team<TEAM, true>(squares, most, lds[turn]);
+            const float s = __builtin_amdgcn_rsqf(fmaf(squares, g.over_width, g.eps));
+            if (g.scales && !g.group_lanes && some && threadIdx.x % TEAM == 0)
+                g.scales[row] = most == 0.0f ? 0.0f * s : fmaxf(most, kLeast) * s * (1.0f / kMost);
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                if (C == 0) {
+                    each<E>([&](auto i) { v[k][i] = 0.0f; });
+                    if (some && n) {
+                        Io::floats(w[k], g.weight, col, n);
+                        value(g, row, col, n, numbers, v[k]);
+                        if (g.sum.p) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k]);
+                    }
+                }
+                float y[E];
+                if (!g.scales) {
+                    each<E>([&](auto i) { y[i] = v[k][i] * s * w[k][i]; });
+                    if (some && n) Io::store(g.out.p, (int64_t)row * g.out.row + col, n, y);
+                    return;
+                }
+                float m = most;
+                if (g.group_lanes) {
+                    m = 0.0f;
+                    each<E>([&](auto i) { m = fmaxf(m, i < n ? fabsf(v[k][i] * w[k][i]) : 0.0f); });
+                    for (uint32_t far = 1; far < g.group_lanes; far *= 2) m = fmaxf(m, __shfl_xor(m, far));
+                    if (some && n && (threadIdx.x & (g.group_lanes - 1)) == 0)
+                        g.scales[row * g.groups + col / (g.group_lanes * E)] =
+                            m == 0.0f ? 0.0f * s : fmaxf(m, kLeast) * s * (1.0f / kMost);
+                }
+                const float up = kMost / fmaxf(m, kLeast);
+                each<E>([&](auto i) { y[i] = v[k][i] * w[k][i] * up; });
+                if (some && n) Io::store8(g.out.p, (int64_t)row * g.out.row + col, n, y);
+            });
+        }
+    }
+
+    static __device__ __forceinline__ void backward(const fg_norm_kargs& g) {
+        __shared__ float2 lds[2][FG_NORM_THREADS / 64];
+        const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
+        float w[KEPT][E], dw[KEPT][E], u[KEPT][E], dy[KEPT][E];
+        float* part = g.part ? g.part + (uint64_t)(blockIdx.x * TEAMS + threadIdx.x / TEAM) * g.width : nullptr;
+        chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+            if (C > 0) Io::floats(w[k], g.weight, col, n);
+            each<E>([&](auto i) { dw[k][i] = 0.0f; });
+            if (C == 0 && part) each<E>([&](auto i) { if (i < n) part[col + i] = 0.0f; });
+        });
+        uint32_t turn = 0;
+        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += (uint64_t)gridDim.x * TEAMS, turn ^= 1) {
+            const uint64_t row = at + threadIdx.x / TEAM;
+            const bool some = row < g.rows;
+            const auto load = [&](auto k, uint32_t col, uint32_t n) {
+                if constexpr (C == 0) Io::floats(w[k], g.weight, col, n);
+                const Raw a = Io::load(g.x.p, (int64_t)row * g.x.row + col, n);
+                const Raw b = Io::load(g.out.p, (int64_t)row * g.out.row + col, n);
+                each<E>([&](auto i) { u[k][i] = T::up(a.v[i]), dy[k][i] = T::up(b.v[i]); });
+            };
+            float squares = 0.0f, along = 0.0f;
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                if (!some || !n) return;
+                load(k, col, n);
+                each<E>([&](auto i) {
+                    squares = fmaf(u[k][i], u[k][i], squares);
+                    if (i < n) along = fmaf(dy[k][i] * w[k][i], u[k][i], along);
+                });
+            });
+            over_team<TEAM, false>(squares, along, lds[turn]);
+            const float s = __builtin_amdgcn_rsqf(fmaf(squares, g.over_width, g.eps));
+            const float back = along * g.over_width * s * s;
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                if (!some || !n) return;
+                if constexpr (C == 0) load(k, col, n);
+                float dv[E];
+                each<E>([&](auto i) { dv[i] = s * fmaf(-u[k][i], back, dy[k][i] * w[k][i]); });
+                if (g.residual.p) {
+                    const Raw r = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
+                    each<E>([&](auto i) { dv[i] += T::up(r.v[i]); });
+                }
+                if (g.dresidual.p) Io::store(g.dresidual.p, (int64_t)row * g.dresidual.row + col, n, dv);
+                if (g.dx.p) {
+                    if (g.drop) Io::drop(dv, g.seed, numbers, row * g.width + col, g.drop, g.drop_all, g.keep);
+                    Io::store(g.dx.p, (int64_t)row * g.dx.row + col, n, dv);
+                }
+                if constexpr (C > 0) {
+                    each<E>([&](auto i) { dw[k][i] = fmaf(dy[k][i], u[k][i] * s, dw[k][i]); });
+                } else if (part) {
+                    each<E>([&](auto i) {
+                        if (i < n) part[col + i] = fmaf(dy[k][i], u[k][i] * s, part[col + i]);
+                    });
+                }
+            });
+        }
+        if (C > 0 && part) {
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                each<E>([&](auto i) { if (i < n) part[col + i] = dw[k][i]; });
+            });
+        }
+    }
+};
+
+// The weight's gradient from the teams' parts: 64 columns of a workgroup, whose
+// waves share the parts.
+__device__ __forceinline__ void reduce(const float* part, float* to, uint32_t width, uint32_t parts) {
+    __shared__ float sums[16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const uint64_t col = (uint64_t)blockIdx.x * 64 + lane;
+    const uint32_t each_wave = (parts + waves - 1) / waves, a = min(parts, wave * each_wave), b = min(parts, a + each_wave);
+    sums[wave][lane] = col < width ? ordered_sum(part + (uint64_t)a * width + col, width, b - a) : 0.0f;
+    __syncthreads();
+    if (wave == 0 && col < width) {
+        float v = 0.0f;
+        for (uint32_t k = 0; k < waves; ++k) v += sums[k][lane];
+        to[col] = v;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void dropout(const fg_dropout_kargs& g) {
+    using Io = Chunk<T>;
+    constexpr int E = Io::E;
+    const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
+    const uint64_t step = (uint64_t)gridDim.x * blockDim.x * E;
+    for (uint64_t at = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * E; at < g.n; at += step) {
+        const uint32_t n = g.n - at < E ? (uint32_t)(g.n - at) : E;
+        const typename Io::Raw x = Io::load(g.x, (int64_t)at, n);
+        float v[E];
+        each<E>([&](auto i) { v[i] = T::up(x.v[i]); });
+        if (g.drop) Io::drop(v, g.seed, numbers, at, g.drop, g.drop_all, g.keep);
+        Io::store(g.out, (int64_t)at, n, v);
+    }
+}
+
+}  // namespace norm
+}  // namespace fg

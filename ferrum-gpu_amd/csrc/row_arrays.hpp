@@ -61,7 +61,9 @@ class Arrays {
 public:
     Arrays(const char* op, int64_t seqs, int64_t rows, uint32_t es) : op_(op), seqs_(seqs), rows_(rows), es_(es) {}
 
-    fg_ssm_view rows(const char* name, const fg_rows& r, int64_t width, bool out, bool optional = false) {
+    // es: bytes of this array's elements where they are not the call's.
+    fg_ssm_view rows(const char* name, const fg_rows& r, int64_t width, bool out, bool optional = false, uint32_t es = 0) {
+        if (!es) es = es_;
         fg_ssm_view v{nullptr, 0, 0};
         if (!r.ptr) {
             if (!optional && seqs_ > 0 && rows_ > 0) invalid(std::string(op_) + ": " + name + ": null buffer");
@@ -70,7 +72,7 @@ public:
         v.p = r.ptr;
         v.seq = seqs_ > 1 ? r.seq_stride : 0;
         v.row = rows_ > 1 ? r.row_stride : 0;
-        if (reinterpret_cast<uintptr_t>(r.ptr) % es_)
+        if (reinterpret_cast<uintptr_t>(r.ptr) % es)
             invalid(std::string(op_) + ": " + name + ": not aligned to its elements");
         if (v.seq < 0 || v.row < 0) invalid(std::string(op_) + ": " + name + ": negative stride");
         if (v.row > kMaxRowStride)
@@ -78,7 +80,7 @@ public:
                     std::to_string(kMaxRowStride));
         if (seqs_ == 0 || rows_ == 0) return v;
         const __int128 last = (__int128)(seqs_ - 1) * v.seq + (__int128)(rows_ - 1) * v.row + width;
-        if (last > kMaxBytes / es_) invalid(std::string(op_) + ": " + name + ": too large");
+        if (last > kMaxBytes / es) invalid(std::string(op_) + ": " + name + ": too large");
         if (out) {
             // rows of all sequences apart: the larger stride steps over all that the smaller one covers
             int64_t small = v.row, small_n = rows_, large = v.seq, large_n = seqs_;
@@ -89,9 +91,9 @@ public:
         Extent e;
         e.name = name;
         e.p = (const char*)r.ptr;
-        e.seq = v.seq * es_;
-        e.row = v.row * es_;
-        e.width = width * es_;
+        e.seq = v.seq * es;
+        e.row = v.row * es;
+        e.width = width * es;
         e.bytes = (seqs_ - 1) * e.seq + (rows_ - 1) * e.row + e.width;
         e.out = out;
         add(e);

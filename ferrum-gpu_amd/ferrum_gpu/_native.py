@@ -132,10 +132,12 @@ _sig("fg_graph_capture_begin", _vp, _P(_vp))
 _sig("fg_graph_capture_end", _vp, _vp, _P(_vp))
 _sig("fg_graph_node_count", _vp, _P(_sz))
 _sig("fg_graph_destroy", _vp)
-for _name in ("fg_conv_plan_create", "fg_scan_plan_create", "fg_recurrence_plan_create"):
+for _name in ("fg_conv_plan_create", "fg_scan_plan_create", "fg_recurrence_plan_create",
+              "fg_norm_plan_create"):
     _sig(_name, _vp, ctypes.c_char_p, _P(_vp))
 for _name in ("fg_conv_forward", "fg_conv_backward", "fg_conv_step", "fg_scan_forward", "fg_scan_backward",
-              "fg_scan_step", "fg_recurrence_forward", "fg_recurrence_backward", "fg_recurrence_step"):
+              "fg_scan_step", "fg_recurrence_forward", "fg_recurrence_backward", "fg_recurrence_step",
+              "fg_norm_forward", "fg_norm_backward", "fg_dropout"):
     _sig(_name, _vp, ctypes.c_char_p, _vp)  # the argument struct, packed
 _sig("fg_conv_plan_destroy", _vp)
 _sig("fg_conv_plan_get_info", _vp, _vp)
@@ -145,6 +147,8 @@ _sig("fg_scan_checkpoint_bytes", _vp, _P(_sz))
 _sig("fg_recurrence_plan_get_info", _vp, _vp)
 _sig("fg_recurrence_plan_destroy", _vp)
 _sig("fg_recurrence_checkpoint_bytes", _vp, _P(_sz))
+_sig("fg_norm_plan_get_info", _vp, _vp)
+_sig("fg_norm_plan_destroy", _vp)
 
 
 def last_error() -> str:

@@ -76,7 +76,7 @@ def _torch_type(dtype: str):
     if t is None:
         import torch  # a tensor has come, so it is there
 
-        for name in (*_DTYPES, "int32"):
+        for name in (*_DTYPES, "int32", "int64", "float8_e4m3fn"):
             _torch_types[name] = getattr(torch, name)
             _type_names[_torch_types[name]] = name
         t = _torch_types[dtype]

@@ -619,6 +619,83 @@ typedef struct fg_recurrence_step_args {
 } fg_recurrence_step_args;
 FG_API int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args *args, fg_stream_t stream);
 
+/* ------------------------------------------------- residual norm, dropout */
+
+/* What stands around the filters of a block, on rows of its residual stream (see
+ * above; row r starts row_stride * r elements from ptr, seq_stride is not used).
+ *
+ *   v = dropout(x) + residual, out = v / sqrt(mean(v^2) + eps) * weight
+ *   sum = v, rounded to the rows' type
+ *
+ * With scales, out is in 8 bits (e4m3, a byte an element): out / scale, one scale
+ * of float32 for each row (group = 0) or for each `group` elements of it, the last
+ * ones' may be fewer; scales is [rows][ceil(width / group)].  A scale is max |out| /
+ * 448, 0 where all of them are 0; it is NaN where a row holds what is not finite.
+ *
+ * Dropout keeps element e = row * width + column where 32 bits are at least p 2^32,
+ * as x / (1 - p): half e % 2 (the lower one first) of the splitmix64 number offset + e / 2
+ * of the seed, the generator of fg_fill_uniform_c64, whose numbers it calls z(0),
+ * z(1), ...  A call uses (rows * width + 1) / 2 of them.  counter (NULL: 0): an int64 on the
+ * device that is added to offset, for calls captured into a graph.  The
+ * backward pass takes the forward pass's p, seed, offset and counter. */
+typedef struct fg_norm_plan *fg_norm_plan_t;
+
+typedef struct fg_norm_shape {
+    int64_t rows, width, dtype; /* rows: the most that a call has */
+    int64_t group;              /* 0, 32, 64 or 128 */
+    double eps;                 /* finite, 0 or more */
+} fg_norm_shape;
+
+/* Optional (NULL): residual, sum, weight (ones), scales (out has the rows' type).
+ * out may be x, unless in 8 bits, and sum may be residual. */
+typedef struct fg_norm_forward_args {
+    int64_t rows;
+    fg_rows x, residual, out, sum;
+    const float *weight; /* [width] */
+    float *scales;
+    double dropout; /* p, 0 .. 1 */
+    uint64_t seed, offset;
+    const int64_t *counter;
+} fg_norm_forward_args;
+
+/* Gradients from grad_out, that of out in the rows' type, and grad_sum (NULL: zeros),
+ * that of sum, given the sum as it was stored.  Each output may be NULL.
+ * grad_residual may be grad_sum and grad_x may be grad_out. */
+typedef struct fg_norm_backward_args {
+    int64_t rows;
+    fg_rows sum, grad_out, grad_sum, grad_x, grad_residual;
+    const float *weight;
+    float *grad_weight;
+    double dropout;
+    uint64_t seed, offset;
+    const int64_t *counter;
+} fg_norm_backward_args;
+
+FG_API int fg_norm_plan_create(fg_device_t dev, const fg_norm_shape *shape, fg_norm_plan_t *out);
+FG_API int fg_norm_plan_destroy(fg_norm_plan_t plan);
+/* Threads that share a row, and the GPU memory that the plan holds (from the first
+ * backward call with a weight's gradient on). */
+typedef struct fg_norm_plan_info {
+    int64_t row_threads, workspace_bytes;
+} fg_norm_plan_info;
+FG_API int fg_norm_plan_get_info(fg_norm_plan_t plan, fg_norm_plan_info *out);
+FG_API int fg_norm_forward(fg_norm_plan_t plan, const fg_norm_forward_args *args, fg_stream_t stream);
+/* The first call with grad_weight allocates the plan's workspace for it, so it
+ * cannot be captured into a graph; later ones can. */
+FG_API int fg_norm_backward(fg_norm_plan_t plan, const fg_norm_backward_args *args, fg_stream_t stream);
+
+/* Dropout on its own: element e of n contiguous ones as above; out may be x.  A
+ * gradient takes the same call with the same p, seed, offset and counter. */
+typedef struct fg_dropout_args {
+    const void *x;
+    void *out;
+    int64_t n, dtype;
+    double p;
+    uint64_t seed, offset;
+    const int64_t *counter;
+} fg_dropout_args;
+FG_API int fg_dropout(fg_device_t dev, const fg_dropout_args *args, fg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
