@@ -7,13 +7,15 @@
 
 #define FG_REC_CHANNELS 64                        /* of a workgroup */
 #define FG_REC_WAVES 8                            /* of a workgroup, at most */
-#define FG_REC_SEGMENT(bytes) ((bytes) == 2 ? 8 : 4) /* tokens of a lane, forward */
-#define FG_REC_BACK_SEGMENT 4                     /* backward */
-#define FG_REC_CHECK (4 * FG_REC_BACK_SEGMENT * FG_REC_WAVES) /* tokens between the states that a
+#define FG_REC_LANE_CHANNELS 2                    /* of a lane; also the rows of lanes of a wave */
+#define FG_REC_SEGMENT(bytes) ((bytes) == 2 ? 16 : 8) /* tokens of a lane, forward */
+#define FG_REC_BACK_SEGMENT 8                     /* backward */
+#define FG_REC_BACK_WAVES 4                       /* backward */
+#define FG_REC_CHECK (FG_REC_LANE_CHANNELS * FG_REC_BACK_SEGMENT * FG_REC_BACK_WAVES) /* tokens between the states that a
                                                     forward pass leaves for its backward pass */
 
 /* Tiles whose pairs a workgroup composes itself, see rec_scan.hpp. */
-#define FG_REC_GROUP 8
+#define FG_REC_GROUP 4
 /* What a plan's tiles pass on: 8-byte words, first the tickets drawn, behind them for
  * each tile FG_REC_WORDS of FG_REC_CHANNELS words. */
 #define FG_REC_WORDS 3
@@ -32,6 +34,7 @@ typedef struct {
     float* part;            /* [parts][3][channels] */
     unsigned long long* chain; /* FG_REC_CHAIN_BYTES(tiles * chains * blocks); null where a chain is one tile */
     uint64_t over_places;   /* (2^64 - 1) / (tiles * chains * blocks) */
+    uint32_t over_across, over_blocks; /* (2^32 - 1) / (chains * blocks), / blocks */
     uint64_t tokens;        /* of a chain: a dense sequence's, packed those of all */
     uint64_t checks;        /* of a chain */
     uint64_t parts;

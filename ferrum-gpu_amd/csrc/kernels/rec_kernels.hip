@@ -7,10 +7,12 @@ using namespace fg::rec;
 
 // _any: for any stride, alignment and number of channels.
 #define FG_REC_ONE(NAME, T, SUFFIX, WIDE, PACKED)                                                               \
-    extern "C" __global__ __launch_bounds__(64 * FG_REC_WAVES) void fg_rec_##NAME##SUFFIX(fg_rec_kargs g) {     \
+    extern "C" __global__ __launch_bounds__(64 * FG_REC_WAVES) __attribute__((amdgpu_waves_per_eu(4)))          \
+    void fg_rec_##NAME##SUFFIX(fg_rec_kargs g) {                                                               \
         Rec<T, WIDE, PACKED>::forward(g);                                                                      \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64 * FG_REC_WAVES) void fg_rec_back_##NAME##SUFFIX(fg_rec_kargs g) { \
+    extern "C" __global__ __launch_bounds__(64 * FG_REC_BACK_WAVES) __attribute__((amdgpu_waves_per_eu(3)))     \
+    void fg_rec_back_##NAME##SUFFIX(fg_rec_kargs g) {                                                          \
         Rec<T, WIDE, PACKED>::backward(g);                                                                     \
     }
 #define FG_REC_STEP(NAME, T, V)                                                                                 \

@@ -5,9 +5,9 @@
 //   a = exp(-rate softplus(decay) r), m = sqrt(1 - a^2)
 //   h_t = a h_{t-1} + m i x,  out = h_t
 //
-// A workgroup has 64 channels.  A lane takes four neighbouring channels through a
-// segment of S tokens, the four rows of 16 lanes of a wave four segments that
-// follow one another, its waves the segments behind those: a tile of 4 S waves
+// A workgroup has 64 channels.  A lane takes two neighbouring channels through a
+// segment of S tokens, the two rows of 32 lanes of a wave two segments that
+// follow one another, its waves the segments behind those: a tile of 2 S waves
 // tokens.  A lane works out a and b = m i x of its tokens once and keeps them in
 // registers; what a segment does to the state that enters it is h -> p h + q, with
 // p the product of its a and q its own state from 0.  These pairs pass from row to
@@ -49,11 +49,10 @@ struct Share {
     float a, m2;
 };
 __device__ __forceinline__ Share share(float k, float r) {
-    const float y = k * r, z = y + y;
-    const float a = exp2_(y);
-    constexpr float c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5;
-    const float near1 = -z * fmaf(z, fmaf(z, fmaf(z, fmaf(z, c5, c4), c3), c2), c1);
-    return {a, z > -0.25f ? near1 : fmaf(-a, a, 1.0f)};
+    const float y = k * r, a = exp2_(y);
+    constexpr float l = 2 * kLn2, c1 = -l, c2 = c1 * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5;
+    const float near1 = y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, c5, c4), c3), c2), c1);
+    return {a, y > -0.125f ? near1 : fmaf(-a, a, 1.0f)};
 }
 
 // What a run of tokens does to the state that enters it: h -> p h + q.  Packed
@@ -76,6 +75,16 @@ __device__ __forceinline__ float through(float p1, float p2) {
 struct Place {
     uint32_t block, chain, tile, tag;
 };
+// n / d and the rest, of over = (2^32 - 1) / d, which gives the quotient or one less.
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t over, uint32_t& rest) {
+    uint32_t q = __umulhi(n, over);
+    rest = n - q * d;
+    if (rest >= d) {
+        rest -= d;
+        ++q;
+    }
+    return q;
+}
 __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
     const uint32_t across = g.blocks * g.chains;
     uint32_t at = blockIdx.x, tag = 0;
@@ -83,33 +92,36 @@ __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
         __shared__ unsigned long long ticket;
         if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(g.chain, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        const uint64_t mine = ticket, places = (uint64_t)across * g.tiles;
+        const uint64_t mine = (uint64_t)uniform((int64_t)ticket), places = (uint64_t)across * g.tiles;
         uint64_t launch = __umul64hi(mine, g.over_places);  // mine / places, or one less
         uint64_t rest = mine - launch * places;
         if (rest >= places) {
             rest -= places;
             ++launch;
         }
-        at = uniform((uint32_t)rest);
-        tag = uniform((uint32_t)(launch % 0xffffffffull) + 1);  // never 0, which memory starts with
+        at = (uint32_t)rest;
+        tag = (uint32_t)launch << 1 | 1;  // never 0, which memory starts with
     }
     Place p;
-    p.tile = at / across;
-    const uint32_t rest = at - p.tile * across;
-    p.chain = rest / g.blocks;
-    p.block = rest - p.chain * g.blocks;
+    uint32_t rest;
+    p.tile = quotient(at, across, g.over_across, rest);
+    p.chain = quotient(rest, g.blocks, g.over_blocks, p.block);
     p.tag = tag;
     return p;
 }
 
-__device__ __forceinline__ unsigned long long* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
-    return g.chain + 8 +
-           (((uint64_t)tile * g.chains + p.chain) * g.blocks + p.block) * (FG_REC_WORDS * FG_REC_CHANNELS);
+// A tile's words; the same for all lanes.
+__device__ __forceinline__ char* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
+    const uint64_t place = ((uint64_t)tile * g.chains + p.chain) * g.blocks + p.block;
+    return (char*)g.chain + 64 + uniform((int64_t)(place * (8 * FG_REC_WORDS * FG_REC_CHANNELS)));
 }
-__device__ __forceinline__ void tell(unsigned long long* to, uint32_t tag, float v) {
+// Word `which` of a lane's channel.
+__device__ __forceinline__ void tell(char* at, int which, uint32_t lane, uint32_t tag, float v) {
+    unsigned long long* to = (unsigned long long*)(at + 8 * FG_REC_CHANNELS * which + 8 * lane);
     __hip_atomic_store(to, (unsigned long long)tag << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ unsigned long long ask(const unsigned long long* from) {
+__device__ __forceinline__ unsigned long long ask(const char* at, int which, uint32_t lane) {
+    const unsigned long long* from = (const unsigned long long*)(at + 8 * FG_REC_CHANNELS * which + 8 * lane);
     return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -119,10 +131,10 @@ template <bool PACKED>
 __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at, float p, float q, float first) {
     const uint32_t lane = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
     const bool last = at.tile + 1 == g.tiles;
-    unsigned long long* mine = words(g, at, at.tile) + lane;
+    char* mine = words(g, at, at.tile);
     if (!last) {
-        tell(mine, at.tag, p);
-        tell(mine + FG_REC_CHANNELS, at.tag, q);
+        tell(mine, 0, lane, at.tag, p);
+        tell(mine, 1, lane, at.tag, q);
     }
     unsigned long long w[2 * FG_REC_GROUP];
     float state = first;
@@ -131,12 +143,12 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         bool all = true;
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) {
-                const unsigned long long* from = words(g, at, at.tile - in_group + k) + lane;
-                w[2 * k] = ask(from);
-                w[2 * k + 1] = ask(from + FG_REC_CHANNELS);
+                const char* from = words(g, at, at.tile - in_group + k);
+                w[2 * k] = ask(from, 0, lane);
+                w[2 * k + 1] = ask(from, 1, lane);
             }
         });
-        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask(words(g, at, at.tile - in_group - 1) + lane + 2 * FG_REC_CHANNELS);
+        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask(words(g, at, at.tile - in_group - 1), 2, lane);
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) all = all && w[2 * k] >> 32 == at.tag && w[2 * k + 1] >> 32 == at.tag;
         });
@@ -154,45 +166,60 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         if (k < in_group)
             state = enter<PACKED>(__uint_as_float((uint32_t)w[2 * k]), __uint_as_float((uint32_t)w[2 * k + 1]), state);
     });
-    if (!last && in_group == FG_REC_GROUP - 1) tell(mine + 2 * FG_REC_CHANNELS, at.tag, enter<PACKED>(p, q, state));
+    if (!last && in_group == FG_REC_GROUP - 1) tell(mine, 2, lane, at.tag, enter<PACKED>(p, q, state));
     return state;
+}
+
+// An infinite x as the largest number of its sign; NaN stays.
+__device__ __forceinline__ float finite(float x) {
+    constexpr float most = 3.402823466e38f;
+    x = x > most ? most : x;
+    return x < -most ? -most : x;
 }
 
 template <class T, bool WIDE, bool PACKED>
 struct Rec {
     using raw = typename T::raw;
-    static constexpr int V = 4;
+    static constexpr int V = FG_REC_LANE_CHANNELS, ROW = 64 / V;  // ROW: lanes that share a token
+    struct __attribute__((aligned(V * 4))) Floats {
+        float v[V];
+    };
     struct __attribute__((aligned(V * sizeof(raw)))) Pack {
         raw v[V];
     };
-
     // A lane's place in the wave's tokens, and its channels.
     struct Lane {
         uint32_t lane, row, ch;  // ch: within the workgroup's 64
         uint32_t left;           // channels from ch on
+        uint32_t off;            // bytes from the workgroup's first channel to what the lane loads: lanes without
+                                 // channels load the first ones
     };
     static __device__ __forceinline__ Lane lane_of(const fg_rec_kargs& g, uint32_t block) {
         Lane l;
         l.lane = threadIdx.x & 63;
-        l.row = l.lane >> 4;
-        l.ch = (l.lane & 15) * V;
+        l.row = l.lane / ROW;
+        l.ch = l.lane % ROW * V;
         const uint32_t all = g.channels - block * FG_REC_CHANNELS;
         l.left = l.ch < all ? all - l.ch : 0;
+        l.off = l.left ? l.ch * (uint32_t)sizeof(raw) : 0;
         return l;
     }
 
-    // Four floats of the workgroup's channels; 0 beyond them.
+    // Floats of the lane's channels, of the workgroup's; 0 beyond them.
     static __device__ __forceinline__ void params(float (&x)[V], const float* p, const Lane& l) {
         if constexpr (WIDE) {
-            const float4 v = p && l.left ? *(const float4*)(p + l.ch) : make_float4(0, 0, 0, 0);
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+            Floats f{};
+            if (p && l.left) f = *(const Floats*)(p + l.ch);
+            each<V>([&](auto c) { x[c] = f.v[c]; });
         } else {
             each<V>([&](auto c) { x[c] = p && c < l.left ? p[l.ch + c] : 0.0f; });
         }
     }
     static __device__ __forceinline__ void put(float* p, const Lane& l, const float (&x)[V]) {
         if constexpr (WIDE) {
-            if (l.left) *(float4*)(p + l.ch) = make_float4(x[0], x[1], x[2], x[3]);
+            Floats f;
+            each<V>([&](auto c) { f.v[c] = x[c]; });
+            if (l.left) *(Floats*)(p + l.ch) = f;
         } else {
             each<V>([&](auto c) {
                 if (c < l.left) p[l.ch + c] = x[c];
@@ -212,7 +239,7 @@ struct Rec {
         } else {
             Pack k;  // channels beyond the last one load it again
             each<V>([&](auto c) {
-                const uint32_t at = l.left == 0 ? 0 : c < l.left ? c : l.left - 1;
+                const uint32_t at = c < l.left ? c : l.left ? l.left - 1 : 0;
                 k.v[c] = *(const raw*)(p + off + at * sizeof(raw));
             });
             return k;
@@ -230,47 +257,55 @@ struct Rec {
         }
     }
 
-    // Which of a segment's S tokens are a sequence's, and where sequences begin
-    // and end; dense: all up to the chain's end.
-    template <int S>
+    // Which of a segment's S tokens are a sequence's, and where packed ones begin and end.
     struct Marks {
         uint32_t in = 0, first = 0, last = 0;
-        int32_t seq[PACKED ? S : 1];
     };
     static __device__ __forceinline__ int64_t offset(const fg_rec_kargs& g, uint32_t s) {
         const int64_t v = g.offsets[s], all = (int64_t)g.tokens;
         return v < 0 ? 0 : v > all ? all : v;
     }
-    template <int S>
-    static __device__ __forceinline__ Marks<S> marks(const fg_rec_kargs& g, int64_t t) {
-        Marks<S> m;
-        const int64_t left = (int64_t)g.tokens - t;
-        if constexpr (!PACKED) {
-            m.in = left >= S ? (1u << S) - 1 : left > 0 ? (1u << left) - 1 : 0;
-        } else {
-            uint32_t lo = 0, hi = g.seqs;  // the sequences whose end is at t or before it
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                if (offset(g, mid + 1) <= t) lo = mid + 1;
-                else hi = mid;
-            }
-            uint32_t s = lo;
-            int64_t a = s < g.seqs ? offset(g, s) : 0, b = s < g.seqs ? offset(g, s + 1) : 0;
-            each<S>([&](auto j) {
-                const int64_t at = t + j;
-                while (s < g.seqs && b <= at) {
-                    ++s;
-                    a = b;
-                    if (s < g.seqs) b = offset(g, s + 1);
-                }
-                const bool in = s < g.seqs && a <= at && j < left;
-                m.in |= (uint32_t)in << j;
-                m.first |= (uint32_t)(in && a == at) << j;
-                m.last |= (uint32_t)(in && b == at + 1) << j;
-                m.seq[j] = (int32_t)s;
-            });
+    // The same for a whole wave, by scalar loads: they wait for no rows that are on their way.
+    static __device__ __forceinline__ int64_t offset_of_wave(const fg_rec_kargs& g, uint32_t s) {
+        using Scalars = const __attribute__((address_space(4))) int32_t*;
+        const int64_t v = ((Scalars)(uint64_t)g.offsets)[uniform(s)], all = (int64_t)g.tokens;
+        return v < 0 ? 0 : v > all ? all : v;
+    }
+    // Of the packed sequences, the first that ends behind row t.
+    template <class F>
+    static __device__ __forceinline__ uint32_t search(const fg_rec_kargs& g, int64_t t, F&& offset_) {
+        uint32_t lo = 0, hi = g.seqs;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (offset_(g, mid + 1) <= t) lo = mid + 1;
+            else hi = mid;
         }
-        return m;
+        return lo;
+    }
+    static __device__ __forceinline__ uint32_t sequence(const fg_rec_kargs& g, int64_t t) { return search(g, t, offset); }
+    // Of the wave's V S tokens from t0 on, those of the lane's segment.
+    template <int S>
+    static __device__ __forceinline__ Marks marks(const fg_rec_kargs& g, int64_t t0, const Lane& l) {
+        static_assert(V * S <= 32, "a bit for each");
+        constexpr uint32_t ALL = (1u << S) - 1;
+        if constexpr (!PACKED) {
+            const int64_t left = (int64_t)g.tokens - t0 - l.row * S;
+            return {left >= S ? ALL : left > 0 ? (1u << (uint32_t)left) - 1 : 0, 0, 0};
+        }
+        const int64_t end = min(t0 + V * S, (int64_t)g.tokens);
+        uint32_t in = 0, first = 0, last = 0;
+        for (uint32_t s = t0 < end ? search(g, t0, offset_of_wave) : g.seqs; s < g.seqs; ++s) {
+            const int64_t a = offset_of_wave(g, s), b = offset_of_wave(g, s + 1);
+            if (a >= end) break;
+            if (b <= a || b <= t0) continue;  // one without tokens
+            const uint32_t lo = (uint32_t)(max(a, t0) - t0), hi = (uint32_t)(min(b, end) - t0);
+            in |= (uint32_t)((1ull << hi) - (1ull << lo));
+            if (a >= t0) first |= 1u << lo;
+            if (b <= end) last |= 1u << (hi - 1);
+            if (b >= end) break;
+        }
+        const uint32_t shift = l.row * S;
+        return {in >> shift & ALL, first >> shift & ALL, last >> shift & ALL};
     }
 
     // The pair of the rows before this one (forward) or behind it (backward) in
@@ -278,9 +313,10 @@ struct Rec {
     template <bool BACK>
     static __device__ __forceinline__ void rows(float (&p)[V], float (&q)[V], float (&ep)[V], float (&eq)[V],
                                                 const Lane& l) {
-        const uint32_t row = BACK ? 3 - l.row : l.row;
-        each<2>([&](auto step) {
-            constexpr int far = 16 << step;
+        const uint32_t row = BACK ? V - 1 - l.row : l.row;
+        static_assert(V == 2, "one step over the rows of lanes");
+        each<1>([&](auto step) {
+            constexpr int far = ROW << step;
             const int from = (int)l.lane + (BACK ? far : -far);
             const bool some = row >= (1u << step);
             each<V>([&](auto c) {
@@ -291,7 +327,7 @@ struct Rec {
                 }
             });
         });
-        const int from = (int)l.lane + (BACK ? 16 : -16);
+        const int from = (int)l.lane + (BACK ? ROW : -ROW);
         each<V>([&](auto c) {
             const float p1 = __shfl(p[c], from & 63), q1 = __shfl(q[c], from & 63);
             ep[c] = row ? p1 : 1.0f;
@@ -306,10 +342,7 @@ struct Rec {
     template <bool BACK>
     static __device__ __forceinline__ void publish(Totals& t, uint32_t wave, const Lane& l, const float (&p)[V],
                                                    const float (&q)[V]) {
-        if (l.row == (BACK ? 0 : 3)) {
-            *(float4*)&t.v[wave][0][l.ch] = make_float4(p[0], p[1], p[2], p[3]);
-            *(float4*)&t.v[wave][1][l.ch] = make_float4(q[0], q[1], q[2], q[3]);
-        }
+        if (l.row == (BACK ? 0 : V - 1)) each<V>([&](auto c) { t.v[wave][0][l.ch + c] = p[c], t.v[wave][1][l.ch + c] = q[c]; });
     }
     // From the state that enters the tile to the one that enters the wave.
     template <bool BACK>
@@ -318,11 +351,8 @@ struct Rec {
         const uint32_t before = BACK ? waves - 1 - wave : wave;
         for (uint32_t k = 0; k < before; ++k) {
             const uint32_t w = BACK ? waves - 1 - k : k;
-            const float4 p = *(const float4*)&t.v[w][0][l.ch], q = *(const float4*)&t.v[w][1][l.ch];
-            h[0] = enter<PACKED>(p.x, q.x, h[0]);
-            h[1] = enter<PACKED>(p.y, q.y, h[1]);
-            h[2] = enter<PACKED>(p.z, q.z, h[2]);
-            h[3] = enter<PACKED>(p.w, q.w, h[3]);
+            const Floats p = *(const Floats*)&t.v[w][0][l.ch], q = *(const Floats*)&t.v[w][1][l.ch];
+            each<V>([&](auto c) { h[c] = enter<PACKED>(p.v[c], q.v[c], h[c]); });
         }
     }
 
@@ -348,8 +378,8 @@ struct Rec {
             lds[l.lane] = entering<PACKED>(g, at, p, q, some ? first[l.lane] : 0.0f);
         }
         __syncthreads();
-        const float4 v = *(const float4*)&lds[l.ch];
-        h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+        const Floats v = *(const Floats*)&lds[l.ch];
+        each<V>([&](auto c) { h[c] = v.v[c]; });
     }
 
     // A packed sequence's row of [sequences][channels].
@@ -385,88 +415,119 @@ struct Rec {
             params(ba, g.bias_a ? g.bias_a + at : nullptr, l);
             params(bx, g.bias_x ? g.bias_x + at : nullptr, l);
             each<V>([&](auto c) {
-                k[c] = -kLog2e * g.rate * softplus(k[c]).value;
-                ba[c] *= -kLog2e;
-                bx[c] *= -kLog2e;
+                // finite, so that a closed gate leaves the state whatever the parameters are
+                k[c] = finite(-kLog2e * g.rate * softplus(k[c]).value);
+                ba[c] = finite(-kLog2e * ba[c]);
+                bx[c] = finite(-kLog2e * bx[c]);
             });
         }
     };
+
+    // What leaves a state as it is: a gate so far closed that a is 1 and b is 0.
+    static __device__ __forceinline__ void nothing(Pack& x, Pack& ga, Pack& gx) {
+        x = gx = Pack{};
+        each<V>([&](auto c) { ga.v[c] = T::down(-__builtin_inff()); });
+    }
+
+    // Of N arrays (x, the gates, the output's gradient) a wave's V S rows, S for each row of
+    // lanes; where only `rows` of them exist, nothing() for those behind.  Token after token of
+    // all arrays, so that the first can be worked on while the others are on their way.
+    template <int N, int S>
+    static __device__ __forceinline__ void fetch_rows(Pack (&to)[N][S], const fg_ssm_view (&v)[N], uint32_t chain,
+                                                      int64_t t0, uint32_t block, const Lane& l, int64_t rows) {
+        const char* p[N];
+        uint32_t step[N], off[N];
+        each<N>([&](auto k) {
+            p[k] = base(v[k], chain, t0, block);
+            step[k] = (uint32_t)v[k].row * (uint32_t)sizeof(raw);
+        });
+        if (rows >= V * S) {
+            each<N>([&](auto k) { off[k] = l.row * S * step[k] + l.off; });
+            each<S>([&](auto j) {
+                each<N>([&](auto k) {
+                    off[k] = fresh(j ? off[k] + step[k] : off[k]);
+                    to[k][j] = fetch(p[k], off[k], l);
+                });
+            });
+        } else {
+            each<S>([&](auto j) {
+                nothing(to[0][j], to[1][j], to[2][j]);
+                if (N > 3) to[N - 1][j] = Pack{};
+                const uint32_t t = l.row * S + j;
+                if (t < rows) each<N>([&](auto k) { to[k][j] = fetch(p[k], t * step[k] + l.off, l); });
+            });
+        }
+    }
 
     static __device__ __forceinline__ void forward(const fg_rec_kargs& g) {
         constexpr int S = FG_REC_SEGMENT(sizeof(raw));
         __shared__ Totals totals;
         __shared__ float4 entered[FG_REC_CHANNELS / 4];
         const Place at = place_of(g);
-        const uint32_t block = at.block, chain = at.chain, tile = at.tile;
+        const uint32_t block = at.block, chain = at.chain;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
+        const int64_t t0 = ((int64_t)at.tile * waves + wave) * (V * S), rows_left = (int64_t)g.tokens - t0;
+        Pack in[3][S];
+        fetch_rows<3, S>(in, {g.x, g.ga, g.gx}, chain, t0, block, l, rows_left);
         Params w;
         w.load(g, block, l);
-        const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
-        {
-            const int64_t t0 = ((int64_t)tile * waves + wave) * (4 * S);
-            const Marks<S> m = marks<S>(g, t0 + l.row * S);
-            float a[S][V], b[S][V], p[V], q[V];
-            const char *px = base(g.x, chain, t0, block), *pa = base(g.ga, chain, t0, block),
-                       *pg = base(g.gx, chain, t0, block);
-            Pack x[S], ga[S], gx[S];
-            each<S>([&](auto j) {
-                if (t0 + l.row * S + j < (int64_t)g.tokens && l.left) {
-                    const uint32_t t = l.row * S + j;
-                    x[j] = fetch(px, (uint32_t)((t * g.x.row + l.ch) * sizeof(raw)), l);
-                    ga[j] = fetch(pa, (uint32_t)((t * g.ga.row + l.ch) * sizeof(raw)), l);
-                    gx[j] = fetch(pg, (uint32_t)((t * g.gx.row + l.ch) * sizeof(raw)), l);
-                }
+        const Marks m = marks<S>(g, t0, l);
+        float a[S][V], b[S][V], p[V], q[V];
+        each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f; });
+        each<S>([&](auto j) {
+            if constexpr (PACKED) {
+                if (!(m.in >> j & 1)) nothing(in[0][j], in[1][j], in[2][j]);
+            }
+            each<V>([&](auto c) {
+                const float r = gate(T::up(in[1][j].v[c]), w.ba[c]), i = gate(T::up(in[2][j].v[c]), w.bx[c]);
+                const Share s = share(w.k[c], r);
+                a[j][c] = s.a;
+                b[j][c] = __builtin_amdgcn_sqrtf(s.m2) * i * T::up(in[0][j].v[c]);
             });
-            each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f; });
-            each<S>([&](auto j) {
-                each<V>([&](auto c) {
-                    const float r = gate(T::up(ga[j].v[c]), w.ba[c]), i = gate(T::up(gx[j].v[c]), w.bx[c]);
-                    const Share s = share(w.k[c], r);
-                    const bool in = m.in >> j & 1;
-                    a[j][c] = in ? s.a : 1.0f;
-                    b[j][c] = in ? __builtin_amdgcn_sqrtf(s.m2) * i * T::up(x[j].v[c]) : 0.0f;
-                });
-                if constexpr (PACKED) {
-                    if (m.first >> j & 1) {
-                        float init[V];
-                        params(init, of(g.initial, g, m.seq[j], block), l);
-                        if (g.check) put(const_cast<float*>(of(inits(g), g, m.seq[j], block)), l, init);
-                        each<V>([&](auto c) { b[j][c] = fmaf(a[j][c], init[c], b[j][c]); });
-                    }
-                }
-                each<V>([&](auto c) {
-                    q[c] = PACKED && (m.first >> j & 1) ? b[j][c] : fmaf(a[j][c], q[c], b[j][c]);
-                    p[c] *= a[j][c];
-                });
+            const bool first = PACKED && (m.first >> j & 1);
+            if (first) {
+                float init[V];
+                const uint32_t s = sequence(g, t0 + l.row * S + j);
+                params(init, of(g.initial, g, s, block), l);
+                if (g.check) put(const_cast<float*>(of(inits(g), g, s, block)), l, init);
+                each<V>([&](auto c) { b[j][c] = fmaf(a[j][c], init[c], b[j][c]); });
+            }
+            each<V>([&](auto c) {
+                q[c] = first ? b[j][c] : fmaf(a[j][c], q[c], b[j][c]);
+                p[c] *= a[j][c];
             });
-            each<V>([&](auto c) { p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast); });
-            float ep[V], eq[V], h[V];
-            rows<false>(p, q, ep, eq, l);
-            publish<false>(totals, wave, l, p, q);
-            __syncthreads();
-            enter_tile<false>(g, at, totals, &entered[0].x, PACKED ? nullptr : of(g.initial, g, chain, block), wave,
-                              waves, l, h);
-            pass<false>(totals, wave, waves, l, h);
-            if (g.check && t0 % FG_REC_CHECK == 0 && l.row == 0 && t0 < (int64_t)g.tokens)
-                put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + at0, l, h);
-            each<V>([&](auto c) { h[c] = enter<PACKED>(ep[c], eq[c], h[c]); });
-            char* po = const_cast<char*>(base(g.out, chain, t0, block));
-            each<S>([&](auto j) {
-                each<V>([&](auto c) {
-                    h[c] = PACKED && (m.first >> j & 1) ? b[j][c] : fmaf(a[j][c], h[c], b[j][c]);
-                });
-                if (m.in >> j & 1) {
-                    store(po, (uint32_t)(((l.row * S + j) * g.out.row + l.ch) * sizeof(raw)), l, h);
-                    if constexpr (PACKED) {
-                        if (g.final && (m.last >> j & 1)) put(const_cast<float*>(of(g.final, g, m.seq[j], block)), l, h);
-                    } else if (g.final && t0 + l.row * S + j + 1 == (int64_t)g.tokens) {
-                        put(const_cast<float*>(of(g.final, g, chain, block)), l, h);
-                    }
-                }
-            });
-            empty(g, g.initial, g.final, block, chain, tile);
+            __builtin_amdgcn_sched_barrier(0);  // tokens mixed would not fit the registers of four waves
+        });
+        each<V>([&](auto c) { p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast); });
+        float ep[V], eq[V], h[V];
+        rows<false>(p, q, ep, eq, l);
+        publish<false>(totals, wave, l, p, q);
+        __syncthreads();
+        enter_tile<false>(g, at, totals, &entered[0].x, PACKED ? nullptr : of(g.initial, g, chain, block), wave, waves,
+                          l, h);
+        pass<false>(totals, wave, waves, l, h);
+        if (g.check && t0 % FG_REC_CHECK == 0 && l.row == 0 && rows_left > 0)
+            put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + (uint64_t)block * FG_REC_CHANNELS, l, h);
+        each<V>([&](auto c) { h[c] = enter<PACKED>(ep[c], eq[c], h[c]); });
+        char* po = const_cast<char*>(base(g.out, chain, t0, block));
+        const uint32_t step = (uint32_t)g.out.row * (uint32_t)sizeof(raw);
+        uint32_t off = l.row * S * step + l.off;
+        each<S>([&](auto j) {
+            const bool first = PACKED && (m.first >> j & 1);
+            each<V>([&](auto c) { h[c] = first ? b[j][c] : fmaf(a[j][c], h[c], b[j][c]); });
+            off = fresh(j ? off + step : off);
+            if (m.in >> j & 1) store(po, off, l, h);
+            if constexpr (PACKED) {
+                if (g.final && (m.last >> j & 1))
+                    put(const_cast<float*>(of(g.final, g, sequence(g, t0 + l.row * S + j), block)), l, h);
+            }
+        });
+        if constexpr (!PACKED) {  // tokens behind the last one left h as it was
+            const int64_t mine = rows_left - l.row * S;
+            if (g.final && mine > 0 && mine <= S) put(const_cast<float*>(of(g.final, g, chain, block)), l, h);
         }
+        empty(g, g.initial, g.final, block, chain, at.tile);
     }
 
     static __device__ __forceinline__ void backward(const fg_rec_kargs& g) {
@@ -478,141 +539,133 @@ struct Rec {
         const uint32_t block = at.block, chain = at.chain, tile = g.tiles - 1 - at.tile;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
+        const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
+        const int64_t t0 = ((int64_t)tile * waves + wave) * (V * S), rows_left = (int64_t)g.tokens - t0;
+        Pack in[4][S];
+        fetch_rows<4, S>(in, {g.x, g.ga, g.gx, g.out}, chain, t0, block, l, rows_left);
         Params w;
         w.load(g, block, l);
-        const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
+        const Marks m = marks<S>(g, t0, l);
+        // Of each token what the gradients go by: mi = m i, e = i x a^2 / m, f = x (1 - i).
+        float a[S][V], r[S][V], mi[S][V], e[S][V], f[S][V], p[V], q[V], rp[V], rq[V];
+        each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f, rq[c] = 0.0f; });
+        each<S>([&](auto j) {
+            const bool first = PACKED && (m.first >> j & 1);
+            if constexpr (PACKED) {
+                if (!(m.in >> j & 1)) {
+                    nothing(in[0][j], in[1][j], in[2][j]);
+                    in[3][j] = Pack{};
+                }
+            }
+            float init[V] = {};
+            if (first) params(init, of(inits(g), g, sequence(g, t0 + l.row * S + j), block), l);
+            each<V>([&](auto c) {
+                const float x = T::up(in[0][j].v[c]), i = gate(T::up(in[2][j].v[c]), w.bx[c]);
+                r[j][c] = gate(T::up(in[1][j].v[c]), w.ba[c]);
+                const Share s = share(w.k[c], r[j][c]);
+                // of a gate so far closed that m^2 is 0, 1 / m is large, not infinite: it meets r, which is 0
+                const float over = __builtin_amdgcn_rsqf(fmaxf(s.m2, 1e-37f));
+                a[j][c] = s.a;
+                mi[j][c] = s.m2 * over * i;
+                e[j][c] = i * x * (s.a * s.a * over);
+                f[j][c] = fmaf(-x, i, x);
+                q[c] = fmaf(a[j][c], first ? init[c] : q[c], mi[j][c] * x);
+                p[c] *= a[j][c];
+            });
+            __builtin_amdgcn_sched_barrier(0);  // tokens mixed would not fit the registers
+        });
+        each<S>([&](auto k) {
+            constexpr int j = S - 1 - k;
+            float end[V] = {};
+            const bool last = PACKED && (m.last >> j & 1);
+            if (last) params(end, of(g.gfinal, g, sequence(g, t0 + l.row * S + j), block), l);
+            each<V>([&](auto c) { rq[c] = a[j][c] * (T::up(in[3][j].v[c]) + (last ? end[c] : rq[c])); });
+        });
+        each<V>([&](auto c) {
+            rp[c] = PACKED && m.last ? -1.0f : fmaxf(p[c], kLeast);
+            p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast);
+        });
+        float ep[V], eq[V], rep[V], req[V], h[V] = {}, d[V];
+        rows<false>(p, q, ep, eq, l);
+        rows<true>(rp, rq, rep, req, l);
+        publish<false>(ta, wave, l, p, q);
+        publish<true>(tb, wave, l, rp, rq);
+        const int64_t first_token = (int64_t)tile * waves * (V * S);
+        if (first_token < (int64_t)g.tokens)
+            params(h, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
+        __syncthreads();
+        pass<false>(ta, wave, waves, l, h);
+        enter_tile<true>(g, at, tb, &entered[0].x, PACKED ? nullptr : of(g.gfinal, g, chain, block), wave, waves, l, d);
+        pass<true>(tb, wave, waves, l, d);
+        each<V>([&](auto c) {
+            h[c] = enter<PACKED>(ep[c], eq[c], h[c]);
+            d[c] = enter<PACKED>(rep[c], req[c], d[c]);
+        });
+        // e becomes a h_{t-1} - e
+        each<S>([&](auto j) {
+            if constexpr (PACKED) {
+                if (m.first >> j & 1) params(h, of(inits(g), g, sequence(g, t0 + l.row * S + j), block), l);
+            }
+            each<V>([&](auto c) {
+                const float kept = a[j][c] * h[c];
+                e[j][c] = kept - e[j][c];
+                h[c] = fmaf(mi[j][c], T::up(in[0][j].v[c]), kept);
+            });
+        });
         float sums[3][V] = {};
-        {
-            const int64_t t0 = ((int64_t)tile * waves + wave) * (4 * S);
-            const Marks<S> m = marks<S>(g, t0 + l.row * S);
-            float a[S][V], b[S][V], p[V], q[V], rp[V], rq[V];
-            const char *px = base(g.x, chain, t0, block), *pa = base(g.ga, chain, t0, block),
-                       *pg = base(g.gx, chain, t0, block), *pd = base(g.out, chain, t0, block);
-            Pack x[S], ga[S], gx[S], dy[S];
-            each<S>([&](auto j) {
-                if (t0 + l.row * S + j < (int64_t)g.tokens && l.left) {
-                    const uint32_t t = l.row * S + j;
-                    x[j] = fetch(px, (uint32_t)((t * g.x.row + l.ch) * sizeof(raw)), l);
-                    ga[j] = fetch(pa, (uint32_t)((t * g.ga.row + l.ch) * sizeof(raw)), l);
-                    gx[j] = fetch(pg, (uint32_t)((t * g.gx.row + l.ch) * sizeof(raw)), l);
-                    dy[j] = fetch(pd, (uint32_t)((t * g.out.row + l.ch) * sizeof(raw)), l);
-                }
-            });
-            each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f, rq[c] = 0.0f; });
-            each<S>([&](auto j) {
-                const bool in = m.in >> j & 1, first = PACKED && (m.first >> j & 1);
-                float init[V] = {};
-                if constexpr (PACKED) {
-                    if (first) params(init, of(inits(g), g, m.seq[j], block), l);
-                }
-                each<V>([&](auto c) {
-                    const float r = gate(T::up(ga[j].v[c]), w.ba[c]), i = gate(T::up(gx[j].v[c]), w.bx[c]);
-                    const Share s = share(w.k[c], r);
-                    a[j][c] = in ? s.a : 1.0f;
-                    b[j][c] = in ? __builtin_amdgcn_sqrtf(s.m2) * i * T::up(x[j].v[c]) : 0.0f;
-                    q[c] = fmaf(a[j][c], first ? init[c] : q[c], b[j][c]);
-                    p[c] *= a[j][c];
-                });
-            });
-            each<S>([&](auto k) {
-                constexpr int j = S - 1 - k;
-                const bool in = m.in >> j & 1, last = PACKED && (m.last >> j & 1);
-                float end[V] = {};
-                if constexpr (PACKED) {
-                    if (last) params(end, of(g.gfinal, g, m.seq[j], block), l);
-                }
-                each<V>([&](auto c) {
-                    const float d = in ? T::up(dy[j].v[c]) : 0.0f;
-                    rq[c] = a[j][c] * (d + (last ? end[c] : rq[c]));
-                });
-            });
+        char* to[3];
+        uint32_t step[3], off[3];
+        const fg_ssm_view* outs[3] = {&g.dx, &g.dga, &g.dgx};
+        each<3>([&](auto k) {
+            to[k] = const_cast<char*>(base(*outs[k], chain, t0, block));
+            step[k] = (uint32_t)outs[k]->row * (uint32_t)sizeof(raw);
+            off[k] = (l.row * S + S - 1) * step[k] + l.off;
+        });
+        each<S>([&](auto k) {
+            constexpr int j = S - 1 - k;
+            each<3>([&](auto n) { off[n] = fresh(k ? off[n] - step[n] : off[n]); });
+            if constexpr (PACKED) {
+                if (m.last >> j & 1) params(d, of(g.gfinal, g, sequence(g, t0 + l.row * S + j), block), l);
+            }
+            float o[3][V];
             each<V>([&](auto c) {
-                rp[c] = PACKED && m.last ? -1.0f : fmaxf(p[c], kLeast);
-                p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast);
+                const float dh = T::up(in[3][j].v[c]) + d[c], log = dh * e[j][c];
+                o[0][c] = dh * mi[j][c];
+                o[1][c] = log * (w.k[c] * kLn2) * fmaf(-r[j][c], r[j][c], r[j][c]);
+                o[2][c] = o[0][c] * f[j][c];
+                sums[0][c] = fmaf(log, r[j][c], sums[0][c]);
+                sums[1][c] += o[1][c];
+                sums[2][c] += o[2][c];
+                d[c] = a[j][c] * dh;
             });
-            float ep[V], eq[V], rep[V], req[V], h[V] = {}, d[V];
-            rows<false>(p, q, ep, eq, l);
-            rows<true>(rp, rq, rep, req, l);
-            publish<false>(ta, wave, l, p, q);
-            publish<true>(tb, wave, l, rp, rq);
-            const int64_t first_token = (int64_t)tile * waves * (4 * S);
-            if (first_token < (int64_t)g.tokens)
-                params(h, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
-            __syncthreads();
-            pass<false>(ta, wave, waves, l, h);
-            enter_tile<true>(g, at, tb, &entered[0].x, PACKED ? nullptr : of(g.gfinal, g, chain, block), wave, waves, l,
-                             d);
-            pass<true>(tb, wave, waves, l, d);
-            each<V>([&](auto c) {
-                h[c] = enter<PACKED>(ep[c], eq[c], h[c]);
-                d[c] = enter<PACKED>(rep[c], req[c], d[c]);
-            });
-            // b becomes a h_{t-1}
-            each<S>([&](auto j) {
-                if constexpr (PACKED) {
-                    if (m.first >> j & 1) params(h, of(inits(g), g, m.seq[j], block), l);
-                }
-                each<V>([&](auto c) {
-                    const float kept = a[j][c] * h[c];
-                    h[c] = fmaf(a[j][c], h[c], b[j][c]);
-                    b[j][c] = kept;
+            if (m.in >> j & 1) {
+                each<3>([&](auto n) {
+                    if (outs[n]->p) store(to[n], off[n], l, o[n]);
                 });
-            });
-            char *qx = const_cast<char*>(base(g.dx, chain, t0, block)), *qa = const_cast<char*>(base(g.dga, chain, t0, block)),
-                 *qg = const_cast<char*>(base(g.dgx, chain, t0, block));
-            each<S>([&](auto k) {
-                constexpr int j = S - 1 - k;
-                if constexpr (PACKED) {
-                    if (m.last >> j & 1) params(d, of(g.gfinal, g, m.seq[j], block), l);
-                }
-                if (m.in >> j & 1) {
-                    float gx_[V], ga_[V], dx_[V];
-                    each<V>([&](auto c) {
-                        const float dh = T::up(dy[j].v[c]) + d[c], xv = T::up(x[j].v[c]);
-                        const float r = gate(T::up(ga[j].v[c]), w.ba[c]), i = gate(T::up(gx[j].v[c]), w.bx[c]);
-                        const Share s = share(w.k[c], r);
-                        // 1 / m, of a gate so far closed that m is 0: 0, as what it is multiplied with tends to
-                        const float inv = s.m2 > 1.2e-38f ? __builtin_amdgcn_rsqf(s.m2) : 0.0f;
-                        const float mi = s.m2 * inv * i;
-                        const float log = dh * fmaf(-i * xv, s.a * s.a * inv, b[j][c]);
-                        dx_[c] = dh * mi;
-                        ga_[c] = log * w.k[c] * kLn2 * r * (1.0f - r);
-                        gx_[c] = dx_[c] * xv * (1.0f - i);
-                        sums[0][c] = fmaf(log, r, sums[0][c]);
-                        sums[1][c] += ga_[c];
-                        sums[2][c] += gx_[c];
-                        d[c] = s.a * dh;
-                    });
-                    const uint32_t t = l.row * S + j;
-                    if (g.dx.p) store(qx, (uint32_t)((t * g.dx.row + l.ch) * sizeof(raw)), l, dx_);
-                    if (g.dga.p) store(qa, (uint32_t)((t * g.dga.row + l.ch) * sizeof(raw)), l, ga_);
-                    if (g.dgx.p) store(qg, (uint32_t)((t * g.dgx.row + l.ch) * sizeof(raw)), l, gx_);
-                    if constexpr (PACKED) {
-                        if (g.ginitial && (m.first >> j & 1)) put(const_cast<float*>(of(g.ginitial, g, m.seq[j], block)), l, d);
-                    } else if (g.ginitial && t0 + t == 0) {
-                        put(const_cast<float*>(of(g.ginitial, g, chain, block)), l, d);
-                    }
-                }
-            });
-            empty(g, g.gfinal, g.ginitial, block, chain, tile);
-        }
+            }
+            if constexpr (PACKED) {
+                if (g.ginitial && (m.first >> j & 1))
+                    put(const_cast<float*>(of(g.ginitial, g, sequence(g, t0 + l.row * S + j), block)), l, d);
+            }
+        });
+        if (!PACKED && g.ginitial && t0 == 0 && l.row == 0 && rows_left > 0)
+            put(const_cast<float*>(of(g.ginitial, g, chain, block)), l, d);
+        empty(g, g.gfinal, g.ginitial, block, chain, tile);
         // the parameters' sums: over the rows of a wave, then over the waves
         __syncthreads();
-        float* to = &both[0].v[0][0][0];  // [wave][3][channel]
+        float* all = &both[0].v[0][0][0];  // [wave][3][channel]
         static_assert(sizeof(both) >= 4 * 3 * FG_REC_WAVES * FG_REC_CHANNELS, "the sums fit");
         each<3>([&](auto k) {
             each<V>([&](auto c) {
-                float v = sums[k][c];
-                v += __shfl_xor(v, 16);
-                v += __shfl_xor(v, 32);
-                if (l.row == 0) to[(wave * 3 + k) * FG_REC_CHANNELS + l.ch + c] = v;
+                const float v = sums[k][c] + __shfl_xor(sums[k][c], ROW);
+                if (l.row == 0) all[(wave * 3 + k) * FG_REC_CHANNELS + l.ch + c] = v;
             });
         });
         __syncthreads();
-        for (uint32_t e = threadIdx.x; e < 3 * FG_REC_CHANNELS; e += blockDim.x) {
-            const uint32_t k = e / FG_REC_CHANNELS, ch = e % FG_REC_CHANNELS;
+        for (uint32_t n = threadIdx.x; n < 3 * FG_REC_CHANNELS; n += blockDim.x) {
+            const uint32_t k = n / FG_REC_CHANNELS, ch = n % FG_REC_CHANNELS;
             float v = 0.0f;
-            for (uint32_t u = 0; u < waves; ++u) v += to[(u * 3 + k) * FG_REC_CHANNELS + ch];
+            for (uint32_t u = 0; u < waves; ++u) v += all[(u * 3 + k) * FG_REC_CHANNELS + ch];
             if (at0 + ch < g.channels) g.part[(((uint64_t)chain * g.tiles + tile) * 3 + k) * g.channels + at0 + ch] = v;
         }
     }

@@ -117,28 +117,32 @@ RecurrencePlan::RecurrencePlan(const HipBackend::DeviceHandle& dev, const Recurr
         backward_[wide] = k.get((int)s.dtype, "fg_rec_back_" + tail + (wide ? "" : "_any"));
     }
     reduce_ = k.get((int)s.dtype, "fg_rec_reduce");
-    ahead_ = chain(FG_REC_SEGMENT(kBytes[s.dtype]));
+    ahead_ = chain(false);
 }
 
-// Tiles of all chains, a workgroup for each 64 channels.
-uint64_t RecurrencePlan::places(uint32_t segment) const {
-    const uint64_t tiles = std::max<uint64_t>(1, ceil_div(rows_, 4 * segment * waves(segment)));
+uint32_t RecurrencePlan::wave_tokens(bool back) const {
+    return FG_REC_LANE_CHANNELS * (back ? FG_REC_BACK_SEGMENT : FG_REC_SEGMENT(kBytes[s_.dtype]));
+}
+
+// As many as the rows of a chain take.
+uint32_t RecurrencePlan::waves(bool back) const {
+    return (uint32_t)std::min<uint64_t>(back ? FG_REC_BACK_WAVES : FG_REC_WAVES,
+                                        std::max<uint64_t>(1, ceil_div(rows_, wave_tokens(back))));
+}
+
+uint64_t RecurrencePlan::places(bool back) const {
+    const uint64_t tiles = std::max<uint64_t>(1, ceil_div(rows_, wave_tokens(back) * waves(back)));
     const uint64_t n = (uint64_t)size_of("recurrence", "launch", {(int64_t)ceil_div(s_.channels, FG_REC_CHANNELS),
                                                                   (int64_t)chains_, (int64_t)tiles});
-    if (n > 0xffffffffull / (64 * waves(segment))) invalid("recurrence: too large for one launch");
+    if (n > 0xffffffffull / (64 * waves(back))) invalid("recurrence: too large for one launch");
     return n;
 }
 
 // None where every chain is one tile.
-Buffer<char, HipBackend> RecurrencePlan::chain(uint32_t segment) const {
-    const uint64_t n = places(segment);
+Buffer<char, HipBackend> RecurrencePlan::chain(bool back) const {
+    const uint64_t n = places(back);
     if (n <= ceil_div(s_.channels, FG_REC_CHANNELS) * chains_) return {};
     return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(n));
-}
-
-// Of a workgroup: as many as the rows of a chain take.
-uint32_t RecurrencePlan::waves(uint32_t segment) const {
-    return (uint32_t)std::min<uint64_t>(FG_REC_WAVES, std::max<uint64_t>(1, ceil_div(rows_, 4 * segment)));
 }
 
 size_t RecurrencePlan::checkpoint_bytes() const {
@@ -148,13 +152,12 @@ size_t RecurrencePlan::checkpoint_bytes() const {
 
 void RecurrencePlan::info(fg_recurrence_plan_info* out) {
     std::lock_guard<std::mutex> lock(mu_);
-    out->forward_tokens = 4 * FG_REC_SEGMENT(kBytes[s_.dtype]) * waves(FG_REC_SEGMENT(kBytes[s_.dtype]));
-    out->backward_tokens = 4 * FG_REC_BACK_SEGMENT * waves(FG_REC_BACK_SEGMENT);
+    out->forward_tokens = wave_tokens(false) * waves(false);
+    out->backward_tokens = wave_tokens(true) * waves(true);
     out->workspace_bytes = (int64_t)(part_.bytes() + ahead_.bytes() + back_.bytes());
 }
 
-fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in, uint32_t segment,
-                                  const Buffer<char, HipBackend>& chain) const {
+fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in, bool back) const {
     if (s_.packed && !in.offsets) invalid(std::string(op) + ": packed sequences need offsets");
     if (!s_.packed && in.offsets) invalid(std::string(op) + ": offsets are for packed sequences");
     fg_rec_kargs g{};
@@ -169,18 +172,20 @@ fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in
     g.channels = (uint32_t)s_.channels;
     g.blocks = (uint32_t)ceil_div(s_.channels, FG_REC_CHANNELS);
     g.rate = (float)s_.rate;
-    const uint64_t n = places(segment), across = (uint64_t)g.blocks * g.chains;
+    const uint64_t n = places(back), across = (uint64_t)g.blocks * g.chains;
     g.tiles = across ? (uint32_t)(n / across) : 1;
     g.parts = chains_ * g.tiles;
-    g.chain = (unsigned long long*)chain.data();
+    g.chain = (unsigned long long*)(back ? back_ : ahead_).data();
     g.over_places = n ? ~0ull / n : 0;
+    g.over_across = across ? (uint32_t)(0xffffffffull / across) : 0;
+    g.over_blocks = g.blocks ? 0xffffffffu / g.blocks : 0;
     return g;
 }
 
 void RecurrencePlan::forward(const fg_recurrence_forward_args& a, hipStream_t stream) const {
     const char* op = "recurrence forward";
-    const uint32_t es = kBytes[s_.dtype], segment = FG_REC_SEGMENT(es);
-    fg_rec_kargs g = base(op, a.in, segment, ahead_);
+    const uint32_t es = kBytes[s_.dtype];
+    fg_rec_kargs g = base(op, a.in, false);
     Arrays all(op, s_.packed ? 1 : s_.sequences, rows_, es);
     const int64_t state = 4 * s_.sequences * s_.channels;
     g.x = all.rows("x", a.in.x, s_.channels, false);
@@ -198,18 +203,18 @@ void RecurrencePlan::forward(const fg_recurrence_forward_args& a, hipStream_t st
     g.initial = a.initial;
     g.final = a.final;
     g.check = (float*)a.checkpoints;
-    bool wide = g.channels % 4 == 0;
-    for (const fg_ssm_view* v : {&g.x, &g.ga, &g.gx, &g.out}) wide = wide && vector_rows(*v, 4, es);
+    bool wide = g.channels % FG_REC_LANE_CHANNELS == 0;
+    for (const fg_ssm_view* v : {&g.x, &g.ga, &g.gx, &g.out}) wide = wide && vector_rows(*v, FG_REC_LANE_CHANNELS, es);
     for (const float* p : {g.decay, g.bias_a, g.bias_x, g.initial, (const float*)g.final, (const float*)g.check})
-        wide = wide && vector_ptr(p, 16);
+        wide = wide && vector_ptr(p, 4 * FG_REC_LANE_CHANNELS);
     void* args[] = {&g};
-    launch(dev_, stream, forward_[wide], (uint64_t)g.blocks * g.chains * g.tiles, 64 * waves(segment), args, op);
+    launch(dev_, stream, forward_[wide], (uint64_t)g.blocks * g.chains * g.tiles, 64 * waves(false), args, op);
 }
 
 void RecurrencePlan::backward(const fg_recurrence_backward_args& a, hipStream_t stream) {
     const char* op = "recurrence backward";
-    const uint32_t es = kBytes[s_.dtype], segment = FG_REC_BACK_SEGMENT;
-    fg_rec_kargs g = base(op, a.in, segment, back_);
+    const uint32_t es = kBytes[s_.dtype];
+    fg_rec_kargs g = base(op, a.in, true);
     Arrays all(op, s_.packed ? 1 : s_.sequences, rows_, es);
     const int64_t state = 4 * s_.sequences * s_.channels;
     g.x = all.rows("x", a.in.x, s_.channels, false);
@@ -240,18 +245,18 @@ void RecurrencePlan::backward(const fg_recurrence_backward_args& a, hipStream_t 
         if (!part_.data() && chains_) {
             refuse_capture(op, dev_, stream);
             size_of(op, "workspace", {4, 3, s_.channels, (int64_t)g.parts});
-            back_ = chain(segment);
+            back_ = chain(true);
             part_ = Buffer<float, HipBackend>(dev_, 3 * (uint64_t)s_.channels * g.parts);
         }
     }
     g.chain = (unsigned long long*)back_.data();
     g.part = part_.data();
-    bool wide = g.channels % 4 == 0;
-    for (const fg_ssm_view* v : {&g.x, &g.ga, &g.gx, &g.out, &g.dx, &g.dga, &g.dgx}) wide = wide && vector_rows(*v, 4, es);
+    bool wide = g.channels % FG_REC_LANE_CHANNELS == 0;
+    for (const fg_ssm_view* v : {&g.x, &g.ga, &g.gx, &g.out, &g.dx, &g.dga, &g.dgx}) wide = wide && vector_rows(*v, FG_REC_LANE_CHANNELS, es);
     for (const float* p : {g.decay, g.bias_a, g.bias_x, g.gfinal, (const float*)g.ginitial, (const float*)g.check})
-        wide = wide && vector_ptr(p, 16);
+        wide = wide && vector_ptr(p, 4 * FG_REC_LANE_CHANNELS);
     void* args[] = {&g};
-    if (chains_) launch(dev_, stream, backward_[wide], (uint64_t)g.blocks * g.chains * g.tiles, 64 * waves(segment), args, op);
+    if (chains_) launch(dev_, stream, backward_[wide], (uint64_t)g.blocks * g.chains * g.tiles, 64 * waves(true), args, op);
     if (g.gdecay || g.gbias_a || g.gbias_x) launch(dev_, stream, reduce_, ceil_div(3 * (uint64_t)g.channels, 256), 256, args, op);
 }
 

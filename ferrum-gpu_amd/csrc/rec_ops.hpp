@@ -38,11 +38,13 @@ public:
     void backward(const fg_recurrence_backward_args& a, hipStream_t stream);
 
 private:
-    uint32_t waves(uint32_t segment) const;
-    uint64_t places(uint32_t segment) const;
-    Buffer<char, HipBackend> chain(uint32_t segment) const;
-    fg_rec_kargs base(const char* op, const fg_recurrence_inputs& in, uint32_t segment,
-                      const Buffer<char, HipBackend>& chain) const;
+    // Of a pass, which has kernels of its own: tokens of a wave, waves of a
+    // workgroup, tiles over all chains and channels, and what they pass on.
+    uint32_t wave_tokens(bool back) const;
+    uint32_t waves(bool back) const;
+    uint64_t places(bool back) const;
+    Buffer<char, HipBackend> chain(bool back) const;
+    fg_rec_kargs base(const char* op, const fg_recurrence_inputs& in, bool back) const;
     HipBackend::DeviceHandle dev_;
     fg_recurrence_shape s_;
     uint64_t chains_, rows_;  // chains of so many rows: dense, the sequences; packed, one
