@@ -16,10 +16,11 @@
 
 /* Tiles whose pairs a workgroup composes itself, see rec_scan.hpp. */
 #define FG_REC_GROUP 4
-/* What a plan's tiles pass on: 8-byte words, first the tickets drawn, behind them for
- * each tile FG_REC_WORDS of FG_REC_CHANNELS words. */
+/* What a plan's tiles pass on: for each chain of 64 channels the tickets drawn, in a line
+ * of 64 bytes of its own, and behind all of them for each tile FG_REC_WORDS of
+ * FG_REC_CHANNELS 8-byte words. */
 #define FG_REC_WORDS 3
-#define FG_REC_CHAIN_BYTES(places) (64 + 8ull * FG_REC_WORDS * FG_REC_CHANNELS * (places))
+#define FG_REC_CHAIN_BYTES(across, tiles) ((across) * (64 + 8ull * FG_REC_WORDS * FG_REC_CHANNELS * (tiles)))
 
 typedef struct {
     fg_ssm_view x, ga, gx, out; /* backward: out is the output's gradient */
@@ -32,8 +33,8 @@ typedef struct {
     float* check;           /* [chains][checks][channels], states before each FG_REC_CHECK tokens;
                                packed, behind them: [sequences][channels] initial states */
     float* part;            /* [parts][3][channels] */
-    unsigned long long* chain; /* FG_REC_CHAIN_BYTES(tiles * chains * blocks); null where a chain is one tile */
-    uint64_t over_places;   /* (2^64 - 1) / (tiles * chains * blocks) */
+    unsigned long long* chain; /* FG_REC_CHAIN_BYTES(chains * blocks, tiles); null where a chain is one tile */
+    uint64_t over_tiles;    /* (2^64 - 1) / tiles */
     uint32_t over_across, over_blocks; /* (2^32 - 1) / (chains * blocks), / blocks */
     uint64_t tokens;        /* of a chain: a dense sequence's, packed those of all */
     uint64_t checks;        /* of a chain */

@@ -20,11 +20,12 @@
 // its pair; a tile composes those of the tiles before it in its group of
 // FG_REC_GROUP and the state that leaves the group before, which that group's last
 // tile writes: from left to right, so that a result does not depend on who was
-// first.  Workgroups take their tiles by a ticket, first tiles first: who waits does
-// so for workgroups that hold earlier tickets, and of those that hold one the
-// earliest waits for nobody, so every wait ends.  The tickets count on from launch
-// to launch, and their number gives the tag: nothing has to be cleared between
-// launches, also when a graph replays them.
+// first.  A chain's workgroups take its tiles by a ticket, first tiles first: who waits
+// does so for workgroups that hold earlier tickets of the chain, and of those that
+// hold one the earliest waits for nobody, so every wait ends.  The tickets count on from
+// launch to launch, and their number gives the tag: nothing has to be cleared
+// between launches, also when a graph replays them.  (A ticket for all chains, taken
+// 512 times at the start, kept the last workgroup waiting for 8 us.)
 //
 // Packed sequences are one chain of rows: a sequence's first token takes its
 // initial state in place of the one before it.
@@ -87,33 +88,32 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t ov
 }
 __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
     const uint32_t across = g.blocks * g.chains;
-    uint32_t at = blockIdx.x, tag = 0;
-    if (g.chain) {
-        __shared__ unsigned long long ticket;
-        if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(g.chain, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        const uint64_t mine = (uint64_t)uniform((int64_t)ticket), places = (uint64_t)across * g.tiles;
-        uint64_t launch = __umul64hi(mine, g.over_places);  // mine / places, or one less
-        uint64_t rest = mine - launch * places;
-        if (rest >= places) {
-            rest -= places;
-            ++launch;
-        }
-        at = (uint32_t)rest;
-        tag = (uint32_t)launch << 1 | 1;  // never 0, which memory starts with
-    }
     Place p;
     uint32_t rest;
-    p.tile = quotient(at, across, g.over_across, rest);
+    p.tile = quotient(blockIdx.x, across, g.over_across, rest);
     p.chain = quotient(rest, g.blocks, g.over_blocks, p.block);
-    p.tag = tag;
+    p.tag = 0;
+    if (g.chain) {
+        __shared__ unsigned long long ticket;
+        if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(g.chain + 8ull * rest, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const uint64_t mine = (uint64_t)uniform((int64_t)ticket);
+        uint64_t launch = __umul64hi(mine, g.over_tiles);  // mine / tiles, or one less
+        uint64_t tile = mine - launch * g.tiles;
+        if (tile >= g.tiles) {
+            tile -= g.tiles;
+            ++launch;
+        }
+        p.tile = (uint32_t)tile;
+        p.tag = (uint32_t)launch << 1 | 1;  // never 0, which memory starts with
+    }
     return p;
 }
 
 // A tile's words; the same for all lanes.
 __device__ __forceinline__ char* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
-    const uint64_t place = ((uint64_t)tile * g.chains + p.chain) * g.blocks + p.block;
-    return (char*)g.chain + 64 + uniform((int64_t)(place * (8 * FG_REC_WORDS * FG_REC_CHANNELS)));
+    const uint64_t across = (uint64_t)g.blocks * g.chains, place = tile * across + (uint64_t)p.chain * g.blocks + p.block;
+    return (char*)g.chain + uniform((int64_t)(64 * across + place * (8 * FG_REC_WORDS * FG_REC_CHANNELS)));
 }
 // Word `which` of a lane's channel.
 __device__ __forceinline__ void tell(char* at, int which, uint32_t lane, uint32_t tag, float v) {

@@ -140,9 +140,9 @@ uint64_t RecurrencePlan::places(bool back) const {
 
 // None where every chain is one tile.
 Buffer<char, HipBackend> RecurrencePlan::chain(bool back) const {
-    const uint64_t n = places(back);
-    if (n <= ceil_div(s_.channels, FG_REC_CHANNELS) * chains_) return {};
-    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(n));
+    const uint64_t n = places(back), across = ceil_div(s_.channels, FG_REC_CHANNELS) * chains_;
+    if (n <= across) return {};
+    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(across, n / across));
 }
 
 size_t RecurrencePlan::checkpoint_bytes() const {
@@ -176,7 +176,7 @@ fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in
     g.tiles = across ? (uint32_t)(n / across) : 1;
     g.parts = chains_ * g.tiles;
     g.chain = (unsigned long long*)(back ? back_ : ahead_).data();
-    g.over_places = n ? ~0ull / n : 0;
+    g.over_tiles = ~0ull / g.tiles;
     g.over_across = across ? (uint32_t)(0xffffffffull / across) : 0;
     g.over_blocks = g.blocks ? 0xffffffffu / g.blocks : 0;
     return g;
