@@ -21,6 +21,7 @@ typedef struct {
     uint32_t group_lanes;              /* lanes that share a scale; 0: a row does */
     uint32_t drop;                     /* kept where the 32 bits are at least this; 0: no dropout */
     uint32_t drop_all;
+    uint32_t stream;                   /* store past the caches */
     float keep;                        /* 1 / (1 - p) */
     float eps, over_width;
 } fg_norm_kargs;
@@ -30,7 +31,7 @@ typedef struct {
     void* out;
     const int64_t* counter;
     uint64_t n, seed, offset;
-    uint32_t drop, drop_all;
+    uint32_t drop, drop_all, stream;
     float keep;
 } fg_dropout_kargs;
 

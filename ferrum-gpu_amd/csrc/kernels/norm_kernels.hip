@@ -5,13 +5,17 @@
 
 using namespace fg::norm;
 
-#define FG_NORM_ONE(NAME, T, C, TEAM)                                                                           \
-    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS) void fg_norm_##NAME##_c##C##_t##TEAM(fg_norm_kargs g) { \
-        Rows<T, C, TEAM>::forward(g);                                                                          \
+// _any: for widths that are not whole chunks.
+#define FG_NORM_FORM(NAME, T, C, TEAM, SUFFIX, EVEN)                                                            \
+    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS)                                                    \
+    void fg_norm_##NAME##_c##C##_t##TEAM##SUFFIX(fg_norm_kargs g) {                                            \
+        Rows<T, C, TEAM, EVEN>::forward(g);                                                                    \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS) void fg_norm_back_##NAME##_c##C##_t##TEAM(fg_norm_kargs g) { \
-        Rows<T, C, TEAM>::backward(g);                                                                         \
+    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS)                                                    \
+    void fg_norm_back_##NAME##_c##C##_t##TEAM##SUFFIX(fg_norm_kargs g) {                                       \
+        Rows<T, C, TEAM, EVEN>::backward(g);                                                                   \
     }
+#define FG_NORM_ONE(NAME, T, C, TEAM) FG_NORM_FORM(NAME, T, C, TEAM, , true) FG_NORM_FORM(NAME, T, C, TEAM, _any, false)
 #define FG_NORM_TYPE(NAME, T)                                                                                   \
     FG_NORM_ONE(NAME, T, 1, 64)                                                                                 \
     FG_NORM_ONE(NAME, T, 2, 64)                                                                                 \

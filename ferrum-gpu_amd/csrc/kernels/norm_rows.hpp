@@ -32,8 +32,20 @@ using namespace ssm;
 constexpr float kMost = 448.0f;            // e4m3's largest
 constexpr float kLeast = 7.888609e-31f;    // 2^-100: what 448 / m is taken of at least
 
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t HalfWords __attribute__((ext_vector_type(2), aligned(1)));
+
+// A store past the caches.  The statement behind it keeps the compiler from making one
+// ordinary store of this one and of that on the branch's other side.
+template <class W>
+__device__ __forceinline__ void past(W v, W* to) {
+    __builtin_nontemporal_store(v, to);
+    asm volatile("; past the caches");
+}
+
 // Chunks of 16 bytes at any address of their elements: the GPU's loads and stores take them.
-template <class T>
+// EVEN: all of them are whole.
+template <class T, bool EVEN>
 struct Chunk {
     using raw = typename T::raw;
     static constexpr int E = 16 / sizeof(raw);
@@ -50,16 +62,18 @@ struct Chunk {
     static __device__ __forceinline__ Raw load(const void* p, int64_t at, uint32_t n) {
         const raw* from = (const raw*)p + at;
         Raw r;
-        if (n >= E) return *(const Raw*)from;
+        if (EVEN || n >= E) return *(const Raw*)from;
         each<E>([&](auto i) { r.v[i] = i < n ? from[i] : raw(0); });
         return r;
     }
-    static __device__ __forceinline__ void store(void* p, int64_t at, uint32_t n, const float (&x)[E]) {
+    static __device__ __forceinline__ void store(void* p, int64_t at, uint32_t n, const float (&x)[E],
+                                                 uint32_t stream) {
         raw* to = (raw*)p + at;
         Raw r;
         each<E>([&](auto i) { r.v[i] = T::down(x[i]); });
-        if (n >= E) {
-            *(Raw*)to = r;
+        if (EVEN || n >= E) {
+            if (stream) past(__builtin_bit_cast(Words, r), (Words*)to);
+            else *(Raw*)to = r;
         } else {
             each<E>([&](auto i) {
                 if (i < n) to[i] = r.v[i];
@@ -69,22 +83,27 @@ struct Chunk {
     static __device__ __forceinline__ void floats(float (&x)[E], const float* p, uint32_t at, uint32_t n) {
         if (!p) {
             each<E>([&](auto i) { x[i] = 1.0f; });
-        } else if (n >= E) {
+        } else if (EVEN || n >= E) {
             const Floats f = *(const Floats*)(p + at);
             each<E>([&](auto i) { x[i] = f.v[i]; });
         } else {
             each<E>([&](auto i) { x[i] = i < n ? p[at + i] : 0.0f; });
         }
     }
-    static __device__ __forceinline__ void store8(void* p, int64_t at, uint32_t n, const float (&x)[E]) {
+    static __device__ __forceinline__ void store8(void* p, int64_t at, uint32_t n, const float (&x)[E], uint32_t stream) {
         uint8_t* to = (uint8_t*)p + at;
         Bytes b;
         each<E / 4>([&](auto i) {
             int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
             b.v[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
         });
-        if (n >= E) {
-            *(Bytes*)to = b;
+        if (EVEN || n >= E) {
+            if constexpr (E == 8) {
+                if (stream) past(__builtin_bit_cast(HalfWords, b), (HalfWords*)to);
+                else *(Bytes*)to = b;
+            } else {
+                *(Bytes*)to = b;
+            }
         } else {
             each<E>([&](auto i) {
                 if (i < n) to[i] = (uint8_t)(b.v[i / 4] >> (8 * (i % 4)));
@@ -132,9 +151,9 @@ __device__ __forceinline__ void over_team(float& a, float& b, float2 (&lds)[FG_N
 }
 
 // C: chunks of a thread; 0: any number of them, read again.
-template <class T, int C, int TEAM>
+template <class T, int C, int TEAM, bool EVEN>
 struct Rows {
-    using Io = Chunk<T>;
+    using Io = Chunk<T, EVEN>;
     using Raw = typename Io::Raw;
     static constexpr int E = Io::E, TEAMS = FG_NORM_THREADS / TEAM, KEPT = C ? C : 1;
 
@@ -182,11 +201,11 @@ struct Rows {
                 if constexpr (C == 0) Io::floats(w[k], g.weight, col, n);
                 value(g, row, col, n, numbers, v[k]);
                 each<E>([&](auto i) {
-                    if (i >= n) v[k][i] = 0.0f;  // a dropped place beyond the row holds nothing else
+                    if (!EVEN && i >= n) v[k][i] = 0.0f;  // a dropped place beyond the row holds nothing else
                     squares = fmaf(v[k][i], v[k][i], squares);
                     most = fmaxf(most, fabsf(v[k][i] * w[k][i]));
                 });
-                if (g.sum.p && C) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k]);
+                if (g.sum.p && C) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k], g.stream);
             });
             over_team<TEAM, true>(squares, most, lds[turn]);
             const float s = __builtin_amdgcn_rsqf(fmaf(squares, g.over_width, g.eps));
@@ -198,19 +217,19 @@ struct Rows {
                     if (some && n) {
                         Io::floats(w[k], g.weight, col, n);
                         value(g, row, col, n, numbers, v[k]);
-                        if (g.sum.p) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k]);
+                        if (g.sum.p) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k], g.stream);
                     }
                 }
                 float y[E];
                 if (!g.scales) {
                     each<E>([&](auto i) { y[i] = v[k][i] * s * w[k][i]; });
-                    if (some && n) Io::store(g.out.p, (int64_t)row * g.out.row + col, n, y);
+                    if (some && n) Io::store(g.out.p, (int64_t)row * g.out.row + col, n, y, g.stream);
                     return;
                 }
                 float m = most;
                 if (g.group_lanes) {
                     m = 0.0f;
-                    each<E>([&](auto i) { m = fmaxf(m, i < n ? fabsf(v[k][i] * w[k][i]) : 0.0f); });
+                    each<E>([&](auto i) { m = fmaxf(m, EVEN || i < n ? fabsf(v[k][i] * w[k][i]) : 0.0f); });
                     for (uint32_t far = 1; far < g.group_lanes; far *= 2) m = fmaxf(m, __shfl_xor(m, far));
                     if (some && n && (threadIdx.x & (g.group_lanes - 1)) == 0)
                         g.scales[row * g.groups + col / (g.group_lanes * E)] =
@@ -218,7 +237,7 @@ struct Rows {
                 }
                 const float up = kMost / fmaxf(m, kLeast);
                 each<E>([&](auto i) { y[i] = v[k][i] * w[k][i] * up; });
-                if (some && n) Io::store8(g.out.p, (int64_t)row * g.out.row + col, n, y);
+                if (some && n) Io::store8(g.out.p, (int64_t)row * g.out.row + col, n, y, g.stream);
             });
         }
     }
@@ -249,7 +268,7 @@ struct Rows {
                 load(k, col, n);
                 each<E>([&](auto i) {
                     squares = fmaf(u[k][i], u[k][i], squares);
-                    if (i < n) along = fmaf(dy[k][i] * w[k][i], u[k][i], along);
+                    if (EVEN || i < n) along = fmaf(dy[k][i] * w[k][i], u[k][i], along);
                 });
             });
             over_team<TEAM, false>(squares, along, lds[turn]);
@@ -264,10 +283,10 @@ struct Rows {
                     const Raw r = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
                     each<E>([&](auto i) { dv[i] += T::up(r.v[i]); });
                 }
-                if (g.dresidual.p) Io::store(g.dresidual.p, (int64_t)row * g.dresidual.row + col, n, dv);
+                if (g.dresidual.p) Io::store(g.dresidual.p, (int64_t)row * g.dresidual.row + col, n, dv, g.stream);
                 if (g.dx.p) {
                     if (g.drop) Io::drop(dv, g.seed, numbers, row * g.width + col, g.drop, g.drop_all, g.keep);
-                    Io::store(g.dx.p, (int64_t)row * g.dx.row + col, n, dv);
+                    Io::store(g.dx.p, (int64_t)row * g.dx.row + col, n, dv, g.stream);
                 }
                 if constexpr (C > 0) {
                     each<E>([&](auto i) { dw[k][i] = fmaf(dy[k][i], u[k][i] * s, dw[k][i]); });
@@ -304,7 +323,7 @@ __device__ __forceinline__ void reduce(const float* part, float* to, uint32_t wi
 
 template <class T>
 __device__ __forceinline__ void dropout(const fg_dropout_kargs& g) {
-    using Io = Chunk<T>;
+    using Io = Chunk<T, false>;
     constexpr int E = Io::E;
     const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
     const uint64_t step = (uint64_t)gridDim.x * blockDim.x * E;
@@ -314,7 +333,7 @@ __device__ __forceinline__ void dropout(const fg_dropout_kargs& g) {
         float v[E];
         each<E>([&](auto i) { v[i] = T::up(x.v[i]); });
         if (g.drop) Io::drop(v, g.seed, numbers, at, g.drop, g.drop_all, g.keep);
-        Io::store(g.out, (int64_t)at, n, v);
+        Io::store(g.out, (int64_t)at, n, v, g.stream);
     }
 }
 

@@ -5,23 +5,25 @@
 
 using namespace fg::rec;
 
-// _any: for any stride, alignment and number of channels.
-#define FG_REC_ONE(NAME, T, SUFFIX, WIDE, PACKED)                                                               \
+// _any: for any stride, alignment and number of channels; _stream: rows past the caches.
+#define FG_REC_ONE(NAME, T, SUFFIX, WIDE, PACKED, STREAM)                                                       \
     extern "C" __global__ __launch_bounds__(64 * FG_REC_WAVES) __attribute__((amdgpu_waves_per_eu(4)))          \
     void fg_rec_##NAME##SUFFIX(fg_rec_kargs g) {                                                               \
-        Rec<T, WIDE, PACKED>::forward(g);                                                                      \
+        Rec<T, WIDE, PACKED, FG_REC_ROWS, STREAM>::forward(g);                                                 \
     }                                                                                                          \
     extern "C" __global__ __launch_bounds__(64 * FG_REC_BACK_WAVES) __attribute__((amdgpu_waves_per_eu(3)))     \
     void fg_rec_back_##NAME##SUFFIX(fg_rec_kargs g) {                                                          \
-        Rec<T, WIDE, PACKED>::backward(g);                                                                     \
+        Rec<T, WIDE, PACKED, FG_REC_BACK_ROWS, STREAM>::backward(g);                                           \
     }
 #define FG_REC_STEP(NAME, T, V)                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void fg_rec_step_##NAME##_v##V(fg_rec_step_kargs g) { step<T, V>(g); }
 #define FG_REC_TYPE(NAME, T)                                                                                    \
-    FG_REC_ONE(NAME, T, , true, false)                                                                          \
-    FG_REC_ONE(NAME, T, _any, false, false)                                                                     \
-    FG_REC_ONE(NAME, T, _packed, true, true)                                                                    \
-    FG_REC_ONE(NAME, T, _packed_any, false, true)                                                               \
+    FG_REC_ONE(NAME, T, , true, false, false)                                                                   \
+    FG_REC_ONE(NAME, T, _stream, true, false, true)                                                             \
+    FG_REC_ONE(NAME, T, _any, false, false, false)                                                              \
+    FG_REC_ONE(NAME, T, _packed, true, true, false)                                                             \
+    FG_REC_ONE(NAME, T, _packed_stream, true, true, true)                                                       \
+    FG_REC_ONE(NAME, T, _packed_any, false, true, false)                                                        \
     FG_REC_STEP(NAME, T, 4)                                                                                     \
     FG_REC_STEP(NAME, T, 1)
 

@@ -5,10 +5,9 @@
 //   a = exp(-rate softplus(decay) r), m = sqrt(1 - a^2)
 //   h_t = a h_{t-1} + m i x,  out = h_t
 //
-// A workgroup has 64 channels.  A lane takes two neighbouring channels through a
-// segment of S tokens, the two rows of 32 lanes of a wave two segments that
-// follow one another, its waves the segments behind those: a tile of 2 S waves
-// tokens.  A lane works out a and b = m i x of its tokens once and keeps them in
+// A workgroup has 128 channels forward, 64 backward.  A lane takes two neighbouring
+// channels through a segment of S tokens; a wave has one segment, or one for each of its two
+// rows of 32 lanes, and its workgroup's waves follow one another: a tile.  A lane works out a and b = m i x of its tokens once and keeps them in
 // registers; what a segment does to the state that enters it is h -> p h + q, with
 // p the product of its a and q its own state from 0.  These pairs pass from row to
 // row by lane exchanges and from wave to wave through LDS, and each lane runs over
@@ -91,6 +90,7 @@ __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
     Place p;
     uint32_t rest;
     p.tile = quotient(blockIdx.x, across, g.over_across, rest);
+    if (across % 8 == 0) rest = rest % 8 * (across / 8) + rest / 8;
     p.chain = quotient(rest, g.blocks, g.over_blocks, p.block);
     p.tag = 0;
     if (g.chain) {
@@ -111,30 +111,33 @@ __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
 }
 
 // A tile's words; the same for all lanes.
+template <int CHANNELS>
 __device__ __forceinline__ char* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
     const uint64_t across = (uint64_t)g.blocks * g.chains, place = tile * across + (uint64_t)p.chain * g.blocks + p.block;
-    return (char*)g.chain + uniform((int64_t)(64 * across + place * (8 * FG_REC_WORDS * FG_REC_CHANNELS)));
+    return (char*)g.chain + uniform((int64_t)(64 * across + place * (8 * FG_REC_WORDS * CHANNELS)));
 }
-// Word `which` of a lane's channel.
-__device__ __forceinline__ void tell(char* at, int which, uint32_t lane, uint32_t tag, float v) {
-    unsigned long long* to = (unsigned long long*)(at + 8 * FG_REC_CHANNELS * which + 8 * lane);
+// Word `which` of a thread's channel.
+template <int CHANNELS>
+__device__ __forceinline__ void tell(char* at, int which, uint32_t ch, uint32_t tag, float v) {
+    unsigned long long* to = (unsigned long long*)(at + 8 * CHANNELS * which + 8 * ch);
     __hip_atomic_store(to, (unsigned long long)tag << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ unsigned long long ask(const char* at, int which, uint32_t lane) {
-    const unsigned long long* from = (const unsigned long long*)(at + 8 * FG_REC_CHANNELS * which + 8 * lane);
+template <int CHANNELS>
+__device__ __forceinline__ unsigned long long ask(const char* at, int which, uint32_t ch) {
+    const unsigned long long* from = (const unsigned long long*)(at + 8 * CHANNELS * which + 8 * ch);
     return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// For the first wave, a lane for each channel: tells the tile's pair p, q and returns
+// For the first waves, a thread for each channel: tells the tile's pair p, q and returns
 // the state that enters the tile, `first` for a chain's first one.
-template <bool PACKED>
+template <bool PACKED, int CHANNELS>
 __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at, float p, float q, float first) {
-    const uint32_t lane = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
+    const uint32_t ch = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
     const bool last = at.tile + 1 == g.tiles;
-    char* mine = words(g, at, at.tile);
+    char* mine = words<CHANNELS>(g, at, at.tile);
     if (!last) {
-        tell(mine, 0, lane, at.tag, p);
-        tell(mine, 1, lane, at.tag, q);
+        tell<CHANNELS>(mine, 0, ch, at.tag, p);
+        tell<CHANNELS>(mine, 1, ch, at.tag, q);
     }
     unsigned long long w[2 * FG_REC_GROUP];
     float state = first;
@@ -143,12 +146,12 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         bool all = true;
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) {
-                const char* from = words(g, at, at.tile - in_group + k);
-                w[2 * k] = ask(from, 0, lane);
-                w[2 * k + 1] = ask(from, 1, lane);
+                const char* from = words<CHANNELS>(g, at, at.tile - in_group + k);
+                w[2 * k] = ask<CHANNELS>(from, 0, ch);
+                w[2 * k + 1] = ask<CHANNELS>(from, 1, ch);
             }
         });
-        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask(words(g, at, at.tile - in_group - 1), 2, lane);
+        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask<CHANNELS>(words<CHANNELS>(g, at, at.tile - in_group - 1), 2, ch);
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) all = all && w[2 * k] >> 32 == at.tag && w[2 * k + 1] >> 32 == at.tag;
         });
@@ -166,21 +169,21 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         if (k < in_group)
             state = enter<PACKED>(__uint_as_float((uint32_t)w[2 * k]), __uint_as_float((uint32_t)w[2 * k + 1]), state);
     });
-    if (!last && in_group == FG_REC_GROUP - 1) tell(mine, 2, lane, at.tag, enter<PACKED>(p, q, state));
+    if (!last && in_group == FG_REC_GROUP - 1) tell<CHANNELS>(mine, 2, ch, at.tag, enter<PACKED>(p, q, state));
     return state;
 }
 
 // An infinite x as the largest number of its sign; NaN stays.
 __device__ __forceinline__ float finite(float x) {
     constexpr float most = 3.402823466e38f;
-    x = x > most ? most : x;
-    return x < -most ? -most : x;
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -most), most);
 }
 
-template <class T, bool WIDE, bool PACKED>
+template <class T, bool WIDE, bool PACKED, int ROWS, bool STREAM>
 struct Rec {
     using raw = typename T::raw;
-    static constexpr int V = FG_REC_LANE_CHANNELS, ROW = 64 / V;  // ROW: lanes that share a token
+    // ROW: lanes that share a token; CHANNELS: of a workgroup.
+    static constexpr int V = FG_REC_LANE_CHANNELS, ROW = 64 / ROWS, CHANNELS = FG_REC_CHANNELS(ROWS);
     struct __attribute__((aligned(V * 4))) Floats {
         float v[V];
     };
@@ -199,7 +202,7 @@ struct Rec {
         l.lane = threadIdx.x & 63;
         l.row = l.lane / ROW;
         l.ch = l.lane % ROW * V;
-        const uint32_t all = g.channels - block * FG_REC_CHANNELS;
+        const uint32_t all = g.channels - block * CHANNELS;
         l.left = l.ch < all ? all - l.ch : 0;
         l.off = l.left ? l.ch * (uint32_t)sizeof(raw) : 0;
         return l;
@@ -231,11 +234,21 @@ struct Rec {
     // channel (uniform); off: token `at` of the wave, at the lane's channels.
     static __device__ __forceinline__ const char* base(const fg_ssm_view& v, uint32_t chain, int64_t t, uint32_t block) {
         return (const char*)v.p +
-               uniform(((int64_t)chain * v.seq + t * v.row + (int64_t)block * FG_REC_CHANNELS) * (int64_t)sizeof(raw));
+               uniform(((int64_t)chain * v.seq + t * v.row + (int64_t)block * CHANNELS) * (int64_t)sizeof(raw));
+    }
+    // The next row's address, by the scalar unit and when it is needed: all rows'
+    // addresses ahead would not fit its registers.
+    template <class P>
+    static __device__ __forceinline__ P further(P p, int64_t step) {
+        p += step;
+        asm volatile("" : "+s"(p));
+        return p;
     }
     static __device__ __forceinline__ Pack fetch(const char* p, uint32_t off, const Lane& l) {
         if constexpr (WIDE) {
-            return *(const Pack*)(p + off);
+            using Word = std::conditional_t<sizeof(Pack) == 4, uint32_t, uint64_t>;
+            const Word* from = (const Word*)(p + off);
+            return __builtin_bit_cast(Pack, STREAM ? __builtin_nontemporal_load(from) : *from);
         } else {
             Pack k;  // channels beyond the last one load it again
             each<V>([&](auto c) {
@@ -249,7 +262,12 @@ struct Rec {
         if constexpr (WIDE) {
             Pack k;
             each<V>([&](auto c) { k.v[c] = T::down(x[c]); });
-            if (l.left) *(Pack*)(p + off) = k;
+            using Word = std::conditional_t<sizeof(Pack) == 4, uint32_t, uint64_t>;
+            Word* to = (Word*)(p + off);
+            if (l.left) {
+                if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Word, k), to);
+                else *to = __builtin_bit_cast(Word, k);
+            }
         } else {
             each<V>([&](auto c) {
                 if (c < l.left) *(raw*)(p + off + c * sizeof(raw)) = T::down(x[c]);
@@ -272,29 +290,47 @@ struct Rec {
         return v < 0 ? 0 : v > all ? all : v;
     }
     // Of the packed sequences, the first that ends behind row t.
-    template <class F>
-    static __device__ __forceinline__ uint32_t search(const fg_rec_kargs& g, int64_t t, F&& offset_) {
+    static __device__ __forceinline__ uint32_t sequence(const fg_rec_kargs& g, int64_t t) {
         uint32_t lo = 0, hi = g.seqs;
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            if (offset_(g, mid + 1) <= t) lo = mid + 1;
+            if (offset(g, mid + 1) <= t) lo = mid + 1;
             else hi = mid;
         }
         return lo;
     }
-    static __device__ __forceinline__ uint32_t sequence(const fg_rec_kargs& g, int64_t t) { return search(g, t, offset); }
-    // Of the wave's V S tokens from t0 on, those of the lane's segment.
+    // The same for a whole wave, a 64th of the sequences for each lane at a time.  The first
+    // look goes out ahead of the rows, so that it is not waited for behind them.
+    struct Probe {
+        uint32_t step;
+        bool before;  // the lane's part of the sequences ends at t or before it
+    };
+    static __device__ __forceinline__ Probe probe(const fg_rec_kargs& g, int64_t t, uint32_t lo, uint32_t n, uint32_t lane) {
+        const uint32_t step = (n + 63) / 64, part = (lane + 1) * step;
+        return {step, part <= n && offset(g, lo + part) <= t};
+    }
+    static __device__ __forceinline__ uint32_t sequence_of_wave(const fg_rec_kargs& g, int64_t t, Probe p, uint32_t lane) {
+        uint32_t lo = 0, n = g.seqs;
+        while (n > 0) {
+            const uint32_t parts = uniform((uint32_t)__popcll(__ballot(p.before)));
+            lo += parts * p.step;
+            n = min(n - parts * p.step, p.step - 1);
+            if (n) p = probe(g, t, lo, n, lane);
+        }
+        return lo;
+    }
+    // Of the wave's ROWS S tokens from t0 on, those of the lane's segment.
     template <int S>
-    static __device__ __forceinline__ Marks marks(const fg_rec_kargs& g, int64_t t0, const Lane& l) {
-        static_assert(V * S <= 32, "a bit for each");
+    static __device__ __forceinline__ Marks marks(const fg_rec_kargs& g, int64_t t0, const Lane& l, const Probe& look) {
+        static_assert(ROWS * S <= 32, "a bit for each");
         constexpr uint32_t ALL = (1u << S) - 1;
         if constexpr (!PACKED) {
             const int64_t left = (int64_t)g.tokens - t0 - l.row * S;
             return {left >= S ? ALL : left > 0 ? (1u << (uint32_t)left) - 1 : 0, 0, 0};
         }
-        const int64_t end = min(t0 + V * S, (int64_t)g.tokens);
+        const int64_t end = min(t0 + ROWS * S, (int64_t)g.tokens);
         uint32_t in = 0, first = 0, last = 0;
-        for (uint32_t s = t0 < end ? search(g, t0, offset_of_wave) : g.seqs; s < g.seqs; ++s) {
+        for (uint32_t s = t0 < end ? sequence_of_wave(g, t0, look, l.lane) : g.seqs; s < g.seqs; ++s) {
             const int64_t a = offset_of_wave(g, s), b = offset_of_wave(g, s + 1);
             if (a >= end) break;
             if (b <= a || b <= t0) continue;  // one without tokens
@@ -313,36 +349,29 @@ struct Rec {
     template <bool BACK>
     static __device__ __forceinline__ void rows(float (&p)[V], float (&q)[V], float (&ep)[V], float (&eq)[V],
                                                 const Lane& l) {
-        const uint32_t row = BACK ? V - 1 - l.row : l.row;
-        static_assert(V == 2, "one step over the rows of lanes");
-        each<1>([&](auto step) {
-            constexpr int far = ROW << step;
-            const int from = (int)l.lane + (BACK ? far : -far);
-            const bool some = row >= (1u << step);
-            each<V>([&](auto c) {
-                const float p1 = __shfl(p[c], from & 63), q1 = __shfl(q[c], from & 63);
-                if (some) {
+        static_assert(ROWS <= 2, "one exchange at most");
+        each<V>([&](auto c) {
+            ep[c] = 1.0f, eq[c] = 0.0f;
+            if constexpr (ROWS == 2) {
+                const bool behind = l.row == (BACK ? 0 : 1);
+                const float p1 = __shfl_xor(p[c], ROW), q1 = __shfl_xor(q[c], ROW);
+                if (behind) {
+                    ep[c] = p1, eq[c] = q1;
                     q[c] = enter<PACKED>(p[c], q[c], q1);
                     p[c] = through<PACKED>(p1, p[c]);
                 }
-            });
-        });
-        const int from = (int)l.lane + (BACK ? ROW : -ROW);
-        each<V>([&](auto c) {
-            const float p1 = __shfl(p[c], from & 63), q1 = __shfl(q[c], from & 63);
-            ep[c] = row ? p1 : 1.0f;
-            eq[c] = row ? q1 : 0.0f;
+            }
         });
     }
 
     // The waves' pairs, [wave][p, q][channel].
     struct Totals {
-        float v[FG_REC_WAVES][2][FG_REC_CHANNELS];
+        float v[FG_REC_WAVES][2][CHANNELS];
     };
     template <bool BACK>
     static __device__ __forceinline__ void publish(Totals& t, uint32_t wave, const Lane& l, const float (&p)[V],
                                                    const float (&q)[V]) {
-        if (l.row == (BACK ? 0 : V - 1)) each<V>([&](auto c) { t.v[wave][0][l.ch + c] = p[c], t.v[wave][1][l.ch + c] = q[c]; });
+        if (l.row == (BACK ? 0 : ROWS - 1)) each<V>([&](auto c) { t.v[wave][0][l.ch + c] = p[c], t.v[wave][1][l.ch + c] = q[c]; });
     }
     // From the state that enters the tile to the one that enters the wave.
     template <bool BACK>
@@ -362,20 +391,22 @@ struct Rec {
     static __device__ __forceinline__ void enter_tile(const fg_rec_kargs& g, const Place& at, const Totals& t, float* lds,
                                                       const float* first, uint32_t wave, uint32_t waves, const Lane& l,
                                                       float (&h)[V]) {
+        static_assert(CHANNELS <= 64 * FG_REC_WAVES, "a thread for each channel, where there are several tiles");
         if (g.tiles == 1) {
             params(h, first, l);
             return;
         }
-        if (wave == 0) {
+        const uint32_t ch = threadIdx.x;
+        if (ch < CHANNELS) {
             float p = 1.0f, q = 0.0f;
             for (uint32_t k = 0; k < waves; ++k) {
                 const uint32_t w = BACK ? waves - 1 - k : k;
-                const float p2 = t.v[w][0][l.lane], q2 = t.v[w][1][l.lane];
+                const float p2 = t.v[w][0][ch], q2 = t.v[w][1][ch];
                 q = enter<PACKED>(p2, q2, q);
                 p = through<PACKED>(p, p2);
             }
-            const bool some = first && at.block * FG_REC_CHANNELS + l.lane < g.channels;
-            lds[l.lane] = entering<PACKED>(g, at, p, q, some ? first[l.lane] : 0.0f);
+            const bool some = first && at.block * CHANNELS + ch < g.channels;
+            lds[ch] = entering<PACKED, CHANNELS>(g, at, p, q, some ? first[ch] : 0.0f);
         }
         __syncthreads();
         const Floats v = *(const Floats*)&lds[l.ch];
@@ -384,7 +415,7 @@ struct Rec {
 
     // A packed sequence's row of [sequences][channels].
     static __device__ __forceinline__ const float* of(const float* p, const fg_rec_kargs& g, uint32_t s, uint32_t block) {
-        return p ? p + (uint64_t)s * g.channels + (uint64_t)block * FG_REC_CHANNELS : nullptr;
+        return p ? p + (uint64_t)s * g.channels + (uint64_t)block * CHANNELS : nullptr;
     }
 
     // Packed: the sequences' initial states, behind the checkpoints of the rows.
@@ -394,23 +425,25 @@ struct Rec {
     // tiles take turns at them.
     static __device__ __forceinline__ void empty(const fg_rec_kargs& g, const float* from, float* to, uint32_t block,
                                                  uint32_t chain, uint32_t tile) {
-        if (!to || threadIdx.x >= FG_REC_CHANNELS || block * FG_REC_CHANNELS + threadIdx.x >= g.channels) return;
-        const uint32_t ch = block * FG_REC_CHANNELS + threadIdx.x;
-        if constexpr (PACKED) {
-            for (uint64_t s = tile; s < g.seqs; s += g.tiles) {
-                const uint64_t at = s * g.channels + ch;
-                if (offset(g, s) >= offset(g, s + 1)) to[at] = from ? from[at] : 0.0f;
+        if (!to) return;
+        for (uint32_t k = threadIdx.x; k < CHANNELS && block * CHANNELS + k < g.channels; k += blockDim.x) {
+            const uint32_t ch = block * CHANNELS + k;
+            if constexpr (PACKED) {
+                for (uint64_t s = tile; s < g.seqs; s += g.tiles) {
+                    const uint64_t at = s * g.channels + ch;
+                    if (offset(g, s) >= offset(g, s + 1)) to[at] = from ? from[at] : 0.0f;
+                }
+            } else if (g.tokens == 0) {
+                const uint64_t at = (uint64_t)chain * g.channels + ch;
+                to[at] = from ? from[at] : 0.0f;
             }
-        } else if (g.tokens == 0) {
-            const uint64_t at = (uint64_t)chain * g.channels + ch;
-            to[at] = from ? from[at] : 0.0f;
         }
     }
 
     struct Params {
         float k[V], ba[V], bx[V];
         __device__ __forceinline__ void load(const fg_rec_kargs& g, uint32_t block, const Lane& l) {
-            const uint64_t at = (uint64_t)block * FG_REC_CHANNELS;
+            const uint64_t at = (uint64_t)block * CHANNELS;
             params(k, g.decay + at, l);
             params(ba, g.bias_a ? g.bias_a + at : nullptr, l);
             params(bx, g.bias_x ? g.bias_x + at : nullptr, l);
@@ -429,61 +462,66 @@ struct Rec {
         each<V>([&](auto c) { ga.v[c] = T::down(-__builtin_inff()); });
     }
 
-    // Of N arrays (x, the gates, the output's gradient) a wave's V S rows, S for each row of
-    // lanes; where only `rows` of them exist, nothing() for those behind.  Token after token of
-    // all arrays, so that the first can be worked on while the others are on their way.
-    template <int N, int S>
-    static __device__ __forceinline__ void fetch_rows(Pack (&to)[N][S], const fg_ssm_view (&v)[N], uint32_t chain,
-                                                      int64_t t0, uint32_t block, const Lane& l, int64_t rows) {
+    // Of N arrays (x, the gates, the output's gradient) a wave's ROWS S rows, S for each row of
+    // lanes, token after token; unless FULL, only `left` of them exist: nothing() for those behind.
+    template <int N, bool FULL>
+    struct Source {
         const char* p[N];
-        uint32_t step[N], off[N];
-        each<N>([&](auto k) {
-            p[k] = base(v[k], chain, t0, block);
-            step[k] = (uint32_t)v[k].row * (uint32_t)sizeof(raw);
-        });
-        if (rows >= V * S) {
-            each<N>([&](auto k) { off[k] = l.row * S * step[k] + l.off; });
-            each<S>([&](auto j) {
-                each<N>([&](auto k) {
-                    off[k] = fresh(j ? off[k] + step[k] : off[k]);
-                    to[k][j] = fetch(p[k], off[k], l);
-                });
-            });
-        } else {
-            each<S>([&](auto j) {
-                nothing(to[0][j], to[1][j], to[2][j]);
-                if (N > 3) to[N - 1][j] = Pack{};
-                const uint32_t t = l.row * S + j;
-                if (t < rows) each<N>([&](auto k) { to[k][j] = fetch(p[k], t * step[k] + l.off, l); });
+        uint32_t step[N], off[N], first;
+        int64_t left;
+        __device__ __forceinline__ Source(const fg_ssm_view (&v)[N], uint32_t chain, int64_t t0, uint32_t block, const Lane& l,
+                                          int64_t rows, uint32_t segment)
+            : first(l.row * segment), left(rows) {
+            each<N>([&](auto k) {
+                p[k] = base(v[k], chain, t0, block);
+                step[k] = (uint32_t)v[k].row * (uint32_t)sizeof(raw);
+                off[k] = fresh(first * step[k] + l.off);
             });
         }
-    }
+        // Token j's, the tokens before it having been fetched.
+        template <int D>
+        __device__ __forceinline__ void next(Pack (&to)[N][D], int at, uint32_t j, const Lane& l) {
+            if constexpr (FULL) {
+                each<N>([&](auto k) { to[k][at] = fetch(p[k], off[k], l); });
+            } else {
+                nothing(to[0][at], to[1][at], to[2][at]);
+                if (N > 3) to[N - 1][at] = Pack{};
+                if (first + j < left) each<N>([&](auto k) { to[k][at] = fetch(p[k], off[k], l); });
+            }
+            each<N>([&](auto k) { p[k] = further(p[k], step[k]); });
+        }
+    };
 
-    static __device__ __forceinline__ void forward(const fg_rec_kargs& g) {
+    template <bool FULL>
+    static __device__ __forceinline__ void forward_tile(const fg_rec_kargs& g, const Place& at, Totals& totals,
+                                                        float4 (&entered)[CHANNELS / 4]) {
         constexpr int S = FG_REC_SEGMENT(sizeof(raw));
-        __shared__ Totals totals;
-        __shared__ float4 entered[FG_REC_CHANNELS / 4];
-        const Place at = place_of(g);
+        constexpr uint32_t ALL = (1u << S) - 1;
         const uint32_t block = at.block, chain = at.chain;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
-        const int64_t t0 = ((int64_t)at.tile * waves + wave) * (V * S), rows_left = (int64_t)g.tokens - t0;
-        Pack in[3][S];
-        fetch_rows<3, S>(in, {g.x, g.ga, g.gx}, chain, t0, block, l, rows_left);
+        const int64_t t0 = ((int64_t)at.tile * waves + wave) * (ROWS * S), rows_left = (int64_t)g.tokens - t0;
+        Probe look{};
+        if constexpr (PACKED) look = probe(g, t0, 0, g.seqs, l.lane);
+        constexpr int D = FG_REC_AHEAD(S);
+        Pack in[3][D];
+        Source<3, FULL> source({g.x, g.ga, g.gx}, chain, t0, block, l, rows_left, S);
+        each<D>([&](auto j) { source.next(in, j, j, l); });
         Params w;
         w.load(g, block, l);
-        const Marks m = marks<S>(g, t0, l);
+        const Marks m = marks<S>(g, t0, l, look);
         float a[S][V], b[S][V], p[V], q[V];
         each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f; });
         each<S>([&](auto j) {
+            constexpr int d = j % D;
             if constexpr (PACKED) {
-                if (!(m.in >> j & 1)) nothing(in[0][j], in[1][j], in[2][j]);
+                if (!(m.in >> j & 1)) nothing(in[0][d], in[1][d], in[2][d]);
             }
             each<V>([&](auto c) {
-                const float r = gate(T::up(in[1][j].v[c]), w.ba[c]), i = gate(T::up(in[2][j].v[c]), w.bx[c]);
+                const float r = gate(T::up(in[1][d].v[c]), w.ba[c]), i = gate(T::up(in[2][d].v[c]), w.bx[c]);
                 const Share s = share(w.k[c], r);
                 a[j][c] = s.a;
-                b[j][c] = __builtin_amdgcn_sqrtf(s.m2) * i * T::up(in[0][j].v[c]);
+                b[j][c] = __builtin_amdgcn_sqrtf(s.m2) * i * T::up(in[0][d].v[c]);
             });
             const bool first = PACKED && (m.first >> j & 1);
             if (first) {
@@ -497,6 +535,9 @@ struct Rec {
                 q[c] = first ? b[j][c] : fmaf(a[j][c], q[c], b[j][c]);
                 p[c] *= a[j][c];
             });
+            // as many rows on their way as memory needs, not all: rows of the workgroups that start
+            // at a time would wait for one another, and all of them for the first
+            if constexpr (j + D < S) source.next(in, d, j + D, l);
             __builtin_amdgcn_sched_barrier(0);  // tokens mixed would not fit the registers of four waves
         });
         each<V>([&](auto c) { p[c] = PACKED && m.first ? -1.0f : fmaxf(p[c], kLeast); });
@@ -508,21 +549,28 @@ struct Rec {
                           l, h);
         pass<false>(totals, wave, waves, l, h);
         if (g.check && t0 % FG_REC_CHECK == 0 && l.row == 0 && rows_left > 0)
-            put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + (uint64_t)block * FG_REC_CHANNELS, l, h);
+            put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + (uint64_t)block * CHANNELS, l, h);
         each<V>([&](auto c) { h[c] = enter<PACKED>(ep[c], eq[c], h[c]); });
         char* po = const_cast<char*>(base(g.out, chain, t0, block));
-        const uint32_t step = (uint32_t)g.out.row * (uint32_t)sizeof(raw);
-        uint32_t off = l.row * S * step + l.off;
-        each<S>([&](auto j) {
-            const bool first = PACKED && (m.first >> j & 1);
-            each<V>([&](auto c) { h[c] = first ? b[j][c] : fmaf(a[j][c], h[c], b[j][c]); });
-            off = fresh(j ? off + step : off);
-            if (m.in >> j & 1) store(po, off, l, h);
-            if constexpr (PACKED) {
-                if (g.final && (m.last >> j & 1))
-                    put(const_cast<float*>(of(g.final, g, sequence(g, t0 + l.row * S + j), block)), l, h);
-            }
-        });
+        const uint32_t step = (uint32_t)g.out.row * (uint32_t)sizeof(raw), off = fresh(l.row * S * step + l.off);
+        if (PACKED ? __all(m.in == ALL && !m.first && !m.last) : FULL) {
+            each<S>([&](auto j) {
+                each<V>([&](auto c) { h[c] = fmaf(a[j][c], h[c], b[j][c]); });
+                store(po, off, l, h);
+                po = further(po, step);
+            });
+        } else {
+            each<S>([&](auto j) {
+                const bool first = PACKED && (m.first >> j & 1);
+                each<V>([&](auto c) { h[c] = first ? b[j][c] : fmaf(a[j][c], h[c], b[j][c]); });
+                if (m.in >> j & 1) store(po, off, l, h);
+                po = further(po, step);
+                if constexpr (PACKED) {
+                    if (g.final && (m.last >> j & 1))
+                        put(const_cast<float*>(of(g.final, g, sequence(g, t0 + l.row * S + j), block)), l, h);
+                }
+            });
+        }
         if constexpr (!PACKED) {  // tokens behind the last one left h as it was
             const int64_t mine = rows_left - l.row * S;
             if (g.final && mine > 0 && mine <= S) put(const_cast<float*>(of(g.final, g, chain, block)), l, h);
@@ -530,22 +578,35 @@ struct Rec {
         empty(g, g.initial, g.final, block, chain, at.tile);
     }
 
-    static __device__ __forceinline__ void backward(const fg_rec_kargs& g) {
-        constexpr int S = FG_REC_BACK_SEGMENT;
-        __shared__ Totals both[2];
-        __shared__ float4 entered[FG_REC_CHANNELS / 4];
-        Totals &ta = both[0], &tb = both[1];
+    // All but a chain's last tile are full; the two are apart from the start, since rows that may
+    // not exist would keep others waiting.
+    static __device__ __forceinline__ void forward(const fg_rec_kargs& g) {
+        __shared__ Totals totals;
+        __shared__ float4 entered[CHANNELS / 4];
         const Place at = place_of(g);
+        const uint64_t tokens = blockDim.x / 64 * (ROWS * FG_REC_SEGMENT(sizeof(raw)));
+        if ((at.tile + 1) * tokens <= g.tokens) forward_tile<true>(g, at, totals, entered);
+        else forward_tile<false>(g, at, totals, entered);
+    }
+
+    template <bool FULL>
+    static __device__ __forceinline__ void backward_tile(const fg_rec_kargs& g, const Place& at, Totals (&both)[2],
+                                                         float4 (&entered)[CHANNELS / 4]) {
+        constexpr int S = FG_REC_BACK_SEGMENT;
+        Totals &ta = both[0], &tb = both[1];
         const uint32_t block = at.block, chain = at.chain, tile = g.tiles - 1 - at.tile;
         const uint32_t wave = uniform(threadIdx.x / 64), waves = blockDim.x / 64;
         const Lane l = lane_of(g, block);
-        const uint64_t at0 = (uint64_t)block * FG_REC_CHANNELS;
-        const int64_t t0 = ((int64_t)tile * waves + wave) * (V * S), rows_left = (int64_t)g.tokens - t0;
+        const uint64_t at0 = (uint64_t)block * CHANNELS;
+        const int64_t t0 = ((int64_t)tile * waves + wave) * (ROWS * S), rows_left = (int64_t)g.tokens - t0;
+        Probe look{};
+        if constexpr (PACKED) look = probe(g, t0, 0, g.seqs, l.lane);
         Pack in[4][S];
-        fetch_rows<4, S>(in, {g.x, g.ga, g.gx, g.out}, chain, t0, block, l, rows_left);
+        Source<4, FULL> source({g.x, g.ga, g.gx, g.out}, chain, t0, block, l, rows_left, S);
+        each<S>([&](auto j) { source.next(in, j, j, l); });
         Params w;
         w.load(g, block, l);
-        const Marks m = marks<S>(g, t0, l);
+        const Marks m = marks<S>(g, t0, l, look);
         // Of each token what the gradients go by: mi = m i, e = i x a^2 / m, f = x (1 - i).
         float a[S][V], r[S][V], mi[S][V], e[S][V], f[S][V], p[V], q[V], rp[V], rq[V];
         each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f, rq[c] = 0.0f; });
@@ -590,7 +651,7 @@ struct Rec {
         rows<true>(rp, rq, rep, req, l);
         publish<false>(ta, wave, l, p, q);
         publish<true>(tb, wave, l, rp, rq);
-        const int64_t first_token = (int64_t)tile * waves * (V * S);
+        const int64_t first_token = (int64_t)tile * waves * (ROWS * S);
         if (first_token < (int64_t)g.tokens)
             params(h, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
         __syncthreads();
@@ -617,13 +678,12 @@ struct Rec {
         uint32_t step[3], off[3];
         const fg_ssm_view* outs[3] = {&g.dx, &g.dga, &g.dgx};
         each<3>([&](auto k) {
-            to[k] = const_cast<char*>(base(*outs[k], chain, t0, block));
             step[k] = (uint32_t)outs[k]->row * (uint32_t)sizeof(raw);
-            off[k] = (l.row * S + S - 1) * step[k] + l.off;
+            to[k] = const_cast<char*>(base(*outs[k], chain, t0 + S - 1, block));
+            off[k] = fresh(l.row * S * step[k] + l.off);
         });
         each<S>([&](auto k) {
             constexpr int j = S - 1 - k;
-            each<3>([&](auto n) { off[n] = fresh(k ? off[n] - step[n] : off[n]); });
             if constexpr (PACKED) {
                 if (m.last >> j & 1) params(d, of(g.gfinal, g, sequence(g, t0 + l.row * S + j), block), l);
             }
@@ -643,6 +703,7 @@ struct Rec {
                     if (outs[n]->p) store(to[n], off[n], l, o[n]);
                 });
             }
+            each<3>([&](auto n) { to[n] = further(to[n], -(int64_t)step[n]); });
             if constexpr (PACKED) {
                 if (g.ginitial && (m.first >> j & 1))
                     put(const_cast<float*>(of(g.ginitial, g, sequence(g, t0 + l.row * S + j), block)), l, d);
@@ -654,20 +715,30 @@ struct Rec {
         // the parameters' sums: over the rows of a wave, then over the waves
         __syncthreads();
         float* all = &both[0].v[0][0][0];  // [wave][3][channel]
-        static_assert(sizeof(both) >= 4 * 3 * FG_REC_WAVES * FG_REC_CHANNELS, "the sums fit");
+        static_assert(sizeof(both) >= 4 * 3 * FG_REC_WAVES * CHANNELS, "the sums fit");
         each<3>([&](auto k) {
             each<V>([&](auto c) {
-                const float v = sums[k][c] + __shfl_xor(sums[k][c], ROW);
-                if (l.row == 0) all[(wave * 3 + k) * FG_REC_CHANNELS + l.ch + c] = v;
+                float v = sums[k][c];
+                if (ROWS == 2) v += __shfl_xor(v, ROW);
+                if (l.row == 0) all[(wave * 3 + k) * CHANNELS + l.ch + c] = v;
             });
         });
         __syncthreads();
-        for (uint32_t n = threadIdx.x; n < 3 * FG_REC_CHANNELS; n += blockDim.x) {
-            const uint32_t k = n / FG_REC_CHANNELS, ch = n % FG_REC_CHANNELS;
+        for (uint32_t n = threadIdx.x; n < 3 * CHANNELS; n += blockDim.x) {
+            const uint32_t k = n / CHANNELS, ch = n % CHANNELS;
             float v = 0.0f;
-            for (uint32_t u = 0; u < waves; ++u) v += all[(u * 3 + k) * FG_REC_CHANNELS + ch];
+            for (uint32_t u = 0; u < waves; ++u) v += all[(u * 3 + k) * CHANNELS + ch];
             if (at0 + ch < g.channels) g.part[(((uint64_t)chain * g.tiles + tile) * 3 + k) * g.channels + at0 + ch] = v;
         }
+    }
+
+    static __device__ __forceinline__ void backward(const fg_rec_kargs& g) {
+        __shared__ Totals both[2];
+        __shared__ float4 entered[CHANNELS / 4];
+        const Place at = place_of(g);
+        const uint64_t tokens = blockDim.x / 64 * (ROWS * FG_REC_BACK_SEGMENT);
+        if ((g.tiles - at.tile) * tokens <= g.tokens) backward_tile<true>(g, at, both, entered);
+        else backward_tile<false>(g, at, both, entered);
     }
 };
 

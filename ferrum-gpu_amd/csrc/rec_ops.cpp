@@ -33,6 +33,12 @@ KernelArtifact rec_code_object(int dtype) {
     return a;
 }
 
+// Bytes of an array of rows from which on rows are loaded and stored past the caches, which
+// several such arrays would leave anyway.  us with ordinary accesses / past the caches, inputs of three sets in
+// turn: 4 x 2048 x 4096 in bfloat16 70.4 / 64.0, 1 x 8192 x 2048 41.0 / 39.5, training step 4 x 1024
+// x 2048 66.2 / 62.8.
+constexpr uint64_t kStreamBytes = 16 << 20;
+
 void check_rate(const char* op, double rate) {
     if (!(rate >= 0) || !std::isfinite((float)rate))
         invalid(std::string(op) + ": rate must be a finite number, 0 or more, got " + std::to_string(rate));
@@ -112,16 +118,22 @@ RecurrencePlan::RecurrencePlan(const HipBackend::DeviceHandle& dev, const Recurr
     chains_ = s.packed ? std::min<int64_t>(s.sequences, 1) : s.sequences;
     rows_ = s.packed ? s.tokens : s.length;
     const std::string tail = std::string(kTypes[s.dtype]) + (s.packed ? "_packed" : "");
+    const bool stream = (uint64_t)s.channels * rows_ * chains_ * kBytes[s.dtype] >= kStreamBytes;
     for (int wide = 0; wide < 2; ++wide) {
-        forward_[wide] = k.get((int)s.dtype, "fg_rec_" + tail + (wide ? "" : "_any"));
-        backward_[wide] = k.get((int)s.dtype, "fg_rec_back_" + tail + (wide ? "" : "_any"));
+        const std::string form = tail + (wide ? stream ? "_stream" : "" : "_any");
+        forward_[wide] = k.get((int)s.dtype, "fg_rec_" + form);
+        backward_[wide] = k.get((int)s.dtype, "fg_rec_back_" + form);
     }
     reduce_ = k.get((int)s.dtype, "fg_rec_reduce");
     ahead_ = chain(false);
 }
 
 uint32_t RecurrencePlan::wave_tokens(bool back) const {
-    return FG_REC_LANE_CHANNELS * (back ? FG_REC_BACK_SEGMENT : FG_REC_SEGMENT(kBytes[s_.dtype]));
+    return back ? FG_REC_BACK_ROWS * FG_REC_BACK_SEGMENT : FG_REC_ROWS * FG_REC_SEGMENT(kBytes[s_.dtype]);
+}
+
+uint32_t RecurrencePlan::blocks(bool back) const {
+    return (uint32_t)ceil_div(s_.channels, FG_REC_CHANNELS(back ? FG_REC_BACK_ROWS : FG_REC_ROWS));
 }
 
 // As many as the rows of a chain take.
@@ -132,17 +144,16 @@ uint32_t RecurrencePlan::waves(bool back) const {
 
 uint64_t RecurrencePlan::places(bool back) const {
     const uint64_t tiles = std::max<uint64_t>(1, ceil_div(rows_, wave_tokens(back) * waves(back)));
-    const uint64_t n = (uint64_t)size_of("recurrence", "launch", {(int64_t)ceil_div(s_.channels, FG_REC_CHANNELS),
-                                                                  (int64_t)chains_, (int64_t)tiles});
+    const uint64_t n = (uint64_t)size_of("recurrence", "launch", {blocks(back), (int64_t)chains_, (int64_t)tiles});
     if (n > 0xffffffffull / (64 * waves(back))) invalid("recurrence: too large for one launch");
     return n;
 }
 
 // None where every chain is one tile.
 Buffer<char, HipBackend> RecurrencePlan::chain(bool back) const {
-    const uint64_t n = places(back), across = ceil_div(s_.channels, FG_REC_CHANNELS) * chains_;
+    const uint64_t n = places(back), across = blocks(back) * chains_;
     if (n <= across) return {};
-    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(across, n / across));
+    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(across, n / across, back ? FG_REC_BACK_ROWS : FG_REC_ROWS));
 }
 
 size_t RecurrencePlan::checkpoint_bytes() const {
@@ -170,7 +181,7 @@ fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in
     g.seqs = (uint32_t)s_.sequences;
     g.chains = (uint32_t)chains_;
     g.channels = (uint32_t)s_.channels;
-    g.blocks = (uint32_t)ceil_div(s_.channels, FG_REC_CHANNELS);
+    g.blocks = blocks(back);
     g.rate = (float)s_.rate;
     const uint64_t n = places(back), across = (uint64_t)g.blocks * g.chains;
     g.tiles = across ? (uint32_t)(n / across) : 1;

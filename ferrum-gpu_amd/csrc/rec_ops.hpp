@@ -38,9 +38,10 @@ public:
     void backward(const fg_recurrence_backward_args& a, hipStream_t stream);
 
 private:
-    // Of a pass, which has kernels of its own: tokens of a wave, waves of a
+    // Of a pass, which has kernels of its own: tokens of a wave, workgroups over the channels, waves of a
     // workgroup, tiles over all chains and channels, and what they pass on.
     uint32_t wave_tokens(bool back) const;
+    uint32_t blocks(bool back) const;
     uint32_t waves(bool back) const;
     uint64_t places(bool back) const;
     Buffer<char, HipBackend> chain(bool back) const;
