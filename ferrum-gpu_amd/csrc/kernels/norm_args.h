@@ -6,7 +6,7 @@
 
 #include "ssm_args.h"
 
-#define FG_NORM_THREADS 256
+#define FG_NORM_THREADS(team) ((team) < 256 ? 256 : (team)) /* of a workgroup, whose teams have a row each */
 
 typedef struct {
     fg_ssm_view x, residual, out, sum; /* .seq unused; may be null: residual, sum.  backward: x is the sum,

@@ -7,11 +7,11 @@ using namespace fg::norm;
 
 // _any: for widths that are not whole chunks.
 #define FG_NORM_FORM(NAME, T, C, TEAM, SUFFIX, EVEN)                                                            \
-    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS)                                                    \
+    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS(TEAM))                                                  \
     void fg_norm_##NAME##_c##C##_t##TEAM##SUFFIX(fg_norm_kargs g) {                                            \
         Rows<T, C, TEAM, EVEN>::forward(g);                                                                    \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS)                                                    \
+    extern "C" __global__ __launch_bounds__(FG_NORM_THREADS(TEAM))                                                  \
     void fg_norm_back_##NAME##_c##C##_t##TEAM##SUFFIX(fg_norm_kargs g) {                                       \
         Rows<T, C, TEAM, EVEN>::backward(g);                                                                   \
     }
@@ -20,10 +20,10 @@ using namespace fg::norm;
     FG_NORM_ONE(NAME, T, 1, 64)                                                                                 \
     FG_NORM_ONE(NAME, T, 2, 64)                                                                                 \
     FG_NORM_ONE(NAME, T, 1, 256)                                                                                \
-    FG_NORM_ONE(NAME, T, 2, 256)                                                                                \
-    FG_NORM_ONE(NAME, T, 4, 256)                                                                                \
-    FG_NORM_ONE(NAME, T, 8, 256)                                                                                \
-    FG_NORM_ONE(NAME, T, 0, 256)                                                                                \
+    FG_NORM_ONE(NAME, T, 1, 512)                                                                                \
+    FG_NORM_ONE(NAME, T, 1, 1024)                                                                               \
+    FG_NORM_ONE(NAME, T, 2, 1024)                                                                               \
+    FG_NORM_ONE(NAME, T, 0, 1024)                                                                               \
     extern "C" __global__ __launch_bounds__(256) void fg_dropout_##NAME(fg_dropout_kargs g) { dropout<T>(g); }
 
 extern "C" __global__ __launch_bounds__(1024) void fg_norm_reduce(const float* part, float* to, uint32_t width,

@@ -35,13 +35,14 @@ constexpr float kLeast = 7.888609e-31f;    // 2^-100: what 448 / m is taken of a
 typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t HalfWords __attribute__((ext_vector_type(2), aligned(1)));
 
-// A store past the caches.  The statement behind it keeps the compiler from making one
+// A store past the caches.  The statements around it keep the compiler from making one
 // ordinary store of this one and of that on the branch's other side.
-template <class W>
-__device__ __forceinline__ void past(W v, W* to) {
-    __builtin_nontemporal_store(v, to);
-    asm volatile("; past the caches");
-}
+#define FG_PAST_THE_CACHES(TYPE, v, to)                                \
+    do {                                                               \
+        asm volatile("; past the caches");                             \
+        __builtin_nontemporal_store(__builtin_bit_cast(TYPE, v), (TYPE*)(to)); \
+        asm volatile("; past the caches");                             \
+    } while (0)
 
 // Chunks of 16 bytes at any address of their elements: the GPU's loads and stores take them.
 // EVEN: all of them are whole.
@@ -72,7 +73,7 @@ struct Chunk {
         Raw r;
         each<E>([&](auto i) { r.v[i] = T::down(x[i]); });
         if (EVEN || n >= E) {
-            if (stream) past(__builtin_bit_cast(Words, r), (Words*)to);
+            if (stream) FG_PAST_THE_CACHES(Words, r, to);
             else *(Raw*)to = r;
         } else {
             each<E>([&](auto i) {
@@ -99,7 +100,7 @@ struct Chunk {
         });
         if (EVEN || n >= E) {
             if constexpr (E == 8) {
-                if (stream) past(__builtin_bit_cast(HalfWords, b), (HalfWords*)to);
+                if (stream) FG_PAST_THE_CACHES(HalfWords, b, to);
                 else *(Bytes*)to = b;
             } else {
                 *(Bytes*)to = b;
@@ -132,14 +133,14 @@ struct Chunk {
 
 // Two sums, or a sum and a largest value, over a team's threads.
 template <int TEAM, bool MAX>
-__device__ __forceinline__ void over_team(float& a, float& b, float2 (&lds)[FG_NORM_THREADS / 64]) {
+__device__ __forceinline__ void over_team(float& a, float& b, float2 (&lds)[TEAM / 64]) {
     each<6>([&](auto i) {
         a += __shfl_xor(a, 1 << i);
         const float o = __shfl_xor(b, 1 << i);
         b = MAX ? fmaxf(b, o) : b + o;
     });
     if constexpr (TEAM > 64) {
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = make_float2(a, b);
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x % TEAM / 64] = make_float2(a, b);
         __syncthreads();
         a = b = 0.0f;
         each<TEAM / 64>([&](auto w) {
@@ -155,7 +156,7 @@ template <class T, int C, int TEAM, bool EVEN>
 struct Rows {
     using Io = Chunk<T, EVEN>;
     using Raw = typename Io::Raw;
-    static constexpr int E = Io::E, TEAMS = FG_NORM_THREADS / TEAM, KEPT = C ? C : 1;
+    static constexpr int E = Io::E, TEAMS = FG_NORM_THREADS(TEAM) / TEAM, KEPT = C ? C : 1;
 
     static __device__ __forceinline__ uint32_t count(const fg_norm_kargs& g, uint32_t col) {
         return col >= g.width ? 0 : g.width - col;
@@ -174,32 +175,49 @@ struct Rows {
         }
     }
 
-    static __device__ __forceinline__ void value(const fg_norm_kargs& g, uint64_t row, uint32_t col, uint32_t n,
+    // A chunk of x and of the residual, and their sum.
+    struct Pair {
+        Raw x, residual;
+    };
+    static __device__ __forceinline__ Pair fetch(const fg_norm_kargs& g, uint64_t row, uint32_t col, uint32_t n) {
+        Pair p{};
+        p.x = Io::load(g.x.p, (int64_t)row * g.x.row + col, n);
+        if (g.residual.p) p.residual = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
+        return p;
+    }
+    static __device__ __forceinline__ void value(const fg_norm_kargs& g, const Pair& p, uint64_t row, uint32_t col,
                                                  uint64_t numbers, float (&v)[E]) {
-        const Raw x = Io::load(g.x.p, (int64_t)row * g.x.row + col, n);
-        each<E>([&](auto i) { v[i] = T::up(x.v[i]); });
+        each<E>([&](auto i) { v[i] = T::up(p.x.v[i]); });
         if (g.drop) Io::drop(v, g.seed, numbers, row * g.width + col, g.drop, g.drop_all, g.keep);
-        if (g.residual.p) {
-            const Raw r = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
-            each<E>([&](auto i) { v[i] += T::up(r.v[i]); });
-        }
+        if (g.residual.p) each<E>([&](auto i) { v[i] += T::up(p.residual.v[i]); });
     }
 
     static __device__ __forceinline__ void forward(const fg_norm_kargs& g) {
-        __shared__ float2 lds[2][FG_NORM_THREADS / 64];
+        __shared__ float2 lds[2][TEAM / 64];
         const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
+        const uint64_t stride = (uint64_t)gridDim.x * TEAMS;
+        uint64_t row = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
         float w[KEPT][E], v[KEPT][E];
-        if constexpr (C > 0) chunks(g, [&](auto k, uint32_t col, uint32_t n) { Io::floats(w[k], g.weight, col, n); });
+        Pair next[KEPT];  // the next row, on its way while this one is worked on
+        if constexpr (C > 0) {
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                if (row < g.rows && n) next[k] = fetch(g, row, col, n);
+            });
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) { Io::floats(w[k], g.weight, col, n); });
+        }
         uint32_t turn = 0;
-        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += (uint64_t)gridDim.x * TEAMS, turn ^= 1) {
-            const uint64_t row = at + threadIdx.x / TEAM;
+        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += stride, row += stride, turn ^= 1) {
             const bool some = row < g.rows;  // a whole team's
             float squares = 0.0f, most = 0.0f;
             chunks(g, [&](auto k, uint32_t col, uint32_t n) {
                 each<E>([&](auto i) { v[k][i] = 0.0f; });
                 if (!some || !n) return;
-                if constexpr (C == 0) Io::floats(w[k], g.weight, col, n);
-                value(g, row, col, n, numbers, v[k]);
+                if constexpr (C == 0) {
+                    Io::floats(w[k], g.weight, col, n);
+                    next[k] = fetch(g, row, col, n);
+                }
+                value(g, next[k], row, col, numbers, v[k]);
+                if (C > 0 && row + stride < g.rows) next[k] = fetch(g, row + stride, col, n);
                 each<E>([&](auto i) {
                     if (!EVEN && i >= n) v[k][i] = 0.0f;  // a dropped place beyond the row holds nothing else
                     squares = fmaf(v[k][i], v[k][i], squares);
@@ -216,7 +234,7 @@ struct Rows {
                     each<E>([&](auto i) { v[k][i] = 0.0f; });
                     if (some && n) {
                         Io::floats(w[k], g.weight, col, n);
-                        value(g, row, col, n, numbers, v[k]);
+                        value(g, fetch(g, row, col, n), row, col, numbers, v[k]);
                         if (g.sum.p) Io::store(g.sum.p, (int64_t)row * g.sum.row + col, n, v[k], g.stream);
                     }
                 }
@@ -243,7 +261,7 @@ struct Rows {
     }
 
     static __device__ __forceinline__ void backward(const fg_norm_kargs& g) {
-        __shared__ float2 lds[2][FG_NORM_THREADS / 64];
+        __shared__ float2 lds[2][TEAM / 64];
         const uint64_t numbers = g.offset + (g.counter ? (uint64_t)*g.counter : 0);
         float w[KEPT][E], dw[KEPT][E], u[KEPT][E], dy[KEPT][E];
         float* part = g.part ? g.part + (uint64_t)(blockIdx.x * TEAMS + threadIdx.x / TEAM) * g.width : nullptr;
@@ -252,20 +270,36 @@ struct Rows {
             each<E>([&](auto i) { dw[k][i] = 0.0f; });
             if (C == 0 && part) each<E>([&](auto i) { if (i < n) part[col + i] = 0.0f; });
         });
+        const uint64_t stride = (uint64_t)gridDim.x * TEAMS;
+        uint64_t row = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+        Raw next[KEPT][3];  // the next row of the sum and of both gradients
+        const auto fetch = [&](uint64_t r, int k, uint32_t col, uint32_t n) {
+            next[k][0] = Io::load(g.x.p, (int64_t)r * g.x.row + col, n);
+            next[k][1] = Io::load(g.out.p, (int64_t)r * g.out.row + col, n);
+            if (g.residual.p) next[k][2] = Io::load(g.residual.p, (int64_t)r * g.residual.row + col, n);
+        };
+        Raw later[KEPT];  // this row's gradient of the sum
+        const auto take = [&](auto k, uint32_t col, uint32_t n) {
+            if constexpr (C == 0) {
+                Io::floats(w[k], g.weight, col, n);
+                fetch(row, k, col, n);
+            }
+            each<E>([&](auto i) { u[k][i] = T::up(next[k][0].v[i]), dy[k][i] = T::up(next[k][1].v[i]); });
+            later[k] = next[k][2];
+        };
+        if constexpr (C > 0) {
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) {
+                if (row < g.rows && n) fetch(row, k, col, n);
+            });
+        }
         uint32_t turn = 0;
-        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += (uint64_t)gridDim.x * TEAMS, turn ^= 1) {
-            const uint64_t row = at + threadIdx.x / TEAM;
+        for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += stride, row += stride, turn ^= 1) {
             const bool some = row < g.rows;
-            const auto load = [&](auto k, uint32_t col, uint32_t n) {
-                if constexpr (C == 0) Io::floats(w[k], g.weight, col, n);
-                const Raw a = Io::load(g.x.p, (int64_t)row * g.x.row + col, n);
-                const Raw b = Io::load(g.out.p, (int64_t)row * g.out.row + col, n);
-                each<E>([&](auto i) { u[k][i] = T::up(a.v[i]), dy[k][i] = T::up(b.v[i]); });
-            };
             float squares = 0.0f, along = 0.0f;
             chunks(g, [&](auto k, uint32_t col, uint32_t n) {
                 if (!some || !n) return;
-                load(k, col, n);
+                take(k, col, n);
+                if (C > 0 && row + stride < g.rows) fetch(row + stride, k, col, n);
                 each<E>([&](auto i) {
                     squares = fmaf(u[k][i], u[k][i], squares);
                     if (EVEN || i < n) along = fmaf(dy[k][i] * w[k][i], u[k][i], along);
@@ -276,13 +310,10 @@ struct Rows {
             const float back = along * g.over_width * s * s;
             chunks(g, [&](auto k, uint32_t col, uint32_t n) {
                 if (!some || !n) return;
-                if constexpr (C == 0) load(k, col, n);
+                if constexpr (C == 0) take(k, col, n);
                 float dv[E];
                 each<E>([&](auto i) { dv[i] = s * fmaf(-u[k][i], back, dy[k][i] * w[k][i]); });
-                if (g.residual.p) {
-                    const Raw r = Io::load(g.residual.p, (int64_t)row * g.residual.row + col, n);
-                    each<E>([&](auto i) { dv[i] += T::up(r.v[i]); });
-                }
+                if (g.residual.p) each<E>([&](auto i) { dv[i] += T::up(later[k].v[i]); });
                 if (g.dresidual.p) Io::store(g.dresidual.p, (int64_t)row * g.dresidual.row + col, n, dv, g.stream);
                 if (g.dx.p) {
                     if (g.drop) Io::drop(dv, g.seed, numbers, row * g.width + col, g.drop, g.drop_all, g.keep);

@@ -38,7 +38,8 @@ public:
     void backward(const fg_norm_backward_args& a, hipStream_t stream);
 
 private:
-    uint64_t workgroups(uint64_t rows, bool back) const;
+    uint32_t teams() const;  // of a workgroup
+    uint64_t workgroups(uint64_t rows) const;
     fg_norm_kargs base(const char* op, int64_t rows, const float* weight, double dropout, uint64_t seed,
                        uint64_t offset, const int64_t* counter) const;
     HipBackend::DeviceHandle dev_;
