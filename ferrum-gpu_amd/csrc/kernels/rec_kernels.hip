@@ -27,7 +27,7 @@ using namespace fg::rec;
     FG_REC_STEP(NAME, T, 4)                                                                                     \
     FG_REC_STEP(NAME, T, 1)
 
-extern "C" __global__ __launch_bounds__(256) void fg_rec_reduce(fg_rec_kargs g) { reduce(g); }
+extern "C" __global__ __launch_bounds__(1024) void fg_rec_reduce(fg_rec_kargs g) { reduce(g); }
 
 // One code object, three builds of this file in parallel: FG_REC_F32, _BF16, _F16.
 #if defined(FG_REC_F32)

@@ -742,14 +742,21 @@ struct Rec {
     }
 };
 
-// The parameters' gradients from the parts' sums.
+// The parameters' gradients from the parts' sums: 64 of them for a workgroup, whose waves
+// share the parts.
 __device__ __forceinline__ void reduce(const fg_rec_kargs& g) {
-    const uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (e >= 3ull * g.channels) return;
+    __shared__ float sums[16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const uint64_t all = 3ull * g.channels, e = (uint64_t)blockIdx.x * 64 + lane;
+    const uint64_t each_wave = (g.parts + waves - 1) / waves, a = min(g.parts, wave * each_wave), b = min(g.parts, a + each_wave);
+    sums[wave][lane] = e < all ? ordered_sum(g.part + a * all + e, all, b - a) : 0.0f;
+    __syncthreads();
+    if (wave || e >= all) return;
     const uint32_t k = e / g.channels, ch = e % g.channels;
     float* to = k == 0 ? g.gdecay : k == 1 ? g.gbias_a : g.gbias_x;
     if (!to) return;
-    const float v = ordered_sum(g.part + e, 3ull * g.channels, g.parts);
+    float v = 0.0f;
+    for (uint32_t w = 0; w < waves; ++w) v += sums[w][lane];
     to[ch] = k == 0 ? v * -g.rate * softplus(g.decay[ch]).slope : v;
 }
 

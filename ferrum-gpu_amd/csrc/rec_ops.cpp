@@ -268,7 +268,7 @@ void RecurrencePlan::backward(const fg_recurrence_backward_args& a, hipStream_t 
         wide = wide && vector_ptr(p, 4 * FG_REC_LANE_CHANNELS);
     void* args[] = {&g};
     if (chains_) launch(dev_, stream, backward_[wide], (uint64_t)g.blocks * g.chains * g.tiles, 64 * waves(true), args, op);
-    if (g.gdecay || g.gbias_a || g.gbias_x) launch(dev_, stream, reduce_, ceil_div(3 * (uint64_t)g.channels, 256), 256, args, op);
+    if (g.gdecay || g.gbias_a || g.gbias_x) launch(dev_, stream, reduce_, ceil_div(3 * (uint64_t)g.channels, 64), 1024, args, op);
 }
 
 }  // namespace fg

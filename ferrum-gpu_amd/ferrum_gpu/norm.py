@@ -14,7 +14,7 @@ import struct
 
 from ferrum_gpu import _native as _n
 from ferrum_gpu.hip import Device
-from ferrum_gpu.ssm import _BYTES, _DTYPES, _Plan, _check_dtype, _dtype_of, _flat, _rows, _stream
+from ferrum_gpu.ssm import _DTYPES, _Plan, _address, _check_dtype, _dtype_of, _flat, _rows, _stream, _torch_types
 
 __all__ = ["NormPlan"]
 
@@ -45,7 +45,7 @@ class NormPlan(_Plan):
     def __init__(self, rows: int, width: int, device: Device, dtype="bfloat16", eps: float = 1e-6, group: int = 0):
         self.device, self.rows, self.width = device, int(rows), int(width)
         self.dtype, self.eps, self.group = _check_dtype(dtype), float(eps), int(group)
-        self._p = ctypes.c_void_p()
+        self._at, self._p = device.ordinal, ctypes.c_void_p()
         shape = _shape_pack(self.rows, self.width, _DTYPES[self.dtype], self.group, self.eps)
         _n.check(_n.lib.fg_norm_plan_create(device.handle, shape, ctypes.byref(self._p)))
         self._groups = -(-self.width // self.group) if self.group else 1
@@ -54,11 +54,13 @@ class NormPlan(_Plan):
         if x is None:
             return 0, 0, 0
         try:  # what a tensor passes in most calls, which may be bound by the host
-            if x.shape == (n, self.width) and _dtype_of(x) == self.dtype and x.get_device() == self.device.ordinal:
+            if x.shape == (n, self.width) and x.dtype is _torch_types[self.dtype] and x.get_device() == self._at:
+                if x.is_contiguous():
+                    return x.data_ptr(), 0, self.width
                 row, element = x.stride()
                 if element == 1:
                     return x.data_ptr(), 0, row
-        except AttributeError:
+        except (AttributeError, KeyError):  # no tensor, or the first one
             pass
         return _rows(x, (n,), self.width, (), self.dtype, self.device.ordinal, what)
 
@@ -75,14 +77,15 @@ class NormPlan(_Plan):
             if element != 1 and self.width > 1:
                 raise ValueError(f"out: the elements of a row must be adjacent (strides {tuple(x.stride())})")
             return x.data_ptr(), 0, row
-        from ferrum_gpu.ssm import _address
-
         return _address(x, n * self.width, "out"), 0, self.width
 
     def _count(self, x, rows) -> int:
         if rows is not None:
             return int(rows)
-        return x.shape[0] if hasattr(x, "data_ptr") and len(x.shape) else self.rows
+        try:
+            return x.shape[0]
+        except (AttributeError, IndexError):  # no tensor, or one that the checks refuse
+            return self.rows
 
     def _weight(self, x, what: str) -> int:
         return _flat(x, (self.width,), "float32", 4 * self.width, self.device.ordinal, what)
