@@ -5,19 +5,17 @@
 
 #include "ssm_args.h"
 
+#define FG_REC_CHANNELS 64                        /* of a workgroup */
 #define FG_REC_LANE_CHANNELS 2                    /* of a lane */
-/* Rows of lanes of a wave, each a segment of tokens: 128 channels of a workgroup
- * forward, 64 backward. */
-#define FG_REC_ROWS 2
-#define FG_REC_BACK_ROWS 2
-#define FG_REC_CHANNELS(rows) (64 * FG_REC_LANE_CHANNELS / (rows))
+#define FG_REC_ROWS 2                             /* rows of lanes of a wave, each a segment of tokens */
 #define FG_REC_WAVES 8                            /* of a workgroup, at most */
-#define FG_REC_BACK_WAVES 4
-#define FG_REC_SEGMENT(bytes) ((bytes) == 2 ? 16 : 8) /* tokens of a lane */
+#define FG_REC_BACK_WAVES 4                       /* backward */
+#define FG_REC_SEGMENT(bytes) ((bytes) == 2 ? 16 : 8) /* tokens of a lane, by its elements' bytes */
 #define FG_REC_BACK_SEGMENT 8
 #define FG_REC_AHEAD(segment) ((segment) / 2)     /* tokens whose rows a lane has on their way */
-#define FG_REC_CHECK (FG_REC_BACK_ROWS * FG_REC_BACK_SEGMENT * FG_REC_BACK_WAVES) /* tokens between the states
-                                                    that a forward pass leaves for its backward pass */
+#define FG_REC_CHECK (FG_REC_ROWS * FG_REC_BACK_SEGMENT * FG_REC_BACK_WAVES) /* tokens between the states that a
+                                                    forward pass leaves for its backward pass, at the
+                                                    starts of waves of both */
 
 /* Tiles whose pairs a workgroup composes itself, see rec_scan.hpp. */
 #define FG_REC_GROUP 4
@@ -25,8 +23,7 @@
  * in a line of 64 bytes of its own, and behind all of them for each tile FG_REC_WORDS
  * 8-byte words of each channel. */
 #define FG_REC_WORDS 3
-#define FG_REC_CHAIN_BYTES(across, tiles, rows) \
-    ((across) * (64 + 8ull * FG_REC_WORDS * FG_REC_CHANNELS(rows) * (tiles)))
+#define FG_REC_CHAIN_BYTES(across, tiles) ((across) * (64 + 8ull * FG_REC_WORDS * FG_REC_CHANNELS * (tiles)))
 
 typedef struct {
     fg_ssm_view x, ga, gx, out; /* backward: out is the output's gradient */
@@ -39,7 +36,7 @@ typedef struct {
     float* check;           /* [chains][checks][channels], states before each FG_REC_CHECK tokens;
                                packed, behind them: [sequences][channels] initial states */
     float* part;            /* [parts][3][channels] */
-    unsigned long long* chain; /* FG_REC_CHAIN_BYTES(chains * blocks, tiles, rows); null where a chain is one tile */
+    unsigned long long* chain; /* FG_REC_CHAIN_BYTES(chains * blocks, tiles); null where a chain is one tile */
     uint64_t over_tiles;    /* (2^64 - 1) / tiles */
     uint32_t over_across, over_blocks; /* (2^32 - 1) / (chains * blocks), / blocks */
     uint64_t tokens;        /* of a chain: a dense sequence's, packed those of all */

@@ -9,11 +9,11 @@ using namespace fg::rec;
 #define FG_REC_ONE(NAME, T, SUFFIX, WIDE, PACKED, STREAM)                                                       \
     extern "C" __global__ __launch_bounds__(64 * FG_REC_WAVES) __attribute__((amdgpu_waves_per_eu(4)))          \
     void fg_rec_##NAME##SUFFIX(fg_rec_kargs g) {                                                               \
-        Rec<T, WIDE, PACKED, FG_REC_ROWS, STREAM>::forward(g);                                                 \
+        Rec<T, WIDE, PACKED, STREAM>::forward(g);                                                 \
     }                                                                                                          \
     extern "C" __global__ __launch_bounds__(64 * FG_REC_BACK_WAVES) __attribute__((amdgpu_waves_per_eu(3)))     \
     void fg_rec_back_##NAME##SUFFIX(fg_rec_kargs g) {                                                          \
-        Rec<T, WIDE, PACKED, FG_REC_BACK_ROWS, STREAM>::backward(g);                                           \
+        Rec<T, WIDE, PACKED, STREAM>::backward(g);                                           \
     }
 #define FG_REC_STEP(NAME, T, V)                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void fg_rec_step_##NAME##_v##V(fg_rec_step_kargs g) { step<T, V>(g); }

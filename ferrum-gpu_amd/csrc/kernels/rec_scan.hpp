@@ -5,13 +5,13 @@
 //   a = exp(-rate softplus(decay) r), m = sqrt(1 - a^2)
 //   h_t = a h_{t-1} + m i x,  out = h_t
 //
-// A workgroup has 128 channels forward, 64 backward.  A lane takes two neighbouring
-// channels through a segment of S tokens; a wave has one segment, or one for each of its two
-// rows of 32 lanes, and its workgroup's waves follow one another: a tile.  A lane works out a and b = m i x of its tokens once and keeps them in
-// registers; what a segment does to the state that enters it is h -> p h + q, with
-// p the product of its a and q its own state from 0.  These pairs pass from row to
-// row by lane exchanges and from wave to wave through LDS, and each lane runs over
-// its tokens again from the state that then enters them.
+// A workgroup has 64 channels.  A lane takes two neighbouring channels through a segment of
+// S tokens, the two rows of 32 lanes of a wave two segments that follow one another, its
+// waves the segments behind those: a tile.  A lane works out a and b = m i x of its tokens
+// once and keeps them in registers; what a segment does to the state that enters it is
+// h -> p h + q, with p the product of its a and q its own state from 0.  These pairs
+// pass from row to row by lane exchanges and from wave to wave through LDS, and each lane runs
+// over its tokens again from the state that then enters them.
 //
 // From tile to tile of a chain they pass through memory, in one launch.  A word of 8
 // bytes holds a float and the launch's tag, so that what is read with the tag is
@@ -28,6 +28,19 @@
 //
 // Packed sequences are one chain of rows: a sequence's first token takes its
 // initial state in place of the one before it.
+//
+// Measured (bfloat16, us; a copy of as many bytes would take): 4 x 2048 tokens x 4096
+// channels forward 65 (40), 1 x 8192 x 2048 40 (20), 4 x 1024 x 2048 forward 21 (10), backward
+// 38 (17) and 3 for the parameters' sums.  Forward is bound by its arithmetic and by memory
+// about alike: 33 us of vector instructions (39 of an element: 6 exponentials, reciprocals and
+// roots, which count twice) and 40 of rows, of which workgroups that start at a time do the
+// one after the other; without arithmetic it would take 59, without the chain 4 less.
+// Backward holds five factors of each token, so a SIMD has three waves of it, four of forward.
+// Other shapes, 4 x 2048 x 4096: four channels of a lane 92 (each wave's share of the
+// parameters, exchanges and addresses falls on half as many tokens), 128 channels of a
+// workgroup 71, four waves of one 72, six 83 (two SIMDs of four get twice the waves), one
+// workgroup through a sequence's tiles one by one 81, and 254 for 1 x 8192 x 2048.  Backward, training
+// step 4 x 1024 x 2048: six waves 85, eight of half as many tokens 67, two 64, 62 so.
 #pragma once
 
 #include "rec_args.h"
@@ -37,6 +50,8 @@ namespace fg {
 namespace rec {
 
 using namespace ssm;
+
+constexpr int CHANNELS = FG_REC_CHANNELS;
 
 __device__ __forceinline__ float gate(float g, float scaled_bias) {
     return __builtin_amdgcn_rcpf(1.0f + exp2_(fmaf(-kLog2e, g, scaled_bias)));
@@ -90,6 +105,9 @@ __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
     Place p;
     uint32_t rest;
     p.tile = quotient(blockIdx.x, across, g.over_across, rest);
+    // Workgroups go to the eight XCDs in turn: neighbouring channels, whose rows share lines where they
+    // are not aligned to them, to the same one (training step 4 x 1024 x 2048 66.2 -> 64.8 us, packed
+    // 7001 x 1500 42.6 -> 42.0).
     if (across % 8 == 0) rest = rest % 8 * (across / 8) + rest / 8;
     p.chain = quotient(rest, g.blocks, g.over_blocks, p.block);
     p.tag = 0;
@@ -111,33 +129,30 @@ __device__ __forceinline__ Place place_of(const fg_rec_kargs& g) {
 }
 
 // A tile's words; the same for all lanes.
-template <int CHANNELS>
 __device__ __forceinline__ char* words(const fg_rec_kargs& g, const Place& p, uint32_t tile) {
     const uint64_t across = (uint64_t)g.blocks * g.chains, place = tile * across + (uint64_t)p.chain * g.blocks + p.block;
     return (char*)g.chain + uniform((int64_t)(64 * across + place * (8 * FG_REC_WORDS * CHANNELS)));
 }
 // Word `which` of a thread's channel.
-template <int CHANNELS>
 __device__ __forceinline__ void tell(char* at, int which, uint32_t ch, uint32_t tag, float v) {
     unsigned long long* to = (unsigned long long*)(at + 8 * CHANNELS * which + 8 * ch);
     __hip_atomic_store(to, (unsigned long long)tag << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int CHANNELS>
 __device__ __forceinline__ unsigned long long ask(const char* at, int which, uint32_t ch) {
     const unsigned long long* from = (const unsigned long long*)(at + 8 * CHANNELS * which + 8 * ch);
     return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// For the first waves, a thread for each channel: tells the tile's pair p, q and returns
+// For the first wave, a thread for each channel: tells the tile's pair p, q and returns
 // the state that enters the tile, `first` for a chain's first one.
-template <bool PACKED, int CHANNELS>
+template <bool PACKED>
 __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at, float p, float q, float first) {
     const uint32_t ch = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
     const bool last = at.tile + 1 == g.tiles;
-    char* mine = words<CHANNELS>(g, at, at.tile);
+    char* mine = words(g, at, at.tile);
     if (!last) {
-        tell<CHANNELS>(mine, 0, ch, at.tag, p);
-        tell<CHANNELS>(mine, 1, ch, at.tag, q);
+        tell(mine, 0, ch, at.tag, p);
+        tell(mine, 1, ch, at.tag, q);
     }
     unsigned long long w[2 * FG_REC_GROUP];
     float state = first;
@@ -146,12 +161,12 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         bool all = true;
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) {
-                const char* from = words<CHANNELS>(g, at, at.tile - in_group + k);
-                w[2 * k] = ask<CHANNELS>(from, 0, ch);
-                w[2 * k + 1] = ask<CHANNELS>(from, 1, ch);
+                const char* from = words(g, at, at.tile - in_group + k);
+                w[2 * k] = ask(from, 0, ch);
+                w[2 * k + 1] = ask(from, 1, ch);
             }
         });
-        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask<CHANNELS>(words<CHANNELS>(g, at, at.tile - in_group - 1), 2, ch);
+        if (at.tile >= FG_REC_GROUP) w[2 * FG_REC_GROUP - 1] = ask(words(g, at, at.tile - in_group - 1), 2, ch);
         each<FG_REC_GROUP - 1>([&](auto k) {
             if (k < in_group) all = all && w[2 * k] >> 32 == at.tag && w[2 * k + 1] >> 32 == at.tag;
         });
@@ -169,7 +184,7 @@ __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at
         if (k < in_group)
             state = enter<PACKED>(__uint_as_float((uint32_t)w[2 * k]), __uint_as_float((uint32_t)w[2 * k + 1]), state);
     });
-    if (!last && in_group == FG_REC_GROUP - 1) tell<CHANNELS>(mine, 2, ch, at.tag, enter<PACKED>(p, q, state));
+    if (!last && in_group == FG_REC_GROUP - 1) tell(mine, 2, ch, at.tag, enter<PACKED>(p, q, state));
     return state;
 }
 
@@ -179,11 +194,11 @@ __device__ __forceinline__ float finite(float x) {
     return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -most), most);
 }
 
-template <class T, bool WIDE, bool PACKED, int ROWS, bool STREAM>
+template <class T, bool WIDE, bool PACKED, bool STREAM>
 struct Rec {
     using raw = typename T::raw;
-    // ROW: lanes that share a token; CHANNELS: of a workgroup.
-    static constexpr int V = FG_REC_LANE_CHANNELS, ROW = 64 / ROWS, CHANNELS = FG_REC_CHANNELS(ROWS);
+    static constexpr int V = FG_REC_LANE_CHANNELS, ROWS = FG_REC_ROWS, ROW = 64 / ROWS;  // ROW: lanes that share a token
+    static_assert(ROW * V == CHANNELS && ROWS == 2, "one exchange between the rows of lanes");
     struct __attribute__((aligned(V * 4))) Floats {
         float v[V];
     };
@@ -349,17 +364,14 @@ struct Rec {
     template <bool BACK>
     static __device__ __forceinline__ void rows(float (&p)[V], float (&q)[V], float (&ep)[V], float (&eq)[V],
                                                 const Lane& l) {
-        static_assert(ROWS <= 2, "one exchange at most");
+        const bool behind = l.row == (BACK ? 0 : 1);
         each<V>([&](auto c) {
-            ep[c] = 1.0f, eq[c] = 0.0f;
-            if constexpr (ROWS == 2) {
-                const bool behind = l.row == (BACK ? 0 : 1);
-                const float p1 = __shfl_xor(p[c], ROW), q1 = __shfl_xor(q[c], ROW);
-                if (behind) {
-                    ep[c] = p1, eq[c] = q1;
-                    q[c] = enter<PACKED>(p[c], q[c], q1);
-                    p[c] = through<PACKED>(p1, p[c]);
-                }
+            const float p1 = __shfl_xor(p[c], ROW), q1 = __shfl_xor(q[c], ROW);
+            ep[c] = behind ? p1 : 1.0f;
+            eq[c] = behind ? q1 : 0.0f;
+            if (behind) {
+                q[c] = enter<PACKED>(p[c], q[c], q1);
+                p[c] = through<PACKED>(p1, p[c]);
             }
         });
     }
@@ -391,7 +403,6 @@ struct Rec {
     static __device__ __forceinline__ void enter_tile(const fg_rec_kargs& g, const Place& at, const Totals& t, float* lds,
                                                       const float* first, uint32_t wave, uint32_t waves, const Lane& l,
                                                       float (&h)[V]) {
-        static_assert(CHANNELS <= 64 * FG_REC_WAVES, "a thread for each channel, where there are several tiles");
         if (g.tiles == 1) {
             params(h, first, l);
             return;
@@ -406,7 +417,7 @@ struct Rec {
                 p = through<PACKED>(p, p2);
             }
             const bool some = first && at.block * CHANNELS + ch < g.channels;
-            lds[ch] = entering<PACKED, CHANNELS>(g, at, p, q, some ? first[ch] : 0.0f);
+            lds[ch] = entering<PACKED>(g, at, p, q, some ? first[ch] : 0.0f);
         }
         __syncthreads();
         const Floats v = *(const Floats*)&lds[l.ch];
@@ -535,8 +546,7 @@ struct Rec {
                 q[c] = first ? b[j][c] : fmaf(a[j][c], q[c], b[j][c]);
                 p[c] *= a[j][c];
             });
-            // as many rows on their way as memory needs, not all: rows of the workgroups that start
-            // at a time would wait for one another, and all of them for the first
+            // rows of half the segment on their way, of all of it no less time (64 us, 65 so) but more registers
             if constexpr (j + D < S) source.next(in, d, j + D, l);
             __builtin_amdgcn_sched_barrier(0);  // tokens mixed would not fit the registers of four waves
         });
@@ -718,8 +728,7 @@ struct Rec {
         static_assert(sizeof(both) >= 4 * 3 * FG_REC_WAVES * CHANNELS, "the sums fit");
         each<3>([&](auto k) {
             each<V>([&](auto c) {
-                float v = sums[k][c];
-                if (ROWS == 2) v += __shfl_xor(v, ROW);
+                const float v = sums[k][c] + __shfl_xor(sums[k][c], ROW);
                 if (l.row == 0) all[(wave * 3 + k) * CHANNELS + l.ch + c] = v;
             });
         });

@@ -117,6 +117,7 @@ RecurrencePlan::RecurrencePlan(const HipBackend::DeviceHandle& dev, const Recurr
     size_of(op, "states", {4, s.sequences, s.channels});
     chains_ = s.packed ? std::min<int64_t>(s.sequences, 1) : s.sequences;
     rows_ = s.packed ? s.tokens : s.length;
+    blocks_ = (uint32_t)ceil_div(s.channels, FG_REC_CHANNELS);
     const std::string tail = std::string(kTypes[s.dtype]) + (s.packed ? "_packed" : "");
     const bool stream = (uint64_t)s.channels * rows_ * chains_ * kBytes[s.dtype] >= kStreamBytes;
     for (int wide = 0; wide < 2; ++wide) {
@@ -129,11 +130,7 @@ RecurrencePlan::RecurrencePlan(const HipBackend::DeviceHandle& dev, const Recurr
 }
 
 uint32_t RecurrencePlan::wave_tokens(bool back) const {
-    return back ? FG_REC_BACK_ROWS * FG_REC_BACK_SEGMENT : FG_REC_ROWS * FG_REC_SEGMENT(kBytes[s_.dtype]);
-}
-
-uint32_t RecurrencePlan::blocks(bool back) const {
-    return (uint32_t)ceil_div(s_.channels, FG_REC_CHANNELS(back ? FG_REC_BACK_ROWS : FG_REC_ROWS));
+    return FG_REC_ROWS * (back ? FG_REC_BACK_SEGMENT : FG_REC_SEGMENT(kBytes[s_.dtype]));
 }
 
 // As many as the rows of a chain take.
@@ -144,16 +141,16 @@ uint32_t RecurrencePlan::waves(bool back) const {
 
 uint64_t RecurrencePlan::places(bool back) const {
     const uint64_t tiles = std::max<uint64_t>(1, ceil_div(rows_, wave_tokens(back) * waves(back)));
-    const uint64_t n = (uint64_t)size_of("recurrence", "launch", {blocks(back), (int64_t)chains_, (int64_t)tiles});
+    const uint64_t n = (uint64_t)size_of("recurrence", "launch", {blocks_, (int64_t)chains_, (int64_t)tiles});
     if (n > 0xffffffffull / (64 * waves(back))) invalid("recurrence: too large for one launch");
     return n;
 }
 
 // None where every chain is one tile.
 Buffer<char, HipBackend> RecurrencePlan::chain(bool back) const {
-    const uint64_t n = places(back), across = blocks(back) * chains_;
+    const uint64_t n = places(back), across = blocks_ * chains_;
     if (n <= across) return {};
-    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(across, n / across, back ? FG_REC_BACK_ROWS : FG_REC_ROWS));
+    return Buffer<char, HipBackend>(dev_, FG_REC_CHAIN_BYTES(across, n / across));
 }
 
 size_t RecurrencePlan::checkpoint_bytes() const {
@@ -181,7 +178,7 @@ fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in
     g.seqs = (uint32_t)s_.sequences;
     g.chains = (uint32_t)chains_;
     g.channels = (uint32_t)s_.channels;
-    g.blocks = blocks(back);
+    g.blocks = blocks_;
     g.rate = (float)s_.rate;
     const uint64_t n = places(back), across = (uint64_t)g.blocks * g.chains;
     g.tiles = across ? (uint32_t)(n / across) : 1;

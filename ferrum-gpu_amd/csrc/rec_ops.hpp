@@ -38,10 +38,9 @@ public:
     void backward(const fg_recurrence_backward_args& a, hipStream_t stream);
 
 private:
-    // Of a pass, which has kernels of its own: tokens of a wave, workgroups over the channels, waves of a
+    // Of a pass, which has kernels of its own: tokens of a wave, waves of a
     // workgroup, tiles over all chains and channels, and what they pass on.
     uint32_t wave_tokens(bool back) const;
-    uint32_t blocks(bool back) const;
     uint32_t waves(bool back) const;
     uint64_t places(bool back) const;
     Buffer<char, HipBackend> chain(bool back) const;
@@ -49,6 +48,7 @@ private:
     HipBackend::DeviceHandle dev_;
     fg_recurrence_shape s_;
     uint64_t chains_, rows_;  // chains of so many rows: dense, the sequences; packed, one
+    uint32_t blocks_;         // workgroups over the channels
     HipBackend::KernelHandle forward_[2] = {}, backward_[2] = {}, reduce_;  // [any, wide]
     Buffer<char, HipBackend> ahead_, back_;  // what the tiles pass on, back_ from the first backward call on
     std::mutex mu_;
