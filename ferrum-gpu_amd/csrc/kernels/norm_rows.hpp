@@ -13,7 +13,18 @@
 //   dweight = sum over rows of grad_out u s
 //
 // A team of threads takes a row, each thread chunks of 16 bytes of it: the row is
-// read once and stays in registers.  Rows that do not fit are read again (C = 0).
+// read once and stays in registers, the weight too, and the next row is loaded while
+// one is summed and written.  Rows that do not fit are read again (C = 0).  The weight's
+// gradient is summed by each team over its rows and then over the teams, in a fixed order.
+//
+// out is taken of the unrounded v; the backward pass, which reads the stored sum, is the
+// gradient at what was stored.
+//
+// Bound by memory.  Measured (8192 rows x 4096, bfloat16, us; a copy of as many bytes would take):
+// with the residual to 8 bits 44 (35), with dropout and the residual 50 (40), backward 68 (50) and 5
+// for the weight's gradient; dropout alone 22 (20).  Dropout is 18 vector instructions of an
+// element, most of them the generator's 64-bit products, backward 24 others: 36 us of the 68.
+// Teams of 256 with two chunks a thread 51, without the next row's loads 53, with ordinary stores 57.
 //
 // Dropout keeps element e (row-major) where 32 bits are at least p 2^32: half e % 2 of
 // the seed's splitmix64 number offset + e / 2 (fill.hpp), so no mask is stored.

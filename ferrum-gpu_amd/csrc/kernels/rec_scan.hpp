@@ -30,9 +30,9 @@
 // initial state in place of the one before it.
 //
 // Measured (bfloat16, us; a copy of as many bytes would take): 4 x 2048 tokens x 4096
-// channels forward 65 (40), 1 x 8192 x 2048 40 (20), 4 x 1024 x 2048 forward 21 (10), backward
-// 38 (17) and 3 for the parameters' sums.  Forward is bound by its arithmetic and by memory
-// about alike: 33 us of vector instructions (39 of an element: 6 exponentials, reciprocals and
+// channels forward 62 (40), 1 x 8192 x 2048 38 (20), 4 x 1024 x 2048 forward 20 (10), backward
+// 39 (17) and 5 for the parameters' sums.  Forward is bound by its arithmetic and by memory
+// about alike: 35 us of vector instructions (35 of an element: 6 exponentials, reciprocals and
 // roots, which count twice) and 40 of rows, of which workgroups that start at a time do the
 // one after the other; without arithmetic it would take 59, without the chain 4 less.
 // Backward holds five factors of each token, so a SIMD has three waves of it, four of forward.

@@ -409,7 +409,8 @@ class RecurrencePlan(_Plan):
         a = exp(-rate softplus(decay) r)
         h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
 
-    With ``tokens`` the sequences are packed; ``length`` is not used then.
+    With ``tokens`` the sequences are packed; ``length`` is not used then.  Both
+    passes use the plan's workspaces, so calls of one plan follow one another.
     """
 
     _destroy, _get_info = _n.lib.fg_recurrence_plan_destroy, _n.lib.fg_recurrence_plan_get_info

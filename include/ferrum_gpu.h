@@ -552,7 +552,8 @@ FG_API int fg_scan_step(fg_device_t dev, const fg_scan_step_args *args, fg_strea
  *   a = exp(-rate softplus(decay[d]) r)
  *   h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
  * Rows, packed sequences (their number of tokens is not held against `length`),
- * states and workspaces as for the scan. */
+ * states and workspaces as for the scan; the forward pass uses the plan's workspaces
+ * too, so all calls of a plan follow one another. */
 typedef struct fg_recurrence_plan *fg_recurrence_plan_t;
 
 typedef struct fg_recurrence_shape {
@@ -594,8 +595,9 @@ typedef struct fg_recurrence_backward_args {
 FG_API int fg_recurrence_plan_create(fg_device_t dev, const fg_recurrence_shape *shape, fg_recurrence_plan_t *out);
 FG_API int fg_recurrence_plan_destroy(fg_recurrence_plan_t plan);
 FG_API int fg_recurrence_checkpoint_bytes(fg_recurrence_plan_t plan, size_t *bytes);
-/* Tokens that a workgroup works through at a time, and the GPU memory that the
- * plan holds (the backward pass's from its first call on). */
+/* Tokens of a workgroup, and the GPU memory that the plan holds (the backward pass's
+ * from its first call on): 1536 bytes for each workgroup of a pass whose sequences take more
+ * than one, and 768 for each of the backward pass's. */
 typedef struct fg_recurrence_plan_info {
     int64_t forward_tokens, backward_tokens, workspace_bytes;
 } fg_recurrence_plan_info;
@@ -621,8 +623,9 @@ FG_API int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args *ar
 
 /* ------------------------------------------------- residual norm, dropout */
 
-/* What stands around the filters of a block, on rows of its residual stream (see
- * above; row r starts row_stride * r elements from ptr, seq_stride is not used).
+/* What stands around the filters of a block, on rows of its residual stream.  Arrays of
+ * rows, types and streams (FG_STREAM_NULL too) as for the filters above; row r starts
+ * row_stride * r elements from ptr, seq_stride is not used.
  *
  *   v = dropout(x) + residual, out = v / sqrt(mean(v^2) + eps) * weight
  *   sum = v, rounded to the rows' type
