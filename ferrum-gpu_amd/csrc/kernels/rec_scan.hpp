@@ -521,12 +521,14 @@ struct Rec {
         Params w;
         w.load(g, block, l);
         const Marks m = marks<S>(g, t0, l, look);
+        // whether a sequence begins or ends in the wave's rows: few waves' do
+        const bool edge = PACKED && !__all(m.in == ALL && !m.first && !m.last);
         float a[S][V], b[S][V], p[V], q[V];
         each<V>([&](auto c) { p[c] = 1.0f, q[c] = 0.0f; });
         each<S>([&](auto j) {
             constexpr int d = j % D;
             if constexpr (PACKED) {
-                if (!(m.in >> j & 1)) nothing(in[0][d], in[1][d], in[2][d]);
+                if (edge && !(m.in >> j & 1)) nothing(in[0][d], in[1][d], in[2][d]);
             }
             each<V>([&](auto c) {
                 const float r = gate(T::up(in[1][d].v[c]), w.ba[c]), i = gate(T::up(in[2][d].v[c]), w.bx[c]);
@@ -534,7 +536,7 @@ struct Rec {
                 a[j][c] = s.a;
                 b[j][c] = __builtin_amdgcn_sqrtf(s.m2) * i * T::up(in[0][d].v[c]);
             });
-            const bool first = PACKED && (m.first >> j & 1);
+            const bool first = PACKED && edge && (m.first >> j & 1);
             if (first) {
                 float init[V];
                 const uint32_t s = sequence(g, t0 + l.row * S + j);
@@ -563,7 +565,7 @@ struct Rec {
         each<V>([&](auto c) { h[c] = enter<PACKED>(ep[c], eq[c], h[c]); });
         char* po = const_cast<char*>(base(g.out, chain, t0, block));
         const uint32_t step = (uint32_t)g.out.row * (uint32_t)sizeof(raw), off = fresh(l.row * S * step + l.off);
-        if (PACKED ? __all(m.in == ALL && !m.first && !m.last) : FULL) {
+        if (PACKED ? !edge : FULL) {
             each<S>([&](auto j) {
                 each<V>([&](auto c) { h[c] = fmaf(a[j][c], h[c], b[j][c]); });
                 store(po, off, l, h);
