@@ -370,6 +370,34 @@ def test_captured_calls_replay(gpu_device):
     assert not torch.equal(masks[0], masks[1])
 
 
+def test_rows_far_apart(gpu_device):
+    """Rows whose offsets pass 32 bits: 2^25 elements between rows, 80 of them in one buffer of 5.4 GB."""
+    from ferrum_gpu import _native as N
+    n, width, row = 80, 200, 1 << 25
+    x = rows((n, width), "bfloat16", 1).contiguous()
+    buf = ferrum_gpu.hip.DeviceBuffer(gpu_device, 2 * ((n - 1) * row + 512))
+    for r in range(n):
+        N.check(N.lib.fg_copy_h2d(gpu_device.handle, buf.ptr + 2 * r * row, x[r].data_ptr(), 2 * width))
+
+    class Rows:
+        shape, dtype = x.shape, x.dtype
+        def __init__(self, at): self.at = at
+        def data_ptr(self): return buf.ptr + 2 * self.at
+        def get_device(self): return gpu_device.ordinal
+        def stride(self): return row, 1
+        def is_contiguous(self): return False
+
+    plan, outs = NormPlan(n, width, gpu_device), [fill((n, width), "bfloat16") for _ in range(3)]
+    plan.forward(up(x), outs[0])
+    plan.forward(Rows(0), outs[1])
+    plan.forward(up(x), Rows(256))
+    gpu_device.sync()
+    for r in range(n):
+        N.check(N.lib.fg_copy_d2h(gpu_device.handle, outs[2].cpu[r].data_ptr(), buf.ptr + 2 * (r * row + 256), 2 * width))
+    assert same(outs[0], outs[1]) and torch.equal(outs[2].cpu, outs[0].get())
+    buf.free()
+
+
 def test_device_buffers_and_addresses(gpu_device):
     n, width = 5, 100
     x, residual = up(rows((n, width), "float32", 1)), up(rows((n, width), "float32", 2))

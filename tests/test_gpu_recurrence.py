@@ -548,3 +548,72 @@ def test_plans_say_how_they_run(gpu_device):
     plan = ssm.RecurrencePlan(2, 40, 64, gpu_device)
     got = plan.describe()
     assert got["forward_tokens"] >= 32 and got["backward_tokens"] >= 32
+
+
+@pytest.mark.parametrize("dtype,channels", [("bfloat16", 64), ("float32", 130), ("float16", 66)])
+def test_rows_at_odd_places(gpu_device, dtype, channels):
+    """Rows that begin at any element give what aligned ones give, forward and backward."""
+    lead = (2, 300)
+    v = inputs(lead, channels, dtype)
+    plan = ssm.RecurrencePlan(*lead, channels, gpu_device, dtype=dtype)
+    grad, decay = torch.randn(*lead, channels).to(TYPES[dtype]), up(v["decay"])
+    seen = []
+    for odd in (0, 1):
+        wide = lambda x: torch.nn.functional.pad(x, (odd, odd))  # noqa: E731
+        cut = lambda x: x[..., odd:odd + channels]  # noqa: E731
+        x, ga, gx, dy = (cut(up(wide(t))) for t in (v["x"], v["gate_a"], v["gate_x"], grad))
+        outs = [fill((*lead, channels + 2 * odd), dtype) for _ in range(4)]
+        check, sums = room(plan.checkpoint_bytes), fill((channels,))
+        plan.forward(x, ga, gx, decay, cut(outs[0]), checkpoints=check)
+        plan.backward(x, ga, gx, decay, dy, check, grad_x=cut(outs[1]), grad_gate_a=cut(outs[2]),
+                      grad_gate_x=cut(outs[3]), grad_decay=sums)
+        seen.append([*(cut(o).get() for o in outs), sums.get()])
+        if odd:
+            assert all((o.get()[..., [0, -1]] == 7).all() for o in outs)
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+
+
+def test_packed_sequences_of_one_token(gpu_device):
+    """As many as three looks of 64 lanes find, against the single token's call; some without any."""
+    n, ch = 9000, 66
+    lengths = torch.ones(n, dtype=torch.int64)
+    lengths[::7] = 0
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]).to(torch.int32)
+    rows = int(offsets[-1])
+    v = inputs((rows,), ch, "float32")
+    d = {k: up(t) for k, t in v.items()}
+    initial = torch.randn(n, ch)
+    out, final = fill((rows, ch)), fill((n, ch))
+    ssm.RecurrencePlan(n, 1, ch, gpu_device, dtype="float32", tokens=rows).forward(
+        d["x"], d["gate_a"], d["gate_x"], d["decay"], out, bias_a=d["bias_a"], bias_x=d["bias_x"], initial=up(initial),
+        final=final, offsets=up(offsets))
+    some = torch.nonzero(lengths)[:, 0]
+    state, want = up(initial), fill((rows, ch))
+    ssm.recurrence_step(gpu_device, **d, state=state, out=want, slots=up(some.to(torch.int32)))
+    assert np.abs(values(out) - values(want)).max() <= 500 * U * 5
+    assert np.abs(values(final) - values(state)).max() <= 500 * U * 5
+    none = torch.nonzero(lengths == 0)[:, 0]
+    assert torch.equal(final.get()[none], initial[none])
+
+
+def test_rows_far_apart(gpu_device):
+    """Rows whose offsets pass 32 bits: 2^25 elements between rows, 96 of them in one buffer of 6.4 GB."""
+    from gpu_tensor import Far
+    from ferrum_gpu.hip import DeviceBuffer
+    n, ch, row = 96, 64, 1 << 25
+    v = inputs((1, n), ch, "bfloat16")
+    buf = DeviceBuffer(gpu_device, 2 * ((n - 1) * row + 4 * ch))
+    far = [Far(buf, t, row, k * ch) for k, t in enumerate((v["x"], v["gate_a"], v["gate_x"], torch.zeros_like(v["x"])))]
+    plan, decay = ssm.RecurrencePlan(1, n, ch, gpu_device), up(v["decay"])
+    check, grad = room(plan.checkpoint_bytes), like(v["x"]).normal_()
+    out, dx, da = like(v["x"]), like(v["x"]), like(v["x"])
+    plan.forward(up(v["x"]), up(v["gate_a"]), up(v["gate_x"]), decay, out, checkpoints=check)
+    plan.backward(up(v["x"]), up(v["gate_a"]), up(v["gate_x"]), decay, grad, check, grad_x=dx, grad_gate_a=da)
+    plan.forward(*far[:3], decay, far[3], checkpoints=check)
+    gpu_device.sync()
+    assert same(out, far[3])
+    ga = like(v["x"])
+    plan.backward(*far[:3], decay, grad, check, grad_x=far[3], grad_gate_a=ga)
+    gpu_device.sync()
+    assert same(dx, far[3]) and same(da, ga)
+    buf.free()
