@@ -92,10 +92,11 @@ struct Chunk {
             });
         }
     }
+    // A team may have more threads than the row has chunks: n is 0 for those, whose `at` lies behind the array.
     static __device__ __forceinline__ void floats(float (&x)[E], const float* p, uint32_t at, uint32_t n) {
         if (!p) {
             each<E>([&](auto i) { x[i] = 1.0f; });
-        } else if (EVEN || n >= E) {
+        } else if (EVEN ? n > 0 : n >= E) {
             const Floats f = *(const Floats*)(p + at);
             each<E>([&](auto i) { x[i] = f.v[i]; });
         } else {
