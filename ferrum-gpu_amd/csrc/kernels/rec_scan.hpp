@@ -304,9 +304,10 @@ struct Rec {
         const int64_t v = ((Scalars)(uint64_t)g.offsets)[uniform(s)], all = (int64_t)g.tokens;
         return v < 0 ? 0 : v > all ? all : v;
     }
-    // Of the packed sequences, the first that ends behind row t.
+    // Of the packed sequences, the first that ends behind row t.  One there is, unless the
+    // offsets fall: the last one then, so that no access leaves the states' arrays.
     static __device__ __forceinline__ uint32_t sequence(const fg_rec_kargs& g, int64_t t) {
-        uint32_t lo = 0, hi = g.seqs;
+        uint32_t lo = 0, hi = g.seqs - 1;
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2;
             if (offset(g, mid + 1) <= t) lo = mid + 1;

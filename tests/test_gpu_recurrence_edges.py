@@ -1,0 +1,45 @@
+"""The recurrence on the GPU where what it is given is at the edge of what it takes: offsets that fall, states in
+one array, parameters that are not finite, arrays large enough for the kernels that pass the caches."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from ferrum_gpu import ssm
+from gpu_tensor import fill, room, up, use, values
+from test_gpu_recurrence import TYPES, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def on_device(gpu_device):
+    yield from use(gpu_device)
+
+
+@pytest.mark.parametrize("dtype,channels", [("bfloat16", 64), ("float32", 37)])
+@pytest.mark.parametrize("tokens,offsets", [
+    (20, [0, 20, 5]), (20, [10, 20, 5]), (40, [9, 5, 40, 1, 1]), (700, [0, 600, 590, 700, 20]),
+    (90, [-4, 2, 9, 5, 2 ** 31 - 1, 1, 1, 1]), (700, [700, 0, 700, 0])])
+def test_falling_offsets_leave_what_lies_around(gpu_device, dtype, channels, tokens, offsets):
+    """Outputs are undefined; what is in front of and behind every array of states and of checkpoints stays."""
+    n = len(offsets) - 1
+    v = inputs((tokens,), channels, dtype)
+    d = {k: up(t) for k, t in v.items()}
+    at = up(torch.tensor(offsets, dtype=torch.int32))
+    plan = ssm.RecurrencePlan(n, tokens, channels, gpu_device, dtype=dtype, tokens=tokens)
+    around = [fill((n + 4, channels)) for _ in range(4)]
+    initial, final, grad_final, grad_initial = (a[2:n + 2] for a in around)
+    check = room(plan.checkpoint_bytes + 4096)
+    out, dx = fill((tokens + 4, channels), dtype), fill((tokens + 4, channels), dtype)
+    main = (d["x"], d["gate_a"], d["gate_x"], d["decay"])
+    grad = up(torch.randn(tokens, channels).to(TYPES[dtype]))
+    plan.forward(*main, out[2:tokens + 2], initial=initial, final=final, offsets=at, checkpoints=check)
+    plan.backward(*main, grad, check, grad_x=dx[2:tokens + 2], grad_final=grad_final, grad_initial=grad_initial, offsets=at)
+    gpu_device.sync()
+    assert (check.get()[plan.checkpoint_bytes:] == 0).all()
+    for a in (*around, out, dx):
+        got = values(a)
+        assert np.all(got[:2] == 7) and np.all(got[-2:] == 7)

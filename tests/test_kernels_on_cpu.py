@@ -37,3 +37,22 @@ def program(tmp_path_factory):
     ("f32", 3, 4100), ("f32", 2, 8188), ("f32", 2, 9001)])
 def test_norm_stays_within_its_arrays(program, dtype, rows, width):
     program("norm", dtype, rows, width)
+
+
+# 64 bits' definition at the sizes of one wave, one tile and several; offsets beyond the rows count as the nearest.
+@pytest.mark.parametrize("args", [
+    "f32 64 40 dense 1", "f32 61 700 dense 1", "bf16 66 300 dense 2", "bf16 64 1100 dense 1", "f32 1 1 dense 3", "f32 130 129 dense 2",
+    "bf16 64 700 packed 0 300 300 310 700", "f32 37 200 packed -5 40 250 300", "f32 66 150 packed 3 10 10 140 145",
+    "bf16 5 64 packed 0 1 2 3 4 5 6 64"])
+def test_recurrence_stays_within_its_arrays(program, args):
+    program("rec", *args.split())
+
+
+# A search over offsets that fall could answer with a sequence behind the last one: where a wave then finds one's first
+# or last token (as in the first three), it read or wrote a row behind the states' arrays.
+@pytest.mark.parametrize("dtype,channels", [("bf16", 64), ("bf16", 7), ("f32", 64), ("f32", 13)])
+@pytest.mark.parametrize("tokens,offsets", [
+    (20, "0 20 5"), (20, "10 20 5"), (16, "0 16 5"), (16, "3 9 16 2"), (40, "9 5 40 1 1"), (700, "0 600 590 700 20"),
+    (90, "-4 2 9 5 2147483647 1 1 1"), (700, "700 0 700 0")])
+def test_falling_offsets_stay_within_the_arrays(program, dtype, channels, tokens, offsets):
+    program("rec", dtype, channels, tokens, "packed", *offsets.split())
