@@ -144,12 +144,15 @@ __device__ __forceinline__ unsigned long long ask(const char* at, int which, uin
 }
 
 // For the first wave, a thread for each channel: tells the tile's pair p, q and returns
-// the state that enters the tile, `first` for a chain's first one.
-template <bool PACKED>
+// the state that enters the tile, `first` for a chain's first one.  ONE: only the chain's
+// first tile is given it, and tells what it makes of it as its q, so that whatever another
+// tile stores hangs on the first states having been read.
+template <bool PACKED, bool ONE>
 __device__ __forceinline__ float entering(const fg_rec_kargs& g, const Place& at, float p, float q, float first) {
     const uint32_t ch = threadIdx.x, in_group = at.tile % FG_REC_GROUP;
     const bool last = at.tile + 1 == g.tiles;
     char* mine = words(g, at, at.tile);
+    if (ONE && at.tile == 0) q = enter<PACKED>(p, q, first);
     if (!last) {
         tell(mine, 0, ch, at.tag, p);
         tell(mine, 1, ch, at.tag, q);
@@ -398,18 +401,32 @@ struct Rec {
         }
     }
 
-    // The state that enters the tile, at the lane's channels.  `first`: a chain's
-    // first one, [channels of the workgroup] or null.
+    // Forward, the last states may lie over the first ones.  Of a packed sequence the first one is part of
+    // what its last one hangs on.  A dense chain's is read by its first tile alone (entering()): its first
+    // wave's threads load it, 0 where p is null, ...
+    static __device__ __forceinline__ float first_state(const fg_rec_kargs& g, const Place& at, const float* p) {
+        const uint32_t ch = threadIdx.x;
+        if (PACKED || !p || at.tile != 0) return 0.0f;
+        return ch < CHANNELS && at.block * CHANNELS + ch < g.channels ? p[ch] : 0.0f;
+    }
+    // ... and leave it in LDS ahead of the barrier that enter_tile() stands behind, so that it has been read
+    // whichever wave then stores the last one first.
+    static __device__ __forceinline__ void keep_first(float* lds, float first) {
+        if (!PACKED && threadIdx.x < CHANNELS) lds[threadIdx.x] = first;
+    }
+
+    // The state that enters the tile, at the lane's channels.  The chain's first one: forward, where
+    // keep_first() left it; backward `first`, [channels of the workgroup] or null, which nothing is stored over.
     template <bool BACK>
     static __device__ __forceinline__ void enter_tile(const fg_rec_kargs& g, const Place& at, const Totals& t, float* lds,
-                                                      const float* first, uint32_t wave, uint32_t waves, const Lane& l,
-                                                      float (&h)[V]) {
-        if (g.tiles == 1) {
+                                                      const float* first, uint32_t waves, const Lane& l, float (&h)[V]) {
+        constexpr bool KEPT = !PACKED && !BACK;
+        if (!KEPT && g.tiles == 1) {
             params(h, first, l);
             return;
         }
         const uint32_t ch = threadIdx.x;
-        if (ch < CHANNELS) {
+        if (g.tiles > 1 && ch < CHANNELS) {
             float p = 1.0f, q = 0.0f;
             for (uint32_t k = 0; k < waves; ++k) {
                 const uint32_t w = BACK ? waves - 1 - k : k;
@@ -417,10 +434,10 @@ struct Rec {
                 q = enter<PACKED>(p2, q2, q);
                 p = through<PACKED>(p, p2);
             }
-            const bool some = first && at.block * CHANNELS + ch < g.channels;
-            lds[ch] = entering<PACKED>(g, at, p, q, some ? first[ch] : 0.0f);
+            const bool some = !KEPT && first && at.block * CHANNELS + ch < g.channels;
+            lds[ch] = entering<PACKED, KEPT>(g, at, p, q, KEPT ? lds[ch] : some ? first[ch] : 0.0f);
         }
-        __syncthreads();
+        if (g.tiles > 1) __syncthreads();
         const Floats v = *(const Floats*)&lds[l.ch];
         each<V>([&](auto c) { h[c] = v.v[c]; });
     }
@@ -519,8 +536,10 @@ struct Rec {
         Pack in[3][D];
         Source<3, FULL> source({g.x, g.ga, g.gx}, chain, t0, block, l, rows_left, S);
         each<D>([&](auto j) { source.next(in, j, j, l); });
+        const float initial = first_state(g, at, PACKED ? nullptr : of(g.initial, g, chain, block));
         Params w;
         w.load(g, block, l);
+        keep_first(&entered[0].x, initial);
         const Marks m = marks<S>(g, t0, l, look);
         // whether a sequence begins or ends in the wave's rows: few waves' do
         const bool edge = PACKED && !__all(m.in == ALL && !m.first && !m.last);
@@ -558,8 +577,7 @@ struct Rec {
         rows<false>(p, q, ep, eq, l);
         publish<false>(totals, wave, l, p, q);
         __syncthreads();
-        enter_tile<false>(g, at, totals, &entered[0].x, PACKED ? nullptr : of(g.initial, g, chain, block), wave, waves,
-                          l, h);
+        enter_tile<false>(g, at, totals, &entered[0].x, nullptr, waves, l, h);
         pass<false>(totals, wave, waves, l, h);
         if (g.check && t0 % FG_REC_CHECK == 0 && l.row == 0 && rows_left > 0)
             put(g.check + (chain * g.checks + t0 / FG_REC_CHECK) * g.channels + (uint64_t)block * CHANNELS, l, h);
@@ -669,7 +687,7 @@ struct Rec {
             params(h, g.check + (chain * g.checks + first_token / FG_REC_CHECK) * g.channels + at0, l);
         __syncthreads();
         pass<false>(ta, wave, waves, l, h);
-        enter_tile<true>(g, at, tb, &entered[0].x, PACKED ? nullptr : of(g.gfinal, g, chain, block), wave, waves, l, d);
+        enter_tile<true>(g, at, tb, &entered[0].x, PACKED ? nullptr : of(g.gfinal, g, chain, block), waves, l, d);
         pass<true>(tb, wave, waves, l, d);
         each<V>([&](auto c) {
             h[c] = enter<PACKED>(ep[c], eq[c], h[c]);

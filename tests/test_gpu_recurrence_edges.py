@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from ferrum_gpu import ssm
-from gpu_tensor import fill, room, up, use, values
+from gpu_tensor import fill, room, same, up, use, values
 from test_gpu_recurrence import TYPES, inputs
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,21 @@ def test_falling_offsets_leave_what_lies_around(gpu_device, dtype, channels, tok
     for a in (*around, out, dx):
         got = values(a)
         assert np.all(got[:2] == 7) and np.all(got[-2:] == 7)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("length", [20, 100, 256, 600, 1300])
+def test_states_in_one_array_carry_on(gpu_device, dtype, length):
+    """Call after call takes its first states where it leaves its last ones, as calls with two arrays do."""
+    lead, ch = (3, length), 132
+    d = {k: up(t) for k, t in inputs(lead, ch, dtype).items()}
+    main = (d["x"], d["gate_a"], d["gate_x"], d["decay"])
+    plan = ssm.RecurrencePlan(*lead, ch, gpu_device, dtype=dtype)
+    start = torch.randn(3, ch)
+    one, turns = up(start), [up(start), fill((3, ch))]
+    outs = [fill((*lead, ch), dtype) for _ in range(2)]
+    for _ in range(8):
+        plan.forward(*main, outs[0], initial=one, final=one)
+        plan.forward(*main, outs[1], initial=turns[0], final=turns[1])
+        turns.reverse()
+        assert same(*outs) and same(one, turns[0])

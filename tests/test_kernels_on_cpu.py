@@ -56,3 +56,11 @@ def test_recurrence_stays_within_its_arrays(program, args):
     (90, "-4 2 9 5 2147483647 1 1 1"), (700, "700 0 700 0")])
 def test_falling_offsets_stay_within_the_arrays(program, dtype, channels, tokens, offsets):
     program("rec", dtype, channels, tokens, "packed", *offsets.split())
+
+
+# A wave, a tile of several waves, several tiles in and beyond one group of them.
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("channels,tokens,sequences", [(64, 20, 1), (64, 100, 1), (37, 128, 2), (64, 256, 1), (66, 600, 2),
+                                                       (64, 1300, 1)])
+def test_last_states_may_lie_over_first_ones(program, dtype, channels, tokens, sequences):
+    program("rec", dtype, channels, tokens, "inplace", sequences)
