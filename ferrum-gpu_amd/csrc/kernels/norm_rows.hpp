@@ -92,11 +92,11 @@ struct Chunk {
             });
         }
     }
-    // A team may have more threads than the row has chunks: n is 0 for those, whose `at` lies behind the array.
+    // Whole chunks: not for n = 0.
     static __device__ __forceinline__ void floats(float (&x)[E], const float* p, uint32_t at, uint32_t n) {
         if (!p) {
             each<E>([&](auto i) { x[i] = 1.0f; });
-        } else if (EVEN ? n > 0 : n >= E) {
+        } else if (EVEN || n >= E) {
             const Floats f = *(const Floats*)(p + at);
             each<E>([&](auto i) { x[i] = f.v[i]; });
         } else {
@@ -215,7 +215,9 @@ struct Rows {
             chunks(g, [&](auto k, uint32_t col, uint32_t n) {
                 if (row < g.rows && n) next[k] = fetch(g, row, col, n);
             });
-            chunks(g, [&](auto k, uint32_t col, uint32_t n) { Io::floats(w[k], g.weight, col, n); });
+            // A team may have more threads than the row has chunks: those load the weight's first one and use
+            // nothing of it (8192 x 4096 to 8 bits 44.6 us so, 45.5 with a branch around the load).
+            chunks(g, [&](auto k, uint32_t col, uint32_t n) { Io::floats(w[k], g.weight, n ? col : 0, n); });
         }
         uint32_t turn = 0;
         for (uint64_t at = (uint64_t)blockIdx.x * TEAMS; at < g.rows; at += stride, row += stride, turn ^= 1) {
@@ -278,7 +280,7 @@ struct Rows {
         float w[KEPT][E], dw[KEPT][E], u[KEPT][E], dy[KEPT][E];
         float* part = g.part ? g.part + (uint64_t)(blockIdx.x * TEAMS + threadIdx.x / TEAM) * g.width : nullptr;
         chunks(g, [&](auto k, uint32_t col, uint32_t n) {
-            if (C > 0) Io::floats(w[k], g.weight, col, n);
+            if (C > 0 && (!EVEN || n)) Io::floats(w[k], g.weight, col, n);
             each<E>([&](auto i) { dw[k][i] = 0.0f; });
             if (C == 0 && part) each<E>([&](auto i) { if (i < n) part[col + i] = 0.0f; });
         });
