@@ -241,8 +241,11 @@ struct Rows {
             });
             over_team<TEAM, true>(squares, most, lds[turn]);
             const float s = __builtin_amdgcn_rsqf(fmaf(squares, g.over_width, g.eps));
+            // s of scales: of an infinite sum it is 0, with which a group beside the infinity, and a row whose
+            // squares pass the range, would be read back as 0
+            const float known = squares < __builtin_inff() ? s : __builtin_nanf("");
             if (g.scales && !g.group_lanes && some && threadIdx.x % TEAM == 0)
-                g.scales[row] = most == 0.0f ? 0.0f * s : fmaxf(most, kLeast) * s * (1.0f / kMost);
+                g.scales[row] = most == 0.0f ? 0.0f * known : fmaxf(most, kLeast) * known * (1.0f / kMost);
             chunks(g, [&](auto k, uint32_t col, uint32_t n) {
                 if (C == 0) {
                     each<E>([&](auto i) { v[k][i] = 0.0f; });
@@ -265,7 +268,7 @@ struct Rows {
                     for (uint32_t far = 1; far < g.group_lanes; far *= 2) m = fmaxf(m, __shfl_xor(m, far));
                     if (some && n && (threadIdx.x & (g.group_lanes - 1)) == 0)
                         g.scales[row * g.groups + col / (g.group_lanes * E)] =
-                            m == 0.0f ? 0.0f * s : fmaxf(m, kLeast) * s * (1.0f / kMost);
+                            m == 0.0f ? 0.0f * known : fmaxf(m, kLeast) * known * (1.0f / kMost);
                 }
                 const float up = kMost / fmaxf(m, kLeast);
                 each<E>([&](auto i) { y[i] = v[k][i] * w[k][i] * up; });

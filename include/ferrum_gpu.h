@@ -633,7 +633,10 @@ FG_API int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args *ar
  * With scales, out is in 8 bits (e4m3, a byte an element): out / scale, one scale
  * of float32 for each row (group = 0) or for each `group` elements of it, the last
  * ones' may be fewer; scales is [rows][ceil(width / group)].  A scale is max |out| /
- * 448, 0 where all of them are 0; it is NaN where a row holds what is not finite.
+ * 448, 0 where all of them are 0; all scales of a row are NaN where v holds what is not finite.
+ *
+ * v^2 is summed in float32.  A row whose sum passes its range (elements of about 1e19) has
+ * scales of NaN too, and without scales an out of 0 where v is finite.
  *
  * Dropout keeps element e = row * width + column where 32 bits are at least p 2^32,
  * as x / (1 - p): half e % 2 (the lower one first) of the splitmix64 number offset + e / 2

@@ -1,5 +1,6 @@
 // The norm's and dropout's kernels on the CPU, each array ending where nothing is mapped:
-// against the definition in 64 bits.  Arguments: f32 or bf16, rows, width.
+// against the definition in 64 bits.  Arguments: f32 or bf16, rows, width; or, with `bad` behind them:
+// what scales say of rows that are not finite, and of their neighbours.
 //
 // Tolerances, u = 2^-24: a thread's sum and a team's take at most 200 + width / 64 roundings and the other
 // steps of a value a dozen, so (240 + width / 64) u of the absolute values that it is a sum of, the weight's
@@ -139,6 +140,31 @@ struct Case {
         }
     }
 
+    // Rows 1 to 4 of 6: an infinity; one where the weight is 0; a NaN; finite values whose squares pass the range.
+    void not_finite(int group) {
+        Rows x = make(0, true);
+        weight[width / 2] = 0;
+        const uint32_t at[] = {width - 1, width / 2, 0};
+        const float v[] = {INFINITY, -INFINITY, NAN};
+        for (int k = 0; k < 3; ++k) (*x.a)[(1 + k) * width + at[k]] = T::down(v[k]);
+        for (uint32_t c = 0; c < width; ++c) (*x.a)[4 * width + c] = T::down(1e25f);
+        fg_norm_kargs g = args();
+        g.x = x.view;
+        g.weight = weight.data();
+        g.groups = group > 0 ? (width + group - 1) / group : 1;
+        g.group_lanes = group > 0 ? group / E : 0;
+        Guarded<float> scales((size_t)rows * g.groups);
+        Guarded<uint8_t> eight((size_t)rows * width);
+        g.scales = scales.data();
+        g.out = {eight.data(), 0, width};
+        launch(g, false);
+        for (uint32_t r = 0; r < rows; ++r)
+            for (uint32_t k = 0; k < g.groups; ++k) {
+                const float s = scales[(size_t)r * g.groups + k];
+                if (std::isnan(s) != (r > 0 && r < 5) || s < 0) check(s, r > 0 && r < 5 ? NAN : 1, -1, "scale", r * g.groups + k);
+            }
+    }
+
     void backward(uint32_t pad) {
         Rows sum = make(pad, true), dy = make(pad + 1, true), ds = make(pad, true), dx = make(pad, false),
              dr = make(pad, false);
@@ -203,9 +229,24 @@ static void all(uint32_t rows, uint32_t width) {
     c.dropped(rows * width);
 }
 
+template <class T>
+static void bad(uint32_t rows, uint32_t width) {
+    Case<T> c(rows, width);
+    for (int group : {0, 32, 64, 128}) {
+        what = "group " + std::to_string(group);
+        c.not_finite(group);
+    }
+}
+
 int main(int argc, char** argv) {
-    if (argc != 4) return 2;
+    if (argc < 4) return 2;
     const uint32_t rows = atoi(argv[2]), width = atoi(argv[3]);
+    if (argc > 4) {
+        if (std::string(argv[1]) == "f32") bad<fg::ssm::F32>(rows, width);
+        else bad<fg::ssm::BF16>(rows, width);
+        printf("%d values off\n", failed);
+        return failed != 0;
+    }
     if (std::string(argv[1]) == "f32") all<fg::ssm::F32>(rows, width);
     else all<fg::ssm::BF16>(rows, width);
     printf("%d values off\n", failed);

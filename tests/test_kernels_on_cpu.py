@@ -39,6 +39,11 @@ def test_norm_stays_within_its_arrays(program, dtype, rows, width):
     program("norm", dtype, rows, width)
 
 
+@pytest.mark.parametrize("dtype,width", [("bf16", 200), ("bf16", 600), ("bf16", 2100), ("f32", 5000), ("bf16", 16400), ("f32", 601)])
+def test_scales_of_rows_that_are_not_finite(program, dtype, width):
+    program("norm", dtype, 6, width, "bad")
+
+
 # 64 bits' definition at the sizes of one wave, one tile and several; offsets beyond the rows count as the nearest.
 @pytest.mark.parametrize("args", [
     "f32 64 40 dense 1", "f32 61 700 dense 1", "bf16 66 300 dense 2", "bf16 64 1100 dense 1", "f32 1 1 dense 3", "f32 130 129 dense 2",
