@@ -197,6 +197,11 @@ __device__ __forceinline__ float finite(float x) {
     return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -most), most);
 }
 
+// A channel's k and its biases as gate() takes them, finite, so that a closed gate leaves the
+// state whatever the parameters are, in sequences and for single tokens.
+__device__ __forceinline__ float full(float rate, float decay) { return finite(-kLog2e * rate * softplus(decay).value); }
+__device__ __forceinline__ float scaled(float bias) { return finite(-kLog2e * bias); }
+
 template <class T, bool WIDE, bool PACKED, bool STREAM>
 struct Rec {
     using raw = typename T::raw;
@@ -477,10 +482,9 @@ struct Rec {
             params(ba, g.bias_a ? g.bias_a + at : nullptr, l);
             params(bx, g.bias_x ? g.bias_x + at : nullptr, l);
             each<V>([&](auto c) {
-                // finite, so that a closed gate leaves the state whatever the parameters are
-                k[c] = finite(-kLog2e * g.rate * softplus(k[c]).value);
-                ba[c] = finite(-kLog2e * ba[c]);
-                bx[c] = finite(-kLog2e * bx[c]);
+                k[c] = full(g.rate, k[c]);
+                ba[c] = scaled(ba[c]);
+                bx[c] = scaled(bx[c]);
             });
         }
     };
@@ -821,8 +825,8 @@ __device__ __forceinline__ void step(const fg_rec_step_kargs& g) {
     if (g.bias_a) ba = *(const Floats*)(g.bias_a + ch);
     if (g.bias_x) bx = *(const Floats*)(g.bias_x + ch);
     each<V>([&](auto c) {
-        const float r = gate(T::up(ga.v[c]), -kLog2e * ba.v[c]), i = gate(T::up(gx.v[c]), -kLog2e * bx.v[c]);
-        const Share s = share(-kLog2e * g.rate * softplus(decay.v[c]).value, r);
+        const float r = gate(T::up(ga.v[c]), scaled(ba.v[c])), i = gate(T::up(gx.v[c]), scaled(bx.v[c]));
+        const Share s = share(full(g.rate, decay.v[c]), r);
         h.v[c] = fmaf(s.a, h.v[c], __builtin_amdgcn_sqrtf(s.m2) * i * T::up(x.v[c]));
         out.v[c] = T::down(h.v[c]);
     });

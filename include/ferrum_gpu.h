@@ -551,6 +551,7 @@ FG_API int fg_scan_step(fg_device_t dev, const fg_scan_step_args *args, fg_strea
  *   r = sigmoid(gate_a + bias_a[d]), i = sigmoid(gate_x + bias_x[d])
  *   a = exp(-rate softplus(decay[d]) r)
  *   h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
+ * Infinite decays and biases count as the largest numbers, so that a gate_a of -inf leaves the state.
  * Rows, packed sequences (their number of tokens is not held against `length`),
  * states and workspaces as for the scan; the forward pass uses the plan's workspaces
  * too, so all calls of a plan follow one another. */

@@ -3,6 +3,8 @@
 //   dense SEQUENCES     against the definition in 64 bits, forward and backward
 //   inplace SEQUENCES   the last states over the first ones, whichever wave goes first, and nothing reads
 //                       the first ones once their sequences' first tiles have ended
+//   step ROWS           the one-token kernel, gates and parameters infinite among them, against sequences of
+//                       one token (TOKENS is 1)
 //   packed OFFSET ...   likewise; offsets that fall: for where accesses go alone
 //
 // Tolerances as for the GPU's results: of a state (240 + 4 tokens) u of the sum of its terms' absolute
@@ -230,10 +232,51 @@ static void in_place(uint32_t channels, uint64_t tokens, uint32_t seqs) {
     }
 }
 
+template <class T, int W>
+static void one_token(uint32_t channels, uint32_t rows) {
+    Call<T> c(false, rows, channels, 1, {});
+    const float far[] = {INFINITY, -INFINITY, 0.5f};
+    const auto pick = [&] { return far[(int)(1e6 * std::fabs(random_number())) % 3]; };
+    for (uint32_t k = 0; k < channels; ++k) c.decay[k] = pick(), c.ba[k] = pick(), c.bx[k] = pick();
+    for (uint32_t i = 0; i < rows * channels; ++i) c.ga[i] = T::down(pick()), c.gx[i] = T::down(pick());
+    c.run(false, false);
+    // the rows' states in slots from the last one on; the first row has none, nor has the last one
+    const uint32_t slots = rows + 1;
+    Guarded<float> state(slots * channels), next(slots * channels);
+    Guarded<int32_t> slot(rows);
+    Guarded<typename T::raw> out(rows * channels);
+    for (uint32_t r = 0; r < rows; ++r) {
+        slot[r] = r == 0 ? -1 : r + 1 == rows && rows > 1 ? (int32_t)slots : (int32_t)(slots - 1 - r);
+        for (uint32_t k = 0; k < channels && slot[r] >= 0 && slot[r] < (int32_t)slots; ++k)
+            state[slot[r] * channels + k] = c.initial[r * channels + k];
+    }
+    fg_rec_step_kargs g{};
+    const auto view = [&](Guarded<typename T::raw>& a) { return fg_ssm_view{a.data(), channels, 0}; };
+    g.x = view(c.x), g.ga = view(c.ga), g.gx = view(c.gx), g.out = view(out);
+    g.decay = c.decay.data(), g.bias_a = c.ba.data(), g.bias_x = c.bx.data();
+    g.state = state.data(), g.state_out = next.data(), g.slots = slot.data();
+    g.state_rows = slots, g.rows = rows, g.channels = channels, g.rate = 8.0f;
+    const uint32_t waves = (channels / W + 63) / 64 * rows;
+    on_cpu::launch((waves + 3) / 4, 256, false, [&] { step<T, W>(g); });
+    for (uint32_t r = 0; r < rows; ++r)
+        for (uint32_t k = 0; k < channels; ++k) {
+            const size_t i = r * channels + k;
+            const bool some = slot[r] >= 0 && slot[r] < (int32_t)slots;
+            const float want = some ? T::up(c.out[i]) : 0, got = T::up(out[i]);
+            if (!(std::isnan(want) && std::isnan(got))) check(got, want, 1e-6 * std::fabs(want) + Call<T>::half * std::fabs(want), "out", i);
+            if (!some) continue;
+            const float to = next[slot[r] * channels + k], end = c.final[i];
+            if (!(std::isnan(to) && std::isnan(end))) check(to, end, 1e-6 * std::fabs(end), "state", i);
+            // a closed gate leaves the state whatever the parameters are
+            if (std::isinf(T::up(c.ga[i])) && T::up(c.ga[i]) < 0) check(to, c.initial[i], 0, "state behind a closed gate", i);
+        }
+}
+
 template <class T>
 static void all(uint32_t channels, uint64_t tokens, const std::string& kind, const std::vector<int32_t>& more) {
     const bool packed = kind == "packed", falls = packed && !std::is_sorted(more.begin(), more.end());
     const uint32_t seqs = packed ? (uint32_t)more.size() - 1 : (uint32_t)more.at(0);
+    if (kind == "step") return channels % 4 ? one_token<T, 1>(channels, seqs) : one_token<T, 4>(channels, seqs);
     if (kind == "inplace") return in_place<T>(channels, tokens, seqs);
     for (bool last : {false, true}) {
         Call<T> c(packed, seqs, channels, tokens, packed ? more : std::vector<int32_t>{});

@@ -61,3 +61,28 @@ def test_states_in_one_array_carry_on(gpu_device, dtype, length):
         plan.forward(*main, outs[1], initial=turns[0], final=turns[1])
         turns.reverse()
         assert same(*outs) and same(one, turns[0])
+
+
+@pytest.mark.parametrize("dtype,channels", [("float32", 64), ("bfloat16", 62)])
+def test_one_token_is_a_sequence_of_one_whatever_the_parameters(gpu_device, dtype, channels):
+    """Infinite decays, biases and gates: the step gives what a plan gives for one token, and a closed gate leaves
+    the state in both."""
+    rows, inf = 60, float("inf")
+    v = inputs((rows,), channels, dtype)
+    far = torch.tensor([inf, -inf, 0.5])
+    for k, lead in (("decay", ()), ("bias_a", ()), ("bias_x", ()), ("gate_a", (rows,)), ("gate_x", (rows,))):
+        v[k] = far[torch.randint(0, 3, (*lead, channels))].to(v[k].dtype)
+    d = {k: up(t) for k, t in v.items()}
+    state = torch.randn(rows, channels)
+    outs, ends = [fill((rows, channels), dtype) for _ in range(2)], [fill((rows, channels)) for _ in range(2)]
+    ssm.recurrence_step(gpu_device, **d, state=up(state), out=outs[0], state_out=ends[0])
+    plan = ssm.RecurrencePlan(rows, 1, channels, gpu_device, dtype=dtype)
+    seq = {k: d[k].view(rows, 1, channels) for k in ("x", "gate_a", "gate_x")}
+    plan.forward(**{**d, **seq}, out=outs[1].view(rows, 1, channels), initial=up(state), final=ends[1])
+    for a, b, step in ((*outs, 0 if dtype == "float32" else torch.finfo(TYPES[dtype]).eps), (*ends, 0)):
+        a, b = values(a), values(b)
+        # the same formula in float32: a dozen roundings of 2^-24, and a half step of the rows on either side
+        assert np.array_equal(np.isnan(a), np.isnan(b))
+        assert (np.abs(a - b) <= (12 * 2.0 ** -24 + step) * np.abs(b))[~np.isnan(b)].all()
+    closed = (v["gate_a"] == -inf).numpy()
+    assert np.array_equal(values(ends[0])[closed], state.double().numpy()[closed])

@@ -63,6 +63,12 @@ def test_falling_offsets_stay_within_the_arrays(program, dtype, channels, tokens
     program("rec", dtype, channels, tokens, "packed", *offsets.split())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("channels,rows", [(64, 7), (37, 5), (1, 3), (260, 9)])
+def test_one_token_is_a_sequence_of_one(program, dtype, channels, rows):
+    program("rec", dtype, channels, 1, "step", rows)
+
+
 # A wave, a tile of several waves, several tiles in and beyond one group of them.
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("channels,tokens,sequences", [(64, 20, 1), (64, 100, 1), (37, 128, 2), (64, 256, 1), (66, 600, 2),
