@@ -48,6 +48,14 @@ typedef struct {
     float rate;
 } fg_rec_kargs;
 
+/* What the kernels divide by (place_of), once blocks, chains and tiles are known. */
+static inline void fg_rec_set_divisors(fg_rec_kargs* g) {
+    const uint64_t across = (uint64_t)g->blocks * g->chains;
+    g->over_tiles = ~0ull / g->tiles;
+    g->over_across = across ? (uint32_t)(0xffffffffull / across) : 0;
+    g->over_blocks = g->blocks ? 0xffffffffu / g->blocks : 0;
+}
+
 typedef struct {
     fg_ssm_view x, ga, gx, out; /* .seq: of rows; .row unused */
     const float *decay, *bias_a, *bias_x, *state;

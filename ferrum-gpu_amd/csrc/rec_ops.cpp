@@ -184,9 +184,7 @@ fg_rec_kargs RecurrencePlan::base(const char* op, const fg_recurrence_inputs& in
     g.tiles = across ? (uint32_t)(n / across) : 1;
     g.parts = chains_ * g.tiles;
     g.chain = (unsigned long long*)(back ? back_ : ahead_).data();
-    g.over_tiles = ~0ull / g.tiles;
-    g.over_across = across ? (uint32_t)(0xffffffffull / across) : 0;
-    g.over_blocks = g.blocks ? 0xffffffffu / g.blocks : 0;
+    fg_rec_set_divisors(&g);
     return g;
 }
 

@@ -5,6 +5,7 @@
 //                       the first ones once their sequences' first tiles have ended
 //   step ROWS           the one-token kernel, gates and parameters infinite among them, against sequences of
 //                       one token (TOKENS is 1)
+//   places FIRST        where workgroups of CHANNELS blocks and TOKENS chains go, from the FIRST-th launch on
 //   packed OFFSET ...   likewise; offsets that fall: for where accesses go alone
 //
 // Tolerances as for the GPU's results: of a state (240 + 4 tokens) u of the sum of its terms' absolute
@@ -79,10 +80,7 @@ struct Call {
         waves = (uint32_t)std::min<uint64_t>(most_waves, std::max<uint64_t>(1, (tokens + wave_tokens - 1) / wave_tokens));
         g.tiles = (uint32_t)std::max<uint64_t>(1, (tokens + wave_tokens * waves - 1) / (wave_tokens * waves));
         g.parts = chains * g.tiles;
-        const uint64_t across = blocks * chains;
-        g.over_tiles = ~0ull / g.tiles;
-        g.over_across = (uint32_t)(0xffffffffull / across);
-        g.over_blocks = 0xffffffffu / g.blocks;
+        fg_rec_set_divisors(&g);
         return g;
     }
 
@@ -272,10 +270,45 @@ static void one_token(uint32_t channels, uint32_t rows) {
         }
 }
 
+// Launches of every number of tiles: each channel block of each chain has its tiles once, in the order of
+// its tickets, with words of its own and a tag that the launch before did not have and new memory does not.
+static void places(uint32_t blocks, uint32_t chains, uint64_t first) {
+    for (uint32_t tiles : {1, 2, 3, 4, 5, 7, 33, 128}) {
+        fg_rec_kargs g{};
+        g.blocks = blocks, g.chains = chains, g.tiles = tiles;
+        fg_rec_set_divisors(&g);
+        const uint64_t across = (uint64_t)blocks * chains, bytes = FG_REC_CHAIN_BYTES(across, tiles);
+        Guarded<char> memory(bytes);
+        for (uint64_t k = 0; k < across; ++k) *(unsigned long long*)(memory.data() + 64 * k) = first * tiles;
+        if (tiles > 1) g.chain = (unsigned long long*)memory.data();
+        uint32_t before = 0;
+        for (uint64_t launch = first; launch < first + 4; ++launch) {
+            std::vector<uint32_t> drawn(across, 0);
+            std::vector<bool> taken(across * tiles, false);
+            uint32_t tag = 0;
+            on_cpu::launch((uint32_t)(across * tiles), 1, false, [&] {
+                const Place p = place_of(g);
+                if (p.block >= blocks || p.chain >= chains || p.tile >= tiles) return check(1, 0, 0, "beyond", blockIdx.x);
+                check(p.tile, drawn[p.chain * blocks + p.block]++, 0, "tile", blockIdx.x);
+                if (tiles == 1) return;
+                if (tag == 0) tag = p.tag;
+                if (p.tag != tag || p.tag == before || p.tag == 0) check(1, 0, 0, "tag", blockIdx.x);
+                const uint64_t at = words(g, p, p.tile) - memory.data(), each = 8 * FG_REC_WORDS * CHANNELS;
+                if (at < 64 * across || at + each > bytes || (at - 64 * across) % each || taken[(at - 64 * across) / each])
+                    return check(1, 0, 0, "words", blockIdx.x);
+                taken[(at - 64 * across) / each] = true;
+            });
+            for (uint64_t k = 0; k < across; ++k) check(drawn[k], tiles, 0, "tiles", k);
+            before = tag;
+        }
+    }
+}
+
 template <class T>
 static void all(uint32_t channels, uint64_t tokens, const std::string& kind, const std::vector<int32_t>& more) {
     const bool packed = kind == "packed", falls = packed && !std::is_sorted(more.begin(), more.end());
     const uint32_t seqs = packed ? (uint32_t)more.size() - 1 : (uint32_t)more.at(0);
+    if (kind == "places") return places(channels, (uint32_t)tokens, (uint64_t)(uint32_t)more.at(0));
     if (kind == "step") return channels % 4 ? one_token<T, 1>(channels, seqs) : one_token<T, 4>(channels, seqs);
     if (kind == "inplace") return in_place<T>(channels, tokens, seqs);
     for (bool last : {false, true}) {

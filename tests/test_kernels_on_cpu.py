@@ -63,6 +63,14 @@ def test_falling_offsets_stay_within_the_arrays(program, dtype, channels, tokens
     program("rec", dtype, channels, tokens, "packed", *offsets.split())
 
 
+# Numbers of channel blocks and chains that the eight XCDs divide and others; launches from the first one on and
+# around the one whose number passes the tags' 31 bits.
+@pytest.mark.parametrize("blocks,chains", [(1, 1), (3, 1), (8, 1), (5, 8), (16, 3), (7, 7), (32, 1), (24, 2), (1, 13)])
+@pytest.mark.parametrize("first", [0, 5, 2 ** 31 - 2])
+def test_workgroups_share_the_tiles(program, blocks, chains, first):
+    program("rec", "f32", blocks, chains, "places", first)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("channels,rows", [(64, 7), (37, 5), (1, 3), (260, 9)])
 def test_one_token_is_a_sequence_of_one(program, dtype, channels, rows):
