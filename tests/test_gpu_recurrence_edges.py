@@ -9,7 +9,7 @@ import torch
 
 from ferrum_gpu import ssm
 from gpu_tensor import fill, room, same, up, use, values
-from test_gpu_recurrence import TYPES, inputs
+from test_gpu_recurrence import TYPES, inputs, run
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,22 @@ def test_one_token_is_a_sequence_of_one_whatever_the_parameters(gpu_device, dtyp
         assert (np.abs(a - b) <= (12 * 2.0 ** -24 + step) * np.abs(b))[~np.isnan(b)].all()
     closed = (v["gate_a"] == -inf).numpy()
     assert np.array_equal(values(ends[0])[closed], state.double().numpy()[closed])
+
+
+LARGE = 16 << 20  # bytes of rows from which on a plan takes the kernels that pass the caches
+
+
+@pytest.mark.parametrize("batch,length,channels,dtype,layout", [
+    (1, 1030, 8192, "bfloat16", "plain"), (2, 1100, 4098, "float16", "plain"), (3, 700, 2050, "float32", "windows"),
+    (1, 2100, 4000, "bfloat16", "windows")])
+def test_large_arrays(gpu_device, batch, length, channels, dtype, layout):
+    assert batch * length * channels * TYPES[dtype].itemsize >= LARGE
+    run(gpu_device, (batch, length), channels, dtype, layout=layout)
+
+
+@pytest.mark.parametrize("channels,dtype,offsets", [
+    (8194, "bfloat16", [0, 300, 300, 310, 1030]), (4100, "float16", [2, 700, 701, 702, 2100]),
+    (4096, "float32", [0, 0, 33, 1024, 1030, 1100])])
+def test_large_packed_arrays(gpu_device, channels, dtype, offsets):
+    assert offsets[-1] * channels * TYPES[dtype].itemsize >= LARGE
+    run(gpu_device, (offsets[-1] + 9,), channels, dtype, offsets=offsets)
