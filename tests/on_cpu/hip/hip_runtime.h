@@ -193,12 +193,10 @@ inline uint32_t to_e4m3(float x) {
     const uint32_t sign = __float_as_uint(x) >> 31 << 7;
     const float a = std::fabs(x);
     if (!(a <= 464.0f)) return sign | 0x7f;
-    uint32_t best = 0;
-    for (uint32_t c = 1; c < 0x7f; ++c) {
-        const float d = std::fabs(e4m3(c) - a), e = std::fabs(e4m3(best) - a);
-        if (d < e || (d == e && c % 2 == 0)) best = c;
-    }
-    return sign | best;
+    uint32_t lo = 0, hi = 0x7e;  // neighbours, in the end
+    while (hi - lo > 1) (e4m3((lo + hi) / 2) <= a ? lo : hi) = (lo + hi) / 2;
+    const float below = a - e4m3(lo), above = e4m3(hi) - a;
+    return sign | (below < above || (below == above && lo % 2 == 0) ? lo : hi);
 }
 
 }  // namespace on_cpu

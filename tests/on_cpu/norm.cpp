@@ -1,5 +1,5 @@
 // The norm's and dropout's kernels on the CPU, each array ending where nothing is mapped:
-// against the definition in 64 bits.  Arguments: f32 or bf16, rows, width; or, with `bad` behind them:
+// against the definition in 64 bits.  Built for TYPE, F32 or BF16.  Arguments: rows, width; or, with `bad` behind them:
 // what scales say of rows that are not finite, and of their neighbours.
 //
 // Tolerances, u = 2^-24: a thread's sum and a team's take at most 200 + width / 64 roundings and the other
@@ -239,16 +239,10 @@ static void bad(uint32_t rows, uint32_t width) {
 }
 
 int main(int argc, char** argv) {
-    if (argc < 4) return 2;
-    const uint32_t rows = atoi(argv[2]), width = atoi(argv[3]);
-    if (argc > 4) {
-        if (std::string(argv[1]) == "f32") bad<fg::ssm::F32>(rows, width);
-        else bad<fg::ssm::BF16>(rows, width);
-        printf("%d values off\n", failed);
-        return failed != 0;
-    }
-    if (std::string(argv[1]) == "f32") all<fg::ssm::F32>(rows, width);
-    else all<fg::ssm::BF16>(rows, width);
+    if (argc < 3) return 2;
+    const uint32_t rows = atoi(argv[1]), width = atoi(argv[2]);
+    if (argc > 3) bad<fg::ssm::TYPE>(rows, width);
+    else all<fg::ssm::TYPE>(rows, width);
     printf("%d values off\n", failed);
     return failed != 0;
 }

@@ -13,8 +13,9 @@ CLANG = "/opt/rocm/llvm/bin/clang++"
 _ASM = re.compile(r'\basm(?: volatile)?\((?:"[^"]*"|[^;"])*\);')
 
 
-def build(program: str, to) -> str:
-    """Builds `program` (.cpp, of this folder) in the folder `to`; the path of what can be run."""
+def build(to) -> dict:
+    """Builds the programs of this folder in the folder `to`, one for each element type, all at a time.
+    (program, type) -> the path of what can be run."""
     copies = os.path.join(str(to), "kernels")
     os.makedirs(copies, exist_ok=True)
     for name in os.listdir(KERNELS):
@@ -23,7 +24,9 @@ def build(program: str, to) -> str:
                 text = f.read()
             with open(os.path.join(copies, name), "w") as f:
                 f.write(_ASM.sub("", text).replace("__attribute__((address_space(4)))", ""))
-    exe = os.path.join(str(to), program.removesuffix(".cpp"))
-    subprocess.run([CLANG, "-std=c++17", "-O1", "-mf16c", "-Wno-everything", "-I", HERE, "-I", copies,
-                    os.path.join(HERE, program), "-o", exe], check=True)
-    return exe
+    built = {(p, t): os.path.join(str(to), f"{p}_{t}") for p in ("rec", "norm") for t in ("f32", "bf16")}
+    running = [subprocess.Popen([CLANG, "-std=c++17", "-O1", "-mf16c", "-w", f"-DTYPE={t.upper()}", "-I", HERE, "-I", copies,
+                                 os.path.join(HERE, p + ".cpp"), "-o", exe]) for (p, t), exe in built.items()]
+    for r in running:
+        assert r.wait() == 0, r.args
+    return built

@@ -1,12 +1,12 @@
 // The recurrence's kernels on the CPU, each array ending where nothing is mapped.
-// Arguments: f32 or bf16, channels, tokens (packed: of all sequences), and
+// Built for TYPE, F32 or BF16.  Arguments: channels, tokens (packed: of all sequences), and
 //   dense SEQUENCES     against the definition in 64 bits, forward and backward
 //   inplace SEQUENCES   the last states over the first ones, whichever wave goes first, and nothing reads
 //                       the first ones once their sequences' first tiles have ended
 //   step ROWS           the one-token kernel, gates and parameters infinite among them, against sequences of
 //                       one token (TOKENS is 1)
 //   places FIRST        where workgroups of CHANNELS blocks and TOKENS chains go, from the FIRST-th launch on
-//   packed OFFSET ...   likewise; offsets that fall: for where accesses go alone
+//   packed OFFSET ...   as dense; offsets that fall: for where accesses go alone
 //
 // Tolerances as for the GPU's results: of a state (240 + 4 tokens) u of the sum of its terms' absolute
 // values, u = 2^-24, of gradients twice that, rows rounded by half a step of their type.
@@ -320,11 +320,10 @@ static void all(uint32_t channels, uint64_t tokens, const std::string& kind, con
 }
 
 int main(int argc, char** argv) {
-    if (argc < 6) return 2;
+    if (argc < 5) return 2;
     std::vector<int32_t> more;
-    for (int k = 5; k < argc; ++k) more.push_back(atoi(argv[k]));
-    if (std::string(argv[1]) == "f32") all<fg::ssm::F32>(atoi(argv[2]), atoi(argv[3]), argv[4], more);
-    else all<fg::ssm::BF16>(atoi(argv[2]), atoi(argv[3]), argv[4], more);
+    for (int k = 4; k < argc; ++k) more.push_back(atoi(argv[k]));
+    all<fg::ssm::TYPE>(atoi(argv[1]), atoi(argv[2]), argv[3], more);
     printf("%d values off\n", failed);
     return failed != 0;
 }

@@ -18,13 +18,11 @@ pytestmark = pytest.mark.skipif(not os.path.exists(programs.CLANG), reason="need
 
 @pytest.fixture(scope="module")
 def program(tmp_path_factory):
-    built = {}
+    built = programs.build(tmp_path_factory.mktemp("on_cpu"))
 
-    def run(name, *args):
-        if name not in built:
-            built[name] = programs.build(name + ".cpp", tmp_path_factory.mktemp(name))
-        got = subprocess.run([built[name], *map(str, args)], capture_output=True, text=True, timeout=300)
-        assert got.returncode == 0, f"{name} {args}: ended with {got.returncode}\n{got.stdout}{got.stderr}"
+    def run(name, dtype, *args):
+        got = subprocess.run([built[name, dtype], *map(str, args)], capture_output=True, text=True, timeout=300)
+        assert got.returncode == 0, f"{name} {dtype} {args}: ended with {got.returncode}\n{got.stdout}{got.stderr}"
 
     return run
 
