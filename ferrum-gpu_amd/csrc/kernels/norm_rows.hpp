@@ -21,9 +21,9 @@
 // gradient at what was stored.
 //
 // Bound by memory.  Measured (8192 rows x 4096, bfloat16, us; a copy of as many bytes would take):
-// with the residual to 8 bits 44 (35), with dropout and the residual 50 (40), backward 68 (50) and 5
+// with the residual to 8 bits 45 (35), with dropout and the residual 50 (40), backward 70 (50) and 5
 // for the weight's gradient; dropout alone 22 (20).  Dropout is 18 vector instructions of an
-// element, most of them the generator's 64-bit products, backward 24 others: 36 us of the 68.
+// element, most of them the generator's 64-bit products, backward 24 others: 36 us of the 70.
 // Teams of 256 with two chunks a thread 51, without the next row's loads 53, with ordinary stores 57.
 //
 // Dropout keeps element e (row-major) where 32 bits are at least p 2^32: half e % 2 of

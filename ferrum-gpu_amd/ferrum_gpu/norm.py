@@ -98,7 +98,8 @@ class NormPlan(_Plan):
         """``weight`` (width) float32 (None: ones).  ``sum_out``: room for v in the
         rows' type, which backward() takes; may be ``residual``, and ``out`` may be
         ``x``.  With ``scales``, (rows, groups) float32, ``out`` is float8_e4m3fn
-        (or uint8): the normed row over its scale, max |out| / 448 of a group."""
+        (or uint8): the normed row over its scale, max |out| / 448 of a group; NaN,
+        like all scales of a row, where the row's sum of squares is not finite."""
         n, at = self._count(x, rows), self.device.ordinal
         args = _forward_pack(n, *self._of(x, n, "x"), *self._of(residual, n, "residual"),
                              *(self._of(out, n, "out") if scales is None else self._out8(out, n)),

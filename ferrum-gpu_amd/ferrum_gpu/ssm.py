@@ -410,7 +410,10 @@ class RecurrencePlan(_Plan):
         h_t[d] = a h_{t-1}[d] + sqrt(1 - a^2) i x,  out = h_t
 
     With ``tokens`` the sequences are packed; ``length`` is not used then.  Both
-    passes use the plan's workspaces, so calls of one plan follow one another.
+    passes use the plan's workspaces, so calls of one plan follow one another; calls
+    that overlap, on two streams or as replayed graphs, mix up their tokens without an
+    error.  A sequence's parts wait for those before them within a launch; a wait of
+    seconds, which no call by itself comes to, gives up, with NaN from there on.
     """
 
     _destroy, _get_info = _n.lib.fg_recurrence_plan_destroy, _n.lib.fg_recurrence_plan_get_info

@@ -554,7 +554,9 @@ FG_API int fg_scan_step(fg_device_t dev, const fg_scan_step_args *args, fg_strea
  * Infinite decays and biases count as the largest numbers, so that a gate_a of -inf leaves the state.
  * Rows, packed sequences (their number of tokens is not held against `length`),
  * states and workspaces as for the scan; the forward pass uses the plan's workspaces
- * too, so all calls of a plan follow one another. */
+ * too, so all calls of a plan follow one another: calls that overlap, on two streams or as replayed
+ * graphs, mix up their tokens without an error.  Within a launch the parts of a sequence wait for those
+ * before them; a wait of seconds, which no call by itself comes to, gives up, with NaN from there on. */
 typedef struct fg_recurrence_plan *fg_recurrence_plan_t;
 
 typedef struct fg_recurrence_shape {
