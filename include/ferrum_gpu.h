@@ -639,7 +639,8 @@ FG_API int fg_recurrence_step(fg_device_t dev, const fg_recurrence_step_args *ar
  * 448, 0 where all of them are 0; all scales of a row are NaN where v holds what is not finite.
  *
  * v^2 is summed in float32.  A row whose sum passes its range (elements of about 1e19) has
- * scales of NaN too, and without scales an out of 0 where v is finite.
+ * scales of NaN too, and without scales an out of 0 where v is finite.  With an eps of 0, a row
+ * whose mean falls below its normal numbers (elements of about 1e-19, zeros) is divided by 0.
  *
  * Dropout keeps element e = row * width + column where 32 bits are at least p 2^32,
  * as x / (1 - p): half e % 2 (the lower one first) of the splitmix64 number offset + e / 2
